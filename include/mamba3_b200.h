@@ -43,7 +43,8 @@ typedef enum m3_dtype {
   M3_FLOAT32 = 0,
   M3_BFLOAT16 = 1,
   M3_FLOAT16 = 2,
-  M3_INT64 = 3 /* token ids (m3_argmax_rows) */
+  M3_INT64 = 3, /* token ids */
+  M3_UINT8 = 4  /* masks: 0 = the position does not count */
 } m3_dtype;
 
 typedef enum m3_status {
@@ -375,6 +376,75 @@ int m3_layer_prologue_bwd(const m3_layer_dims* dims, const m3_tensor* zxbcdt, co
                           size_t workspace_bytes, void* stream);
 int m3_silu_gate_bwd(const m3_tensor* y, const m3_tensor* z, const m3_tensor* dout, m3_tensor* dy,
                      m3_tensor* dz, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Losses over the tokens of a language model's logits, for fine-tuning (no counterpart in
+ * the reference, whose train.py takes a cross-entropy of the logits). With s = 1 /
+ * temperature and logp = s l[tok] - log sum_v exp(s l[v]) of a position's logits l:
+ *   m3_token_logprobs   logp of every position
+ *   m3_policy_loss      sum_t w_t [ -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *                       + kl_coef (exp(d) - d - 1) ],  r = exp(logp - old), d = ref - logp;
+ *                       w = 1 / (positions that count), or with by_sequence 1 / (those of the
+ *                       sequence) / (sequences with any)
+ *   m3_preference_loss  mean over pairs of -(1 - e) log sigma(z) - e log sigma(-z), z = reward of
+ *                       sequence i (chosen) - reward of sequence N + i (rejected), reward =
+ *                       beta sum_t (logp - ref), e = label_smoothing
+ *   m3_token_grad       dlogits = up * coef * s * (one-hot - softmax), the gradient of all three
+ * Operands:
+ *   logits (batch, seqlen, V) f32 / bf16 / f16, innermost stride 1; tokens (batch, seqlen) i64;
+ *   mask (batch, seqlen) u8, optional: a position counts where it is not 0 and the token is
+ *   not ignore_index. Other positions are not read: their logp and gradient rows are 0. A
+ *   token outside [0, V) that is not ignore_index makes its position's results NaN.
+ *   old_logprobs, advantages, ref_logprobs, coef (batch, seqlen) f32, any strides (0 where one
+ *   value serves a sequence); ref_logprobs optional (absent: no KL term / reference 0).
+ *   logprobs (batch, seqlen) f32 contiguous, stats (batch, seqlen, 2) f32 contiguous: what
+ *   m3_token_grad needs of each row; optional. temperature > 0, finite.
+ *   m3_policy_loss: loss, kl (mean), clip_fraction: one f32 each; coef (batch, seqlen) f32
+ *   contiguous optional: d loss / d logp; dlogits optional (logits' dtype, innermost stride 1):
+ *   the gradient for an upstream gradient of 1, written while the row is at hand.
+ *   m3_preference_loss: loss (one f32), rewards (2 N), seq_coef (2 N) f32: d loss / d logp of a
+ *   sequence's positions, which m3_token_grad takes as a coef of strides (1, 0).
+ *   m3_token_grad: up optional, one f32 on the device; with keep_if_one the call leaves
+ *   dlogits as it is where *up is 1 (m3_policy_loss has written it).
+ *   workspace: as the _workspace_size functions say, 16-byte aligned.
+ * ------------------------------------------------------------------------------- */
+int m3_token_logprobs(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                      double temperature, int64_t ignore_index, m3_tensor* logprobs, m3_tensor* stats,
+                      void* stream);
+size_t m3_policy_loss_workspace_size(int64_t batch, int64_t seqlen);
+int m3_policy_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                   const m3_tensor* old_logprobs, const m3_tensor* advantages, const m3_tensor* ref_logprobs,
+                   double temperature, int64_t ignore_index, double clip_low, double clip_high, double kl_coef,
+                   int by_sequence, m3_tensor* loss, m3_tensor* kl, m3_tensor* clip_fraction,
+                   m3_tensor* logprobs, m3_tensor* stats, m3_tensor* coef, m3_tensor* dlogits, void* workspace,
+                   size_t workspace_bytes, void* stream);
+size_t m3_preference_loss_workspace_size(int64_t batch, int64_t seqlen);
+int m3_preference_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                       const m3_tensor* ref_logprobs, double temperature, int64_t ignore_index, double beta,
+                       double label_smoothing, m3_tensor* loss, m3_tensor* rewards, m3_tensor* logprobs,
+                       m3_tensor* stats, m3_tensor* seq_coef, void* workspace, size_t workspace_bytes,
+                       void* stream);
+int m3_token_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                  const m3_tensor* stats, const m3_tensor* coef, const m3_tensor* up, double temperature,
+                  int64_t ignore_index, int keep_if_one, m3_tensor* dlogits, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Global norm of many gradient tensors, with scaling and clipping (the reference's train.py
+ * calls torch's clip_grad_norm_):
+ *   norm = scale * sqrt(sum g^2), or scale * max |g| with largest;
+ *   g <- g * scale * min(1, max_norm / (norm + 1e-6)), or out <- that with outs.
+ * The tensors are dense runs of elements, given as host arrays (a model has hundreds, and
+ * four arrays are quicker to build than as many m3_tensor records): device pointers, element
+ * counts and m3_dtype (f32 / bf16 / f16). outs NULL: in place, and nothing is written where
+ * scale is 1 and nothing is clipped. out_dtypes: the gradient's own or M3_FLOAT32. Tensors
+ * that are written must not overlap one another or another gradient. max_norm infinite: no
+ * clipping. A NaN gradient makes the norm and every scaled gradient NaN.
+ *   norm (1) f32. workspace: m3_clip_grads_workspace_size(count) bytes, 16-byte aligned.
+ * ------------------------------------------------------------------------------- */
+size_t m3_clip_grads_workspace_size(int64_t count);
+int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel, const int32_t* dtypes,
+                  void* const* outs, const int32_t* out_dtypes, int largest, double max_norm, double scale,
+                  m3_tensor* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Health word of the warp-specialised kernels and of the single-pass MIMO forward on the

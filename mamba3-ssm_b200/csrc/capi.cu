@@ -2,18 +2,22 @@
 // kernels, and the thread-local error string. Nothing here allocates device memory.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <mutex>
 #include <string>
+#include <vector>
 
 #include "argmax.cuh"
 #include "decode_step.cuh"
+#include "grad_clip.cuh"
 #include "m3_common.cuh"
 #include "mimo_scan.cuh"
 #include "prologue.cuh"
 #include "rmsnorm.cuh"
 #include "siso_chunk.cuh"
 #include "siso_scan.cuh"
+#include "token_loss.cuh"
 
 namespace m3 {
 
@@ -1096,6 +1100,248 @@ int m3_silu_gate(const m3_tensor* y, const m3_tensor* z, m3_tensor* out, void* s
   p.rows = sh[0] * sh[1] * sh[2]; p.L = (int)sh[1]; p.H = (int)sh[2]; p.P = (int)sh[3];
   p.y = y->data; p.sy = s3(y); p.z = z->data; p.sz = s3(z); p.out = out->data; p.so = s3(out);
   return launch_gate(p, y->dtype, z->dtype, out->dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------
+// token losses
+// ------------------------------------------------------------------------------------
+namespace m3 {
+namespace {
+
+// A (batch, seqlen) operand of the token losses: one dtype, any strides.
+template <typename T>
+int map2(const m3_tensor* t, const char* name, int dtype, const int64_t* bt, bool optional, bool devcheck,
+         Map2<T>* out) {
+  *out = Map2<T>{nullptr, 0, 0};
+  if (!present(t)) {
+    if (optional) return M3_OK;
+    return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": missing");
+  }
+  if (t->ndim != 2 || t->shape[0] != bt[0] || t->shape[1] != bt[1])
+    return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": expected (batch, seqlen) = (" + std::to_string(bt[0]) +
+                                             "," + std::to_string(bt[1]) + ")");
+  if (t->dtype != dtype)
+    return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": unsupported dtype " + std::to_string(t->dtype));
+  if (t->stride[0] < 0 || t->stride[1] < 0)
+    return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": negative stride");
+  if (devcheck) M3_TRY(check_device_ptr(t->data, name));
+  *out = Map2<T>{static_cast<T*>(t->data), t->stride[0], t->stride[1]};
+  return M3_OK;
+}
+
+// The rows that every token loss reads; *empty: there is no position.
+int token_rows(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask, double temperature,
+               int64_t ignore_index, TokenRows* p, bool* empty) {
+  if (!present(logits)) return fail(M3_ERR_INVALID_ARGUMENT, "logits: missing");
+  if (logits->ndim != 3) return fail(M3_ERR_INVALID_ARGUMENT, "logits: expected (batch, seqlen, vocabulary)");
+  const int64_t* sh = logits->shape;
+  if (sh[0] < 0 || sh[1] < 0 || sh[2] <= 0) return fail(M3_ERR_INVALID_ARGUMENT, "logits: empty vocabulary");
+  if (sh[1] > INT32_MAX || sh[2] > INT32_MAX / 2 || (sh[0] > 0 && sh[1] > INT32_MAX / 8 / sh[0]))
+    return fail(M3_ERR_UNSUPPORTED, "logits: dimension too large");
+  *empty = sh[0] * sh[1] == 0;
+  M3_TRY(check(logits, "logits", 3, sh, kAnyFloat, false, false, !*empty));
+  if (!(temperature > 1e-6 && temperature < 1e6))
+    return fail(M3_ERR_INVALID_ARGUMENT, "temperature: expected a number between 1e-6 and 1e6");
+  M3_TRY(map2(tokens, "tokens", M3_INT64, sh, false, !*empty, &p->tok));
+  M3_TRY(map2(mask, "mask", M3_UINT8, sh, true, !*empty, &p->mask));
+  p->logits = logits->data;
+  p->sb = logits->stride[0]; p->st = logits->stride[1];
+  p->R = sh[0] * sh[1]; p->T = (int)sh[1]; p->V = (int)sh[2];
+  p->ignore = ignore_index;
+  p->scale = 1.0 / temperature;
+  // c in two floats, the upper one rounded down so that the lower one is positive
+  const double c = p->scale * 1.44269504088896340736;
+  float hi = (float)c;
+  if ((double)hi >= c) hi = std::nextafterf(hi, 0.f);
+  p->c_hi = hi;
+  p->c_lo = (float)(c - (double)hi);
+  return M3_OK;
+}
+
+// One f32 value on the device, 0-d or of one element.
+int scalar_out(const m3_tensor* t, const char* name, bool optional) {
+  if (!present(t) && optional) return M3_OK;
+  const int64_t one[1] = {1};
+  return check(t, name, present(t) && t->ndim == 0 ? 0 : 1, one, kF32, true, false, true);
+}
+
+int optional_out(const m3_tensor* t, const char* name, int ndim, const int64_t* shape, bool devcheck) {
+  return check(t, name, ndim, shape, kF32, true, true, devcheck);
+}
+
+int workspace_ok(const void* ws, size_t have, size_t need, const char* what) {
+  if (ws == nullptr || have < need || (reinterpret_cast<uintptr_t>(ws) & 15) != 0)
+    return fail(M3_ERR_WORKSPACE, std::string(what) + ": workspace of " + std::to_string(need) + " bytes required");
+  return M3_OK;
+}
+
+}  // namespace
+}  // namespace m3
+
+extern "C" {
+
+int m3_token_logprobs(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask, double temperature,
+                      int64_t ignore_index, m3_tensor* logprobs, m3_tensor* stats, void* stream) {
+  TokenRows p{};
+  bool empty = false;
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  const int64_t bt[3] = {logits->shape[0], logits->shape[1], 2};
+  M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
+  M3_TRY(optional_out(stats, "stats", 3, bt, !empty));
+  if (empty) return M3_OK;
+  return launch_token_logprobs(p, logits->dtype, fptr<float>(logprobs), fptr<float2>(stats),
+                               reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t m3_policy_loss_workspace_size(int64_t batch, int64_t seqlen) {
+  if (batch < 0 || seqlen < 0) return 0;
+  return policy_workspace_bytes(batch, batch * seqlen);
+}
+
+int m3_policy_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                   const m3_tensor* old_logprobs, const m3_tensor* advantages, const m3_tensor* ref_logprobs,
+                   double temperature, int64_t ignore_index, double clip_low, double clip_high, double kl_coef,
+                   int by_sequence, m3_tensor* loss, m3_tensor* kl, m3_tensor* clip_fraction, m3_tensor* logprobs,
+                   m3_tensor* stats, m3_tensor* coef, m3_tensor* dlogits, void* workspace, size_t workspace_bytes, void* stream) {
+  TokenRows p{};
+  bool empty = false;
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  const int64_t* sh = logits->shape;
+  const int64_t bt[3] = {sh[0], sh[1], 2};
+  if (!(clip_low >= 0 && clip_low <= 1)) return fail(M3_ERR_INVALID_ARGUMENT, "clip_low: expected a number from 0 to 1");
+  if (!(clip_high >= 0)) return fail(M3_ERR_INVALID_ARGUMENT, "clip_high: expected a number from 0 on");
+  if (!(kl_coef >= 0 && std::isfinite(kl_coef))) return fail(M3_ERR_INVALID_ARGUMENT, "kl_coef: expected a finite number from 0 on");
+  if (by_sequence != 0 && by_sequence != 1) return fail(M3_ERR_INVALID_ARGUMENT, "by_sequence: expected 0 or 1");
+  PolicyArgs a{};
+  M3_TRY(map2(old_logprobs, "old_logprobs", M3_FLOAT32, sh, false, !empty, &a.old_logp));
+  M3_TRY(map2(advantages, "advantages", M3_FLOAT32, sh, false, !empty, &a.adv));
+  M3_TRY(map2(ref_logprobs, "ref_logprobs", M3_FLOAT32, sh, true, !empty, &a.ref));
+  M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
+  M3_TRY(optional_out(stats, "stats", 3, bt, !empty));
+  M3_TRY(optional_out(coef, "coef", 2, bt, !empty));
+  M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, true, !empty));
+  M3_TRY(scalar_out(loss, "loss", false));
+  M3_TRY(scalar_out(kl, "kl", false));
+  M3_TRY(scalar_out(clip_fraction, "clip_fraction", false));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (empty) {
+    M3_TRY(memset_async(loss->data, sizeof(float), s, "loss"));
+    M3_TRY(memset_async(kl->data, sizeof(float), s, "kl"));
+    return memset_async(clip_fraction->data, sizeof(float), s, "clip_fraction");
+  }
+  M3_TRY(workspace_ok(workspace, workspace_bytes, policy_workspace_bytes(sh[0], p.R), "policy loss"));
+  a.clip_lo = 1.0 - clip_low; a.clip_hi = 1.0 + clip_high; a.kl_coef = kl_coef; a.by_sequence = by_sequence;
+  const bool grad = present(dlogits);
+  return launch_policy_loss(p, logits->dtype, a, sh[0], fptr<float>(loss), fptr<float>(kl),
+                            fptr<float>(clip_fraction), fptr<float>(logprobs), fptr<float2>(stats), fptr<float>(coef), fptr<void>(dlogits), grad ? dlogits->stride[0] : 0,
+                            grad ? dlogits->stride[1] : 0, workspace, s);
+}
+
+size_t m3_preference_loss_workspace_size(int64_t batch, int64_t seqlen) {
+  if (batch < 0 || seqlen < 0) return 0;
+  return preference_workspace_bytes(batch, batch * seqlen);
+}
+
+int m3_preference_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                       const m3_tensor* ref_logprobs, double temperature, int64_t ignore_index, double beta,
+                       double label_smoothing, m3_tensor* loss, m3_tensor* rewards, m3_tensor* logprobs,
+                       m3_tensor* stats, m3_tensor* seq_coef, void* workspace, size_t workspace_bytes, void* stream) {
+  TokenRows p{};
+  bool empty = false;
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  const int64_t* sh = logits->shape;
+  if (sh[0] % 2 != 0 || sh[0] == 0)
+    return fail(M3_ERR_INVALID_ARGUMENT, "logits: an even number of sequences expected, chosen before rejected");
+  if (!(beta >= 0 && std::isfinite(beta))) return fail(M3_ERR_INVALID_ARGUMENT, "beta: expected a finite number from 0 on");
+  if (!(label_smoothing >= 0 && label_smoothing <= 1))
+    return fail(M3_ERR_INVALID_ARGUMENT, "label_smoothing: expected a number from 0 to 1");
+  const int64_t bt[3] = {sh[0], sh[1], 2};
+  Map2<const float> ref;
+  M3_TRY(map2(ref_logprobs, "ref_logprobs", M3_FLOAT32, sh, true, !empty, &ref));
+  M3_TRY(scalar_out(loss, "loss", false));
+  M3_TRY(check(rewards, "rewards", 1, bt, kF32, true, false, true));
+  M3_TRY(check(seq_coef, "seq_coef", 1, bt, kF32, true, false, true));
+  M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
+  M3_TRY(optional_out(stats, "stats", 3, bt, !empty));
+  M3_TRY(workspace_ok(workspace, workspace_bytes, preference_workspace_bytes(sh[0], p.R), "preference loss"));
+  return launch_preference_loss(p, logits->dtype, ref, beta, label_smoothing, sh[0] / 2, fptr<float>(loss),
+                                fptr<float>(rewards), fptr<float>(logprobs), fptr<float2>(stats),
+                                fptr<float>(seq_coef), workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int m3_token_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask, const m3_tensor* stats,
+                  const m3_tensor* coef, const m3_tensor* up, double temperature, int64_t ignore_index,
+                  int keep_if_one, m3_tensor* dlogits, void* stream) {
+  TokenRows p{};
+  bool empty = false;
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  const int64_t* sh = logits->shape;
+  const int64_t bt[3] = {sh[0], sh[1], 2};
+  if (keep_if_one != 0 && keep_if_one != 1) return fail(M3_ERR_INVALID_ARGUMENT, "keep_if_one: expected 0 or 1");
+  Map2<const float> c;
+  M3_TRY(check(stats, "stats", 3, bt, kF32, true, false, !empty));
+  M3_TRY(map2(coef, "coef", M3_FLOAT32, sh, false, !empty, &c));
+  M3_TRY(scalar_out(up, "up", true));
+  M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, false, !empty));
+  if (empty) return M3_OK;
+  return launch_token_grad(p, logits->dtype, fptr<const float2>(stats), c, fptr<const float>(up), keep_if_one != 0,
+                           dlogits->data, dlogits->stride[0], dlogits->stride[1],
+                           reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t m3_clip_grads_workspace_size(int64_t count) { return count < 0 ? 0 : clip_grads_workspace_bytes(count); }
+
+int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel, const int32_t* dtypes,
+                  void* const* outs, const int32_t* out_dtypes, int largest, double max_norm, double scale,
+                  m3_tensor* norm, void* workspace, size_t workspace_bytes, void* stream) try {
+  if (count < 0 || (count > 0 && (!grads || !numel || !dtypes)))
+    return fail(M3_ERR_INVALID_ARGUMENT, "grads: missing");
+  if (outs && !out_dtypes) return fail(M3_ERR_INVALID_ARGUMENT, "out_dtypes: missing");
+  if (largest != 0 && largest != 1) return fail(M3_ERR_INVALID_ARGUMENT, "largest: expected 0 or 1");
+  if (!(max_norm >= 0)) return fail(M3_ERR_INVALID_ARGUMENT, "max_norm: expected a number from 0 on");
+  if (!(scale > 0 && std::isfinite(scale))) return fail(M3_ERR_INVALID_ARGUMENT, "scale: expected a positive finite number");
+  // what is written (and, with outs, what is read) as address ranges, to find overlaps
+  struct Range { uintptr_t lo, hi; bool written; int64_t index; };
+  const bool writes = outs || scale != 1.0 || !std::isinf(max_norm);
+  std::vector<Range> ranges;
+  if (writes) ranges.reserve((size_t)count * (outs ? 2 : 1));
+  for (int64_t i = 0; i < count; ++i) {
+    auto name = [&](const char* what) { return std::string(what) + "[" + std::to_string(i) + "]"; };
+    if (numel[i] < 0) return fail(M3_ERR_INVALID_ARGUMENT, name("numel") + ": negative");
+    if (dtypes[i] < 0 || dtypes[i] > M3_FLOAT16) return fail(M3_ERR_INVALID_ARGUMENT, name("grads") + ": unsupported dtype");
+    if (outs && out_dtypes[i] != dtypes[i] && out_dtypes[i] != M3_FLOAT32)
+      return fail(M3_ERR_INVALID_ARGUMENT, name("outs") + ": dtype must be the gradient's own or float32");
+    if (numel[i] == 0) continue;
+    if (!grads[i] || (outs && !outs[i])) return fail(M3_ERR_INVALID_ARGUMENT, name("grads") + ": missing");
+    const uintptr_t g = reinterpret_cast<uintptr_t>(grads[i]), o = outs ? reinterpret_cast<uintptr_t>(outs[i]) : g;
+    const size_t gs = dtype_size(dtypes[i]), os = outs ? dtype_size(out_dtypes[i]) : gs;
+    if (g % gs != 0 || o % os != 0) return fail(M3_ERR_INVALID_ARGUMENT, name("grads") + ": not aligned to its elements");
+    if (i == 0) {
+      M3_TRY(check_device_ptr(grads[0], "grads[0]"));
+      if (outs) M3_TRY(check_device_ptr(outs[0], "outs[0]"));
+    }
+    if (!writes) continue;
+    ranges.push_back(Range{o, o + os * (size_t)numel[i], true, i});
+    if (outs && !(o == g && os == gs)) ranges.push_back(Range{g, g + gs * (size_t)numel[i], false, i});
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
+  // sorted by their starts, a range meets an earlier one exactly if it begins before the
+  // furthest end so far (of the written ones, or of any where it is written itself)
+  uintptr_t end_any = 0, end_written = 0;
+  for (const Range& r : ranges) {
+    if (r.lo < (r.written ? end_any : end_written))
+      return fail(M3_ERR_INVALID_ARGUMENT, "grads[" + std::to_string(r.index) + "]: shares memory with another tensor of the call");
+    end_any = std::max(end_any, r.hi);
+    if (r.written) end_written = std::max(end_written, r.hi);
+  }
+  M3_TRY(scalar_out(norm, "norm", false));
+  if (count > 0) M3_TRY(workspace_ok(workspace, workspace_bytes, clip_grads_workspace_bytes(count), "clip_grads"));
+  ClipArgs a{count, grads, numel, dtypes, outs, out_dtypes, largest != 0, max_norm, scale, fptr<float>(norm)};
+  return launch_clip_grads(a, workspace, reinterpret_cast<cudaStream_t>(stream));
+} catch (const std::exception& e) {
+  return fail(M3_ERR_INVALID_ARGUMENT, std::string("clip_grads: ") + e.what());
 }
 
 }  // extern "C"

@@ -1,0 +1,54 @@
+// Losses over the tokens of a language model's logits: log-probabilities, the clipped policy
+// loss, the preference loss, and the gradient of the logits.
+#pragma once
+#include <stdint.h>
+
+#include <cuda_runtime.h>
+
+namespace m3 {
+
+// (batch, positions) operand with element strides (0 where it is broadcast)
+template <typename T>
+struct Map2 {
+  T* p;
+  int64_t sb, st;
+};
+
+// The rows of the logits and what is known of each: (batch, positions, V), innermost stride 1.
+struct TokenRows {
+  const void* logits;
+  int64_t sb, st;
+  int64_t R;           // rows = batch * T
+  int T, V;
+  Map2<const int64_t> tok;
+  Map2<const uint8_t> mask;  // p may be null: every position counts
+  int64_t ignore;      // token id of positions that do not count
+  double scale;        // 1 / temperature
+  float c_hi, c_lo;    // scale * log2(e) in two floats
+};
+
+struct PolicyArgs {
+  Map2<const float> old_logp, adv, ref;  // ref.p null: no KL term
+  double clip_lo, clip_hi;               // bounds of the ratio
+  double kl_coef;
+  int by_sequence;                       // mean of the sequences' means
+};
+
+// Workspace of the policy loss: counts and the sums' partial results (token_loss.cu).
+size_t policy_workspace_bytes(int64_t batch, int64_t rows);
+size_t preference_workspace_bytes(int64_t batch, int64_t rows);
+
+// logp (R) and, where given, stats (R) = (maximum, sum) of each row
+int launch_token_logprobs(const TokenRows& p, int dtype, float* logp, float2* stats, cudaStream_t s);
+// loss, mean KL, share of clipped tokens; coef (R) and dlogits where given
+int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64_t batch, float* loss, float* kl,
+                       float* clipped, float* logp, float2* stats, float* coef, void* dlogits, int64_t dsb, int64_t dst, void* ws, cudaStream_t s);
+// loss (1), rewards (2 N), seq_coef (2 N): d loss / d logp of each sequence's positions
+int launch_preference_loss(const TokenRows& p, int dtype, Map2<const float> ref, double beta, double smoothing,
+                           int64_t pairs, float* loss, float* rewards, float* logp, float2* stats, float* seq_coef,
+                           void* ws, cudaStream_t s);
+// dlogits = up * coef * scale * (one-hot - softmax); keep_if_one: leaves dlogits where *up is 1
+int launch_token_grad(const TokenRows& p, int dtype, const float2* stats, Map2<const float> coef, const float* up,
+                      bool keep_if_one, void* dlogits, int64_t dsb, int64_t dst, cudaStream_t s);
+
+}  // namespace m3

@@ -17,9 +17,9 @@ MAX_DIMS = 6
 
 M3_FLOAT32, M3_BFLOAT16, M3_FLOAT16 = 0, 1, 2
 M3_OK, M3_ERR_INVALID_ARGUMENT, M3_ERR_UNSUPPORTED, M3_ERR_CUDA, M3_ERR_WORKSPACE = 0, 1, 2, 3, 4
-M3_INT64 = 3
+M3_INT64, M3_UINT8 = 3, 4
 _DTYPE_CODE = {torch.float32: M3_FLOAT32, torch.bfloat16: M3_BFLOAT16, torch.float16: M3_FLOAT16,
-               torch.int64: M3_INT64}
+               torch.int64: M3_INT64, torch.bool: M3_UINT8, torch.uint8: M3_UINT8}
 _STATUS = {1: "invalid argument", 2: "unsupported", 3: "CUDA error", 4: "workspace"}
 
 
@@ -86,6 +86,17 @@ _SIGS = {
                               ctypes.c_int),
     "m3_silu_gate_bwd": ([_P] * 5 + [ctypes.c_void_p], ctypes.c_int),
     "m3_argmax_rows": ([_P, _P, ctypes.c_void_p], ctypes.c_int),
+    "m3_token_logprobs": ([_P] * 3 + [ctypes.c_double, ctypes.c_int64] + [_P] * 2 + [ctypes.c_void_p], ctypes.c_int),
+    "m3_policy_loss_workspace_size": ([ctypes.c_int64] * 2, ctypes.c_size_t),
+    "m3_policy_loss": ([_P] * 6 + [ctypes.c_double, ctypes.c_int64] + [ctypes.c_double] * 3 + [ctypes.c_int] +
+                       [_P] * 7 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
+    "m3_preference_loss_workspace_size": ([ctypes.c_int64] * 2, ctypes.c_size_t),
+    "m3_preference_loss": ([_P] * 4 + [ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double] + [_P] * 5 +
+                           [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
+    "m3_token_grad": ([_P] * 6 + [ctypes.c_double, ctypes.c_int64, ctypes.c_int, _P, ctypes.c_void_p], ctypes.c_int),
+    "m3_clip_grads_workspace_size": ([ctypes.c_int64], ctypes.c_size_t),
+    "m3_clip_grads": ([ctypes.c_int64] + [ctypes.c_void_p] * 5 + [ctypes.c_int, ctypes.c_double, ctypes.c_double, _P,
+                       ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
 }
 
 _lib = None
@@ -168,6 +179,11 @@ class Packed:
 
 def pack(*ts):
     return Packed(ts)
+
+
+def address(b):
+    """Address of a bytes object's contents; it must stay alive until the call returns."""
+    return ctypes.cast(ctypes.c_char_p(b), ctypes.c_void_p).value
 
 
 def ref(m):

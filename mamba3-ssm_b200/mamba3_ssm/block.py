@@ -11,6 +11,7 @@ import torch.nn.functional as F
 
 from .config import MambaConfig
 from .layer import Mamba3
+from .losses import token_logprobs
 from .ops import RMSNorm, argmax_rows, rmsnorm
 
 
@@ -76,6 +77,14 @@ class MambaLMHeadModel(nn.Module):
             if self.mlp_layers is not None:
                 x = x + self.mlp_layers[i](self.mlp_norms[i](x))
         return self.lm_head(self.norm_f(x))
+
+    def token_logprobs(self, input_ids: torch.Tensor, mask: torch.Tensor = None,
+                       temperature: float = 1.0) -> torch.Tensor:
+        """log p(input_ids[:, t + 1] | input_ids[:, :t + 1]) in fp32, (B, L - 1), from the logits
+        by losses.token_logprobs: what a policy, a reference model or an evaluation records
+        of given answers. mask (B, L - 1), optional: positions with 0 give 0."""
+        logits = self.forward(input_ids)[:, :-1]
+        return token_logprobs(logits, input_ids[:, 1:], mask=mask, temperature=temperature)
 
     def allocate_inference_cache(self, batch_size: int) -> List[Tuple[torch.Tensor, ...]]:
         return [blk.mixer.allocate_inference_cache(batch_size) for blk in self.layers]

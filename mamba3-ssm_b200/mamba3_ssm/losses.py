@@ -1,0 +1,281 @@
+"""Losses over the tokens of a language model's logits, for fine-tuning MambaLMHeadModel.
+
+    logits = model(input_ids)                                  # (batch, length, vocabulary)
+    token_logprobs(logits, tokens)                             # scoring, or a loss of one's own
+    policy_loss(logits, tokens, old_logprobs, advantages).loss.backward()
+    preference_loss(logits, tokens, ref_logprobs).loss.backward()
+
+``tokens[b, t]`` is the token that ``logits[b, t]`` predicts, i.e. the input shifted by one.
+``logits[:, :-1]`` with ``input_ids[:, 1:]`` is read in place; keeping the logits whole and
+giving the last position ``ignore_index`` also spares autograd the padding of that slice.
+
+Positions with mask 0 or the token ``ignore_index`` do not count: their logits are not read,
+their log-probability is 0 and their gradient is 0, whatever is stored there. A token id
+outside the vocabulary that is not ``ignore_index`` makes its position NaN. Gradients flow to
+the logits alone; old and reference log-probabilities, advantages and masks are constants.
+No counterpart in the reference (its train.py takes a cross-entropy of the logits).
+"""
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from .ops import _inner, _require_cuda
+
+__all__ = ["PolicyLoss", "PreferenceLoss", "policy_loss", "preference_loss", "token_logprobs"]
+
+_LOGIT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class PolicyLoss(NamedTuple):
+    """loss: scalar, differentiable by the logits. logprobs: of the tokens, in fp32 (0 where a
+    position does not count). kl, clip_fraction: means over the positions that count."""
+    loss: torch.Tensor
+    logprobs: torch.Tensor
+    kl: torch.Tensor
+    clip_fraction: torch.Tensor
+
+
+class PreferenceLoss(NamedTuple):
+    """loss: scalar, differentiable by the logits. rewards (2 N): beta * sum(logp - ref) of each
+    sequence. logprobs: of the tokens, in fp32 (0 where a position does not count)."""
+    loss: torch.Tensor
+    rewards: torch.Tensor
+    logprobs: torch.Tensor
+
+
+def _rows(name, logits, tokens):
+    """Logits as (batch, length, V) and tokens as (batch, length), without a copy where the
+    strides allow."""
+    _require_cuda(name, logits, tokens)
+    if logits.dtype not in _LOGIT_DTYPES:
+        raise TypeError(f"{name}: logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
+        raise ValueError(f"{name}: logits (..., V) and tokens (...) expected, got {tuple(logits.shape)} and "
+                         f"{tuple(tokens.shape)}")
+    if logits.shape[-1] == 0:
+        raise ValueError(f"{name}: empty vocabulary")
+    if tokens.dtype != torch.int64:
+        if tokens.dtype not in (torch.int32, torch.int16, torch.uint8):
+            raise TypeError(f"{name}: tokens must be integers, got {tokens.dtype}")
+        tokens = tokens.long()
+    if tokens.device != logits.device:
+        raise RuntimeError(f"{name}: tokens are on {tokens.device}, logits on {logits.device}")
+    n = tokens.dim()
+    if n < 2:
+        logits, tokens = logits.reshape(1, -1, logits.shape[-1]), tokens.reshape(1, -1)
+    elif n > 2:
+        logits, tokens = logits.flatten(0, n - 2), tokens.flatten(0, n - 2)
+    return _inner(logits), tokens
+
+
+def _per_token(name, what, v, logits, tokens, shape, dtype=torch.float32):
+    """A constant operand as (batch, length); it may be of any shape that broadcasts to
+    ``shape``, the shape the caller gave its tokens in."""
+    if v is None:
+        return None
+    if not isinstance(v, torch.Tensor):
+        raise TypeError(f"{name}: {what} must be a tensor")
+    if v.device != logits.device:
+        raise RuntimeError(f"{name}: {what} is on {v.device}, logits on {logits.device}")
+    v = v.detach()
+    if dtype is torch.bool:
+        v = v if v.dtype in (torch.bool, torch.uint8) else v != 0
+    elif v.dtype != dtype:
+        v = v.to(dtype)
+    if v.shape != shape:
+        try:
+            v = v.expand(shape)
+        except RuntimeError:
+            raise ValueError(f"{name}: {what} of shape {tuple(v.shape)} does not broadcast to the tokens' "
+                             f"{tuple(shape)}") from None
+    if v.dim() == 2:
+        return v
+    return v.reshape(tokens.shape)
+
+
+def _like_rows(logits):
+    """The gradient's tensor: rows of the logits' pitch where these are cut from wider rows, so
+    that both start on the same boundaries."""
+    if logits.is_contiguous():
+        return torch.empty_like(logits)
+    B, T, V = logits.shape
+    pitch = logits.stride(1)
+    if V < pitch < 2 * V:
+        return torch.empty(B, T, pitch, dtype=logits.dtype, device=logits.device)[..., :V]
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
+def _token_grad(logits, tokens, mask, stats, coef, up, temperature, ignore_index, dlogits=None):
+    """dlogits = up * coef / temperature * (one-hot - softmax) on m3_token_grad. A given
+    ``dlogits`` holds that for up = 1 already and is kept where up is 1."""
+    keep = dlogits is not None
+    if not keep:
+        dlogits = _like_rows(logits)
+    lib = L.load()
+    a = L.pack(logits, tokens, mask, stats, coef, up, dlogits)
+    with torch.cuda.device(logits.device):
+        L.check(lib.m3_token_grad(*a.ptrs[:6], temperature, ignore_index, int(keep), a.ptrs[6], L.stream_of(logits)),
+                "m3_token_grad")
+    return dlogits
+
+
+def _f32(logits, *shape):
+    return torch.empty(shape, dtype=torch.float32, device=logits.device)
+
+
+def _wants_grad(logits):
+    return torch.is_grad_enabled() and logits.requires_grad
+
+
+def _workspace(logits, nbytes):
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=logits.device)
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, temperature, ignore_index, need):
+        lib = L.load()
+        logp = _f32(logits, *tokens.shape)
+        stats = _f32(logits, *tokens.shape, 2) if need else None
+        a = L.pack(logits, tokens, mask, logp, stats)
+        with torch.cuda.device(logits.device):
+            L.check(lib.m3_token_logprobs(*a.ptrs[:3], temperature, ignore_index, *a.ptrs[3:], L.stream_of(logits)),
+                    "m3_token_logprobs")
+        if need:
+            ctx.save_for_backward(logits, tokens, mask, stats)
+            ctx.args = (temperature, ignore_index)
+        return logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogp):
+        logits, tokens, mask, stats = ctx.saved_tensors
+        return (_token_grad(logits, tokens, mask, stats, dlogp.float(), None, *ctx.args),) + (None,) * 5
+
+
+class _PolicyLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, old, adv, ref, temperature, ignore_index, clip_low, clip_high, kl_coef,
+                by_sequence, need):
+        lib = L.load()
+        B, T = tokens.shape
+        loss, kl, clipped = _f32(logits), _f32(logits), _f32(logits)
+        logp = _f32(logits, B, T)
+        stats = coef = dlogits = None
+        if need:
+            # the gradient for an upstream gradient of 1, while each row is at hand; backward
+            # forms it again only where the upstream gradient is another
+            stats, coef, dlogits = _f32(logits, B, T, 2), _f32(logits, B, T), _like_rows(logits)
+        ws = _workspace(logits, lib.m3_policy_loss_workspace_size(B, T))
+        a = L.pack(logits, tokens, mask, old, adv, ref, loss, kl, clipped, logp, stats, coef, dlogits)
+        with torch.cuda.device(logits.device):
+            L.check(lib.m3_policy_loss(*a.ptrs[:6], temperature, ignore_index, clip_low, clip_high, kl_coef,
+                                       int(by_sequence), *a.ptrs[6:], ws.data_ptr(), ws.numel(), L.stream_of(logits)),
+                    "m3_policy_loss")
+        if need:
+            ctx.save_for_backward(logits, tokens, mask, stats, coef)
+            ctx.args = (temperature, ignore_index)
+            ctx.dlogits = dlogits
+        ctx.mark_non_differentiable(logp, kl, clipped)
+        return loss, logp, kl, clipped
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up, _dlogp, _dkl, _dclipped):
+        logits, tokens, mask, stats, coef = ctx.saved_tensors
+        # handed out once: what receives it may write to it
+        dlogits, ctx.dlogits = ctx.dlogits, None
+        d = _token_grad(logits, tokens, mask, stats, coef, up.float(), *ctx.args, dlogits=dlogits)
+        return (d,) + (None,) * 12
+
+
+class _PreferenceLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, ref, temperature, ignore_index, beta, label_smoothing, need):
+        lib = L.load()
+        B, T = tokens.shape
+        loss, rewards, coef = _f32(logits), _f32(logits, B), _f32(logits, B)
+        logp = _f32(logits, B, T)
+        stats = _f32(logits, B, T, 2) if need else None
+        ws = _workspace(logits, lib.m3_preference_loss_workspace_size(B, T))
+        a = L.pack(logits, tokens, mask, ref, loss, rewards, logp, stats, coef)
+        with torch.cuda.device(logits.device):
+            L.check(lib.m3_preference_loss(*a.ptrs[:4], temperature, ignore_index, beta, label_smoothing, *a.ptrs[4:],
+                                           ws.data_ptr(), ws.numel(), L.stream_of(logits)), "m3_preference_loss")
+        if need:
+            ctx.save_for_backward(logits, tokens, mask, stats, coef)
+            ctx.args = (temperature, ignore_index)
+        ctx.mark_non_differentiable(rewards, logp)
+        return loss, rewards, logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up, _drewards, _dlogp):
+        logits, tokens, mask, stats, coef = ctx.saved_tensors
+        d = _token_grad(logits, tokens, mask, stats, coef.unsqueeze(1).expand(tokens.shape), up.float(),
+                        *ctx.args)
+        return (d,) + (None,) * 8
+
+
+def token_logprobs(logits, tokens, *, mask=None, temperature=1.0, ignore_index=-100):
+    """log softmax(logits / temperature) at ``tokens``, in fp32: logits (..., V) in fp32, bf16 or
+    fp16, tokens (...) integers, mask broadcastable to the tokens (nonzero = counts).
+    Differentiable by the logits; without the (..., V) tensor of all log-probabilities."""
+    x, t = _rows("token_logprobs", logits, tokens)
+    m = _per_token("token_logprobs", "mask", mask, x, t, tokens.shape, torch.bool)
+    return _TokenLogprobsFn.apply(x, t, m, float(temperature), int(ignore_index), _wants_grad(x)).reshape(tokens.shape)
+
+
+def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, mask=None, clip_low=0.2,
+                clip_high=None, kl_coef=0.0, temperature=1.0, reduction="token", ignore_index=-100):
+    """Clipped policy loss with a KL term: per position, with r = exp(logp - old_logprobs) and
+    d = ref_logprobs - logp,
+
+        -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1)
+
+    ``reduction`` "token": the mean over the positions that count; "sequence": the mean over
+    the sequences (last dimension of tokens) that have any, of each one's mean. 0 where no
+    position counts. ``advantages`` may be per token or broadcast (e.g. (batch, 1)).
+    ``clip_high`` defaults to ``clip_low``. Without ``ref_logprobs`` there is no KL term (and
+    ``kl_coef`` must be 0); with them ``kl`` is reported also for kl_coef 0.
+    Where the logits need a gradient it is formed in the forward pass, so that they are read
+    once; a loss that is scaled before backward() costs a second pass over them.
+    Returns PolicyLoss(loss, logprobs, kl, clip_fraction)."""
+    name = "policy_loss"
+    if reduction not in ("token", "sequence"):
+        raise ValueError(f"{name}: reduction is 'token' or 'sequence', got {reduction!r}")
+    if ref_logprobs is None and kl_coef != 0:
+        raise ValueError(f"{name}: kl_coef needs ref_logprobs")
+    x, t = _rows(name, logits, tokens)
+    m = _per_token(name, "mask", mask, x, t, tokens.shape, torch.bool)
+    old = _per_token(name, "old_logprobs", old_logprobs, x, t, tokens.shape)
+    adv = _per_token(name, "advantages", advantages, x, t, tokens.shape)
+    ref = _per_token(name, "ref_logprobs", ref_logprobs, x, t, tokens.shape)
+    loss, logp, kl, clipped = _PolicyLossFn.apply(
+        x, t, m, old, adv, ref, float(temperature), int(ignore_index), float(clip_low),
+        float(clip_low if clip_high is None else clip_high), float(kl_coef), reduction == "sequence", _wants_grad(x))
+    return PolicyLoss(loss, logp.reshape(tokens.shape), kl, clipped)
+
+
+def preference_loss(logits, tokens, ref_logprobs=None, *, mask=None, beta=0.1, label_smoothing=0.0, temperature=1.0,
+                    ignore_index=-100):
+    """Preference loss over pairs of answers: logits (2 N, T, V), tokens (2 N, T), sequence i the
+    chosen and sequence N + i the rejected answer of pair i. With reward = beta * sum over
+    the positions that count of (logp - ref_logprobs) and z = reward_i - reward_{N+i}:
+
+        loss = mean_i of -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z)
+
+    ``ref_logprobs`` (2 N, T): the reference model's, as token_logprobs returns them; None: 0.
+    Returns PreferenceLoss(loss, rewards, logprobs)."""
+    name = "preference_loss"
+    if logits.dim() != 3 or logits.shape[0] == 0 or logits.shape[0] % 2:
+        raise ValueError(f"{name}: logits (2 N, T, V) expected, the N chosen answers before the N rejected ones, got "
+                         f"{tuple(logits.shape)}")
+    x, t = _rows(name, logits, tokens)
+    m = _per_token(name, "mask", mask, x, t, tokens.shape, torch.bool)
+    ref = _per_token(name, "ref_logprobs", ref_logprobs, x, t, tokens.shape)
+    return PreferenceLoss(*_PreferenceLossFn.apply(x, t, m, ref, float(temperature), int(ignore_index), float(beta),
+                                                   float(label_smoothing), _wants_grad(x)))
