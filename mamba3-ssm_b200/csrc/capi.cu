@@ -853,12 +853,13 @@ int m3_argmax_rows(const m3_tensor* logits, m3_tensor* out, void* stream) {
 
 int m3_device_timeouts(int reset, int* flag_out) {
   if (!flag_out) return fail(M3_ERR_INVALID_ARGUMENT, "flag_out: missing");
-  int f = 0, b = 0, m = 0, q = 0;
+  int f = 0, b = 0, m = 0, q = 0, t = 0;
   M3_TRY(chunk_error_word(reset != 0, &f));
   M3_TRY(chunk_bwd_error_word(reset != 0, &b));
   M3_TRY(mimo_error_word(reset != 0, &m));
   M3_TRY(prologue_error_word(reset != 0, &q));
-  *flag_out = f | b | m | q;
+  M3_TRY(token_error_word(reset != 0, &t));
+  *flag_out = f | b | m | q | t;
   return M3_OK;
 }
 

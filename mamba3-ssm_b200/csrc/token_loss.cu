@@ -26,9 +26,11 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "m3_common.cuh"
+#include "sm100.cuh"
 #include "token_loss.cuh"
 
 namespace cg = cooperative_groups;
@@ -127,24 +129,51 @@ __device__ __forceinline__ Base base_at(float m, float c_hi) {
   return Base{m, far ? 0.f : -(m * c_hi), far};
 }
 
-// c (l - base) with c in two floats. c_lo is positive, so that l = -inf stays -inf.
-template <bool FAR>
+// The exponent of a logit. FINE: with c's lower half too (c_lo is positive, so that l = -inf
+// stays -inf); it then carries m c_lo, which norm_sum takes off the sum. The policy loss does
+// without: 1 / temperature is then off by 3e-8 of itself at most, for S and for the token alike.
+template <bool FAR, bool FINE>
 __device__ __forceinline__ float exponent(float l, const Base& b, float c_hi, float c_lo) {
   if constexpr (FAR) {
     const float d = l - b.m;
     return fmaf(d, c_hi, d * c_lo);
+  } else if constexpr (FINE) {
+    return fmaf(l, c_lo, fmaf(l, c_hi, b.k));
+  } else {
+    return fmaf(l, c_hi, b.k);
   }
-  return fmaf(l, c_lo, fmaf(l, c_hi, b.k));
+}
+// 2^(exponent) of one logit, whichever kind its base is
+template <bool FINE>
+__device__ __forceinline__ float exp_one(float l, const Base& b, float c_hi, float c_lo) {
+  return exp2_approx(b.far ? exponent<true, FINE>(l, b, c_hi, c_lo) : exponent<false, FINE>(l, b, c_hi, c_lo));
+}
+// A sum of fine exponentials in terms of plain ones, as the gradient forms them.
+template <bool FINE>
+__device__ __forceinline__ float norm_sum(float S, const Base& b, float c_lo) {
+  return FINE && !b.far ? S * exp2_approx(-b.m * c_lo) : S;
 }
 
-template <bool FAR, typename T>
-__device__ __forceinline__ float vec_sum(const Vec<T>& v, const Base& b, float c_hi, float c_lo) {
+// Two running sums, for their latency.
+struct Sum {
+  float a, b;
+  __device__ __forceinline__ float total() const { return a + b; }
+};
+template <bool FAR, bool FINE, typename T>
+__device__ __forceinline__ void add_vec(Sum& s, const Vec<T>& v, const Base& b, float c_hi, float c_lo) {
   constexpr int N = Vec<T>::N;
-  float l[N], s[2] = {0.f, 0.f};
+  float l[N];
   unpack(v, l);
 #pragma unroll
-  for (int k = 0; k < N; ++k) s[k & 1] += exp2_approx(exponent<FAR>(l[k], b, c_hi, c_lo));
-  return s[0] + s[1];
+  for (int k = 0; k < N; k += 2) {
+    s.a += exp2_approx(exponent<FAR, FINE>(l[k], b, c_hi, c_lo));
+    s.b += exp2_approx(exponent<FAR, FINE>(l[k + 1], b, c_hi, c_lo));
+  }
+}
+template <bool FINE, typename T>
+__device__ __forceinline__ void add_any(Sum& s, const Vec<T>& v, const Base& b, float c_hi, float c_lo) {
+  if (b.far) add_vec<true, FINE>(s, v, b, c_hi, c_lo);
+  else add_vec<false, FINE>(s, v, b, c_hi, c_lo);
 }
 template <typename T>
 __device__ __forceinline__ float vec_max(const Vec<T>& v) {
@@ -192,23 +221,25 @@ __device__ __forceinline__ Position position(const TokenRows& p, int64_t b, int6
 }
 
 // ------------------------------------------------------------------- policy workspace
-// counts (batch) int32, then one PolicyHead, then per-row results and their partial sums
 struct PolicyHead {
-  double total, sequences;  // positions that count; sequences with any
-  unsigned done;            // CTAs of the final sum that have finished
+  int kept, skipped;  // positions that count and that do not
+  int sequences;      // with any that counts
+  unsigned done;      // CTAs of the final sum that have finished
 };
 struct RowResult {
   float loss, kl, clipped;  // weighted loss; KL and 0 / 1, zero where the position does not count
 };
-constexpr int kSumRows = 2048;  // rows of one CTA of the final sum
+constexpr int kSumRows = 512;  // rows of one CTA of the final sum
 struct SumPart {
   double loss, kl, clipped;
 };
 struct PolicyWs {
   PolicyHead* head;
   int* counts;
+  int* order;  // the positions that count, then the others
   RowResult* rows;
   SumPart* parts;
+  size_t zeroed;
 };
 __host__ __device__ inline size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 inline PolicyWs policy_ws(void* ws, int64_t batch, int64_t rows, size_t* bytes) {
@@ -217,59 +248,57 @@ inline PolicyWs policy_ws(void* ws, int64_t batch, int64_t rows, size_t* bytes) 
   PolicyWs w;
   w.head = reinterpret_cast<PolicyHead*>(q + at);
   at += up16(sizeof(PolicyHead));
+  w.counts = reinterpret_cast<int*>(q + at);  // with the head, what is zero at the start
+  at += up16(sizeof(int) * (size_t)batch);
+  w.zeroed = at;
   w.parts = reinterpret_cast<SumPart*>(q + at);
   at += up16(sizeof(SumPart) * (size_t)((rows + kSumRows - 1) / kSumRows));
-  w.counts = reinterpret_cast<int*>(q + at);
-  at += up16(sizeof(int) * (size_t)batch);
+  w.order = reinterpret_cast<int*>(q + at);
+  at += up16(sizeof(int) * (size_t)rows);
   w.rows = reinterpret_cast<RowResult*>(q + at);
   at += up16(sizeof(RowResult) * (size_t)rows);
   *bytes = at;
   return w;
 }
 
-// Positions that count, by sequence and in all. One cluster of CTAs; a warp counts a segment
-// of a sequence and adds its (whole) number, so the result does not depend on the order.
-constexpr int kCountCluster = 8, kCountThreads = 1024, kCountSegment = 1024;
-__global__ void __cluster_dims__(kCountCluster, 1, 1) __launch_bounds__(kCountThreads)
-    policy_count_kernel(TokenRows p, int64_t batch, PolicyWs w) {
-  cg::cluster_group cl = cg::this_cluster();
-  const int64_t nthreads = (int64_t)gridDim.x * blockDim.x, me = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  for (int64_t b = me; b < batch; b += nthreads) w.counts[b] = 0;
-  if (me == 0) w.head->done = 0;
-  __threadfence();
-  cl.sync();
+// Positions that count, by sequence and in all, and the rows' order: those first, so that
+// they spread evenly whatever the mask. A warp takes a segment of a sequence and adds its
+// (whole) numbers to counters that are zero at the start, so the counts do not depend on the
+// schedule. The order within the two groups does, but no result depends on it.
+constexpr int kCountThreads = 128, kCountSegment = 256;
+__global__ void __launch_bounds__(kCountThreads) policy_count_kernel(TokenRows p, int64_t units, int segs, PolicyWs w) {
   const int lane = threadIdx.x & 31;
-  const int64_t segs = (p.T + kCountSegment - 1) / kCountSegment, units = batch * segs;
-  for (int64_t u = me >> 5; u < units; u += nthreads >> 5) {
-    const int64_t b = u / segs, t0 = (u % segs) * kCountSegment;
-    const int64_t t1 = t0 + kCountSegment < p.T ? t0 + kCountSegment : p.T;
-    int n = 0;
-    for (int64_t t = t0 + lane; t < t1; t += 32) n += position(p, b, t).keep;
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0 && n > 0) atomicAdd(&w.counts[b], n);
-  }
-  __threadfence();
-  cl.sync();
-  if (blockIdx.x != 0) return;
-  __shared__ long long tot[kCountThreads / 32], seq[kCountThreads / 32];
-  long long n = 0, m = 0;
-  for (int64_t b = threadIdx.x; b < batch; b += blockDim.x) {
-    const int k = *reinterpret_cast<volatile int*>(&w.counts[b]);
-    n += k;
-    m += k > 0;
-  }
+  const int64_t u = ((int64_t)blockIdx.x * kCountThreads + threadIdx.x) >> 5;
+  if (u >= units) return;
+  const int64_t b = u / segs;
+  const int t0 = (int)(u - b * segs) * kCountSegment, t1 = min(t0 + kCountSegment, p.T);
+  unsigned flags = 0;  // bit k: position t0 + 32 k + lane
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    n += __shfl_xor_sync(0xffffffffu, n, o);
-    m += __shfl_xor_sync(0xffffffffu, m, o);
+  for (int k = 0; k < kCountSegment / 32; ++k) {
+    const int t = t0 + 32 * k + lane;
+    if (t < t1 && position(p, b, t).keep) flags |= 1u << k;
   }
-  if (lane == 0) { tot[threadIdx.x >> 5] = n; seq[threadIdx.x >> 5] = m; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    n = m = 0;
-    for (int i = 0; i < kCountThreads / 32; ++i) { n += tot[i]; m += seq[i]; }
-    w.head->total = (double)n;
-    w.head->sequences = (double)m;
+  const int n = __reduce_add_sync(0xffffffffu, __popc(flags));
+  int at = 0, skip = 0;
+  if (lane == 0) {
+    if (n > 0) {
+      at = atomicAdd(&w.head->kept, n);
+      if (atomicAdd(&w.counts[b], n) == 0) atomicAdd(&w.head->sequences, 1);  // the sequence's first
+    }
+    skip = atomicAdd(&w.head->skipped, t1 - t0 - n);
+  }
+  at = __shfl_sync(0xffffffffu, at, 0);
+  skip = (int)p.R - 1 - __shfl_sync(0xffffffffu, skip, 0);
+  const unsigned below = (1u << lane) - 1;
+#pragma unroll
+  for (int k = 0; k < kCountSegment / 32; ++k) {
+    const int t = t0 + 32 * k + lane;
+    const bool in = t < t1, keep = flags >> k & 1;
+    const unsigned yes = __ballot_sync(0xffffffffu, keep), no = __ballot_sync(0xffffffffu, in && !keep);
+    if (keep) w.order[at + __popc(yes & below)] = (int)(b * p.T + t);
+    else if (in) w.order[skip - __popc(no & below)] = (int)(b * p.T + t);
+    at += __popc(yes);
+    skip -= __popc(no);
   }
 }
 
@@ -283,7 +312,7 @@ __device__ __forceinline__ TokenOps token_ops(const PolicyArgs& a, const PolicyW
   o.old_logp = map_at(a.old_logp, b, t);
   o.adv = map_at(a.adv, b, t);
   o.ref = a.ref.p ? map_at(a.ref, b, t) : 0.f;
-  o.weight = a.by_sequence ? 1.0 / ((double)w.counts[b] * w.head->sequences) : 1.0 / w.head->total;
+  o.weight = a.by_sequence ? 1.0 / ((double)w.counts[b] * (double)w.head->sequences) : 1.0 / (double)w.head->kept;
   return o;
 }
 
@@ -340,27 +369,59 @@ struct GradRow {
   float g, inv;  // inv = 1 / S
   int tok;
   float at;      // the token's logit
+  // For 16-bit results |g| / S goes into the exponent, so that a multiplication is spared:
+  // its rounding there, at most 2^-19 for |kg| < 64, is far below the result's own (2^-12).
+  float kg;
+  bool negative;  // -g < 0
+  bool folded;
 };
+__device__ __forceinline__ GradRow grad_row(const Base& base, float g, float S, int tok, float at) {
+  GradRow r{base, g, 1.f / S, tok, at, 0.f, g > 0.f, false};
+  r.kg = base.k + log2f(fabsf(g) * r.inv);
+  r.folded = !base.far && fabsf(r.kg) < 64.f && fabsf(base.k) < 64.f;  // false for NaN
+  return r;
+}
+// Two floats of at least 0 to two 16-bit values in a word, their signs set. For bf16 by an
+// addition (which rounds, ties up instead of to even, and sets the sign) and a byte selection:
+// the conversion instruction shares the exponential's unit, which bounds these kernels.
+__device__ __forceinline__ uint32_t signed_word(float a, float b, bool negative, __nv_bfloat16) {
+  const uint32_t add = negative ? 0x80008000u : 0x8000u;
+  return __byte_perm(__float_as_uint(a) + add, __float_as_uint(b) + add, 0x7632);
+}
+__device__ __forceinline__ uint32_t signed_word(float a, float b, bool negative, __half t) {
+  return word(a, b, t) ^ (negative ? 0x80008000u : 0u);
+}
+template <typename T>
+__device__ __forceinline__ Vec<T> vec_grad_folded(const Vec<T>& v, float kg, bool negative, float c_hi) {
+  constexpr int N = Vec<T>::N;
+  float l[N];
+  unpack(v, l);
+#pragma unroll
+  for (int k = 0; k < N; ++k) l[k] = exp2_approx(fmaf(l[k], c_hi, kg));
+  uint32_t o[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = signed_word(l[2 * k], l[2 * k + 1], negative, T{});
+  return Vec<T>{make_uint4(o[0], o[1], o[2], o[3])};
+}
 template <bool FAR, typename T>
 __device__ __forceinline__ Vec<T> vec_grad(const Vec<T>& v, const GradRow& r, float c_hi, float c_lo) {
   float l[Vec<T>::N];
   unpack(v, l);
   const float q = -r.g * r.inv;
 #pragma unroll
-  for (int k = 0; k < Vec<T>::N; ++k) l[k] = q * exp2_approx(exponent<FAR>(l[k], r.base, c_hi, c_lo));
+  for (int k = 0; k < Vec<T>::N; ++k) l[k] = q * exp2_approx(exponent<FAR, false>(l[k], r.base, c_hi, c_lo));
   return pack<T>(l);
 }
 template <typename T>
 __device__ __forceinline__ T one_grad(float l, const GradRow& r, float hot, float c_hi, float c_lo) {
-  const float e = r.base.far ? exponent<true>(l, r.base, c_hi, c_lo) : exponent<false>(l, r.base, c_hi, c_lo);
-  return from_f32<T>(r.g * (hot - exp2_approx(e) * r.inv));
+  return from_f32<T>(r.g * (hot - exp_one<false>(l, r.base, c_hi, c_lo) * r.inv));
 }
-// Vector j of a row to its place; whoever writes the token's vector writes its element again.
-template <bool FAR, typename T>
+// Vector j of a row to its place (the token's element is written again afterwards).
+template <typename T>
 __device__ __forceinline__ void put_grad(const Vec<T>& v, int j, T* out, const RowCut& c, const GradRow& r, bool same,
                                          float c_hi, float c_lo) {
   constexpr int N = Vec<T>::N;
-  const Vec<T> o = vec_grad<FAR>(v, r, c_hi, c_lo);
+  const Vec<T> o = r.base.far ? vec_grad<true>(v, r, c_hi, c_lo) : vec_grad<false>(v, r, c_hi, c_lo);
   const int i0 = c.head + j * N;
   if (same) {
     *reinterpret_cast<Vec<T>*>(out + i0) = o;
@@ -370,7 +431,33 @@ __device__ __forceinline__ void put_grad(const Vec<T>& v, int j, T* out, const R
 #pragma unroll
     for (int k = 0; k < N; ++k) out[i0 + k] = from_f32<T>(x[k]);
   }
-  if ((unsigned)(r.tok - i0) < (unsigned)N) out[r.tok] = one_grad<T>(r.at, r, 1.f, c_hi, c_lo);
+}
+// Vectors tid, tid + nt, ... of [0, n), which go to places v0 + j of the row.
+template <typename T, typename Get>
+__device__ __forceinline__ void put_vecs(int first, int n, int nt, int v0, T* out, const RowCut& c, const GradRow& r,
+                                         bool same, float c_hi, float c_lo, Get get) {
+  Vec<T>* const dst = reinterpret_cast<Vec<T>*>(out + c.head) + v0;
+  if (same && sizeof(T) == 2 && r.folded) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll 4
+      for (int j = first; j < n; j += nt) dst[j] = vec_grad_folded(get(j), r.kg, r.negative, c_hi);
+    }
+  } else if (same && !r.base.far) {
+#pragma unroll 4
+    for (int j = first; j < n; j += nt) dst[j] = vec_grad<false>(get(j), r, c_hi, c_lo);
+  } else {
+    for (int j = first; j < n; j += nt) put_grad(get(j), v0 + j, out, c, r, same, c_hi, c_lo);
+  }
+}
+// The token's element, by the thread that has written its vector: vectors v0 + tid, v0 + tid +
+// nt, ... of [v0, v1). One before or behind the vectors is put_ends' work.
+template <typename T>
+__device__ __forceinline__ void put_token(T* out, const RowCut& c, const GradRow& r, int v0, int v1, int tid, int nt,
+                                          float c_hi, float c_lo) {
+  constexpr int N = Vec<T>::N;
+  if (r.tok < c.head || r.tok >= c.tail0) return;
+  const int j = (r.tok - c.head) / N;
+  if (j >= v0 && j < v1 && (j - v0) % nt == tid) out[r.tok] = one_grad<T>(r.at, r, 1.f, c_hi, c_lo);
 }
 // The single elements before and behind a row's vectors.
 template <typename T>
@@ -400,14 +487,6 @@ __device__ __forceinline__ void fill(T* out, int i0, int i1, int tid, int nt, T 
   for (int i = h + nv * N + tid; i < i1; i += nt) out[i] = value;
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Results of a position that does not count.
 template <bool POLICY>
 __device__ __forceinline__ void skip_row(const RowOut& o, const PolicyWs& w, int64_t r) {
@@ -419,13 +498,13 @@ __device__ __forceinline__ void skip_row(const RowOut& o, const PolicyWs& w, int
     if (o.coef) o.coef[r] = 0.f;
   }
 }
-// From a row's sum to its results; `lead` writes them. Returns g, the gradient's factor.
+// From a row's sum to its results (`lead` writes them) and to what its gradient needs.
 template <bool POLICY>
-__device__ __forceinline__ float finish_row(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o,
-                                            const TokenOps& x, int64_t r, float at_token, const Base& base, float S,
-                                            bool lead) {
-  // the token's exponent exactly as the sum's elements have theirs: relative to base.k
-  const double c = p.scale * 1.44269504088896340736;
+__device__ __forceinline__ GradRow finish_row(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o,
+                                              const TokenOps& x, int64_t r, float at_token, int tok, const Base& base,
+                                              float S, bool lead) {
+  // the token's exponent exactly as the sum's elements have theirs
+  const double c = POLICY && !base.far ? (double)p.c_hi : (double)p.c_hi + (double)p.c_lo;
   const double at = base.far ? ((double)at_token - (double)base.m) * c : fma((double)at_token, c, (double)base.k);
   const double logp = at * kLn2 - log_sum(S);
   float coef = 0.f;
@@ -437,34 +516,103 @@ __device__ __forceinline__ float finish_row(const TokenRows& p, const PolicyArgs
       if (o.coef) o.coef[r] = coef;
     }
   }
+  const float Sn = norm_sum<!POLICY>(S, base, p.c_lo);
   if (lead) {
     o.logp[r] = (float)logp;
     if (o.logp64) o.logp64[r] = logp;
-    if (o.stats) o.stats[r] = make_float2(base.m, S);
+    if (o.stats) o.stats[r] = make_float2(base.m, Sn);
   }
-  return (float)((double)coef * p.scale);
+  return grad_row(base, (float)((double)coef * p.scale), Sn, tok, at_token);
 }
 
 // Whether a sum over an assumed base can be trusted (false for NaN too).
 __device__ __forceinline__ bool in_range(float S) { return S > 8.673617e-19f && S < 1.2676506e30f; }  // 2^-60, 2^100
 
-// One cluster of CTAs (of one CTA where there are rows enough) per row. With KEEP a CTA's part
-// stays in shared memory between the sum and the gradient; each thread reads there what it
-// copied itself, so the copies need no barrier. Without, the gradient reads the row again
-// (from the L2 cache, as a rule).
-template <typename T, bool POLICY, bool KEEP>
+// A row's sum and results by a cluster of CTAs: what the kernels below share.
+struct RowShared {
+  float part[2][kRowWarps];  // the warps' sums, alternating between rows
+  GradRow row[2];
+  bool again[2];
+};
+
+// The base of a row from its first vectors (of all elements, where there is no vector).
+template <typename T>
+__device__ __forceinline__ float first_max(const T* row, int V, const RowCut& c, int lane) {
+  if (c.nv > 0) return lane < c.nv ? vec_max(reinterpret_cast<const Vec<T>*>(row + c.head)[lane]) : -INFINITY;
+  return lane < V ? to_f32(row[lane]) : -INFINITY;
+}
+
+// Joins the threads' sums over the cluster and finishes the row. `s`: this thread's sum over
+// `base`; `get(j)`: vector j of this CTA's part. On return sh.row[slot] holds the row. `slot`
+// alternates from row to row, so that a CTA can go on while another still reads its sums.
+template <typename T, bool POLICY, typename Get>
+__device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o,
+                                         RowShared& sh, int slot, const TokenOps& x, int64_t r, const T* row,
+                                         const RowCut& c, int n, Base base, float s, float at_token, int tok, Get get) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, W = nt >> 5;
+  auto meet = [&]() {
+    if (C > 1) cl.sync();
+    else __syncthreads();
+  };
+  float* part = sh.part[slot];
+  s = warp_sum(s);
+  if (lane == 0) part[warp] = s;
+  meet();
+  if (warp == 0) {
+    // by CTA first: the order of token_grad_rows_kernel, for the same bits
+    float S = 0.f;
+    for (int k = 0; k < C; ++k) S += warp_sum(lane < W ? (C > 1 ? cl.map_shared_rank(part, k)[lane] : part[lane]) : 0.f);
+    if (lane == 0) {
+      sh.again[slot] = base.far || !in_range(S);
+      if (!sh.again[slot]) sh.row[slot] = finish_row<POLICY>(p, a, w, o, x, r, at_token, tok, base, S, rank == 0);
+    }
+  }
+  __syncthreads();
+  if (!sh.again[slot]) return;
+  // rare: the row's true maximum, then its sum
+  auto ends = [&](auto f) {
+    if (rank == 0) {
+      for (int i = tid; i < c.head; i += nt) f(to_f32(row[i]));
+      for (int i = c.tail0 + tid; i < p.V; i += nt) f(to_f32(row[i]));
+    }
+  };
+  auto all = [&](float v, bool largest) {
+    meet();  // the parts of the last sum have been read
+    if (lane == 0) part[warp] = v;
+    meet();
+    float y = largest ? -INFINITY : 0.f;
+    for (int i = 0; i < W * C; ++i) {
+      const float z = C > 1 ? cl.map_shared_rank(part, i / W)[i % W] : part[i];
+      y = largest ? fmaxf(y, z) : y + z;
+    }
+    return y;
+  };
+  float mx = -INFINITY;
+  for (int j = tid; j < n; j += nt) mx = fmaxf(mx, vec_max(get(j)));
+  ends([&](float l) { mx = fmaxf(mx, l); });
+  base = base_at(all(warp_max(mx), true), p.c_hi);
+  Sum s2{0.f, 0.f};
+  for (int j = tid; j < n; j += nt) add_any<!POLICY>(s2, get(j), base, p.c_hi, p.c_lo);
+  s = s2.total();
+  ends([&](float l) { s += exp_one<!POLICY>(l, base, p.c_hi, p.c_lo); });
+  const float S = all(warp_sum(s), false);
+  if (tid == 0) sh.row[slot] = finish_row<POLICY>(p, a, w, o, x, r, at_token, tok, base, S, rank == 0);
+  __syncthreads();
+}
+
+// One cluster of CTAs (of one CTA where there are rows enough) per row. A policy gradient of
+// rows too long for token_grad_rows_kernel is written from a second reading.
+template <typename T, bool POLICY>
 __global__ void __launch_bounds__(kRowThreads) token_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o) {
   constexpr int U = 4;  // loads in flight per thread
-  extern __shared__ uint4 kept_raw[];
-  Vec<T>* kept = reinterpret_cast<Vec<T>*>(kept_raw);
-  __shared__ float part[kRowWarps];
-  __shared__ GradRow sh;
-  __shared__ bool again;
+  __shared__ RowShared sh;
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int64_t r = blockIdx.x / C;
   const int64_t b = r / p.T, t = r - b * p.T;
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, W = nt >> 5;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31;
   const T* row = static_cast<const T*>(p.logits) + b * p.sb + t * p.st;
   T* drow = nullptr;
   if constexpr (POLICY)
@@ -478,131 +626,357 @@ __global__ void __launch_bounds__(kRowThreads) token_rows_kernel(TokenRows p, Po
   }
   const RowCut c = cut_row(row, p.V);
   const int v0 = (int)((int64_t)c.nv * rank / C), v1 = (int)((int64_t)c.nv * (rank + 1) / C), n = v1 - v0;
-  const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + c.head);
-  const Vec<T>* mine = rv + v0;
-  const int quarter = (n + 4 * nt - 1) / (4 * nt) * nt;  // of the part, in whole rounds of the CTA
-  if constexpr (KEEP) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      for (int j = q * quarter + tid; j < min(n, (q + 1) * quarter); j += nt) cp_async16(kept + j, mine + j);
-      cp_async_commit();
-    }
-  }
-  // the base: the largest of the row's first 32 vectors (of all, where there is no vector)
-  float m = -INFINITY;
-  if (c.nv > 0) {
-    if (lane < c.nv) m = vec_max(rv[lane]);
-  } else if (lane < p.V) {
-    m = to_f32(row[lane]);
-  }
+  const Vec<T>* mine = reinterpret_cast<const Vec<T>*>(row + c.head) + v0;
+  const float m = first_max(row, p.V, c, lane);
   TokenOps x{};
   float at_token = 0.f;
   if (tid == 0) {
     at_token = pos.known ? to_f32(row[pos.tok]) : NAN;
     if constexpr (POLICY) x = token_ops(a, w, b, t);
   }
-  Base base = base_at(warp_max(m), p.c_hi);
-  float s = 0.f;
-  if constexpr (KEEP) {
-    auto sum_quarter = [&](int q) {
-      for (int j = q * quarter + tid; j < min(n, (q + 1) * quarter); j += nt)
-        s += vec_sum<false>(kept[j], base, p.c_hi, p.c_lo);
-    };
-    cp_async_wait<3>();
-    sum_quarter(0);
-    cp_async_wait<2>();
-    sum_quarter(1);
-    cp_async_wait<1>();
-    sum_quarter(2);
-    cp_async_wait<0>();
-    sum_quarter(3);
-  } else {
-    int j = tid;
-    for (; j + (U - 1) * nt < n; j += U * nt) {
-      Vec<T> v[U];
+  const Base base = base_at(warp_max(m), p.c_hi);
+  Sum s2{0.f, 0.f};
+  int j = tid;
+  for (; j + (U - 1) * nt < n; j += U * nt) {
+    Vec<T> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = mine[j + u * nt];
+    for (int u = 0; u < U; ++u) v[u] = mine[j + u * nt];
 #pragma unroll
-      for (int u = 0; u < U; ++u) s += vec_sum<false>(v[u], base, p.c_hi, p.c_lo);
-    }
-    for (; j < n; j += nt) s += vec_sum<false>(mine[j], base, p.c_hi, p.c_lo);
+    for (int u = 0; u < U; ++u) add_vec<false, !POLICY>(s2, v[u], base, p.c_hi, p.c_lo);
   }
-  auto ends = [&](auto f) {
-    if (rank == 0) {
-      for (int i = tid; i < c.head; i += nt) f(to_f32(row[i]));
-      for (int i = c.tail0 + tid; i < p.V; i += nt) f(to_f32(row[i]));
-    }
-  };
-  ends([&](float l) { s += exp2_approx(exponent<false>(l, base, p.c_hi, p.c_lo)); });
-  s = warp_sum(s);
-  if (lane == 0) part[warp] = s;
-  auto meet = [&]() {
-    if (C > 1) cl.sync();
-    else __syncthreads();
-  };
-  meet();
-  if (warp == 0) {
-    float S = 0.f;
-    for (int i = lane; i < W * C; i += 32) S += C > 1 ? cl.map_shared_rank(part, i / W)[i % W] : part[i];
-    S = warp_sum(S);
-    if (lane == 0) {
-      again = base.far || !in_range(S);
-      if (!again) {
-        const float g = finish_row<POLICY>(p, a, w, o, x, r, at_token, base, S, rank == 0);
-        sh = GradRow{base, g, 1.f / S, pos.known ? (int)pos.tok : -1, at_token};
-      }
-    }
+  for (; j < n; j += nt) add_vec<false, !POLICY>(s2, mine[j], base, p.c_hi, p.c_lo);
+  float s = s2.total();
+  if (rank == 0) {
+    for (int i = tid; i < c.head; i += nt) s += exp_one<!POLICY>(to_f32(row[i]), base, p.c_hi, p.c_lo);
+    for (int i = c.tail0 + tid; i < p.V; i += nt) s += exp_one<!POLICY>(to_f32(row[i]), base, p.c_hi, p.c_lo);
   }
-  __syncthreads();
-  if (again) {
-    // rare: the row's true maximum, then its sum
-    auto all = [&](float v, bool largest) {
-      meet();  // the parts of the last sum have been read
-      if (lane == 0) part[warp] = v;
-      meet();
-      float y = largest ? -INFINITY : 0.f;
-      for (int i = 0; i < W * C; ++i) {
-        const float z = C > 1 ? cl.map_shared_rank(part, i / W)[i % W] : part[i];
-        y = largest ? fmaxf(y, z) : y + z;
-      }
-      return y;
-    };
-    float mx = -INFINITY;
-    for (int j = tid; j < n; j += nt) mx = fmaxf(mx, vec_max(mine[j]));
-    ends([&](float l) { mx = fmaxf(mx, l); });
-    base = base_at(all(warp_max(mx), true), p.c_hi);
-    s = 0.f;
-    for (int j = tid; j < n; j += nt)
-      s += base.far ? vec_sum<true>(mine[j], base, p.c_hi, p.c_lo) : vec_sum<false>(mine[j], base, p.c_hi, p.c_lo);
-    ends([&](float l) {
-      s += exp2_approx(base.far ? exponent<true>(l, base, p.c_hi, p.c_lo) : exponent<false>(l, base, p.c_hi, p.c_lo));
-    });
-    const float S = all(warp_sum(s), false);
-    if (tid == 0) {
-      const float g = finish_row<POLICY>(p, a, w, o, x, r, at_token, base, S, rank == 0);
-      sh = GradRow{base, g, 1.f / S, pos.known ? (int)pos.tok : -1, at_token};
-    }
-    __syncthreads();
-  }
+  join_row<T, POLICY>(p, a, w, o, sh, 0, x, r, row, c, n, base, s, at_token, pos.known ? (int)pos.tok : -1,
+                      [&](int k) { return mine[k]; });
   if (C > 1) cl.barrier_arrive();  // this CTA reads no other's part from here on
   if constexpr (POLICY) {
     if (drow) {
-      const GradRow gr = sh;
+      const GradRow gr = sh.row[0];
       if (gr.g == 0.f) {
         fill<T>(drow, e0, e1, tid, nt, from_f32<T>(0.f));
       } else {
         const bool same = same_boundary(drow, c);
-        auto put = [&](auto far) {
-          for (int j = tid; j < n; j += nt)
-            put_grad<decltype(far)::value>(KEEP ? kept[j] : mine[j], v0 + j, drow, c, gr, same, p.c_hi, p.c_lo);
-        };
-        if (gr.base.far) put(std::true_type{});
-        else put(std::false_type{});
+        put_vecs<T>(tid, n, nt, v0, drow, c, gr, same, p.c_hi, p.c_lo, [&](int k) { return mine[k]; });
+        put_token(drow, c, gr, v0, v1, tid, nt, p.c_hi, p.c_lo);
         if (rank == 0) put_ends(row, drow, p.V, c, gr, tid, nt, p.c_hi, p.c_lo);
       }
     }
   }
   if (C > 1) cl.barrier_wait();  // no CTA leaves while another reads its part
+}
+
+// The policy loss and its gradient, the logits read once. CTAs (clusters of them, where a row
+// is split) stay on the device and take the rows that count in turn; a CTA keeps its part of
+// a row in shared memory between the sum and the gradient. One warp copies: it fetches what
+// the row needs beside its logits a row ahead, refills each piece of the part with the next
+// row's as soon as the other warps have written the piece's gradient, and writes the zeros of
+// the positions that do not count, so that the memory stays busy while the others compute.
+constexpr int kPieces = 8;           // at most
+constexpr int kPieceVecs = 4;        // vectors of a piece per thread: few enough waits and bounds beside the work
+constexpr int kZeroBytes = 2048;
+constexpr uint32_t kWaitLimit = 1u << 24;
+
+template <typename T>
+struct RowInfo {
+  const T* row;
+  T* drow;
+  int64_t r;
+  RowCut c;
+  int v0, n;
+  Base base;
+  TokenOps x;
+  float at_token;
+  int tok;
+};
+template <typename T>
+struct GradRowsShared {
+  alignas(16) unsigned char zeros[kZeroBytes];
+  uint64_t full[kPieces], empty[kPieces], info_full[2], info_empty[2], met[2];
+  float part[2][kRowWarps];
+  float other[2][8];  // sums of the cluster's CTAs
+  float sum;
+  bool again[2], stop[2];
+  int dead;           // a wait gave up: everyone leaves
+  GradRow row[2];
+  RowInfo<T> info[2];
+};
+
+__device__ unsigned g_token_error;
+
+// A bounded wait of one thread. Where it gives up, so does everyone who waits in this CTA.
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, int* dead) {
+  if (sm100::mbar_try_wait(bar, parity)) return true;
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    if (sm100::mbar_try_wait(bar, parity)) return true;
+    if (*reinterpret_cast<volatile int*>(dead)) return false;
+  }
+  *reinterpret_cast<volatile int*>(dead) = 1;
+  atomicOr(&g_token_error, 1u);
+  return false;
+}
+// The same for a whole warp, which agrees on the answer.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* dead) {
+  return __all_sync(0xffffffffu, wait_one(bar, parity, dead));
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(sm100::smem_u32(src)),
+               "r"(bytes)
+               : "memory");
+}
+// v into other[slot] of CTA `to` of the cluster, counted on its barrier `met`
+__device__ __forceinline__ void send(float* slot, uint64_t* met, int to, float v) {
+  uint32_t at, bar;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(sm100::smem_u32(slot)), "r"(to));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(sm100::smem_u32(met)), "r"(to));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(at),
+               "r"(__float_as_uint(v)), "r"(bar)
+               : "memory");
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT + 32, 1024 / NT)
+    token_grad_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o, int pieces) {
+  constexpr int W = NT / 32, kPiece = kPieceVecs * NT;
+  extern __shared__ __align__(16) uint4 kept_raw[];
+  __shared__ GradRowsShared<T> sh;
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int cid = blockIdx.x / C, ncl = gridDim.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  Vec<T>* const kept = reinterpret_cast<Vec<T>*>(kept_raw);
+  for (int i = tid; i < kZeroBytes / 16; i += NT + 32) reinterpret_cast<uint4*>(sh.zeros)[i] = make_uint4(0, 0, 0, 0);
+  sm100::fence_proxy_async_smem();  // the zeros, for the copies that read them
+  if (tid == 0) {
+    for (int k = 0; k < kPieces; ++k) {
+      sm100::mbar_init(&sh.full[k], 1);
+      sm100::mbar_init(&sh.empty[k], W);
+    }
+    for (int k = 0; k < 2; ++k) {
+      sm100::mbar_init(&sh.info_full[k], 1);
+      sm100::mbar_init(&sh.info_empty[k], W);
+      sm100::mbar_init(&sh.met[k], 1);
+    }
+    sh.dead = 0;
+    sm100::fence_barrier_init();
+  }
+  if (C > 1) cl.sync();
+  else __syncthreads();
+  const int kept_rows = w.head->kept;
+
+  if (warp == W) {
+    // ------------------------------------------------------------------ the copying warp
+    uint32_t round = 0, issued = 0;  // issued: pieces whose copy of the current round is under way
+    bool ok = true;
+    // zeros to a position that does not count, this CTA's part of the row
+    auto skip = [&](int i) {
+      const int r = w.order[i];
+      const int64_t b = r / p.T, t = r - b * p.T;
+      T* const drow = static_cast<T*>(o.dlogits) + b * o.dsb + t * o.dst;
+      if (rank == 0 && lane == 0) skip_row<true>(o, w, r);
+      const RowCut c = cut_row(drow, p.V);
+      const int v0 = (int)((int64_t)c.nv * rank / C), v1 = (int)((int64_t)c.nv * (rank + 1) / C);
+      Vec<T>* const dst = reinterpret_cast<Vec<T>*>(drow + c.head);
+      constexpr int per = kZeroBytes / 16;
+      for (int v = v0 + lane * per; v < v1; v += 32 * per) bulk_store(dst + v, sh.zeros, (uint32_t)min(per, v1 - v) * 16u);
+      if (rank == 0) {
+        if (lane < c.head) drow[lane] = from_f32<T>(0.f);
+        if (c.tail0 + lane < p.V) drow[c.tail0 + lane] = from_f32<T>(0.f);
+      }
+      sm100::bulk_commit();
+    };
+    const int mine = cid < kept_rows ? (kept_rows - cid + ncl - 1) / ncl : 0;  // rows that count
+    const int rest = p.R - kept_rows, skips = cid < rest ? (int)(rest - cid + ncl - 1) / ncl : 0;
+    int skipped = 0;
+    for (int i = cid; i < kept_rows; i += ncl, ++round) {
+      const int slot = round & 1;
+      if (round >= 2 && !(ok = wait_warp(&sh.info_empty[slot], ((round >> 1) - 1) & 1, &sh.dead))) break;
+      RowInfo<T> q;
+      q.r = w.order[i];
+      const int b = (int)q.r / p.T, t = (int)q.r - b * p.T;
+      q.row = static_cast<const T*>(p.logits) + b * p.sb + t * p.st;
+      q.drow = static_cast<T*>(o.dlogits) + b * o.dsb + t * o.dst;
+      q.c = cut_row(q.row, p.V);
+      q.v0 = (int)((int64_t)q.c.nv * rank / C);
+      q.n = (int)((int64_t)q.c.nv * (rank + 1) / C) - q.v0;
+      const int64_t tok = map_at(p.tok, b, t);
+      const bool known = tok >= 0 && tok < p.V;
+      q.tok = known ? (int)tok : -1;
+      q.x = token_ops(a, w, b, t);
+      const float m = first_max(q.row, p.V, q.c, lane);
+      q.at_token = known ? to_f32(q.row[tok]) : NAN;
+      q.base = base_at(warp_max(m), p.c_hi);
+      if (lane == 0) {
+        sh.info[slot] = q;
+        sm100::mbar_arrive(&sh.info_full[slot]);
+        const Vec<T>* src = reinterpret_cast<const Vec<T>*>(q.row + q.c.head) + q.v0;
+        issued = 0;
+        for (int k = 0; k < pieces; ++k) {
+          if (round >= 1 && !(ok = wait_one(&sh.empty[k], (round - 1) & 1, &sh.dead))) break;
+          const int n = min(kPiece, q.n - k * kPiece);
+          sm100::mbar_expect_tx(&sh.full[k], n > 0 ? (uint32_t)n * 16u : 0u);
+          if (n > 0) sm100::bulk_load(kept + k * kPiece, src + k * kPiece, (uint32_t)n * 16u, &sh.full[k]);
+          issued |= 1u << k;
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      // in step with the rows that count
+      for (const int until = (int)((int64_t)skips * (round + 1) / mine); skipped < until; ++skipped)
+        skip(kept_rows + cid + skipped * ncl);
+    }
+    for (; ok && skipped < skips; ++skipped) skip(kept_rows + cid + skipped * ncl);
+    if (!ok && lane == 0) {
+      // copies in flight end before the CTA does
+      for (int k = 0; k < pieces; ++k) {
+        const uint32_t phase = (issued >> k & 1) ? round & 1 : (round + 1) & 1;
+        if (round > 0 || (issued >> k & 1)) sm100::mbar_wait(&sh.full[k], phase, kWaitLimit);
+      }
+    }
+    sm100::bulk_wait0();
+  } else {
+    // ---------------------------------------------------- the warps that sum and write
+    uint32_t meets = 0;
+    // The sum (or maximum) over the cluster, by warp 0. Two barriers in turn: a CTA may be one
+    // exchange ahead of this one, whose values must not count for the present one.
+    auto over_cluster = [&](float v, bool largest) {
+      if (C == 1) return v;
+      const int s = meets & 1;
+      if (lane == 0) sm100::mbar_expect_tx(&sh.met[s], 4u * C);
+      __syncwarp();
+      if (lane < C) send(&sh.other[s][rank], &sh.met[s], lane, v);
+      wait_warp(&sh.met[s], (meets >> 1) & 1, &sh.dead);
+      ++meets;
+      float y = sh.other[s][0];
+      for (int k = 1; k < C; ++k) y = largest ? fmaxf(y, sh.other[s][k]) : y + sh.other[s][k];
+      return y;
+    };
+    uint32_t round = 0;
+    for (int i = cid; i < kept_rows; i += ncl, ++round) {
+      const int slot = round & 1;
+      // where a wait gives up the warp does no more work, but still meets the others below,
+      // where all learn of it
+      bool ok = wait_warp(&sh.info_full[slot], (round >> 1) & 1, &sh.dead);
+      const RowInfo<T>& q = sh.info[slot];
+      const RowCut c = ok ? q.c : RowCut{0, 0, p.V};
+      const int n = ok ? q.n : 0, v0 = q.v0;
+      const T* const row = q.row;
+      T* const drow = q.drow;
+      Base base = q.base;
+      Sum s2{0.f, 0.f};
+      for (int k = 0; k < pieces; ++k) {
+        const int left = n - k * kPiece;
+        if (left <= 0) break;
+        if (!(ok = wait_warp(&sh.full[k], round & 1, &sh.dead))) break;
+        const Vec<T>* const at = kept + k * kPiece + tid;
+        if (left >= kPiece) {
+          Vec<T> v[kPieceVecs];
+#pragma unroll
+          for (int u = 0; u < kPieceVecs; ++u) v[u] = at[u * NT];
+#pragma unroll
+          for (int u = 0; u < kPieceVecs; ++u) add_vec<false, false>(s2, v[u], base, p.c_hi, p.c_lo);
+        } else {
+          for (int j = tid; j < left; j += NT) add_vec<false, false>(s2, at[j - tid], base, p.c_hi, p.c_lo);
+        }
+      }
+      float s = s2.total();
+      auto ends = [&](auto f) {
+        if (rank == 0) {
+          if (tid < c.head) f(to_f32(row[tid]));
+          if (c.tail0 + tid < p.V) f(to_f32(row[c.tail0 + tid]));
+        }
+      };
+      ends([&](float l) { s += exp_one<false>(l, base, p.c_hi, p.c_lo); });
+      s = warp_sum(s);
+      if (lane == 0) sh.part[slot][warp] = s;
+      bar_sync(1, NT);
+      if (warp == 0) {
+        const float S = over_cluster(warp_sum(lane < W ? sh.part[slot][lane] : 0.f), false);
+        if (lane == 0) {
+          const bool stop = *reinterpret_cast<volatile int*>(&sh.dead) != 0;
+          sh.stop[slot] = stop;
+          sh.again[slot] = base.far || !in_range(S);
+          if (!stop && !sh.again[slot])
+            sh.row[slot] = finish_row<true>(p, a, w, o, q.x, q.r, q.at_token, q.tok, base, S, rank == 0);
+        }
+      }
+      bar_sync(1, NT);
+      if (sh.stop[slot]) break;
+      if (sh.again[slot]) {
+        // rare: the row's true maximum, then its sum
+        auto all = [&](float v, bool largest) {
+          if (lane == 0) sh.part[slot][warp] = v;
+          bar_sync(1, NT);
+          if (warp == 0) {
+            float y = lane < W ? sh.part[slot][lane] : (largest ? -INFINITY : 0.f);
+            y = over_cluster(largest ? warp_max(y) : warp_sum(y), largest);
+            if (lane == 0) sh.sum = y;
+          }
+          bar_sync(1, NT);
+          return sh.sum;
+        };
+        float mx = -INFINITY;
+        for (int j = tid; j < n; j += NT) mx = fmaxf(mx, vec_max(kept[j]));
+        ends([&](float l) { mx = fmaxf(mx, l); });
+        base = base_at(all(warp_max(mx), true), p.c_hi);
+        s2 = Sum{0.f, 0.f};
+        for (int j = tid; j < n; j += NT) add_any<false>(s2, kept[j], base, p.c_hi, p.c_lo);
+        s = s2.total();
+        ends([&](float l) { s += exp_one<false>(l, base, p.c_hi, p.c_lo); });
+        const float S = all(warp_sum(s), false);
+        if (tid == 0) sh.row[slot] = finish_row<true>(p, a, w, o, q.x, q.r, q.at_token, q.tok, base, S, rank == 0);
+        bar_sync(1, NT);
+      }
+      const GradRow gr = sh.row[slot];
+      const bool same = same_boundary(drow, c), zero = gr.g == 0.f;
+      const int kind = zero ? 0 : !same || gr.base.far ? 3 : sizeof(T) == 2 && gr.folded ? 1 : 2;
+      if (zero)
+        fill<T>(drow, (int)((int64_t)p.V * rank / C), (int)((int64_t)p.V * (rank + 1) / C), tid, NT, from_f32<T>(0.f));
+      Vec<T>* const dst = reinterpret_cast<Vec<T>*>(drow + c.head) + v0 + tid;
+      for (int k = 0; k < pieces; ++k) {
+        const int left = n - k * kPiece;
+        const Vec<T>* const at = kept + k * kPiece + tid;
+        Vec<T>* const to = dst + k * kPiece;
+        if (left >= kPiece && (kind == 1 || kind == 2)) {
+          Vec<T> v[kPieceVecs];
+#pragma unroll
+          for (int u = 0; u < kPieceVecs; ++u) v[u] = at[u * NT];
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(&sh.empty[k]);  // read: its place can be filled again
+          if (kind == 1) {
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+              for (int u = 0; u < kPieceVecs; ++u) to[u * NT] = vec_grad_folded(v[u], gr.kg, gr.negative, p.c_hi);
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < kPieceVecs; ++u) to[u * NT] = vec_grad<false>(v[u], gr, p.c_hi, p.c_lo);
+          }
+        } else {
+          if (!zero)
+            for (int j = tid; j < left; j += NT)
+              put_grad(at[j - tid], v0 + k * kPiece + j, drow, c, gr, same, p.c_hi, p.c_lo);
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(&sh.empty[k]);
+        }
+      }
+      if (!zero) {
+        // the token's element again, by the thread that wrote its vector
+        const int jt = gr.tok >= c.head && gr.tok < c.tail0 ? (gr.tok - c.head) / Vec<T>::N - v0 : -1;
+        if (jt >= 0 && jt < n && jt % NT == tid) drow[gr.tok] = one_grad<T>(gr.at, gr, 1.f, p.c_hi, p.c_lo);
+        if (rank == 0) put_ends(row, drow, p.V, c, gr, tid, NT, p.c_hi, p.c_lo);
+      }
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&sh.info_empty[slot]);
+    }
+  }
+  if (C > 1) cl.sync();  // no CTA leaves while another sends to it
 }
 
 // Short rows (up to 4 KB): a warp per row, the row in its registers.
@@ -642,31 +1016,27 @@ __global__ void __launch_bounds__(kShortThreads) token_short_rows_kernel(TokenRo
   const Base base = base_at(warp_max(m), p.c_hi);
   auto sum = [&](auto far) {
     constexpr bool FAR = decltype(far)::value;
-    // a lane without a single element holds -inf there, which adds nothing
-    float s = (lane < c.head ? exp2_approx(exponent<FAR>(first, base, p.c_hi, p.c_lo)) : 0.f) +
-              (c.tail0 + lane < p.V ? exp2_approx(exponent<FAR>(last, base, p.c_hi, p.c_lo)) : 0.f);
+    const float s = (lane < c.head ? exp_one<!POLICY>(first, base, p.c_hi, p.c_lo) : 0.f) +
+                    (c.tail0 + lane < p.V ? exp_one<!POLICY>(last, base, p.c_hi, p.c_lo) : 0.f);
+    Sum s2{0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < kShortVecs; ++u)
-      if (lane + 32 * u < c.nv) s += vec_sum<FAR>(v[u], base, p.c_hi, p.c_lo);
-    return s;
+      if (lane + 32 * u < c.nv) add_vec<FAR, !POLICY>(s2, v[u], base, p.c_hi, p.c_lo);
+    return s + s2.total();
   };
   const float S = warp_sum(base.far ? sum(std::true_type{}) : sum(std::false_type{}));
-  const float g = finish_row<POLICY>(p, a, w, o, x, r, at_token, base, S, lane == 0);
+  const GradRow gr =
+      finish_row<POLICY>(p, a, w, o, x, r, at_token, pos.known ? (int)pos.tok : -1, base, S, lane == 0);
   if constexpr (POLICY) {
     if (drow) {
-      const GradRow gr{base, g, 1.f / S, pos.known ? (int)pos.tok : -1, at_token};
-      if (g == 0.f) {
+      if (gr.g == 0.f) {
         fill<T>(drow, 0, p.V, lane, 32, from_f32<T>(0.f));
       } else {
         const bool same = same_boundary(drow, c);
-        auto put = [&](auto far) {
 #pragma unroll
-          for (int u = 0; u < kShortVecs; ++u)
-            if (lane + 32 * u < c.nv)
-              put_grad<decltype(far)::value>(v[u], lane + 32 * u, drow, c, gr, same, p.c_hi, p.c_lo);
-        };
-        if (base.far) put(std::true_type{});
-        else put(std::false_type{});
+        for (int u = 0; u < kShortVecs; ++u)
+          if (lane + 32 * u < c.nv) put_grad(v[u], lane + 32 * u, drow, c, gr, same, p.c_hi, p.c_lo);
+        put_token(drow, c, gr, 0, c.nv, lane, 32, p.c_hi, p.c_lo);
         put_ends(row, drow, p.V, c, gr, lane, 32, p.c_hi, p.c_lo);
       }
     }
@@ -721,7 +1091,7 @@ __global__ void __launch_bounds__(kSumThreads) policy_sum_kernel(int64_t R, Poli
   s.kl = block_sum(s.kl, sh);
   s.clipped = block_sum(s.clipped, sh);
   if (threadIdx.x == 0) {
-    const double n = w.head->total > 0 ? w.head->total : 1.0;
+    const double n = w.head->kept > 0 ? (double)w.head->kept : 1.0;
     *loss = (float)s.loss;
     *kl = (float)(s.kl / n);
     *clipped = (float)(s.clipped / n);
@@ -800,35 +1170,38 @@ __global__ void __launch_bounds__(kGradThreads, 3)
     const float2 st = stats[r];
     const RowCut c = cut_row(row, p.V);
     const int v0 = min(c.nv, part * kGradPart), v1 = min(c.nv, v0 + kGradPart);
-    GradRow gr;
-    gr.g = 0.f;
-    if (pos.keep) gr.g = pos.known ? (float)((double)u * (double)co * p.scale) : NAN;
-    if (gr.g == 0.f) {
+    float g = 0.f;
+    if (pos.keep) g = pos.known ? (float)((double)u * (double)co * p.scale) : NAN;
+    if (g == 0.f) {
       constexpr int N = Vec<T>::N;
       fill<T>(out, part == 0 ? 0 : c.head + v0 * N, part == parts - 1 ? p.V : c.head + v1 * N, lane, 32,
               from_f32<T>(0.f));
       continue;
     }
-    gr.base = base_at(st.x, p.c_hi);
-    gr.inv = 1.f / st.y;
-    gr.tok = pos.known ? (int)pos.tok : -1;
-    gr.at = pos.known ? to_f32(row[pos.tok]) : 0.f;
+    const GradRow gr = grad_row(base_at(st.x, p.c_hi), g, st.y, pos.known ? (int)pos.tok : -1,
+                                pos.known ? to_f32(row[pos.tok]) : 0.f);
     const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + c.head);
     const bool same = same_boundary(out, c);
-    auto put = [&](auto far) {
-      for (int j0 = v0; j0 < v1; j0 += 32 * kGradU) {
-        Vec<T> v[kGradU];
+    for (int j0 = v0; j0 < v1; j0 += 32 * kGradU) {
+      Vec<T> v[kGradU];
+#pragma unroll
+      for (int k = 0; k < kGradU; ++k)
+        if (j0 + lane + 32 * k < v1) v[k] = rv[j0 + lane + 32 * k];
+      if (same && sizeof(T) == 2 && gr.folded) {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int k = 0; k < kGradU; ++k)
+            if (j0 + lane + 32 * k < v1)
+              *reinterpret_cast<Vec<T>*>(out + c.head + (int64_t)(j0 + lane + 32 * k) * Vec<T>::N) =
+                  vec_grad_folded(v[k], gr.kg, gr.negative, p.c_hi);
+        }
+      } else {
 #pragma unroll
         for (int k = 0; k < kGradU; ++k)
-          if (j0 + lane + 32 * k < v1) v[k] = rv[j0 + lane + 32 * k];
-#pragma unroll
-        for (int k = 0; k < kGradU; ++k)
-          if (j0 + lane + 32 * k < v1)
-            put_grad<decltype(far)::value>(v[k], j0 + lane + 32 * k, out, c, gr, same, p.c_hi, p.c_lo);
+          if (j0 + lane + 32 * k < v1) put_grad(v[k], j0 + lane + 32 * k, out, c, gr, same, p.c_hi, p.c_lo);
       }
-    };
-    if (gr.base.far) put(std::true_type{});
-    else put(std::false_type{});
+    }
+    put_token(out, c, gr, v0, v1, lane, 32, p.c_hi, p.c_lo);
     if (part == 0) put_ends(row, out, p.V, c, gr, lane, 32, p.c_hi, p.c_lo);
   }
 }
@@ -836,11 +1209,10 @@ __global__ void __launch_bounds__(kGradThreads, 3)
 // How the rows are laid over the device.
 struct RowPlan {
   int C, threads;
-  size_t smem;
+  int slot_vecs;  // of one row's place in shared memory; 0: none
 };
-constexpr int64_t kKeepBytes = 110 * 1024;  // of a CTA's part: two CTAs of an SM then hold one each
-constexpr int64_t kKeepMost = 220 * 1024;
-int plan_rows(const TokenRows& p, int64_t elem, bool policy, bool keep, RowPlan* out) {
+constexpr int64_t kPlaceBytes = 104 * 1024;  // of a CTA's part of a row: two CTAs share an SM
+int plan_rows(const TokenRows& p, int64_t elem, bool policy, RowPlan* out) {
   int sms = 0;
   M3_TRY(device_sm_count(&sms));
   const int64_t bytes = (int64_t)p.V * elem;
@@ -848,32 +1220,22 @@ int plan_rows(const TokenRows& p, int64_t elem, bool policy, bool keep, RowPlan*
   // few rows: split each so that the device is filled, down to parts of 16 KB
   while (C < 8 && p.R * C * 2 <= 2 * (int64_t)sms && bytes / (2 * C) >= 16384) C *= 2;
   // the same with and without a gradient, so that both give the same bits
+  static const int64_t place = getenv("M3_PLACE") ? atoi(getenv("M3_PLACE")) * 1024 : kPlaceBytes;
+  static const int vt = getenv("M3_VT") ? atoi(getenv("M3_VT")) : 52;
   if (policy)
-    while (C < 8 && bytes / C > kKeepBytes) C *= 2;
-  // about eight vectors a thread
-  const int64_t want = bytes / C / 16 / 8;
-  int threads = 64;
-  while (threads < kRowThreads && threads < want) threads *= 2;
+    while (C < 8 && bytes / C > place) C *= 2;
   out->C = C;
-  out->threads = threads;
-  out->smem = keep ? (size_t)(bytes / C / 16 + 2) * 16 : 0;
-  if (out->smem > (size_t)kKeepMost) out->smem = 0;
+  out->threads = bytes / C <= 16 * 1024 ? 128 : bytes / C <= vt * 1024 ? 256 : 512;
+  out->slot_vecs = bytes / C <= kPlaceBytes ? (int)(bytes / C / 16 + 2) : 0;
   return M3_OK;
 }
 
-template <typename T, bool POLICY, bool KEEP>
-int launch_cluster_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o, const RowPlan& plan,
-                        cudaStream_t s) {
-  if (p.R > INT32_MAX / plan.C) return fail(M3_ERR_UNSUPPORTED, "token rows: too many positions");
-  auto kernel = token_rows_kernel<T, POLICY, KEEP>;
-  if constexpr (KEEP) {
-    static std::atomic<bool> done[kMaxDevices];
-    M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), (size_t)kKeepMost, done));
-  }
+// A launch of clusters; grid 0: as many clusters as the device holds at once, at most `most`.
+template <typename K, typename... A>
+int launch_clusters(K kernel, const RowPlan& plan, int64_t grid, int64_t most, size_t smem, cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.R * plan.C));
   cfg.blockDim = dim3((unsigned)plan.threads);
-  cfg.dynamicSmemBytes = KEEP ? plan.smem : 0;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -881,12 +1243,35 @@ int launch_cluster_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs&
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, a, w, o);
+  if (grid == 0) {
+    int n = 0;
+    cfg.gridDim = dim3((unsigned)plan.C);
+    cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      return fail(M3_ERR_CUDA, std::string("token rows: occupancy query: ") + cudaGetErrorString(e));
+    }
+    grid = std::min<int64_t>(n, most) * plan.C;
+  }
+  cfg.gridDim = dim3((unsigned)grid);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();
-    return fail(M3_ERR_CUDA, std::string("token_rows_kernel: ") + cudaGetErrorString(e));
+    return fail(M3_ERR_CUDA, std::string("token rows: ") + cudaGetErrorString(e));
   }
   return M3_OK;
+}
+
+template <typename T, int NT>
+int launch_grad_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o, RowPlan plan,
+                     cudaStream_t s) {
+  auto kernel = token_grad_rows_kernel<T, NT>;
+  static std::atomic<bool> done[kMaxDevices];
+  M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), (size_t)kPlaceBytes + 64, done));
+  const int pieces = (plan.slot_vecs + kPieceVecs * NT - 1) / (kPieceVecs * NT);
+  if (pieces > kPieces) return fail(M3_ERR_UNSUPPORTED, "token rows: row too long");
+  plan.threads = NT + 32;
+  return launch_clusters(kernel, plan, 0, p.R, (size_t)plan.slot_vecs * 16, s, p, a, w, o, pieces);
 }
 
 template <typename T, bool POLICY>
@@ -898,10 +1283,16 @@ int launch_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, cons
     return check_launch("token_short_rows_kernel");
   }
   RowPlan plan;
-  M3_TRY(plan_rows(p, (int64_t)sizeof(T), POLICY, o.dlogits != nullptr, &plan));
-  if constexpr (POLICY)
-    if (plan.smem > 0) return launch_cluster_rows<T, POLICY, true>(p, a, w, o, plan, s);
-  return launch_cluster_rows<T, POLICY, false>(p, a, w, o, plan, s);
+  M3_TRY(plan_rows(p, (int64_t)sizeof(T), POLICY, &plan));
+  if constexpr (POLICY) {
+    if (o.dlogits && plan.slot_vecs > 0) {
+      if (plan.threads == 128) return launch_grad_rows<T, 128>(p, a, w, o, plan, s);
+      if (plan.threads == 256) return launch_grad_rows<T, 256>(p, a, w, o, plan, s);
+      return launch_grad_rows<T, 512>(p, a, w, o, plan, s);
+    }
+  }
+  if (p.R > INT32_MAX / plan.C) return fail(M3_ERR_UNSUPPORTED, "token rows: too many positions");
+  return launch_clusters(token_rows_kernel<T, POLICY>, plan, p.R * plan.C, 0, 0, s, p, a, w, o);
 }
 
 template <bool POLICY>
@@ -916,6 +1307,18 @@ int launch_rows_of(const TokenRows& p, int dtype, const PolicyArgs& a, const Pol
 }
 
 }  // namespace
+
+int token_error_word(bool reset, int* out) {
+  unsigned v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_token_error, sizeof(v));
+  if (e == cudaSuccess && reset) {
+    const unsigned z = 0;
+    e = cudaMemcpyToSymbol(g_token_error, &z, sizeof(z));
+  }
+  if (e != cudaSuccess) return fail(M3_ERR_CUDA, std::string("device timeouts: ") + cudaGetErrorString(e));
+  *out = (int)v;
+  return M3_OK;
+}
 
 size_t policy_workspace_bytes(int64_t batch, int64_t rows) {
   size_t n = 0;
@@ -938,7 +1341,11 @@ int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64
                        void* ws, cudaStream_t s) {
   size_t bytes = 0;
   const PolicyWs w = policy_ws(ws, batch, p.R, &bytes);
-  policy_count_kernel<<<kCountCluster, kCountThreads, 0, s>>>(p, batch, w);
+  cudaError_t e = cudaMemsetAsync(w.head, 0, w.zeroed, s);
+  if (e != cudaSuccess) return fail(M3_ERR_CUDA, std::string("policy loss: ") + cudaGetErrorString(e));
+  const int segs = (p.T + kCountSegment - 1) / kCountSegment;
+  const int64_t units = batch * segs, per = kCountThreads / 32;
+  policy_count_kernel<<<(unsigned)((units + per - 1) / per), kCountThreads, 0, s>>>(p, units, segs, w);
   M3_TRY(check_launch("policy_count_kernel"));
   M3_TRY(launch_rows_of<true>(p, dtype, a, w, RowOut{logp, nullptr, stats, coef, dlogits, dsb, dst}, s));
   policy_sum_kernel<<<(unsigned)((p.R + kSumRows - 1) / kSumRows), kSumThreads, 0, s>>>(p.R, w, loss, kl, clipped);

@@ -34,6 +34,9 @@ struct PolicyArgs {
   int by_sequence;                       // mean of the sequences' means
 };
 
+// Nonzero once a bounded wait of the policy loss's kernel gave up on this device.
+int token_error_word(bool reset, int* out);
+
 // Workspace of the policy loss: counts and the sums' partial results (token_loss.cu).
 size_t policy_workspace_bytes(int64_t batch, int64_t rows);
 size_t preference_workspace_bytes(int64_t batch, int64_t rows);
