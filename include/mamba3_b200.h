@@ -389,44 +389,49 @@ int m3_silu_gate_bwd(const m3_tensor* y, const m3_tensor* z, const m3_tensor* do
  *   m3_preference_loss  mean over pairs of -(1 - e) log sigma(z) - e log sigma(-z), z = reward of
  *                       sequence i (chosen) - reward of sequence N + i (rejected), reward =
  *                       beta sum_t (logp - ref), e = label_smoothing
- *   m3_token_grad       dlogits = up * coef * s * (one-hot - softmax), the gradient of all three
+ *   m3_*_grad           dlogits = up * (d loss / d logp) * s * (one-hot - softmax)
  * Operands:
  *   logits (batch, seqlen, V) f32 / bf16 / f16, innermost stride 1; tokens (batch, seqlen) i64;
  *   mask (batch, seqlen) u8, optional: a position counts where it is not 0 and the token is
  *   not ignore_index. Other positions are not read: their logp and gradient rows are 0. A
  *   token outside [0, V) that is not ignore_index makes its position's results NaN.
- *   old_logprobs, advantages, ref_logprobs, coef (batch, seqlen) f32, any strides (0 where one
- *   value serves a sequence); ref_logprobs optional (absent: no KL term / reference 0).
- *   logprobs (batch, seqlen) f32 contiguous, stats (batch, seqlen, 2) f32 contiguous: what
- *   m3_token_grad needs of each row; optional. temperature > 0, finite.
- *   m3_policy_loss: loss, kl (mean), clip_fraction: one f32 each; coef (batch, seqlen) f32
- *   contiguous optional: d loss / d logp; dlogits optional (logits' dtype, innermost stride 1):
- *   the gradient for an upstream gradient of 1, written while the row is at hand.
- *   m3_preference_loss: loss (one f32), rewards (2 N), seq_coef (2 N) f32: d loss / d logp of a
- *   sequence's positions, which m3_token_grad takes as a coef of strides (1, 0).
- *   m3_token_grad: up optional, one f32 on the device; with keep_if_one the call leaves
- *   dlogits as it is where *up is 1 (m3_policy_loss has written it).
+ *   old_logprobs, advantages, ref_logprobs, dlogprobs (batch, seqlen) f32, any strides (0 where
+ *   one value serves a sequence); ref_logprobs optional (absent: no KL term / reference 0).
+ *   logprobs (batch, seqlen) f32 contiguous. temperature: between 1e-6 and 1e6.
+ *   m3_token_logprobs: stats (batch, seqlen, 2) f32 contiguous, optional: what
+ *   m3_token_logprobs_grad needs of each row.
+ *   m3_policy_loss: loss, kl (mean), clip_fraction: one f32 each; dlogits optional (logits'
+ *   dtype, innermost stride 1): the gradient for an upstream gradient of 1, written while the
+ *   row is at hand.
+ *   m3_preference_loss: batch = 2 N; loss (one f32), rewards (2 N) f32.
+ *   m3_policy_loss_grad, m3_preference_loss_grad: the workspace as the loss's call left it; up
+ *   optional, one f32 on the device (absent: 1). With keep_if_one the call leaves dlogits as
+ *   it is where *up is 1, because m3_policy_loss has written it.
  *   workspace: as the _workspace_size functions say, 16-byte aligned.
  * ------------------------------------------------------------------------------- */
 int m3_token_logprobs(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
                       double temperature, int64_t ignore_index, m3_tensor* logprobs, m3_tensor* stats,
                       void* stream);
+int m3_token_logprobs_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                           const m3_tensor* stats, const m3_tensor* dlogprobs, double temperature,
+                           int64_t ignore_index, m3_tensor* dlogits, void* stream);
 size_t m3_policy_loss_workspace_size(int64_t batch, int64_t seqlen);
 int m3_policy_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
                    const m3_tensor* old_logprobs, const m3_tensor* advantages, const m3_tensor* ref_logprobs,
                    double temperature, int64_t ignore_index, double clip_low, double clip_high, double kl_coef,
                    int by_sequence, m3_tensor* loss, m3_tensor* kl, m3_tensor* clip_fraction,
-                   m3_tensor* logprobs, m3_tensor* stats, m3_tensor* coef, m3_tensor* dlogits, void* workspace,
-                   size_t workspace_bytes, void* stream);
+                   m3_tensor* logprobs, m3_tensor* dlogits, void* workspace, size_t workspace_bytes, void* stream);
+int m3_policy_loss_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                        const m3_tensor* up, double temperature, int64_t ignore_index, int keep_if_one,
+                        m3_tensor* dlogits, const void* workspace, size_t workspace_bytes, void* stream);
 size_t m3_preference_loss_workspace_size(int64_t batch, int64_t seqlen);
 int m3_preference_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
                        const m3_tensor* ref_logprobs, double temperature, int64_t ignore_index, double beta,
                        double label_smoothing, m3_tensor* loss, m3_tensor* rewards, m3_tensor* logprobs,
-                       m3_tensor* stats, m3_tensor* seq_coef, void* workspace, size_t workspace_bytes,
-                       void* stream);
-int m3_token_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
-                  const m3_tensor* stats, const m3_tensor* coef, const m3_tensor* up, double temperature,
-                  int64_t ignore_index, int keep_if_one, m3_tensor* dlogits, void* stream);
+                       void* workspace, size_t workspace_bytes, void* stream);
+int m3_preference_loss_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                            const m3_tensor* up, double temperature, int64_t ignore_index, m3_tensor* dlogits,
+                            const void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Global norm of many gradient tensors, with scaling and clipping (the reference's train.py

@@ -1168,10 +1168,6 @@ int scalar_out(const m3_tensor* t, const char* name, bool optional) {
   return check(t, name, present(t) && t->ndim == 0 ? 0 : 1, one, kF32, true, false, true);
 }
 
-int optional_out(const m3_tensor* t, const char* name, int ndim, const int64_t* shape, bool devcheck) {
-  return check(t, name, ndim, shape, kF32, true, true, devcheck);
-}
-
 int workspace_ok(const void* ws, size_t have, size_t need, const char* what) {
   if (ws == nullptr || have < need || (reinterpret_cast<uintptr_t>(ws) & 15) != 0)
     return fail(M3_ERR_WORKSPACE, std::string(what) + ": workspace of " + std::to_string(need) + " bytes required");
@@ -1190,7 +1186,7 @@ int m3_token_logprobs(const m3_tensor* logits, const m3_tensor* tokens, const m3
   M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
   const int64_t bt[3] = {logits->shape[0], logits->shape[1], 2};
   M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
-  M3_TRY(optional_out(stats, "stats", 3, bt, !empty));
+  M3_TRY(check(stats, "stats", 3, bt, kF32, true, true, !empty));
   if (empty) return M3_OK;
   return launch_token_logprobs(p, logits->dtype, fptr<float>(logprobs), fptr<float2>(stats),
                                reinterpret_cast<cudaStream_t>(stream));
@@ -1205,12 +1201,12 @@ int m3_policy_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_te
                    const m3_tensor* old_logprobs, const m3_tensor* advantages, const m3_tensor* ref_logprobs,
                    double temperature, int64_t ignore_index, double clip_low, double clip_high, double kl_coef,
                    int by_sequence, m3_tensor* loss, m3_tensor* kl, m3_tensor* clip_fraction, m3_tensor* logprobs,
-                   m3_tensor* stats, m3_tensor* coef, m3_tensor* dlogits, void* workspace, size_t workspace_bytes, void* stream) {
+                   m3_tensor* dlogits, void* workspace, size_t workspace_bytes, void* stream) {
   TokenRows p{};
   bool empty = false;
   M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
   const int64_t* sh = logits->shape;
-  const int64_t bt[3] = {sh[0], sh[1], 2};
+  const int64_t bt[2] = {sh[0], sh[1]};
   if (!(clip_low >= 0 && clip_low <= 1)) return fail(M3_ERR_INVALID_ARGUMENT, "clip_low: expected a number from 0 to 1");
   if (!(clip_high >= 0)) return fail(M3_ERR_INVALID_ARGUMENT, "clip_high: expected a number from 0 on");
   if (!(kl_coef >= 0 && std::isfinite(kl_coef))) return fail(M3_ERR_INVALID_ARGUMENT, "kl_coef: expected a finite number from 0 on");
@@ -1220,8 +1216,6 @@ int m3_policy_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_te
   M3_TRY(map2(advantages, "advantages", M3_FLOAT32, sh, false, !empty, &a.adv));
   M3_TRY(map2(ref_logprobs, "ref_logprobs", M3_FLOAT32, sh, true, !empty, &a.ref));
   M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
-  M3_TRY(optional_out(stats, "stats", 3, bt, !empty));
-  M3_TRY(optional_out(coef, "coef", 2, bt, !empty));
   M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, true, !empty));
   M3_TRY(scalar_out(loss, "loss", false));
   M3_TRY(scalar_out(kl, "kl", false));
@@ -1236,8 +1230,8 @@ int m3_policy_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_te
   a.clip_lo = 1.0 - clip_low; a.clip_hi = 1.0 + clip_high; a.kl_coef = kl_coef; a.by_sequence = by_sequence;
   const bool grad = present(dlogits);
   return launch_policy_loss(p, logits->dtype, a, sh[0], fptr<float>(loss), fptr<float>(kl),
-                            fptr<float>(clip_fraction), fptr<float>(logprobs), fptr<float2>(stats), fptr<float>(coef), fptr<void>(dlogits), grad ? dlogits->stride[0] : 0,
-                            grad ? dlogits->stride[1] : 0, workspace, s);
+                            fptr<float>(clip_fraction), fptr<float>(logprobs), fptr<void>(dlogits),
+                            grad ? dlogits->stride[0] : 0, grad ? dlogits->stride[1] : 0, workspace, s);
 }
 
 size_t m3_preference_loss_workspace_size(int64_t batch, int64_t seqlen) {
@@ -1248,7 +1242,7 @@ size_t m3_preference_loss_workspace_size(int64_t batch, int64_t seqlen) {
 int m3_preference_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
                        const m3_tensor* ref_logprobs, double temperature, int64_t ignore_index, double beta,
                        double label_smoothing, m3_tensor* loss, m3_tensor* rewards, m3_tensor* logprobs,
-                       m3_tensor* stats, m3_tensor* seq_coef, void* workspace, size_t workspace_bytes, void* stream) {
+                       void* workspace, size_t workspace_bytes, void* stream) {
   TokenRows p{};
   bool empty = false;
   M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
@@ -1258,38 +1252,69 @@ int m3_preference_loss(const m3_tensor* logits, const m3_tensor* tokens, const m
   if (!(beta >= 0 && std::isfinite(beta))) return fail(M3_ERR_INVALID_ARGUMENT, "beta: expected a finite number from 0 on");
   if (!(label_smoothing >= 0 && label_smoothing <= 1))
     return fail(M3_ERR_INVALID_ARGUMENT, "label_smoothing: expected a number from 0 to 1");
-  const int64_t bt[3] = {sh[0], sh[1], 2};
+  const int64_t bt[2] = {sh[0], sh[1]};
   Map2<const float> ref;
   M3_TRY(map2(ref_logprobs, "ref_logprobs", M3_FLOAT32, sh, true, !empty, &ref));
   M3_TRY(scalar_out(loss, "loss", false));
   M3_TRY(check(rewards, "rewards", 1, bt, kF32, true, false, true));
-  M3_TRY(check(seq_coef, "seq_coef", 1, bt, kF32, true, false, true));
   M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
-  M3_TRY(optional_out(stats, "stats", 3, bt, !empty));
   M3_TRY(workspace_ok(workspace, workspace_bytes, preference_workspace_bytes(sh[0], p.R), "preference loss"));
   return launch_preference_loss(p, logits->dtype, ref, beta, label_smoothing, sh[0] / 2, fptr<float>(loss),
-                                fptr<float>(rewards), fptr<float>(logprobs), fptr<float2>(stats),
-                                fptr<float>(seq_coef), workspace, reinterpret_cast<cudaStream_t>(stream));
+                                fptr<float>(rewards), fptr<float>(logprobs), workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int m3_token_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask, const m3_tensor* stats,
-                  const m3_tensor* coef, const m3_tensor* up, double temperature, int64_t ignore_index,
-                  int keep_if_one, m3_tensor* dlogits, void* stream) {
+namespace m3 {
+namespace {
+// The gradient of a loss from its workspace.
+int loss_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask, const m3_tensor* up,
+              double temperature, int64_t ignore_index, bool keep_if_one, m3_tensor* dlogits, const void* workspace,
+              size_t workspace_bytes, bool policy, cudaStream_t s) {
+  TokenRows p{};
+  bool empty = false;
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  const int64_t* sh = logits->shape;
+  M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, false, !empty));
+  M3_TRY(scalar_out(up, "up", true));
+  if (empty) return M3_OK;
+  const size_t need = policy ? policy_workspace_bytes(sh[0], p.R) : preference_workspace_bytes(sh[0], p.R);
+  M3_TRY(workspace_ok(workspace, workspace_bytes, need, policy ? "policy loss" : "preference loss"));
+  const Map2<const float> coef = policy ? policy_coef(workspace, p) : preference_coef(workspace, p);
+  return launch_token_grad(p, logits->dtype, workspace_stats(workspace), coef, fptr<const float>(up), keep_if_one,
+                           dlogits->data, dlogits->stride[0], dlogits->stride[1], s);
+}
+}  // namespace
+}  // namespace m3
+
+int m3_policy_loss_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask, const m3_tensor* up,
+                        double temperature, int64_t ignore_index, int keep_if_one, m3_tensor* dlogits,
+                        const void* workspace, size_t workspace_bytes, void* stream) {
+  if (keep_if_one != 0 && keep_if_one != 1) return fail(M3_ERR_INVALID_ARGUMENT, "keep_if_one: expected 0 or 1");
+  return loss_grad(logits, tokens, mask, up, temperature, ignore_index, keep_if_one != 0, dlogits, workspace,
+                   workspace_bytes, true, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int m3_preference_loss_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                            const m3_tensor* up, double temperature, int64_t ignore_index, m3_tensor* dlogits,
+                            const void* workspace, size_t workspace_bytes, void* stream) {
+  return loss_grad(logits, tokens, mask, up, temperature, ignore_index, false, dlogits, workspace, workspace_bytes,
+                   false, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int m3_token_logprobs_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask,
+                           const m3_tensor* stats, const m3_tensor* dlogprobs, double temperature,
+                           int64_t ignore_index, m3_tensor* dlogits, void* stream) {
   TokenRows p{};
   bool empty = false;
   M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
   const int64_t* sh = logits->shape;
   const int64_t bt[3] = {sh[0], sh[1], 2};
-  if (keep_if_one != 0 && keep_if_one != 1) return fail(M3_ERR_INVALID_ARGUMENT, "keep_if_one: expected 0 or 1");
   Map2<const float> c;
   M3_TRY(check(stats, "stats", 3, bt, kF32, true, false, !empty));
-  M3_TRY(map2(coef, "coef", M3_FLOAT32, sh, false, !empty, &c));
-  M3_TRY(scalar_out(up, "up", true));
+  M3_TRY(map2(dlogprobs, "dlogprobs", M3_FLOAT32, sh, false, !empty, &c));
   M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, false, !empty));
   if (empty) return M3_OK;
-  return launch_token_grad(p, logits->dtype, fptr<const float2>(stats), c, fptr<const float>(up), keep_if_one != 0,
-                           dlogits->data, dlogits->stride[0], dlogits->stride[1],
-                           reinterpret_cast<cudaStream_t>(stream));
+  return launch_token_grad(p, logits->dtype, fptr<const float2>(stats), c, nullptr, false, dlogits->data,
+                           dlogits->stride[0], dlogits->stride[1], reinterpret_cast<cudaStream_t>(stream));
 }
 
 size_t m3_clip_grads_workspace_size(int64_t count) { return count < 0 ? 0 : clip_grads_workspace_bytes(count); }

@@ -234,6 +234,8 @@ struct SumPart {
   double loss, kl, clipped;
 };
 struct PolicyWs {
+  float2* stats;
+  float* coef;
   PolicyHead* head;
   int* counts;
   int* order;  // the positions that count, then the others
@@ -246,11 +248,15 @@ inline PolicyWs policy_ws(void* ws, int64_t batch, int64_t rows, size_t* bytes) 
   char* q = static_cast<char*>(ws);
   size_t at = 0;
   PolicyWs w;
+  w.stats = reinterpret_cast<float2*>(q + at);
+  at += up16(sizeof(float2) * (size_t)rows);
+  w.coef = reinterpret_cast<float*>(q + at);
+  at += up16(sizeof(float) * (size_t)rows);
   w.head = reinterpret_cast<PolicyHead*>(q + at);
   at += up16(sizeof(PolicyHead));
   w.counts = reinterpret_cast<int*>(q + at);  // with the head, what is zero at the start
   at += up16(sizeof(int) * (size_t)batch);
-  w.zeroed = at;
+  w.zeroed = (size_t)(q + at - reinterpret_cast<char*>(w.head));
   w.parts = reinterpret_cast<SumPart*>(q + at);
   at += up16(sizeof(SumPart) * (size_t)((rows + kSumRows - 1) / kSumRows));
   w.order = reinterpret_cast<int*>(q + at);
@@ -604,15 +610,16 @@ __device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a
 
 // One cluster of CTAs (of one CTA where there are rows enough) per row. A policy gradient of
 // rows too long for token_grad_rows_kernel is written from a second reading.
-template <typename T, bool POLICY>
-__global__ void __launch_bounds__(kRowThreads) token_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o) {
+template <typename T, bool POLICY, int NT>
+__global__ void __launch_bounds__(NT, POLICY ? 1024 / NT : 1536 / NT) token_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o) {
   constexpr int U = 4;  // loads in flight per thread
   __shared__ RowShared sh;
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int64_t r = blockIdx.x / C;
   const int64_t b = r / p.T, t = r - b * p.T;
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31;
+  constexpr int nt = NT;
+  const int tid = threadIdx.x, lane = tid & 31;
   const T* row = static_cast<const T*>(p.logits) + b * p.sb + t * p.st;
   T* drow = nullptr;
   if constexpr (POLICY)
@@ -1101,22 +1108,33 @@ __global__ void __launch_bounds__(kSumThreads) policy_sum_kernel(int64_t R, Poli
 // Rewards of the answers, then (by the CTA that finishes last) the loss of the pairs and the
 // derivative by each answer's log-probabilities. One CTA per answer.
 struct PrefWs {
+  float2* stats;
+  float* coef;      // (2 N)
   unsigned* done;
   double* rewards;  // (2 N)
   double* logp;     // (2 N, T)
 };
 inline PrefWs pref_ws(void* ws, int64_t batch, int64_t rows, size_t* bytes) {
+  char* q = static_cast<char*>(ws);
+  size_t at = 0;
   PrefWs w;
-  w.done = static_cast<unsigned*>(ws);
-  w.rewards = reinterpret_cast<double*>(static_cast<char*>(ws) + 16);
-  w.logp = w.rewards + batch;
-  *bytes = 16 + sizeof(double) * (size_t)(batch + rows);
+  w.stats = reinterpret_cast<float2*>(q + at);
+  at += up16(sizeof(float2) * (size_t)rows);
+  w.coef = reinterpret_cast<float*>(q + at);
+  at += up16(sizeof(float) * (size_t)batch);
+  w.done = reinterpret_cast<unsigned*>(q + at);
+  at += 16;
+  w.rewards = reinterpret_cast<double*>(q + at);
+  at += up16(sizeof(double) * (size_t)batch);
+  w.logp = reinterpret_cast<double*>(q + at);
+  at += up16(sizeof(double) * (size_t)rows);
+  *bytes = at;
   return w;
 }
 
 __global__ void __launch_bounds__(kSumThreads)
     preference_pairs_kernel(TokenRows p, Map2<const float> ref, double beta, double smoothing, int pairs,
-                            PrefWs w, float* loss, float* rewards, float* seq_coef) {
+                            PrefWs w, float* loss, float* rewards) {
   __shared__ double sh[kSumThreads / 32];
   __shared__ bool last;
   const int64_t b = blockIdx.x;
@@ -1140,69 +1158,69 @@ __global__ void __launch_bounds__(kSumThreads)
     const double l = log1p(exp(-fabs(z)));  // softplus(-|z|)
     s += (1.0 - smoothing) * (l + fmax(-z, 0.0)) + smoothing * (l + fmax(z, 0.0));
     const double dz = (1.0 / (1.0 + exp(-z)) - (1.0 - smoothing)) * beta / pairs;
-    seq_coef[i] = (float)dz;
-    seq_coef[pairs + i] = (float)-dz;
+    w.coef[i] = (float)dz;
+    w.coef[pairs + i] = (float)-dz;
   }
   s = block_sum(s, sh);
   if (threadIdx.x == 0) *loss = (float)(s / pairs);
 }
 
-// The gradient of the logits from the rows' (m, S). A warp takes a part of a row at a time,
-// parts from the end (the forward read the end last, so some of it is still in the L2 cache).
-constexpr int kGradThreads = 256, kGradWarps = kGradThreads / 32;
-constexpr int kGradU = 4;                    // loads in flight per lane
-constexpr int kGradPart = 32 * kGradU * 4;   // vectors of one part
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads, 3)
+// The gradient of the logits from the rows' (m, S). A group of G threads takes a part of a row
+// at a time, parts from the end (the forward read the end last, so some of it is still in the
+// L2 cache; the stores are marked to leave it there).
+constexpr int kGradThreads = 256;
+constexpr int kGradU = 4;  // loads in flight per thread
+template <typename T, int G>
+__global__ void __launch_bounds__(kGradThreads, 4)
     token_grad_kernel(TokenRows p, const float2* stats, Map2<const float> coef, const float* up, bool keep_if_one,
-                      T* dlogits, int64_t dsb, int64_t dst, int parts, int64_t units) {
+                      T* dlogits, int64_t dsb, int64_t dst, int parts, int units) {
   const float u = up ? *up : 1.f;
   if (keep_if_one && u == 1.f) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t step = (int64_t)gridDim.x * kGradWarps;
-  for (int64_t i = (int64_t)blockIdx.x * kGradWarps + (threadIdx.x >> 5); i < units; i += step) {
-    const int64_t at = units - 1 - i, r = at / parts, b = r / p.T, t = r - b * p.T;
-    const int part = (int)(at - r * parts);
+  constexpr int groups = kGradThreads / G;
+  const int tid = threadIdx.x % G;
+  const int step = gridDim.x * groups;
+  for (int i = blockIdx.x * groups + threadIdx.x / G; i < units; i += step) {
+    const int at = units - 1 - i, r = at / parts, part = at - r * parts, b = r / p.T, t = r - b * p.T;
     const T* row = static_cast<const T*>(p.logits) + b * p.sb + t * p.st;
     T* out = dlogits + b * dsb + t * dst;
     const Position pos = position(p, b, t);
     const float co = map_at(coef, b, t);
     const float2 st = stats[r];
     const RowCut c = cut_row(row, p.V);
-    const int v0 = min(c.nv, part * kGradPart), v1 = min(c.nv, v0 + kGradPart);
+    const int v0 = (int)((int64_t)c.nv * part / parts), v1 = (int)((int64_t)c.nv * (part + 1) / parts);
     float g = 0.f;
     if (pos.keep) g = pos.known ? (float)((double)u * (double)co * p.scale) : NAN;
     if (g == 0.f) {
       constexpr int N = Vec<T>::N;
-      fill<T>(out, part == 0 ? 0 : c.head + v0 * N, part == parts - 1 ? p.V : c.head + v1 * N, lane, 32,
-              from_f32<T>(0.f));
+      fill<T>(out, part == 0 ? 0 : c.head + v0 * N, part == parts - 1 ? p.V : c.head + v1 * N, tid, G, from_f32<T>(0.f));
       continue;
     }
     const GradRow gr = grad_row(base_at(st.x, p.c_hi), g, st.y, pos.known ? (int)pos.tok : -1,
                                 pos.known ? to_f32(row[pos.tok]) : 0.f);
     const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + c.head);
+    uint4* const to = reinterpret_cast<uint4*>(out + c.head);
     const bool same = same_boundary(out, c);
-    for (int j0 = v0; j0 < v1; j0 += 32 * kGradU) {
-      Vec<T> v[kGradU];
+    const int kind = !same || gr.base.far ? 3 : sizeof(T) == 2 && gr.folded ? 1 : 2;
+    int j = v0 + tid;
+    if (kind != 3) {
+      for (; j + (kGradU - 1) * G < v1; j += kGradU * G) {
+        Vec<T> v[kGradU];
 #pragma unroll
-      for (int k = 0; k < kGradU; ++k)
-        if (j0 + lane + 32 * k < v1) v[k] = rv[j0 + lane + 32 * k];
-      if (same && sizeof(T) == 2 && gr.folded) {
-        if constexpr (sizeof(T) == 2) {
+        for (int k = 0; k < kGradU; ++k) v[k] = rv[j + k * G];
+        if (kind == 1) {
+          if constexpr (sizeof(T) == 2) {
 #pragma unroll
-          for (int k = 0; k < kGradU; ++k)
-            if (j0 + lane + 32 * k < v1)
-              *reinterpret_cast<Vec<T>*>(out + c.head + (int64_t)(j0 + lane + 32 * k) * Vec<T>::N) =
-                  vec_grad_folded(v[k], gr.kg, gr.negative, p.c_hi);
+            for (int k = 0; k < kGradU; ++k) __stcs(to + j + k * G, vec_grad_folded(v[k], gr.kg, gr.negative, p.c_hi).u);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < kGradU; ++k) __stcs(to + j + k * G, vec_grad<false>(v[k], gr, p.c_hi, p.c_lo).u);
         }
-      } else {
-#pragma unroll
-        for (int k = 0; k < kGradU; ++k)
-          if (j0 + lane + 32 * k < v1) put_grad(v[k], j0 + lane + 32 * k, out, c, gr, same, p.c_hi, p.c_lo);
       }
     }
-    put_token(out, c, gr, v0, v1, lane, 32, p.c_hi, p.c_lo);
-    if (part == 0) put_ends(row, out, p.V, c, gr, lane, 32, p.c_hi, p.c_lo);
+    for (; j < v1; j += G) put_grad(rv[j], j, out, c, gr, same, p.c_hi, p.c_lo);
+    put_token(out, c, gr, v0, v1, tid, G, p.c_hi, p.c_lo);
+    if (part == 0) put_ends(row, out, p.V, c, gr, tid, G, p.c_hi, p.c_lo);
   }
 }
 
@@ -1225,14 +1243,24 @@ int plan_rows(const TokenRows& p, int64_t elem, bool policy, RowPlan* out) {
   if (policy)
     while (C < 8 && bytes / C > place) C *= 2;
   out->C = C;
-  out->threads = bytes / C <= 16 * 1024 ? 128 : bytes / C <= vt * 1024 ? 256 : 512;
+  static const int fw = getenv("M3_FW") ? atoi(getenv("M3_FW")) : 256;
+  out->threads = bytes / C <= 16 * 1024 ? 128 : bytes / C <= vt * 1024 || !policy ? 256 : 512;
+  if (!policy && out->threads == 256) out->threads = fw;
   out->slot_vecs = bytes / C <= kPlaceBytes ? (int)(bytes / C / 16 + 2) : 0;
   return M3_OK;
 }
 
-// A launch of clusters; grid 0: as many clusters as the device holds at once, at most `most`.
+// Clusters of one kernel that the device holds at once, remembered for the last launch shape of
+// each device: (shared memory << 32) | (cluster size << 16) | clusters.
+struct ClusterCache {
+  std::atomic<long long> word[kMaxDevices];
+};
+
+// A launch of clusters. With a cache: as many as the device holds at once, at most `most`;
+// without: `most` of them.
 template <typename K, typename... A>
-int launch_clusters(K kernel, const RowPlan& plan, int64_t grid, int64_t most, size_t smem, cudaStream_t s, A... args) {
+int launch_clusters(K kernel, const RowPlan& plan, int64_t most, ClusterCache* cache, size_t smem, cudaStream_t s,
+                    A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3((unsigned)plan.threads);
   cfg.dynamicSmemBytes = smem;
@@ -1243,17 +1271,24 @@ int launch_clusters(K kernel, const RowPlan& plan, int64_t grid, int64_t most, s
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (grid == 0) {
-    int n = 0;
-    cfg.gridDim = dim3((unsigned)plan.C);
-    cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-    if (e != cudaSuccess || n <= 0) {
-      cudaGetLastError();
-      return fail(M3_ERR_CUDA, std::string("token rows: occupancy query: ") + cudaGetErrorString(e));
+  if (cache) {
+    int dev = 0;
+    M3_TRY(current_device(&dev));
+    const long long shape = ((long long)smem << 16) | plan.C, word = cache->word[dev].load(std::memory_order_acquire);
+    int n = (int)(word & 0xffff);
+    if (n == 0 || (word >> 16) != shape) {
+      cfg.gridDim = dim3((unsigned)plan.C);
+      cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+      if (e != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        return fail(M3_ERR_CUDA, std::string("token rows: occupancy query: ") + cudaGetErrorString(e));
+      }
+      n = std::min(n, 0xffff);
+      cache->word[dev].store((shape << 16) | n, std::memory_order_release);
     }
-    grid = std::min<int64_t>(n, most) * plan.C;
+    most = std::min<int64_t>(n, most);
   }
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = dim3((unsigned)(most * plan.C));
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -1271,7 +1306,8 @@ int launch_grad_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w,
   const int pieces = (plan.slot_vecs + kPieceVecs * NT - 1) / (kPieceVecs * NT);
   if (pieces > kPieces) return fail(M3_ERR_UNSUPPORTED, "token rows: row too long");
   plan.threads = NT + 32;
-  return launch_clusters(kernel, plan, 0, p.R, (size_t)plan.slot_vecs * 16, s, p, a, w, o, pieces);
+  static ClusterCache cache;
+  return launch_clusters(kernel, plan, p.R, &cache, (size_t)plan.slot_vecs * 16, s, p, a, w, o, pieces);
 }
 
 template <typename T, bool POLICY>
@@ -1292,7 +1328,9 @@ int launch_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, cons
     }
   }
   if (p.R > INT32_MAX / plan.C) return fail(M3_ERR_UNSUPPORTED, "token rows: too many positions");
-  return launch_clusters(token_rows_kernel<T, POLICY>, plan, p.R * plan.C, 0, 0, s, p, a, w, o);
+  if (plan.threads == 128) return launch_clusters(token_rows_kernel<T, POLICY, 128>, plan, p.R, nullptr, 0, s, p, a, w, o);
+  if (plan.threads == 256) return launch_clusters(token_rows_kernel<T, POLICY, 256>, plan, p.R, nullptr, 0, s, p, a, w, o);
+  return launch_clusters(token_rows_kernel<T, POLICY, 512>, plan, p.R, nullptr, 0, s, p, a, w, o);
 }
 
 template <bool POLICY>
@@ -1337,8 +1375,7 @@ int launch_token_logprobs(const TokenRows& p, int dtype, float* logp, float2* st
 }
 
 int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64_t batch, float* loss, float* kl,
-                       float* clipped, float* logp, float2* stats, float* coef, void* dlogits, int64_t dsb, int64_t dst,
-                       void* ws, cudaStream_t s) {
+                       float* clipped, float* logp, void* dlogits, int64_t dsb, int64_t dst, void* ws, cudaStream_t s) {
   size_t bytes = 0;
   const PolicyWs w = policy_ws(ws, batch, p.R, &bytes);
   cudaError_t e = cudaMemsetAsync(w.head, 0, w.zeroed, s);
@@ -1347,23 +1384,32 @@ int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64
   const int64_t units = batch * segs, per = kCountThreads / 32;
   policy_count_kernel<<<(unsigned)((units + per - 1) / per), kCountThreads, 0, s>>>(p, units, segs, w);
   M3_TRY(check_launch("policy_count_kernel"));
-  M3_TRY(launch_rows_of<true>(p, dtype, a, w, RowOut{logp, nullptr, stats, coef, dlogits, dsb, dst}, s));
+  M3_TRY(launch_rows_of<true>(p, dtype, a, w, RowOut{logp, nullptr, w.stats, w.coef, dlogits, dsb, dst}, s));
   policy_sum_kernel<<<(unsigned)((p.R + kSumRows - 1) / kSumRows), kSumThreads, 0, s>>>(p.R, w, loss, kl, clipped);
   return check_launch("policy_sum_kernel");
 }
 
 int launch_preference_loss(const TokenRows& p, int dtype, Map2<const float> ref, double beta, double smoothing,
-                           int64_t pairs, float* loss, float* rewards, float* logp, float2* stats, float* seq_coef,
-                           void* ws, cudaStream_t s) {
+                           int64_t pairs, float* loss, float* rewards, float* logp, void* ws, cudaStream_t s) {
   size_t bytes = 0;
   const PrefWs w = pref_ws(ws, 2 * pairs, p.R, &bytes);
   cudaError_t e = cudaMemsetAsync(w.done, 0, sizeof(unsigned), s);
   if (e != cudaSuccess) return fail(M3_ERR_CUDA, std::string("preference loss: ") + cudaGetErrorString(e));
   M3_TRY(launch_rows_of<false>(p, dtype, PolicyArgs{}, PolicyWs{},
-                               RowOut{logp, w.logp, stats, nullptr, nullptr, 0, 0}, s));
+                               RowOut{logp, w.logp, w.stats, nullptr, nullptr, 0, 0}, s));
   preference_pairs_kernel<<<(unsigned)(2 * pairs), kSumThreads, 0, s>>>(p, ref, beta, smoothing, (int)pairs, w, loss,
-                                                                       rewards, seq_coef);
+                                                                       rewards);
   return check_launch("preference_pairs_kernel");
+}
+
+const float2* workspace_stats(const void* ws) { return static_cast<const float2*>(ws); }
+Map2<const float> policy_coef(const void* ws, const TokenRows& p) {
+  size_t bytes = 0;
+  return Map2<const float>{policy_ws(const_cast<void*>(ws), p.R / p.T, p.R, &bytes).coef, p.T, 1};
+}
+Map2<const float> preference_coef(const void* ws, const TokenRows& p) {
+  size_t bytes = 0;
+  return Map2<const float>{pref_ws(const_cast<void*>(ws), p.R / p.T, p.R, &bytes).coef, 1, 0};
 }
 
 template <typename T>
@@ -1371,12 +1417,22 @@ static int launch_grad(const TokenRows& p, const float2* stats, Map2<const float
                        bool keep_if_one, void* dlogits, int64_t dsb, int64_t dst, cudaStream_t s) {
   int sms = 0;
   M3_TRY(device_sm_count(&sms));
-  const int N = 16 / (int)sizeof(T);
-  const int parts = std::max(1, (p.V / N + kGradPart - 1) / kGradPart);
-  const int64_t units = p.R * parts;
-  const unsigned grid = (unsigned)std::min<int64_t>((units + kGradWarps - 1) / kGradWarps, (int64_t)sms * 8);
-  token_grad_kernel<T><<<grid, kGradThreads, 0, s>>>(p, stats, coef, up, keep_if_one, static_cast<T*>(dlogits), dsb,
-                                                    dst, parts, units);
+  const int64_t bytes = (int64_t)p.V * (int64_t)sizeof(T), ctas = (int64_t)sms * 4;
+  T* const d = static_cast<T*>(dlogits);
+  if (bytes <= 8192) {  // a warp per row
+    const int units = (int)p.R;
+    const unsigned grid = (unsigned)std::min<int64_t>((units + 7) / 8, ctas);
+    token_grad_kernel<T, 32><<<grid, kGradThreads, 0, s>>>(p, stats, coef, up, keep_if_one, d, dsb, dst, 1, units);
+  } else {
+    // a CTA per row, or per part of a row where the rows do not fill the device (parts of 8 KB
+    // or more) or where there are few for each CTA, whose last ones would then be uneven
+    int64_t parts = 1;
+    while (p.R * parts < 4 * ctas && bytes / (2 * parts) >= 8192) parts *= 2;
+    const int units = (int)(p.R * parts);
+    const unsigned grid = (unsigned)std::min<int64_t>(units, ctas);
+    token_grad_kernel<T, kGradThreads><<<grid, kGradThreads, 0, s>>>(p, stats, coef, up, keep_if_one, d, dsb, dst,
+                                                                     (int)parts, units);
+  }
   return check_launch("token_grad_kernel");
 }
 

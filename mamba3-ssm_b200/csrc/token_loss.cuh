@@ -37,21 +37,25 @@ struct PolicyArgs {
 // Nonzero once a bounded wait of the policy loss's kernel gave up on this device.
 int token_error_word(bool reset, int* out);
 
-// Workspace of the policy loss: counts and the sums' partial results (token_loss.cu).
+// Workspaces of the two losses. They begin with what the gradient needs: stats (R) and the
+// coefficients d loss / d logp (by position, or by sequence for the preference loss).
 size_t policy_workspace_bytes(int64_t batch, int64_t rows);
 size_t preference_workspace_bytes(int64_t batch, int64_t rows);
 
 // logp (R) and, where given, stats (R) = (maximum, sum) of each row
 int launch_token_logprobs(const TokenRows& p, int dtype, float* logp, float2* stats, cudaStream_t s);
-// loss, mean KL, share of clipped tokens; coef (R) and dlogits where given
+// loss, mean KL, share of clipped tokens; dlogits where given
 int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64_t batch, float* loss, float* kl,
-                       float* clipped, float* logp, float2* stats, float* coef, void* dlogits, int64_t dsb, int64_t dst, void* ws, cudaStream_t s);
-// loss (1), rewards (2 N), seq_coef (2 N): d loss / d logp of each sequence's positions
+                       float* clipped, float* logp, void* dlogits, int64_t dsb, int64_t dst, void* ws, cudaStream_t s);
+// loss (1), rewards (2 N)
 int launch_preference_loss(const TokenRows& p, int dtype, Map2<const float> ref, double beta, double smoothing,
-                           int64_t pairs, float* loss, float* rewards, float* logp, float2* stats, float* seq_coef,
-                           void* ws, cudaStream_t s);
+                           int64_t pairs, float* loss, float* rewards, float* logp, void* ws, cudaStream_t s);
 // dlogits = up * coef * scale * (one-hot - softmax); keep_if_one: leaves dlogits where *up is 1
 int launch_token_grad(const TokenRows& p, int dtype, const float2* stats, Map2<const float> coef, const float* up,
                       bool keep_if_one, void* dlogits, int64_t dsb, int64_t dst, cudaStream_t s);
+// stats and coefficients in a loss's workspace
+const float2* workspace_stats(const void* ws);
+Map2<const float> policy_coef(const void* ws, const TokenRows& p);
+Map2<const float> preference_coef(const void* ws, const TokenRows& p);
 
 }  // namespace m3

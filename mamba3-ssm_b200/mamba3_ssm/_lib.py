@@ -5,6 +5,7 @@ directory. There is deliberately no fallback: if the library is missing or a cal
 a RuntimeError is raised with the library's own error text.
 """
 
+import contextlib
 import ctypes
 import os
 import struct
@@ -87,13 +88,17 @@ _SIGS = {
     "m3_silu_gate_bwd": ([_P] * 5 + [ctypes.c_void_p], ctypes.c_int),
     "m3_argmax_rows": ([_P, _P, ctypes.c_void_p], ctypes.c_int),
     "m3_token_logprobs": ([_P] * 3 + [ctypes.c_double, ctypes.c_int64] + [_P] * 2 + [ctypes.c_void_p], ctypes.c_int),
+    "m3_token_logprobs_grad": ([_P] * 5 + [ctypes.c_double, ctypes.c_int64, _P, ctypes.c_void_p], ctypes.c_int),
     "m3_policy_loss_workspace_size": ([ctypes.c_int64] * 2, ctypes.c_size_t),
     "m3_policy_loss": ([_P] * 6 + [ctypes.c_double, ctypes.c_int64] + [ctypes.c_double] * 3 + [ctypes.c_int] +
-                       [_P] * 7 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
+                       [_P] * 5 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
+    "m3_policy_loss_grad": ([_P] * 4 + [ctypes.c_double, ctypes.c_int64, ctypes.c_int, _P, ctypes.c_void_p,
+                                       ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
     "m3_preference_loss_workspace_size": ([ctypes.c_int64] * 2, ctypes.c_size_t),
-    "m3_preference_loss": ([_P] * 4 + [ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double] + [_P] * 5 +
+    "m3_preference_loss": ([_P] * 4 + [ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double] + [_P] * 3 +
                            [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
-    "m3_token_grad": ([_P] * 6 + [ctypes.c_double, ctypes.c_int64, ctypes.c_int, _P, ctypes.c_void_p], ctypes.c_int),
+    "m3_preference_loss_grad": ([_P] * 4 + [ctypes.c_double, ctypes.c_int64, _P, ctypes.c_void_p, ctypes.c_size_t,
+                                           ctypes.c_void_p], ctypes.c_int),
     "m3_clip_grads_workspace_size": ([ctypes.c_int64], ctypes.c_size_t),
     "m3_clip_grads": ([ctypes.c_int64] + [ctypes.c_void_p] * 5 + [ctypes.c_int, ctypes.c_double, ctypes.c_double, _P,
                        ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
@@ -147,6 +152,12 @@ def tensor(t):
     return m
 
 
+_PADS = tuple((0,) * (MAX_DIMS - n) for n in range(MAX_DIMS + 1))
+_RECS = [struct.Struct("=" + "qii" + "q" * (2 * MAX_DIMS))]
+for _n in range(2, 25):
+    _RECS.append(struct.Struct("=" + ("qii" + "q" * (2 * MAX_DIMS)) * _n))
+
+
 class Packed:
     """m3_tensor records of several tensors in one buffer (built with struct, which is
     several times cheaper than filling ctypes structures). ``ptrs[i]`` is the address
@@ -156,29 +167,67 @@ class Packed:
     __slots__ = ("buf", "ptrs")
 
     def __init__(self, ts):
-        n = len(ts)
-        self.buf = ctypes.create_string_buffer(_REC.size * n)
-        base = ctypes.addressof(self.buf)
+        vals = []
         ptrs = []
-        for i, t in enumerate(ts):
+        n = 0
+        for t in ts:
             if t is None:
                 ptrs.append(None)
                 continue
             code = _DTYPE_CODE.get(t.dtype)
             if code is None:
                 raise TypeError(f"dtype {t.dtype} is not supported by libmamba3_b200")
-            nd = t.dim()
+            shape = t.shape
+            nd = len(shape)
             if nd > MAX_DIMS:
                 raise ValueError("tensor has too many dimensions for the C ABI")
-            pad = (0,) * (MAX_DIMS - nd)
-            ptr = t.data_ptr() or (1 if t.numel() == 0 else 0)
-            _REC.pack_into(self.buf, _REC.size * i, ptr, code, nd, *t.shape, *pad, *t.stride(), *pad)
-            ptrs.append(base + _REC.size * i)
+            pad = _PADS[nd]
+            vals += (t.data_ptr() or (1 if t.numel() == 0 else 0), code, nd, *shape, *pad, *t.stride(), *pad)
+            ptrs.append(n)
+            n += _REC.size
+        if n:
+            self.buf = _RECS[n // _REC.size - 1].pack(*vals)
+            base = address(self.buf)
+            ptrs = [None if p is None else base + p for p in ptrs]
+        else:
+            self.buf = None
         self.ptrs = ptrs
 
 
 def pack(*ts):
     return Packed(ts)
+
+
+class Records:
+    """Records whose fields the caller knows already (an entry point with a dozen operands of
+    one shape would otherwise spend more time on packing than on its launches): ``vals`` holds
+    rec2 / rec3 / NO_RECORD tuples one after the other. ``at(i)`` is the address of record i."""
+
+    __slots__ = ("buf", "base")
+
+    def __init__(self, vals):
+        self.buf = _RECS[len(vals) // 15 - 1].pack(*vals)
+        self.base = address(self.buf)
+
+    def at(self, i):
+        return self.base + _REC.size * i
+
+
+NO_RECORD = (0,) * 15  # data NULL: an absent optional argument
+
+
+def rec2(t, code, a, b):
+    """The record of a two-dimensional (a, b) tensor of dtype ``code``."""
+    return (t.data_ptr() or 1, code, 2, a, b, 0, 0, 0, 0, *t.stride(), 0, 0, 0, 0)
+
+
+def rec3(t, code, a, b, c):
+    return (t.data_ptr() or 1, code, 3, a, b, c, 0, 0, 0, *t.stride(), 0, 0, 0)
+
+
+def rec0(ptr, code):
+    """The record of one value at an address."""
+    return (ptr, code, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
 def address(b):
@@ -196,8 +245,27 @@ def check(rc, what):
         raise RuntimeError(f"{what} failed ({_STATUS.get(rc, rc)}): {msg}")
 
 
+# the current stream's handle as an integer: the public Stream object costs as much as a launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream_ptr(device):
+    """Handle of the current stream of a CUDA device, as an integer."""
+    if _raw_stream is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
+
+
 def stream_of(t):
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    return ctypes.c_void_p(stream_ptr(t.device))
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(device):
+    """The context of a call on ``device``: the switch to it, or nothing where it is current."""
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def device_timeouts(reset=False, device=None):

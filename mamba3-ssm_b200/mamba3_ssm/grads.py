@@ -94,10 +94,10 @@ def clip_grads_(grads, max_norm, norm_type=2.0, *, scale=1.0, out=None):
     a = L.pack(norm)
     base = L.address(tables)
     obase = L.address(out_tables) if out_tables is not None else None
-    with torch.cuda.device(dev):
+    with L.on_device(dev):
         rc = lib.m3_clip_grads(n, base, base + 8 * n, base + 16 * n, obase, obase + 8 * n if obase else None,
                                int(norm_type == math.inf), max_norm, scale, a.ptrs[0], ws.data_ptr(), ws.numel(),
-                               L.stream_of(norm))
+                               L.stream_ptr(dev))
     L.check(rc, "m3_clip_grads")
     if out is not None or scale != 1.0 or max_norm != math.inf:
         torch.autograd.graph.increment_version(out if out is not None else grads)

@@ -49,21 +49,23 @@ class PreferenceLoss(NamedTuple):
 def _rows(name, logits, tokens):
     """Logits as (batch, length, V) and tokens as (batch, length), without a copy where the
     strides allow."""
-    _require_cuda(name, logits, tokens)
+    if not (logits.is_cuda and tokens.is_cuda):
+        _require_cuda(name, logits, tokens)
     if logits.dtype not in _LOGIT_DTYPES:
         raise TypeError(f"{name}: logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
+    shape = tokens.shape
+    if logits.dim() < 1 or logits.shape[:-1] != shape:
         raise ValueError(f"{name}: logits (..., V) and tokens (...) expected, got {tuple(logits.shape)} and "
-                         f"{tuple(tokens.shape)}")
+                         f"{tuple(shape)}")
     if logits.shape[-1] == 0:
         raise ValueError(f"{name}: empty vocabulary")
-    if tokens.dtype != torch.int64:
+    if tokens.dtype is not torch.int64:
         if tokens.dtype not in (torch.int32, torch.int16, torch.uint8):
             raise TypeError(f"{name}: tokens must be integers, got {tokens.dtype}")
         tokens = tokens.long()
-    if tokens.device != logits.device:
+    if tokens.get_device() != logits.get_device():
         raise RuntimeError(f"{name}: tokens are on {tokens.device}, logits on {logits.device}")
-    n = tokens.dim()
+    n = len(shape)
     if n < 2:
         logits, tokens = logits.reshape(1, -1, logits.shape[-1]), tokens.reshape(1, -1)
     elif n > 2:
@@ -78,20 +80,21 @@ def _per_token(name, what, v, logits, tokens, shape, dtype=torch.float32):
         return None
     if not isinstance(v, torch.Tensor):
         raise TypeError(f"{name}: {what} must be a tensor")
-    if v.device != logits.device:
+    if v.get_device() != logits.get_device():
         raise RuntimeError(f"{name}: {what} is on {v.device}, logits on {logits.device}")
-    v = v.detach()
-    if dtype is torch.bool:
-        v = v if v.dtype in (torch.bool, torch.uint8) else v != 0
-    elif v.dtype != dtype:
-        v = v.to(dtype)
+    if v.dtype is not dtype:
+        v = v.detach()
+        if dtype is not torch.bool:
+            v = v.to(dtype)
+        elif v.dtype is not torch.uint8:
+            v = v != 0
     if v.shape != shape:
         try:
             v = v.expand(shape)
         except RuntimeError:
             raise ValueError(f"{name}: {what} of shape {tuple(v.shape)} does not broadcast to the tokens' "
                              f"{tuple(shape)}") from None
-    if v.dim() == 2:
+    if len(shape) == 2:
         return v
     return v.reshape(tokens.shape)
 
@@ -108,116 +111,159 @@ def _like_rows(logits):
     return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
 
 
-def _token_grad(logits, tokens, mask, stats, coef, up, temperature, ignore_index, dlogits=None):
-    """dlogits = up * coef / temperature * (one-hot - softmax) on m3_token_grad. A given
-    ``dlogits`` holds that for up = 1 already and is kept where up is 1."""
-    keep = dlogits is not None
-    if not keep:
-        dlogits = _like_rows(logits)
-    lib = L.load()
-    a = L.pack(logits, tokens, mask, stats, coef, up, dlogits)
-    with torch.cuda.device(logits.device):
-        L.check(lib.m3_token_grad(*a.ptrs[:6], temperature, ignore_index, int(keep), a.ptrs[6], L.stream_of(logits)),
-                "m3_token_grad")
-    return dlogits
-
-
-def _f32(logits, *shape):
-    return torch.empty(shape, dtype=torch.float32, device=logits.device)
-
-
 def _wants_grad(logits):
     return torch.is_grad_enabled() and logits.requires_grad
 
 
-def _workspace(logits, nbytes):
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=logits.device)
+def _records(logits, tokens, *per_token):
+    """The records of logits, tokens and optional operands of the tokens' shape: a mask first,
+    then fp32."""
+    B, T, V = logits.shape
+    vals = [*L.rec3(logits, L._DTYPE_CODE[logits.dtype], B, T, V), *L.rec2(tokens, L.M3_INT64, B, T)]
+    code = L.M3_UINT8
+    for v in per_token:
+        vals += L.NO_RECORD if v is None else L.rec2(v, code, B, T)
+        code = L.M3_FLOAT32
+    return vals
 
 
+# The functions take the logits and one tuple of everything else, none of which has a gradient.
+# What a user could change between forward and backward (logits, tokens, mask) is saved through
+# autograd, which notices it; what is made here is held by the context.
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, mask, temperature, ignore_index, need):
-        lib = L.load()
-        logp = _f32(logits, *tokens.shape)
-        stats = _f32(logits, *tokens.shape, 2) if need else None
-        a = L.pack(logits, tokens, mask, logp, stats)
-        with torch.cuda.device(logits.device):
-            L.check(lib.m3_token_logprobs(*a.ptrs[:3], temperature, ignore_index, *a.ptrs[3:], L.stream_of(logits)),
-                    "m3_token_logprobs")
+    def forward(ctx, logits, rest):
+        tokens, mask, temperature, ignore_index, need = rest
+        B, T = tokens.shape
+        dev = logits.device
+        logp = torch.empty((B, T), dtype=torch.float32, device=dev)
+        stats = torch.empty((B, T, 2), dtype=torch.float32, device=dev) if need else None
+        vals = _records(logits, tokens, mask, logp)
+        vals += L.rec3(stats, L.M3_FLOAT32, B, T, 2) if need else L.NO_RECORD
+        a = L.Records(vals)
+        with L.on_device(dev):
+            L.check(L.load().m3_token_logprobs(a.at(0), a.at(1), a.at(2), temperature, ignore_index, a.at(3), a.at(4),
+                                               L.stream_ptr(dev)), "m3_token_logprobs")
         if need:
-            ctx.save_for_backward(logits, tokens, mask, stats)
-            ctx.args = (temperature, ignore_index)
+            ctx.save_for_backward(logits, tokens, mask)
+            ctx.held = (stats, temperature, ignore_index)
         return logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogp):
-        logits, tokens, mask, stats = ctx.saved_tensors
-        return (_token_grad(logits, tokens, mask, stats, dlogp.float(), None, *ctx.args),) + (None,) * 5
+        logits, tokens, mask = ctx.saved_tensors
+        stats, temperature, ignore_index = ctx.held
+        dlogits = _like_rows(logits)
+        a = L.pack(logits, tokens, mask, stats, dlogp.float(), dlogits)
+        dev = logits.device
+        with L.on_device(dev):
+            L.check(L.load().m3_token_logprobs_grad(*a.ptrs[:5], temperature, ignore_index, a.ptrs[5],
+                                                    L.stream_ptr(dev)), "m3_token_logprobs_grad")
+        return dlogits, None
+
+
+def _grad_records(logits, tokens, mask, up, dlogits):
+    vals = _records(logits, tokens, mask)
+    up = up if up.dtype is torch.float32 else up.float()
+    B, T, V = logits.shape
+    vals += L.rec0(up.data_ptr(), L.M3_FLOAT32)
+    vals += L.rec3(dlogits, L._DTYPE_CODE[logits.dtype], B, T, V)
+    return L.Records(vals), up
 
 
 class _PolicyLossFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, mask, old, adv, ref, temperature, ignore_index, clip_low, clip_high, kl_coef,
-                by_sequence, need):
+    def forward(ctx, logits, rest):
+        tokens, mask, old, adv, ref, temperature, ignore_index, clip_low, clip_high, kl_coef, by_sequence, need = rest
         lib = L.load()
-        B, T = tokens.shape
-        loss, kl, clipped = _f32(logits), _f32(logits), _f32(logits)
-        logp = _f32(logits, B, T)
-        stats = coef = dlogits = None
+        B, T, V = logits.shape
+        dev = logits.device
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        means = torch.empty((2,), dtype=torch.float32, device=dev)  # KL, share of clipped positions
+        logp = torch.empty((B, T), dtype=torch.float32, device=dev)
+        # the gradient for an upstream gradient of 1, while each row is at hand; backward forms it
+        # again only where the upstream gradient is another
+        dlogits = _like_rows(logits) if need else None
+        nbytes = lib.m3_policy_loss_workspace_size(B, T)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        f32, m = L.M3_FLOAT32, means.data_ptr()
+        vals = _records(logits, tokens, mask, old, adv, ref, logp)
+        vals += L.rec0(loss.data_ptr(), f32)
+        vals += L.rec0(m, f32)
+        vals += L.rec0(m + 4, f32)
+        vals += L.rec3(dlogits, L._DTYPE_CODE[logits.dtype], B, T, V) if need else L.NO_RECORD
+        a = L.Records(vals)
+        with L.on_device(dev):
+            L.check(lib.m3_policy_loss(a.at(0), a.at(1), a.at(2), a.at(3), a.at(4), a.at(5), temperature, ignore_index,
+                                       clip_low, clip_high, kl_coef, by_sequence, a.at(7), a.at(8), a.at(9), a.at(6),
+                                       a.at(10), ws.data_ptr(), nbytes, L.stream_ptr(dev)), "m3_policy_loss")
         if need:
-            # the gradient for an upstream gradient of 1, while each row is at hand; backward
-            # forms it again only where the upstream gradient is another
-            stats, coef, dlogits = _f32(logits, B, T, 2), _f32(logits, B, T), _like_rows(logits)
-        ws = _workspace(logits, lib.m3_policy_loss_workspace_size(B, T))
-        a = L.pack(logits, tokens, mask, old, adv, ref, loss, kl, clipped, logp, stats, coef, dlogits)
-        with torch.cuda.device(logits.device):
-            L.check(lib.m3_policy_loss(*a.ptrs[:6], temperature, ignore_index, clip_low, clip_high, kl_coef,
-                                       int(by_sequence), *a.ptrs[6:], ws.data_ptr(), ws.numel(), L.stream_of(logits)),
-                    "m3_policy_loss")
-        if need:
-            ctx.save_for_backward(logits, tokens, mask, stats, coef)
-            ctx.args = (temperature, ignore_index)
+            ctx.save_for_backward(logits, tokens, mask)
+            ctx.held = (ws, temperature, ignore_index)
             ctx.dlogits = dlogits
-        ctx.mark_non_differentiable(logp, kl, clipped)
-        return loss, logp, kl, clipped
+        ctx.mark_non_differentiable(logp, means)
+        return loss, logp, means
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, up, _dlogp, _dkl, _dclipped):
-        logits, tokens, mask, stats, coef = ctx.saved_tensors
+    def backward(ctx, up, _dlogp, _dmeans):
+        logits, tokens, mask = ctx.saved_tensors
+        ws, temperature, ignore_index = ctx.held
         # handed out once: what receives it may write to it
         dlogits, ctx.dlogits = ctx.dlogits, None
-        d = _token_grad(logits, tokens, mask, stats, coef, up.float(), *ctx.args, dlogits=dlogits)
-        return (d,) + (None,) * 12
+        keep = dlogits is not None
+        if not keep:
+            dlogits = _like_rows(logits)
+        a, up = _grad_records(logits, tokens, mask, up, dlogits)
+        dev = logits.device
+        with L.on_device(dev):
+            L.check(L.load().m3_policy_loss_grad(a.at(0), a.at(1), a.at(2), a.at(3), temperature, ignore_index, keep,
+                                                 a.at(4), ws.data_ptr(), ws.numel(), L.stream_ptr(dev)),
+                    "m3_policy_loss_grad")
+        return dlogits, None
 
 
 class _PreferenceLossFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, mask, ref, temperature, ignore_index, beta, label_smoothing, need):
+    def forward(ctx, logits, rest):
+        tokens, mask, ref, temperature, ignore_index, beta, label_smoothing, need = rest
         lib = L.load()
         B, T = tokens.shape
-        loss, rewards, coef = _f32(logits), _f32(logits, B), _f32(logits, B)
-        logp = _f32(logits, B, T)
-        stats = _f32(logits, B, T, 2) if need else None
-        ws = _workspace(logits, lib.m3_preference_loss_workspace_size(B, T))
-        a = L.pack(logits, tokens, mask, ref, loss, rewards, logp, stats, coef)
-        with torch.cuda.device(logits.device):
-            L.check(lib.m3_preference_loss(*a.ptrs[:4], temperature, ignore_index, beta, label_smoothing, *a.ptrs[4:],
-                                           ws.data_ptr(), ws.numel(), L.stream_of(logits)), "m3_preference_loss")
+        dev = logits.device
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        rewards = torch.empty((B,), dtype=torch.float32, device=dev)
+        logp = torch.empty((B, T), dtype=torch.float32, device=dev)
+        nbytes = lib.m3_preference_loss_workspace_size(B, T)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        f32 = L.M3_FLOAT32
+        vals = _records(logits, tokens, mask, ref, logp)
+        vals += L.rec0(loss.data_ptr(), f32)
+        vals += (rewards.data_ptr(), f32, 1, B, 0, 0, 0, 0, 0, 1, 0, 0, 0, 0, 0)
+        a = L.Records(vals)
+        with L.on_device(dev):
+            L.check(lib.m3_preference_loss(a.at(0), a.at(1), a.at(2), a.at(3), temperature, ignore_index, beta,
+                                           label_smoothing, a.at(5), a.at(6), a.at(4), ws.data_ptr(), nbytes,
+                                           L.stream_ptr(dev)), "m3_preference_loss")
         if need:
-            ctx.save_for_backward(logits, tokens, mask, stats, coef)
-            ctx.args = (temperature, ignore_index)
+            ctx.save_for_backward(logits, tokens, mask)
+            ctx.held = (ws, temperature, ignore_index)
         ctx.mark_non_differentiable(rewards, logp)
         return loss, rewards, logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, up, _drewards, _dlogp):
-        logits, tokens, mask, stats, coef = ctx.saved_tensors
-        d = _token_grad(logits, tokens, mask, stats, coef.unsqueeze(1).expand(tokens.shape), up.float(),
-                        *ctx.args)
-        return (d,) + (None,) * 8
+        logits, tokens, mask = ctx.saved_tensors
+        ws, temperature, ignore_index = ctx.held
+        dlogits = _like_rows(logits)
+        a, up = _grad_records(logits, tokens, mask, up, dlogits)
+        dev = logits.device
+        with L.on_device(dev):
+            L.check(L.load().m3_preference_loss_grad(a.at(0), a.at(1), a.at(2), a.at(3), temperature, ignore_index,
+                                                     a.at(4), ws.data_ptr(), ws.numel(), L.stream_ptr(dev)),
+                    "m3_preference_loss_grad")
+        return dlogits, None
 
 
 def token_logprobs(logits, tokens, *, mask=None, temperature=1.0, ignore_index=-100):
@@ -226,7 +272,8 @@ def token_logprobs(logits, tokens, *, mask=None, temperature=1.0, ignore_index=-
     Differentiable by the logits; without the (..., V) tensor of all log-probabilities."""
     x, t = _rows("token_logprobs", logits, tokens)
     m = _per_token("token_logprobs", "mask", mask, x, t, tokens.shape, torch.bool)
-    return _TokenLogprobsFn.apply(x, t, m, float(temperature), int(ignore_index), _wants_grad(x)).reshape(tokens.shape)
+    logp = _TokenLogprobsFn.apply(x, (t, m, float(temperature), int(ignore_index), _wants_grad(x)))
+    return logp if logp.shape == tokens.shape else logp.reshape(tokens.shape)
 
 
 def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, mask=None, clip_low=0.2,
@@ -254,10 +301,11 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
     old = _per_token(name, "old_logprobs", old_logprobs, x, t, tokens.shape)
     adv = _per_token(name, "advantages", advantages, x, t, tokens.shape)
     ref = _per_token(name, "ref_logprobs", ref_logprobs, x, t, tokens.shape)
-    loss, logp, kl, clipped = _PolicyLossFn.apply(
-        x, t, m, old, adv, ref, float(temperature), int(ignore_index), float(clip_low),
-        float(clip_low if clip_high is None else clip_high), float(kl_coef), reduction == "sequence", _wants_grad(x))
-    return PolicyLoss(loss, logp.reshape(tokens.shape), kl, clipped)
+    loss, logp, means = _PolicyLossFn.apply(
+        x, (t, m, old, adv, ref, float(temperature), int(ignore_index), float(clip_low),
+            float(clip_low if clip_high is None else clip_high), float(kl_coef), int(reduction == "sequence"),
+            _wants_grad(x)))
+    return PolicyLoss(loss, logp if logp.shape == tokens.shape else logp.reshape(tokens.shape), *means.unbind(0))
 
 
 def preference_loss(logits, tokens, ref_logprobs=None, *, mask=None, beta=0.1, label_smoothing=0.0, temperature=1.0,
@@ -277,5 +325,5 @@ def preference_loss(logits, tokens, ref_logprobs=None, *, mask=None, beta=0.1, l
     x, t = _rows(name, logits, tokens)
     m = _per_token(name, "mask", mask, x, t, tokens.shape, torch.bool)
     ref = _per_token(name, "ref_logprobs", ref_logprobs, x, t, tokens.shape)
-    return PreferenceLoss(*_PreferenceLossFn.apply(x, t, m, ref, float(temperature), int(ignore_index), float(beta),
-                                                   float(label_smoothing), _wants_grad(x)))
+    return PreferenceLoss(*_PreferenceLossFn.apply(
+        x, (t, m, ref, float(temperature), int(ignore_index), float(beta), float(label_smoothing), _wants_grad(x))))
