@@ -148,40 +148,38 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
   if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
+// `n` gradients, scaled. A thread moves as many elements at once as make one 16-byte store, so
+// that the stores of a warp are one run of memory also where a 16-bit gradient becomes an fp32
+// one (its loads are then 8 bytes wide).
 template <typename T, typename O>
 __device__ __forceinline__ void scale_part(const T* g, O* o, int n, float f) {
-  constexpr int N = Vec<T>::N, M = Vec<O>::N < N ? Vec<O>::N : N;  // M elements make one store
-  const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / sizeof(T)));
-  const int nv = (n - head) / N;
-  const bool same = (reinterpret_cast<uintptr_t>(o + head) & 15) == 0;
-  const Vec<T>* v = reinterpret_cast<const Vec<T>*>(g + head);
-  auto put = [&](int j, const Vec<T>& x) {
-    O* at = o + head + (int64_t)j * N;
-    if (same) {
+  constexpr int M = 16 / sizeof(O), kBytes = M * sizeof(T);
+  struct alignas(kBytes) In { T e[M]; };
+  struct alignas(16) Out { O e[M]; };
+  const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(o) & 15)) & 15) / sizeof(O)));
+  const bool same = (reinterpret_cast<uintptr_t>(g + head) & (kBytes - 1)) == 0;
+  const int nv = same ? (n - head) / M : 0;
+  const In* v = reinterpret_cast<const In*>(g + head);
+  Out* w = reinterpret_cast<Out*>(o + head);
+  auto put = [&](int j, const In& x) {
+    Out y;
 #pragma unroll
-      for (int k = 0; k < N; k += M) {
-        Vec<O> y;
-#pragma unroll
-        for (int q = 0; q < M; ++q) y.e[q] = from_f32<O>(to_f32(x.e[k + q]) * f);
-        *reinterpret_cast<Vec<O>*>(at + k) = y;
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < N; ++k) at[k] = from_f32<O>(to_f32(x.e[k]) * f);
-    }
+    for (int k = 0; k < M; ++k) y.e[k] = from_f32<O>(to_f32(x.e[k]) * f);
+    __stcs(reinterpret_cast<float4*>(w + j), *reinterpret_cast<const float4*>(&y));  // not needed again here
   };
-  constexpr int U = 4;
+  constexpr int U = kBytes == 16 ? 4 : 8;
   int j = threadIdx.x;
   for (; j + (U - 1) * kThreads < nv; j += U * kThreads) {
-    Vec<T> x[U];
+    In x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) x[u] = v[j + u * kThreads];
 #pragma unroll
     for (int u = 0; u < U; ++u) put(j + u * kThreads, x[u]);
   }
   for (; j < nv; j += kThreads) put(j, v[j]);
+  // before the vectors and behind them (everything, where the two sides' boundaries differ)
   for (int i = threadIdx.x; i < head; i += kThreads) o[i] = from_f32<O>(to_f32(g[i]) * f);
-  for (int i = head + nv * N + threadIdx.x; i < n; i += kThreads) o[i] = from_f32<O>(to_f32(g[i]) * f);
+  for (int i = head + nv * M + threadIdx.x; i < n; i += kThreads) o[i] = from_f32<O>(to_f32(g[i]) * f);
 }
 
 template <int K, bool LARGEST>

@@ -26,7 +26,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 #include "m3_common.cuh"
@@ -611,8 +610,8 @@ __device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a
 // One cluster of CTAs (of one CTA where there are rows enough) per row. A policy gradient of
 // rows too long for token_grad_rows_kernel is written from a second reading.
 template <typename T, bool POLICY, int NT>
-__global__ void __launch_bounds__(NT, POLICY ? 1024 / NT : 1536 / NT) token_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o) {
-  constexpr int U = 4;  // loads in flight per thread
+__global__ void __launch_bounds__(NT, 1024 / NT) token_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o) {
+  constexpr int U = 8;  // loads in flight per thread
   __shared__ RowShared sh;
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
@@ -748,7 +747,7 @@ __device__ __forceinline__ void send(float* slot, uint64_t* met, int to, float v
 }
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT + 32, 1024 / NT)
+__global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
     token_grad_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o, int pieces) {
   constexpr int W = NT / 32, kPiece = kPieceVecs * NT;
   extern __shared__ __align__(16) uint4 kept_raw[];
@@ -1195,8 +1194,7 @@ __global__ void __launch_bounds__(kGradThreads, 4)
       fill<T>(out, part == 0 ? 0 : c.head + v0 * N, part == parts - 1 ? p.V : c.head + v1 * N, tid, G, from_f32<T>(0.f));
       continue;
     }
-    const GradRow gr = grad_row(base_at(st.x, p.c_hi), g, st.y, pos.known ? (int)pos.tok : -1,
-                                pos.known ? to_f32(row[pos.tok]) : 0.f);
+    GradRow gr = grad_row(base_at(st.x, p.c_hi), g, st.y, pos.known ? (int)pos.tok : -1, 0.f);
     const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + c.head);
     uint4* const to = reinterpret_cast<uint4*>(out + c.head);
     const bool same = same_boundary(out, c);
@@ -1219,6 +1217,7 @@ __global__ void __launch_bounds__(kGradThreads, 4)
       }
     }
     for (; j < v1; j += G) put_grad(rv[j], j, out, c, gr, same, p.c_hi, p.c_lo);
+    if (gr.tok >= 0) gr.at = to_f32(row[gr.tok]);  // a row's loads need not wait for it
     put_token(out, c, gr, v0, v1, tid, G, p.c_hi, p.c_lo);
     if (part == 0) put_ends(row, out, p.V, c, gr, tid, G, p.c_hi, p.c_lo);
   }
@@ -1237,15 +1236,13 @@ int plan_rows(const TokenRows& p, int64_t elem, bool policy, RowPlan* out) {
   int C = 1;
   // few rows: split each so that the device is filled, down to parts of 16 KB
   while (C < 8 && p.R * C * 2 <= 2 * (int64_t)sms && bytes / (2 * C) >= 16384) C *= 2;
-  // the same with and without a gradient, so that both give the same bits
-  static const int64_t place = getenv("M3_PLACE") ? atoi(getenv("M3_PLACE")) * 1024 : kPlaceBytes;
-  static const int vt = getenv("M3_VT") ? atoi(getenv("M3_VT")) : 52;
+  // a place for each part, with and without a gradient, so that both give the same bits
   if (policy)
-    while (C < 8 && bytes / C > place) C *= 2;
+    while (C < 8 && bytes / C > kPlaceBytes) C *= 2;
   out->C = C;
-  static const int fw = getenv("M3_FW") ? atoi(getenv("M3_FW")) : 256;
-  out->threads = bytes / C <= 16 * 1024 ? 128 : bytes / C <= vt * 1024 || !policy ? 256 : 512;
-  if (!policy && out->threads == 256) out->threads = fw;
+  // small CTAs stream best (1200 rows of 100 KB: 24.9 us with 128 threads, 25.4 with 256, 31.7
+  // with 512); a CTA that keeps its part needs warps enough for the whole of it
+  out->threads = !policy || bytes / C <= 16 * 1024 ? 128 : bytes / C <= 52 * 1024 ? 256 : 512;
   out->slot_vecs = bytes / C <= kPlaceBytes ? (int)(bytes / C / 16 + 2) : 0;
   return M3_OK;
 }
@@ -1328,9 +1325,11 @@ int launch_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, cons
     }
   }
   if (p.R > INT32_MAX / plan.C) return fail(M3_ERR_UNSUPPORTED, "token rows: too many positions");
-  if (plan.threads == 128) return launch_clusters(token_rows_kernel<T, POLICY, 128>, plan, p.R, nullptr, 0, s, p, a, w, o);
-  if (plan.threads == 256) return launch_clusters(token_rows_kernel<T, POLICY, 256>, plan, p.R, nullptr, 0, s, p, a, w, o);
-  return launch_clusters(token_rows_kernel<T, POLICY, 512>, plan, p.R, nullptr, 0, s, p, a, w, o);
+  if constexpr (POLICY) {
+    if (plan.threads == 512) return launch_clusters(token_rows_kernel<T, POLICY, 512>, plan, p.R, nullptr, 0, s, p, a, w, o);
+    if (plan.threads == 256) return launch_clusters(token_rows_kernel<T, POLICY, 256>, plan, p.R, nullptr, 0, s, p, a, w, o);
+  }
+  return launch_clusters(token_rows_kernel<T, POLICY, 128>, plan, p.R, nullptr, 0, s, p, a, w, o);
 }
 
 template <bool POLICY>
@@ -1419,19 +1418,18 @@ static int launch_grad(const TokenRows& p, const float2* stats, Map2<const float
   M3_TRY(device_sm_count(&sms));
   const int64_t bytes = (int64_t)p.V * (int64_t)sizeof(T), ctas = (int64_t)sms * 4;
   T* const d = static_cast<T*>(dlogits);
+  // where the kernel may find nothing to do its grid is small, else as large as the work
   if (bytes <= 8192) {  // a warp per row
-    const int units = (int)p.R;
-    const unsigned grid = (unsigned)std::min<int64_t>((units + 7) / 8, ctas);
-    token_grad_kernel<T, 32><<<grid, kGradThreads, 0, s>>>(p, stats, coef, up, keep_if_one, d, dsb, dst, 1, units);
+    const int64_t need = (p.R + kGradThreads / 32 - 1) / (kGradThreads / 32);
+    token_grad_kernel<T, 32><<<(unsigned)(keep_if_one ? std::min(need, ctas) : need), kGradThreads, 0, s>>>(
+        p, stats, coef, up, keep_if_one, d, dsb, dst, 1, (int)p.R);
   } else {
-    // a CTA per row, or per part of a row where the rows do not fill the device (parts of 8 KB
-    // or more) or where there are few for each CTA, whose last ones would then be uneven
+    // a CTA per row, or per part of a row (16 KB or more) where there are few rows
     int64_t parts = 1;
-    while (p.R * parts < 4 * ctas && bytes / (2 * parts) >= 8192) parts *= 2;
-    const int units = (int)(p.R * parts);
-    const unsigned grid = (unsigned)std::min<int64_t>(units, ctas);
-    token_grad_kernel<T, kGradThreads><<<grid, kGradThreads, 0, s>>>(p, stats, coef, up, keep_if_one, d, dsb, dst,
-                                                                     (int)parts, units);
+    while (p.R * parts < 4 * ctas && bytes / (2 * parts) >= 16384) parts *= 2;
+    const int64_t units = p.R * parts;
+    token_grad_kernel<T, kGradThreads><<<(unsigned)(keep_if_one ? std::min(units, ctas) : units), kGradThreads, 0, s>>>(
+        p, stats, coef, up, keep_if_one, d, dsb, dst, (int)parts, (int)units);
   }
   return check_launch("token_grad_kernel");
 }

@@ -90,13 +90,14 @@ def clip_grads_(grads, max_norm, norm_type=2.0, *, scale=1.0, out=None):
     out_tables = struct.pack(f"={n}q{n}i", *outs, *out_codes) if outs is not None else None
     lib = L.load()
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(lib.m3_clip_grads_workspace_size(n), dtype=torch.uint8, device=dev)
-    a = L.pack(norm)
+    nbytes = lib.m3_clip_grads_workspace_size(n)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    a = L.Records(L.rec0(norm.data_ptr(), L.M3_FLOAT32))
     base = L.address(tables)
     obase = L.address(out_tables) if out_tables is not None else None
     with L.on_device(dev):
         rc = lib.m3_clip_grads(n, base, base + 8 * n, base + 16 * n, obase, obase + 8 * n if obase else None,
-                               int(norm_type == math.inf), max_norm, scale, a.ptrs[0], ws.data_ptr(), ws.numel(),
+                               int(norm_type == math.inf), max_norm, scale, a.at(0), ws.data_ptr(), nbytes,
                                L.stream_ptr(dev))
     L.check(rc, "m3_clip_grads")
     if out is not None or scale != 1.0 or max_norm != math.inf:
