@@ -4,9 +4,10 @@
 //   logp = s l[tok] - log sum_v exp(s l[v]) = ln 2 (c (l[tok] - m) - log2 S),
 //   S = sum_v 2^(c (l[v] - m)),  m any value near max(l)
 //   d logp / d l[v] = s (1[v = tok] - 2^(c (l[v] - m)) / S)
-// m is the largest of the row's first elements: every warp finds the same one by itself, sums
-// of all warps (and CTAs) join by addition, and no element passes through a second rounding
-// exponential. Where S then leaves 2^-60 .. 2^100 the row is done again with its true maximum.
+// m is the largest of the row's first elements and the token's own (a likely one, in earnest):
+// every warp finds the same m by itself, sums of all warps (and CTAs) join by addition, and no
+// element passes through a second rounding exponential. Where S then leaves 2^-60 .. 2^100 the
+// row is done again with its true maximum.
 // c is held in two floats: one float's rounding (up to 3e-8 of c) would move every
 // log-probability of a sequence the same way, and the preference loss sums them.
 // The element work runs in 32 bits, what happens once a row (the logarithm, the ratio, the
@@ -183,7 +184,12 @@ __device__ __forceinline__ float vec_max(const Vec<T>& v) {
   for (int k = 1; k < Vec<T>::N; ++k) m = fmaxf(m, l[k]);
   return m;
 }
-__device__ __forceinline__ float warp_sum(float v) {
+// The type in which a row's partial sums are joined: a thread's own sum is of 32 bits, but what
+// is rounded here is a whole row's, and sums of log-probabilities (the rewards) add it up.
+template <bool POLICY>
+using Joined = std::conditional_t<POLICY, float, double>;
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v) {
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
   return v;
@@ -194,16 +200,22 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// log S. ex2.approx falls short by 5.1e-8 of its value on average (measured over its whole
-// range of fractions); all terms but the base's own, which is exact, carry that. The integer
-// part of the logarithm is scaled in 64 bits, so that the result is off by 3e-8 at most
-// instead of half a step of a value near 10 (5e-7).
+// log S. ex2.approx falls short by kExpShort of its value on average (measured for negative
+// exponents over the whole range of fractions; about 3e-8 too much for positive ones, which are
+// few); all terms but the base's own, which is exact, carry that. From a 32-bit
+// S the integer part of the logarithm is scaled in 64 bits, so that the result is off by 3e-8
+// at most instead of half a step of a value near 10 (5e-7).
+constexpr double kExpShort = 5.05e-8;
+__device__ __forceinline__ double log_sum(double S) {
+  if (!(S > 0.0 && S < INFINITY)) return (double)NAN;
+  return log(S) + (S > 1.0 ? kExpShort * ((S - 1.0) / S) : 0.0);
+}
 __device__ __forceinline__ double log_sum(float S) {
   if (!(S > 0.f && S < INFINITY)) return (double)NAN;
   int e;
   float m = frexpf(S, &e);  // 0.5 .. 1
   if (m < 0.75f) { m *= 2.f; --e; }
-  return (double)e * kLn2 + (double)log1pf(m - 1.f) + (S > 1.f ? 5.1e-8 * (double)((S - 1.f) / S) : 0.0);
+  return (double)e * kLn2 + (double)log1pf(m - 1.f) + (S > 1.f ? kExpShort * (double)((S - 1.f) / S) : 0.0);
 }
 
 // Whether a position counts, its token, and whether that token is one of the vocabulary.
@@ -507,7 +519,7 @@ __device__ __forceinline__ void skip_row(const RowOut& o, const PolicyWs& w, int
 template <bool POLICY>
 __device__ __forceinline__ GradRow finish_row(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o,
                                               const TokenOps& x, int64_t r, float at_token, int tok, const Base& base,
-                                              float S, bool lead) {
+                                              Joined<POLICY> S, bool lead) {
   // the token's exponent exactly as the sum's elements have theirs
   const double c = POLICY && !base.far ? (double)p.c_hi : (double)p.c_hi + (double)p.c_lo;
   const double at = base.far ? ((double)at_token - (double)base.m) * c : fma((double)at_token, c, (double)base.k);
@@ -521,7 +533,7 @@ __device__ __forceinline__ GradRow finish_row(const TokenRows& p, const PolicyAr
       if (o.coef) o.coef[r] = coef;
     }
   }
-  const float Sn = norm_sum<!POLICY>(S, base, p.c_lo);
+  const float Sn = norm_sum<!POLICY>((float)S, base, p.c_lo);
   if (lead) {
     o.logp[r] = (float)logp;
     if (o.logp64) o.logp64[r] = logp;
@@ -534,13 +546,14 @@ __device__ __forceinline__ GradRow finish_row(const TokenRows& p, const PolicyAr
 __device__ __forceinline__ bool in_range(float S) { return S > 8.673617e-19f && S < 1.2676506e30f; }  // 2^-60, 2^100
 
 // A row's sum and results by a cluster of CTAs: what the kernels below share.
+template <bool POLICY>
 struct RowShared {
-  float part[2][kRowWarps];  // the warps' sums, alternating between rows
+  Joined<POLICY> part[2][kRowWarps];  // the warps' sums, alternating between rows
   GradRow row[2];
   bool again[2];
 };
 
-// The base of a row from its first vectors (of all elements, where there is no vector).
+// The largest of a row's first vectors (of all elements, where there is no vector).
 template <typename T>
 __device__ __forceinline__ float first_max(const T* row, int V, const RowCut& c, int lane) {
   if (c.nv > 0) return lane < c.nv ? vec_max(reinterpret_cast<const Vec<T>*>(row + c.head)[lane]) : -INFINITY;
@@ -552,7 +565,7 @@ __device__ __forceinline__ float first_max(const T* row, int V, const RowCut& c,
 // alternates from row to row, so that a CTA can go on while another still reads its sums.
 template <typename T, bool POLICY, typename Get>
 __device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o,
-                                         RowShared& sh, int slot, const TokenOps& x, int64_t r, const T* row,
+                                         RowShared<POLICY>& sh, int slot, const TokenOps& x, int64_t r, const T* row,
                                          const RowCut& c, int n, Base base, float s, float at_token, int tok, Get get) {
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
@@ -561,16 +574,17 @@ __device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a
     if (C > 1) cl.sync();
     else __syncthreads();
   };
-  float* part = sh.part[slot];
-  s = warp_sum(s);
-  if (lane == 0) part[warp] = s;
+  using F = Joined<POLICY>;
+  F* part = sh.part[slot];
+  const F mine = warp_sum((F)s);
+  if (lane == 0) part[warp] = mine;
   meet();
   if (warp == 0) {
     // by CTA first: the order of token_grad_rows_kernel, for the same bits
-    float S = 0.f;
-    for (int k = 0; k < C; ++k) S += warp_sum(lane < W ? (C > 1 ? cl.map_shared_rank(part, k)[lane] : part[lane]) : 0.f);
+    F S = 0;
+    for (int k = 0; k < C; ++k) S += warp_sum(lane < W ? (C > 1 ? cl.map_shared_rank(part, k)[lane] : part[lane]) : F(0));
     if (lane == 0) {
-      sh.again[slot] = base.far || !in_range(S);
+      sh.again[slot] = base.far || !in_range((float)S);
       if (!sh.again[slot]) sh.row[slot] = finish_row<POLICY>(p, a, w, o, x, r, at_token, tok, base, S, rank == 0);
     }
   }
@@ -583,26 +597,26 @@ __device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a
       for (int i = c.tail0 + tid; i < p.V; i += nt) f(to_f32(row[i]));
     }
   };
-  auto all = [&](float v, bool largest) {
+  auto all = [&](F v, bool largest) {
     meet();  // the parts of the last sum have been read
     if (lane == 0) part[warp] = v;
     meet();
-    float y = largest ? -INFINITY : 0.f;
+    F y = largest ? -INFINITY : F(0);
     for (int i = 0; i < W * C; ++i) {
-      const float z = C > 1 ? cl.map_shared_rank(part, i / W)[i % W] : part[i];
-      y = largest ? fmaxf(y, z) : y + z;
+      const F z = C > 1 ? cl.map_shared_rank(part, i / W)[i % W] : part[i];
+      y = largest ? (z > y ? z : y) : y + z;
     }
     return y;
   };
   float mx = -INFINITY;
   for (int j = tid; j < n; j += nt) mx = fmaxf(mx, vec_max(get(j)));
   ends([&](float l) { mx = fmaxf(mx, l); });
-  base = base_at(all(warp_max(mx), true), p.c_hi);
+  base = base_at((float)all(warp_max(mx), true), p.c_hi);
   Sum s2{0.f, 0.f};
   for (int j = tid; j < n; j += nt) add_any<!POLICY>(s2, get(j), base, p.c_hi, p.c_lo);
   s = s2.total();
   ends([&](float l) { s += exp_one<!POLICY>(l, base, p.c_hi, p.c_lo); });
-  const float S = all(warp_sum(s), false);
+  const F S = all(warp_sum((F)s), false);
   if (tid == 0) sh.row[slot] = finish_row<POLICY>(p, a, w, o, x, r, at_token, tok, base, S, rank == 0);
   __syncthreads();
 }
@@ -612,7 +626,7 @@ __device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a
 template <typename T, bool POLICY, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) token_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o) {
   constexpr int U = 8;  // loads in flight per thread
-  __shared__ RowShared sh;
+  __shared__ RowShared<POLICY> sh;
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int64_t r = blockIdx.x / C;
@@ -633,14 +647,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_rows_kernel(TokenRows p, 
   const RowCut c = cut_row(row, p.V);
   const int v0 = (int)((int64_t)c.nv * rank / C), v1 = (int)((int64_t)c.nv * (rank + 1) / C), n = v1 - v0;
   const Vec<T>* mine = reinterpret_cast<const Vec<T>*>(row + c.head) + v0;
-  const float m = first_max(row, p.V, c, lane);
+  const float at_token = pos.known ? to_f32(row[pos.tok]) : NAN;
   TokenOps x{};
-  float at_token = 0.f;
-  if (tid == 0) {
-    at_token = pos.known ? to_f32(row[pos.tok]) : NAN;
-    if constexpr (POLICY) x = token_ops(a, w, b, t);
-  }
-  const Base base = base_at(warp_max(m), p.c_hi);
+  if constexpr (POLICY)
+    if (tid == 0) x = token_ops(a, w, b, t);
+  const Base base = base_at(fmaxf(warp_max(first_max(row, p.V, c, lane)), at_token), p.c_hi);
   Sum s2{0.f, 0.f};
   int j = tid;
   for (; j + (U - 1) * nt < n; j += U * nt) {
@@ -815,9 +826,8 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
       const bool known = tok >= 0 && tok < p.V;
       q.tok = known ? (int)tok : -1;
       q.x = token_ops(a, w, b, t);
-      const float m = first_max(q.row, p.V, q.c, lane);
       q.at_token = known ? to_f32(q.row[tok]) : NAN;
-      q.base = base_at(warp_max(m), p.c_hi);
+      q.base = base_at(fmaxf(warp_max(first_max(q.row, p.V, q.c, lane)), q.at_token), p.c_hi);
       if (lane == 0) {
         sh.info[slot] = q;
         sm100::mbar_arrive(&sh.info_full[slot]);
@@ -1030,7 +1040,7 @@ __global__ void __launch_bounds__(kShortThreads) token_short_rows_kernel(TokenRo
       if (lane + 32 * u < c.nv) add_vec<FAR, !POLICY>(s2, v[u], base, p.c_hi, p.c_lo);
     return s + s2.total();
   };
-  const float S = warp_sum(base.far ? sum(std::true_type{}) : sum(std::false_type{}));
+  const Joined<POLICY> S = warp_sum((Joined<POLICY>)(base.far ? sum(std::true_type{}) : sum(std::false_type{})));
   const GradRow gr =
       finish_row<POLICY>(p, a, w, o, x, r, at_token, pos.known ? (int)pos.tok : -1, base, S, lane == 0);
   if constexpr (POLICY) {
