@@ -1127,9 +1127,19 @@ int map2(const m3_tensor* t, const char* name, int dtype, const int64_t* bt, boo
     return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": unsupported dtype " + std::to_string(t->dtype));
   if (t->stride[0] < 0 || t->stride[1] < 0)
     return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": negative stride");
-  if (devcheck) M3_TRY(check_device_ptr(t->data, name));
+  if (devcheck) {
+    if (reinterpret_cast<uintptr_t>(t->data) % sizeof(T) != 0)
+      return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": address not aligned to its elements");
+    M3_TRY(check_device_ptr(t->data, name));
+  }
   *out = Map2<T>{static_cast<T*>(t->data), t->stride[0], t->stride[1]};
   return M3_OK;
+}
+
+// Vector and element accesses need addresses that are multiples of the element's size.
+int aligned(const m3_tensor* t, const char* name, size_t bytes) {
+  if (!present(t) || reinterpret_cast<uintptr_t>(t->data) % bytes == 0) return M3_OK;
+  return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": address not aligned to " + std::to_string(bytes) + " bytes");
 }
 
 // The rows that every token loss reads; *empty: there is no position.
@@ -1143,6 +1153,7 @@ int token_rows(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor
     return fail(M3_ERR_UNSUPPORTED, "logits: dimension too large");
   *empty = sh[0] * sh[1] == 0;
   M3_TRY(check(logits, "logits", 3, sh, kAnyFloat, false, false, !*empty));
+  if (!*empty) M3_TRY(aligned(logits, "logits", dtype_size(logits->dtype)));
   if (!(temperature > 1e-6 && temperature < 1e6))
     return fail(M3_ERR_INVALID_ARGUMENT, "temperature: expected a number between 1e-6 and 1e6");
   M3_TRY(map2(tokens, "tokens", M3_INT64, sh, false, !*empty, &p->tok));
@@ -1187,6 +1198,7 @@ int m3_token_logprobs(const m3_tensor* logits, const m3_tensor* tokens, const m3
   const int64_t bt[3] = {logits->shape[0], logits->shape[1], 2};
   M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
   M3_TRY(check(stats, "stats", 3, bt, kF32, true, true, !empty));
+  if (!empty) M3_TRY(aligned(stats, "stats", 8));
   if (empty) return M3_OK;
   return launch_token_logprobs(p, logits->dtype, fptr<float>(logprobs), fptr<float2>(stats),
                                reinterpret_cast<cudaStream_t>(stream));
@@ -1217,6 +1229,7 @@ int m3_policy_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_te
   M3_TRY(map2(ref_logprobs, "ref_logprobs", M3_FLOAT32, sh, true, !empty, &a.ref));
   M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
   M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, true, !empty));
+  if (!empty) M3_TRY(aligned(dlogits, "dlogits", dtype_size(logits->dtype)));
   M3_TRY(scalar_out(loss, "loss", false));
   M3_TRY(scalar_out(kl, "kl", false));
   M3_TRY(scalar_out(clip_fraction, "clip_fraction", false));
@@ -1274,6 +1287,7 @@ int loss_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor*
   M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
   const int64_t* sh = logits->shape;
   M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, false, !empty));
+  if (!empty) M3_TRY(aligned(dlogits, "dlogits", dtype_size(logits->dtype)));
   M3_TRY(scalar_out(up, "up", true));
   if (empty) return M3_OK;
   const size_t need = policy ? policy_workspace_bytes(sh[0], p.R) : preference_workspace_bytes(sh[0], p.R);
@@ -1310,8 +1324,10 @@ int m3_token_logprobs_grad(const m3_tensor* logits, const m3_tensor* tokens, con
   const int64_t bt[3] = {sh[0], sh[1], 2};
   Map2<const float> c;
   M3_TRY(check(stats, "stats", 3, bt, kF32, true, false, !empty));
+  if (!empty) M3_TRY(aligned(stats, "stats", 8));
   M3_TRY(map2(dlogprobs, "dlogprobs", M3_FLOAT32, sh, false, !empty, &c));
   M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, false, !empty));
+  if (!empty) M3_TRY(aligned(dlogits, "dlogits", dtype_size(logits->dtype)));
   if (empty) return M3_OK;
   return launch_token_grad(p, logits->dtype, fptr<const float2>(stats), c, nullptr, false, dlogits->data,
                            dlogits->stride[0], dlogits->stride[1], reinterpret_cast<cudaStream_t>(stream));
@@ -1331,6 +1347,7 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
   // what is written (and, with outs, what is read) as address ranges, to find overlaps
   struct Range { uintptr_t lo, hi; bool written; int64_t index; };
   const bool writes = outs || scale != 1.0 || !std::isinf(max_norm);
+  int64_t first = -1;  // tensor with elements
   std::vector<Range> ranges;
   if (writes) ranges.reserve((size_t)count * (outs ? 2 : 1));
   for (int64_t i = 0; i < count; ++i) {
@@ -1344,10 +1361,7 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
     const uintptr_t g = reinterpret_cast<uintptr_t>(grads[i]), o = outs ? reinterpret_cast<uintptr_t>(outs[i]) : g;
     const size_t gs = dtype_size(dtypes[i]), os = outs ? dtype_size(out_dtypes[i]) : gs;
     if (g % gs != 0 || o % os != 0) return fail(M3_ERR_INVALID_ARGUMENT, name("grads") + ": not aligned to its elements");
-    if (i == 0) {
-      M3_TRY(check_device_ptr(grads[0], "grads[0]"));
-      if (outs) M3_TRY(check_device_ptr(outs[0], "outs[0]"));
-    }
+    if (first < 0) first = i;
     if (!writes) continue;
     ranges.push_back(Range{o, o + os * (size_t)numel[i], true, i});
     if (outs && !(o == g && os == gs)) ranges.push_back(Range{g, g + gs * (size_t)numel[i], false, i});
@@ -1361,6 +1375,11 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
       return fail(M3_ERR_INVALID_ARGUMENT, "grads[" + std::to_string(r.index) + "]: shares memory with another tensor of the call");
     end_any = std::max(end_any, r.hi);
     if (r.written) end_written = std::max(end_written, r.hi);
+  }
+  // one address of each kind is looked up: hundreds would cost more than the launches
+  if (first >= 0) {
+    M3_TRY(check_device_ptr(grads[first], "grads"));
+    if (outs) M3_TRY(check_device_ptr(outs[first], "outs"));
   }
   M3_TRY(scalar_out(norm, "norm", false));
   if (count > 0) M3_TRY(workspace_ok(workspace, workspace_bytes, clip_grads_workspace_bytes(count), "clip_grads"));

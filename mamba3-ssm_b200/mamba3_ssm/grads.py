@@ -101,7 +101,8 @@ def clip_grads_(grads, max_norm, norm_type=2.0, *, scale=1.0, out=None):
                                L.stream_ptr(dev))
     L.check(rc, "m3_clip_grads")
     if out is not None or scale != 1.0 or max_norm != math.inf:
-        torch.autograd.graph.increment_version(out if out is not None else grads)
+        written = out if out is not None else grads
+        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
     return norm
 
 
