@@ -111,10 +111,6 @@ def _like_rows(logits):
     return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
 
 
-def _wants_grad(logits):
-    return torch.is_grad_enabled() and logits.requires_grad
-
-
 def _records(logits, tokens, *per_token):
     """The records of logits, tokens and optional operands of the tokens' shape: a mask first,
     then fp32."""
@@ -125,6 +121,15 @@ def _records(logits, tokens, *per_token):
         vals += L.NO_RECORD if v is None else L.rec2(v, code, B, T)
         code = L.M3_FLOAT32
     return vals
+
+
+def _apply(fn, logits, *rest):
+    """fn on logits that may need a gradient; where they do not, its forward alone (autograd's
+    bookkeeping would cost as much as a small call's launches)."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return fn.apply(logits, (*rest, True))
+    with torch.no_grad():
+        return fn.forward(None, logits, (*rest, False))
 
 
 # The functions take the logits and one tuple of everything else, none of which has a gradient.
@@ -202,7 +207,7 @@ class _PolicyLossFn(torch.autograd.Function):
             ctx.save_for_backward(logits, tokens, mask)
             ctx.held = (ws, temperature, ignore_index)
             ctx.dlogits = dlogits
-        ctx.mark_non_differentiable(logp, means)
+            ctx.mark_non_differentiable(logp, means)
         return loss, logp, means
 
     @staticmethod
@@ -248,7 +253,7 @@ class _PreferenceLossFn(torch.autograd.Function):
         if need:
             ctx.save_for_backward(logits, tokens, mask)
             ctx.held = (ws, temperature, ignore_index)
-        ctx.mark_non_differentiable(rewards, logp)
+            ctx.mark_non_differentiable(rewards, logp)
         return loss, rewards, logp
 
     @staticmethod
@@ -272,7 +277,7 @@ def token_logprobs(logits, tokens, *, mask=None, temperature=1.0, ignore_index=-
     Differentiable by the logits; without the (..., V) tensor of all log-probabilities."""
     x, t = _rows("token_logprobs", logits, tokens)
     m = _per_token("token_logprobs", "mask", mask, x, t, tokens.shape, torch.bool)
-    logp = _TokenLogprobsFn.apply(x, (t, m, float(temperature), int(ignore_index), _wants_grad(x)))
+    logp = _apply(_TokenLogprobsFn, x, t, m, float(temperature), int(ignore_index))
     return logp if logp.shape == tokens.shape else logp.reshape(tokens.shape)
 
 
@@ -301,10 +306,9 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
     old = _per_token(name, "old_logprobs", old_logprobs, x, t, tokens.shape)
     adv = _per_token(name, "advantages", advantages, x, t, tokens.shape)
     ref = _per_token(name, "ref_logprobs", ref_logprobs, x, t, tokens.shape)
-    loss, logp, means = _PolicyLossFn.apply(
-        x, (t, m, old, adv, ref, float(temperature), int(ignore_index), float(clip_low),
-            float(clip_low if clip_high is None else clip_high), float(kl_coef), int(reduction == "sequence"),
-            _wants_grad(x)))
+    loss, logp, means = _apply(
+        _PolicyLossFn, x, t, m, old, adv, ref, float(temperature), int(ignore_index), float(clip_low),
+        float(clip_low if clip_high is None else clip_high), float(kl_coef), int(reduction == "sequence"))
     return PolicyLoss(loss, logp if logp.shape == tokens.shape else logp.reshape(tokens.shape), *means.unbind(0))
 
 
@@ -325,5 +329,5 @@ def preference_loss(logits, tokens, ref_logprobs=None, *, mask=None, beta=0.1, l
     x, t = _rows(name, logits, tokens)
     m = _per_token(name, "mask", mask, x, t, tokens.shape, torch.bool)
     ref = _per_token(name, "ref_logprobs", ref_logprobs, x, t, tokens.shape)
-    return PreferenceLoss(*_PreferenceLossFn.apply(
-        x, (t, m, ref, float(temperature), int(ignore_index), float(beta), float(label_smoothing), _wants_grad(x))))
+    return PreferenceLoss(*_apply(_PreferenceLossFn, x, t, m, ref, float(temperature), int(ignore_index), float(beta),
+                                  float(label_smoothing)))
