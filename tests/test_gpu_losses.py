@@ -662,3 +662,88 @@ def test_refusals():
     d, = torch.autograd.grad(token_logprobs(x, tokens).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(d.sum(), x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [700, 9000, 60001, 140000])
+def test_rows_whose_first_elements_mislead(V, dtype):
+    """Rows whose first elements and token lie far below the rest (the sum over an assumed base
+    then overflows), are excluded, or are all there is; one row of each kind in turn, with
+    ordinary rows between: forward, policy gradient and the gradient of log-probabilities."""
+    from mamba3_ssm import policy_loss, token_logprobs
+    from mamba3_ssm import _lib
+    B, T = 2, 12
+    x, tokens = _inputs((B, T, V), dtype, 70)
+    few = min(300, V // 2)
+    tokens %= few
+    x[:, 1::6, :few] = -150.0
+    x[:, 2::6, :few] = float("-inf")
+    x[:, 2::6, 0] = -120.0
+    tokens[:, 2::6] = 0
+    x[:, 3::6, :] = torch.finfo(dtype).min
+    x[:, 4::6, :few] = torch.finfo(dtype).min
+    tokens[:, 4::6] = V - 1
+    ref = _logp64(x, tokens)
+    y = x.clone().requires_grad_(True)
+    out = token_logprobs(y, tokens)
+    _assert_logp(out.detach(), ref)
+    dout = torch.randn(B, T, device=DEV, generator=_gen(71))
+    d, = torch.autograd.grad(out, y, dout)
+    _assert_grad(d, x, tokens, dout.double())
+    old = ref.float()  # ratios of 1
+    r = policy_loss(y, tokens, old, dout)
+    # off by the rounding of old to 32 bits and the log-probability's tolerance
+    loss = -dout.double().mean()
+    slack = (dout.double().abs() * (LOGP_TOL + 2.0 ** -23 * ref.abs())).mean()
+    assert abs(r.loss.item() - loss.item()) <= slack.item() + 1e-6 * abs(loss.item())
+    d, = torch.autograd.grad(r.loss, y)
+    p = torch.softmax(x.double(), -1)
+    hot = torch.zeros_like(p).scatter_(-1, tokens.unsqueeze(-1), 1.0)
+    g = (-dout.double() / (B * T)).unsqueeze(-1)
+    exact = g * (hot - p)
+    loose = (LOGP_TOL + 2.0 ** -22 * ref.abs()).unsqueeze(-1)
+    tol = exact.abs() * (loose + torch.finfo(dtype).eps / 2 * 1.001) + g.abs() * (2.0 ** -18 * p + 2.0 ** -23) + 1e-37
+    assert ((d.double() - exact).abs() <= tol).all()
+    assert _lib.device_timeouts() == 0
+
+
+def test_two_calls_at_once():
+    """Two policy steps and two clippings on two streams beside each other: the results of each
+    alone."""
+    from mamba3_ssm import clip_grads_, policy_loss
+    data = [_inputs((8, 100, 50001), torch.bfloat16, 80 + i) for i in range(2)]
+    adv = torch.randn(8, 100, device=DEV, generator=_gen(82))
+    old = torch.full((8, 100), -9.0, device=DEV)
+    leaves = [x.requires_grad_(True) for x, _ in data]
+    grads = [torch.randn(3000001, device=DEV, generator=_gen(83 + i)) for i in range(2)]
+
+    def step(i):
+        r = policy_loss(leaves[i], data[i][1], old, adv, clip_low=1.0, clip_high=1e6)
+        g = grads[i].clone()
+        return [r.loss.detach(), r.logprobs, torch.autograd.grad(r.loss, leaves[i])[0], clip_grads_([g], 1.0), g]
+
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = [None, None]
+        for i in range(2):
+            streams[i].wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(streams[i]):
+                got[i] = step(i)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_changed_inputs_are_noticed():
+    """What backward reads again must not have changed in between."""
+    from mamba3_ssm import token_logprobs
+    x, tokens = _inputs((2, 3, 64), torch.float32, 90)
+    x = x.requires_grad_(True)
+    y = x * 1.0
+    out = token_logprobs(y, tokens)
+    with torch.no_grad():
+        y.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
