@@ -284,43 +284,46 @@ inline PolicyWs policy_ws(void* ws, int64_t batch, int64_t rows, size_t* bytes) 
 }
 
 // Positions that count, by sequence and in all, and the rows' order: those first, so that
-// they spread evenly whatever the mask. A warp takes a segment of a sequence and adds its
-// (whole) numbers to counters that are zero at the start, so the counts do not depend on the
-// schedule. The order within the two groups does, but no result depends on it.
-constexpr int kCountThreads = 128, kCountSegment = 256;
-__global__ void __launch_bounds__(kCountThreads) policy_count_kernel(TokenRows p, int64_t units, int segs, PolicyWs w) {
-  const int lane = threadIdx.x & 31;
-  const int64_t u = ((int64_t)blockIdx.x * kCountThreads + threadIdx.x) >> 5;
-  if (u >= units) return;
-  const int64_t b = u / segs;
-  const int t0 = (int)(u - b * segs) * kCountSegment, t1 = min(t0 + kCountSegment, p.T);
-  unsigned flags = 0;  // bit k: position t0 + 32 k + lane
+// they spread evenly whatever the mask. A warp takes 256 positions and adds its (whole) numbers
+// to counters that are zero at the start, so the counts do not depend on the schedule. The
+// order within the two groups does, but no result depends on it.
+constexpr int kCountThreads = 128, kCountRows = 256;
+__global__ void __launch_bounds__(kCountThreads) policy_count_kernel(TokenRows p, bool by_sequence, PolicyWs w) {
+  const int lane = threadIdx.x & 31, R = (int)p.R;
+  const int r0 = ((blockIdx.x * kCountThreads + threadIdx.x) >> 5) * kCountRows;
+  if (r0 >= R) return;
+  unsigned flags = 0;  // bit k: position r0 + 32 k + lane
 #pragma unroll
-  for (int k = 0; k < kCountSegment / 32; ++k) {
-    const int t = t0 + 32 * k + lane;
-    if (t < t1 && position(p, b, t).keep) flags |= 1u << k;
+  for (int k = 0; k < kCountRows / 32; ++k) {
+    const int r = r0 + 32 * k + lane, b = r / p.T;
+    if (r < R && position(p, b, r - b * p.T).keep) flags |= 1u << k;
   }
   const int n = __reduce_add_sync(0xffffffffu, __popc(flags));
   int at = 0, skip = 0;
   if (lane == 0) {
-    if (n > 0) {
-      at = atomicAdd(&w.head->kept, n);
-      if (atomicAdd(&w.counts[b], n) == 0) atomicAdd(&w.head->sequences, 1);  // the sequence's first
-    }
-    skip = atomicAdd(&w.head->skipped, t1 - t0 - n);
+    if (n > 0) at = atomicAdd(&w.head->kept, n);
+    skip = atomicAdd(&w.head->skipped, min(kCountRows, R - r0) - n);
   }
   at = __shfl_sync(0xffffffffu, at, 0);
-  skip = (int)p.R - 1 - __shfl_sync(0xffffffffu, skip, 0);
+  skip = R - 1 - __shfl_sync(0xffffffffu, skip, 0);
   const unsigned below = (1u << lane) - 1;
 #pragma unroll
-  for (int k = 0; k < kCountSegment / 32; ++k) {
-    const int t = t0 + 32 * k + lane;
-    const bool in = t < t1, keep = flags >> k & 1;
+  for (int k = 0; k < kCountRows / 32; ++k) {
+    const int r = r0 + 32 * k + lane;
+    const bool in = r < R, keep = flags >> k & 1;
     const unsigned yes = __ballot_sync(0xffffffffu, keep), no = __ballot_sync(0xffffffffu, in && !keep);
-    if (keep) w.order[at + __popc(yes & below)] = (int)(b * p.T + t);
-    else if (in) w.order[skip - __popc(no & below)] = (int)(b * p.T + t);
+    if (keep) w.order[at + __popc(yes & below)] = r;
+    else if (in) w.order[skip - __popc(no & below)] = r;
     at += __popc(yes);
     skip -= __popc(no);
+    if (by_sequence && yes != 0) {
+      // one addition where the 32 positions are of one sequence
+      const int b = r / p.T, first = __shfl_sync(0xffffffffu, b, 0);
+      const bool one = __all_sync(0xffffffffu, b == first || !in);
+      const int add = one ? (lane == 0 ? __popc(yes) : 0) : keep ? 1 : 0;
+      // whoever finds a sequence's counter at zero is its first
+      if (add > 0 && atomicAdd(&w.counts[b], add) == 0) atomicAdd(&w.head->sequences, 1);
+    }
   }
 }
 
@@ -1403,9 +1406,8 @@ int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64
   const PolicyWs w = policy_ws(ws, batch, p.R, &bytes);
   cudaError_t e = cudaMemsetAsync(w.head, 0, w.zeroed, s);
   if (e != cudaSuccess) return fail(M3_ERR_CUDA, std::string("policy loss: ") + cudaGetErrorString(e));
-  const int segs = (p.T + kCountSegment - 1) / kCountSegment;
-  const int64_t units = batch * segs, per = kCountThreads / 32;
-  policy_count_kernel<<<(unsigned)((units + per - 1) / per), kCountThreads, 0, s>>>(p, units, segs, w);
+  const int64_t warps = (p.R + kCountRows - 1) / kCountRows, per = kCountThreads / 32;
+  policy_count_kernel<<<(unsigned)((warps + per - 1) / per), kCountThreads, 0, s>>>(p, a.by_sequence != 0, w);
   M3_TRY(check_launch("policy_count_kernel"));
   M3_TRY(launch_rows_of<true>(p, dtype, a, w, RowOut{logp, nullptr, w.stats, w.coef, dlogits, dsb, dst}, s));
   policy_sum_kernel<<<(unsigned)((p.R + kSumRows - 1) / kSumRows), kSumThreads, 0, s>>>(p.R, w, loss, kl, clipped);

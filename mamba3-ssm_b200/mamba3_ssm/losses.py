@@ -160,11 +160,18 @@ class _TokenLogprobsFn(torch.autograd.Function):
         logits, tokens, mask = ctx.saved_tensors
         stats, temperature, ignore_index = ctx.held
         dlogits = _like_rows(logits)
-        a = L.pack(logits, tokens, mask, stats, dlogp.float(), dlogits)
+        B, T, V = logits.shape
+        dlogp = dlogp if dlogp.dtype is torch.float32 else dlogp.float()
+        vals = _records(logits, tokens, mask)
+        vals += L.rec2(dlogp, L.M3_FLOAT32, B, T)
+        vals += L.rec3(stats, L.M3_FLOAT32, B, T, 2)
+        vals += L.rec3(dlogits, L._DTYPE_CODE[logits.dtype], B, T, V)
+        a = L.Records(vals)
         dev = logits.device
         with L.on_device(dev):
-            L.check(L.load().m3_token_logprobs_grad(*a.ptrs[:5], temperature, ignore_index, a.ptrs[5],
-                                                    L.stream_ptr(dev)), "m3_token_logprobs_grad")
+            L.check(L.load().m3_token_logprobs_grad(a.at(0), a.at(1), a.at(2), a.at(4), a.at(3), temperature,
+                                                    ignore_index, a.at(5), L.stream_ptr(dev)),
+                    "m3_token_logprobs_grad")
         return dlogits, None
 
 

@@ -264,6 +264,9 @@ def _off_border(x, tokens, lo, hi, temperature, g):
     ((3, 700, 257), "sequence", True, False, 0.0, 0.5, 1.3),
     ((300, 2, 64), "sequence", False, True, 1.0, 0.2, 1.0),
     ((1, 2500, 300), "token", True, True, 0.2, 0.2, 1.0),
+    ((700, 1, 600), "sequence", False, True, 0.2, 0.2, 1.0),
+    ((60, 17, 520), "sequence", True, True, 0.2, 0.2, 1.0),
+    ((2, 2, 900001), "token", True, True, 0.2, 0.2, 1.0),
 ])
 def test_policy_loss(shape, reduction, with_ref, masked, lo, hi, temperature, dtype):
     from mamba3_ssm import policy_loss
@@ -747,3 +750,32 @@ def test_changed_inputs_are_noticed():
         y.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["cut", "wide", "shifted", "transposed", "offset", "expanded"])
+@pytest.mark.parametrize("V", [513, 9001, 70003])
+def test_policy_loss_layouts(V, layout, dtype):
+    """Rows of every layout, whose gradient may start on other boundaries than the logits, at
+    lengths that each of the kernels takes; advantages and masks broadcast."""
+    from mamba3_ssm import policy_loss
+    x, tokens = _inputs((3, 7, V), dtype, 95, layout)
+    logp = _logp64(x, tokens)
+    old = (logp - 0.1).float()
+    adv = torch.tensor([[1.0], [-2.0], [0.5]], device=DEV)
+    mask = torch.arange(7, device=DEV) != 2
+    leaf = x.detach().requires_grad_(True)
+    r = policy_loss(leaf, tokens, old, adv, mask=mask, clip_low=0.5, clip_high=0.5)
+    d, = torch.autograd.grad(r.loss, leaf)
+    ratio = (logp - old.double()).exp()
+    keep = mask.expand(3, 7)
+    dlogp = torch.where(keep, -ratio * adv.double() / 18, torch.zeros_like(ratio))
+    assert torch.equal(r.logprobs == 0, ~keep)
+    _assert_logp(r.logprobs[keep], logp[keep])
+    # the ratio carries the log-probability's tolerance: 2^-19 of the gradient, beside p's 2^-18
+    p = torch.softmax(x.double(), -1)
+    hot = torch.zeros_like(p).scatter_(-1, tokens.unsqueeze(-1), 1.0)
+    exact = dlogp.unsqueeze(-1) * (hot - p)
+    u = torch.finfo(dtype).eps / 2
+    tol = exact.abs() * (u * 1.001 + 2.0 ** -18) + dlogp.abs().unsqueeze(-1) * (2.0 ** -18 * p + 2.0 ** -23) + 1e-37
+    assert ((d.double() - exact).abs() <= tol).all()
