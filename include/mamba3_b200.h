@@ -379,8 +379,7 @@ int m3_silu_gate_bwd(const m3_tensor* y, const m3_tensor* z, const m3_tensor* do
 
 /* ---------------------------------------------------------------------------------
  * Losses over the tokens of a language model's logits, for fine-tuning (no counterpart in
- * the reference, whose train.py takes a cross-entropy of the logits). With s = 1 /
- * temperature and logp = s l[tok] - log sum_v exp(s l[v]) of a position's logits l:
+ * the reference's package). With s = 1 / temperature and logp = s l[tok] - log sum_v exp(s l[v]) of a position's logits l:
  *   m3_token_logprobs   logp of every position
  *   m3_policy_loss      sum_t w_t [ -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
  *                       + kl_coef (exp(d) - d - 1) ],  r = exp(logp - old), d = ref - logp;
@@ -434,8 +433,8 @@ int m3_preference_loss_grad(const m3_tensor* logits, const m3_tensor* tokens, co
                             const void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
- * Global norm of many gradient tensors, with scaling and clipping (the reference's train.py
- * calls torch's clip_grad_norm_):
+ * Global norm of many gradient tensors, with scaling and clipping, between backward and the
+ * optimiser's step (no counterpart in the reference's package):
  *   norm = scale * sqrt(sum g^2), or scale * max |g| with largest;
  *   g <- g * scale * min(1, max_norm / (norm + 1e-6)), or out <- that with outs.
  * The tensors are dense runs of elements, given as host arrays (a model has hundreds, and

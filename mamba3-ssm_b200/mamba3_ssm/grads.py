@@ -1,10 +1,10 @@
 """Global norm of a model's gradients, and their scaling and clipping, on m3_clip_grads (two
 kernel launches for up to a thousand tensors, no host synchronisation, deterministic).
 
-``clip_grad_norm_`` takes parameters, with the arguments of torch.nn.utils.clip_grad_norm_
-(which the reference's train.py calls between backward and the optimiser's step);
-``clip_grads_`` takes the gradients themselves and can also unscale them and write fp32
-gradients for an optimiser from bf16 ones.
+``clip_grad_norm_`` takes parameters, with the arguments of torch.nn.utils.clip_grad_norm_;
+``clip_grads_`` takes the gradients themselves and can also unscale them (loss scaling,
+accumulated micro-batches) and write fp32 gradients for an optimiser from 16-bit ones. No
+counterpart in the reference's package.
 """
 
 import math

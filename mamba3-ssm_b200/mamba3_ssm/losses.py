@@ -13,7 +13,7 @@ Positions with mask 0 or the token ``ignore_index`` do not count: their logits a
 their log-probability is 0 and their gradient is 0, whatever is stored there. A token id
 outside the vocabulary that is not ``ignore_index`` makes its position NaN. Gradients flow to
 the logits alone; old and reference log-probabilities, advantages and masks are constants.
-No counterpart in the reference (its train.py takes a cross-entropy of the logits).
+No counterpart in the reference's package.
 """
 
 from typing import NamedTuple
