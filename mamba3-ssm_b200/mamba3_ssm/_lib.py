@@ -7,6 +7,7 @@ a RuntimeError is raised with the library's own error text.
 
 import contextlib
 import ctypes
+import functools
 import os
 import struct
 
@@ -20,7 +21,7 @@ M3_FLOAT32, M3_BFLOAT16, M3_FLOAT16 = 0, 1, 2
 M3_OK, M3_ERR_INVALID_ARGUMENT, M3_ERR_UNSUPPORTED, M3_ERR_CUDA, M3_ERR_WORKSPACE = 0, 1, 2, 3, 4
 M3_INT64, M3_UINT8 = 3, 4
 _DTYPE_CODE = {torch.float32: M3_FLOAT32, torch.bfloat16: M3_BFLOAT16, torch.float16: M3_FLOAT16,
-               torch.int64: M3_INT64, torch.bool: M3_UINT8, torch.uint8: M3_UINT8}
+               torch.int64: M3_INT64}
 _STATUS = {1: "invalid argument", 2: "unsupported", 3: "CUDA error", 4: "workspace"}
 
 
@@ -153,9 +154,11 @@ def tensor(t):
 
 
 _PADS = tuple((0,) * (MAX_DIMS - n) for n in range(MAX_DIMS + 1))
-_RECS = [struct.Struct("=" + "qii" + "q" * (2 * MAX_DIMS))]
-for _n in range(2, 25):
-    _RECS.append(struct.Struct("=" + ("qii" + "q" * (2 * MAX_DIMS)) * _n))
+
+
+@functools.lru_cache(maxsize=64)
+def _records_struct(n):
+    return struct.Struct("=" + ("qii" + "q" * (2 * MAX_DIMS)) * n)
 
 
 class Packed:
@@ -186,7 +189,7 @@ class Packed:
             ptrs.append(n)
             n += _REC.size
         if n:
-            self.buf = _RECS[n // _REC.size - 1].pack(*vals)
+            self.buf = _records_struct(n // _REC.size).pack(*vals)
             base = address(self.buf)
             ptrs = [None if p is None else base + p for p in ptrs]
         else:
@@ -206,7 +209,7 @@ class Records:
     __slots__ = ("buf", "base")
 
     def __init__(self, vals):
-        self.buf = _RECS[len(vals) // 15 - 1].pack(*vals)
+        self.buf = _records_struct(len(vals) // 15).pack(*vals)
         self.base = address(self.buf)
 
     def at(self, i):

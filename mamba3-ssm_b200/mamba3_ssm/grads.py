@@ -102,7 +102,10 @@ def clip_grads_(grads, max_norm, norm_type=2.0, *, scale=1.0, out=None):
     L.check(rc, "m3_clip_grads")
     if out is not None or scale != 1.0 or max_norm != math.inf:
         written = out if out is not None else grads
-        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+        try:
+            torch.autograd.graph.increment_version(written)
+        except RuntimeError:  # inference tensors have no version
+            torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
     return norm
 
 
