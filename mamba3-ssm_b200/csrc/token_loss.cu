@@ -608,9 +608,10 @@ __device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a
     if (lane == 0) part[warp] = v;
     meet();
     F y = largest ? -INFINITY : F(0);
-    for (int i = 0; i < W * C; ++i) {
-      const F z = C > 1 ? cl.map_shared_rank(part, i / W)[i % W] : part[i];
-      y = largest ? (z > y ? z : y) : y + z;
+    for (int k = 0; k < C; ++k) {  // in the same order as the first sum
+      const F z = lane >= W ? (largest ? -INFINITY : F(0)) : C > 1 ? cl.map_shared_rank(part, k)[lane] : part[lane];
+      if (largest) y = fmaxf((float)y, warp_max((float)z));
+      else y += warp_sum(z);
     }
     return y;
   };

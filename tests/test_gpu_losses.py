@@ -779,3 +779,19 @@ def test_policy_loss_layouts(V, layout, dtype):
     u = torch.finfo(dtype).eps / 2
     tol = exact.abs() * (u * 1.001 + 2.0 ** -18) + dlogp.abs().unsqueeze(-1) * (2.0 ** -18 * p + 2.0 ** -23) + 1e-37
     assert ((d.double() - exact).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [12000, 60001, 140000])
+def test_misleading_rows_without_grad_have_the_same_bits(V, dtype):
+    """Rows that are summed a second time, over their true maximum, too."""
+    from mamba3_ssm import policy_loss
+    B, T = 10, 40
+    x, tokens = _inputs((B, T, V), dtype, 105)
+    x[..., :V // 2] = -150.0
+    adv = torch.randn(B, T, device=DEV, generator=_gen(106))
+    old = torch.full((B, T), -11.0, device=DEV)
+    plain = policy_loss(x, tokens, old, adv)
+    r = policy_loss(x.requires_grad_(True), tokens, old, adv)
+    for a, b in zip(plain, r):
+        assert torch.equal(a, b.detach())
