@@ -332,12 +332,16 @@ struct TokenOps {
   float old_logp, adv, ref;
   double weight;
 };
-__device__ __forceinline__ TokenOps token_ops(const PolicyArgs& a, const PolicyWs& w, int64_t b, int64_t t) {
+// The weight of a position, where it is the same for all.
+__device__ __forceinline__ double even_weight(const PolicyArgs& a, const PolicyWs& w) {
+  return a.by_sequence ? 0.0 : 1.0 / (double)w.head->kept;
+}
+__device__ __forceinline__ TokenOps token_ops(const PolicyArgs& a, const PolicyWs& w, int64_t b, int64_t t, double even) {
   TokenOps o;
   o.old_logp = map_at(a.old_logp, b, t);
   o.adv = map_at(a.adv, b, t);
   o.ref = a.ref.p ? map_at(a.ref, b, t) : 0.f;
-  o.weight = a.by_sequence ? 1.0 / ((double)w.counts[b] * (double)w.head->sequences) : 1.0 / (double)w.head->kept;
+  o.weight = a.by_sequence ? 1.0 / ((double)w.counts[b] * (double)w.head->sequences) : even;
   return o;
 }
 
@@ -660,7 +664,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_rows_kernel(TokenRows p, 
   const float at_token = pos.known ? to_f32(row[pos.tok]) : NAN;
   TokenOps x{};
   if constexpr (POLICY)
-    if (tid == 0) x = token_ops(a, w, b, t);
+    if (tid == 0) x = token_ops(a, w, b, t, even_weight(a, w));
   const Base base = base_at(fmaxf(warp_max(first_max(row, p.V, c, lane)), at_token), p.c_hi);
   Sum s2{0.f, 0.f};
   int j = tid;
@@ -805,6 +809,7 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
 
   if (warp == W) {
     // ------------------------------------------------------------------ the copying warp
+    const double even = even_weight(a, w);
     uint32_t round = 0, issued = 0;  // issued: pieces whose copy of the current round is under way
     bool ok = true;
     // zeros to a position that does not count, this CTA's part of the row
@@ -841,7 +846,7 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
       const int64_t tok = map_at(p.tok, b, t);
       const bool known = tok >= 0 && tok < p.V;
       q.tok = known ? (int)tok : -1;
-      q.x = token_ops(a, w, b, t);
+      q.x = token_ops(a, w, b, t, even);
       q.at_token = known ? to_f32(q.row[tok]) : NAN;
       q.base = base_at(fmaxf(warp_max(first_max(q.row, p.V, q.c, lane)), q.at_token), p.c_hi);
       if (lane == 0) {
@@ -1011,68 +1016,203 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
   if (C > 1) cl.sync();  // no CTA leaves while another sends to it
 }
 
-// Short rows (up to 4 KB): a warp per row, the row in its registers. A CTA per row would spend
-// more time on its two barriers than on the row.
-constexpr int kShortBytes = 4096, kShortVecs = kShortBytes / (16 * 32), kShortThreads = 128;
-template <typename T, bool POLICY>
-__global__ void __launch_bounds__(kShortThreads) token_short_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o) {
-  const int lane = threadIdx.x & 31;
-  const int64_t r = (int64_t)blockIdx.x * (kShortThreads / 32) + (threadIdx.x >> 5);
-  if (r >= p.R) return;
-  const int64_t b = r / p.T, t = r - b * p.T;
-  const T* row = static_cast<const T*>(p.logits) + b * p.sb + t * p.st;
-  T* drow = nullptr;
-  if constexpr (POLICY)
-    if (o.dlogits) drow = static_cast<T*>(o.dlogits) + b * o.dsb + t * o.dst;
-  const Position pos = position(p, b, t);
-  if (!pos.keep) {
-    if (lane == 0) skip_row<POLICY>(o, w, r);
-    if (drow) fill<T>(drow, 0, p.V, lane, 32, from_f32<T>(0.f));
-    return;
+// Rows of up to 24 KB. A warp takes 32 / G consecutive rows at a time, which bulk copies bring to
+// its place in shared memory, sums each with G lanes and writes their gradients from there. A lane
+// is a row where a row's few numbers are concerned: its token, logarithm, loss and gradient's
+// factor cost a warp as much for one row as for eight. No warp waits for another, and none copies
+// ahead: twice the warps hide a copy better than a second place each (4096 bf16 logits a row, loss
+// and gradient: 5.1 TB/s read and written against 4.3). What bounds it: with 24 and more warps of
+// an SM in flight the instructions per logit in 16 bits and per row in short rows, the memory else.
+// 400 million logits, at most 262144 rows, TB/s, without a gradient | with the policy's:
+//   bf16, rows of 300, 1000, 2500, 4096, 8192: 2.9 4.3 4.7 5.5 5.7 | 2.8 4.2 4.7 5.4 5.4
+//   fp32, rows of 300, 1000, 2500, 4096, 6000: 5.8 6.5 6.6 6.9 6.6 | 4.5 5.4 5.6 5.6 6.1
+// A warp per row in registers (up to 4 KB) and a CTA per row (above) had 0.9 2.7 1.2 2.3 3.9 for
+// bf16 rows without a gradient and 0.9 2.7 2.1 2.9 4.0 with it.
+constexpr int kWarpThreads = 64;
+template <bool POLICY>
+constexpr int kWarpCtas = POLICY ? 14 : 16;  // of an SM at most: 72 and 64 registers
+constexpr int64_t kWarpRow = 24 * 1024;      // rows of fp32 logits of 32 KB: a CTA per row 6.8 TB/s, this 6.2
+constexpr int64_t kSmSmem = 227 * 1024;
+template <typename T, int G>
+struct WarpRowsShared {
+  static constexpr int E = 32 / sizeof(T);  // single elements before and behind a row's vectors: fewer than this
+  uint64_t full[kWarpThreads / 32];
+  int dead;
+  T ends[kWarpThreads / 32][32 / G * E];
+};
+struct LaneRow {
+  int r, b, t, tok, head, nv;
+  bool mine, keep;
+  float at_token;
+  TokenOps x;
+};
+template <typename T, bool POLICY, int G>
+__global__ void __launch_bounds__(kWarpThreads, kWarpCtas<POLICY>)
+    token_warp_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o, int row_vecs) {
+  constexpr int N = Vec<T>::N, E = WarpRowsShared<T, G>::E, W = kWarpThreads / 32;
+  constexpr int each = 32 / G;  // rows of a batch
+  using F = Joined<POLICY>;
+  extern __shared__ __align__(16) uint4 places_raw[];
+  __shared__ WarpRowsShared<T, G> sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Vec<T>* const place = reinterpret_cast<Vec<T>*>(places_raw) + (size_t)warp * each * row_vecs;
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < W; ++k) sm100::mbar_init(&sh.full[k], 1);
+    sh.dead = 0;
+    sm100::fence_barrier_init();
   }
-  const RowCut c = cut_row(row, p.V);
-  const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + c.head);
-  Vec<T> v[kShortVecs];
+  __syncthreads();
+  const T* const logits = static_cast<const T*>(p.logits);
+  auto row_at = [&](int b, int t) { return logits + b * p.sb + t * p.st; };
+  auto of = [](auto v, int i) { return __shfl_sync(0xffffffffu, v, i); };
+
+  double even = 0.0;
+  if constexpr (POLICY) even = even_weight(a, w);
+
+  // the rows of a batch: their vectors on the way to its place, the rest here
+  auto fetch = [&](int batch) {
+    const int r0 = batch * each, rows = min(each, (int)p.R - r0);
+    LaneRow q;
+    q.mine = lane < rows;
+    q.r = r0 + min(lane, rows - 1);
+    q.b = q.r / p.T;
+    q.t = q.r - q.b * p.T;
+    const Position pos = position(p, q.b, q.t);
+    q.keep = q.mine && pos.keep;
+    q.tok = pos.known ? (int)pos.tok : -1;
+    const T* const row = row_at(q.b, q.t);
+    const RowCut c = cut_row(row, p.V);
+    q.head = c.head;
+    q.nv = c.nv;
+    const uint32_t bytes = q.keep ? 16u * c.nv : 0u, all = __reduce_add_sync(0xffffffffu, bytes);
+    if (lane == 0) sm100::mbar_expect_tx(&sh.full[warp], all);
+    __syncwarp();
+    if (bytes) sm100::bulk_load(place + lane * row_vecs, row + c.head, bytes, &sh.full[warp]);
+    q.at_token = NAN;
+    q.x = TokenOps{};
+    if (q.keep) {
+      if (pos.known) q.at_token = to_f32(row[pos.tok]);
+      if constexpr (POLICY) q.x = token_ops(a, w, q.b, q.t, even);
+    }
+    if (__any_sync(0xffffffffu, q.keep && p.V != c.nv * N)) {
+      T* const ends = sh.ends[warp];
 #pragma unroll
-  for (int u = 0; u < kShortVecs; ++u)
-    if (lane + 32 * u < c.nv) v[u] = rv[lane + 32 * u];
-  // at most seven single elements on each side
-  const float first = lane < c.head ? to_f32(row[lane]) : -INFINITY;
-  const float last = c.tail0 + lane < p.V ? to_f32(row[c.tail0 + lane]) : -INFINITY;
-  const float at_token = pos.known ? to_f32(row[pos.tok]) : NAN;
-  TokenOps x{};
-  if constexpr (POLICY) x = token_ops(a, w, b, t);
-  float m = fmaxf(first, last);
-#pragma unroll
-  for (int u = 0; u < kShortVecs; ++u)
-    if (lane + 32 * u < c.nv) m = fmaxf(m, vec_max(v[u]));
-  const Base base = base_at(warp_max(m), p.c_hi);
-  auto sum = [&](auto far) {
-    constexpr bool FAR = decltype(far)::value;
-    const float s = (lane < c.head ? exp_one<!POLICY>(first, base, p.c_hi, p.c_lo) : 0.f) +
-                    (c.tail0 + lane < p.V ? exp_one<!POLICY>(last, base, p.c_hi, p.c_lo) : 0.f);
-    Sum s2{0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < kShortVecs; ++u)
-      if (lane + 32 * u < c.nv) add_vec<FAR, !POLICY>(s2, v[u], base, p.c_hi, p.c_lo);
-    return s + s2.total();
-  };
-  const Joined<POLICY> S = warp_sum((Joined<POLICY>)(base.far ? sum(std::true_type{}) : sum(std::false_type{})));
-  const GradRow gr =
-      finish_row<POLICY>(p, a, w, o, x, r, at_token, pos.known ? (int)pos.tok : -1, base, S, lane == 0);
-  if constexpr (POLICY) {
-    if (drow) {
-      if (gr.g == 0.f) {
-        fill<T>(drow, 0, p.V, lane, 32, from_f32<T>(0.f));
-      } else {
-        const bool same = same_boundary(drow, c);
-#pragma unroll
-        for (int u = 0; u < kShortVecs; ++u)
-          if (lane + 32 * u < c.nv) put_grad(v[u], lane + 32 * u, drow, c, gr, same, p.c_hi, p.c_lo);
-        put_token(drow, c, gr, 0, c.nv, lane, 32, p.c_hi, p.c_lo);
-        put_ends(row, drow, p.V, c, gr, lane, 32, p.c_hi, p.c_lo);
+      for (int k0 = 0; k0 < each; k0 += 32 / E) {
+        const int k = k0 + lane / E, e = lane % E;
+        const int head = of(q.head, k), nv = of(q.nv, k), b = of(q.b, k), t = of(q.t, k);
+        if (k < rows && e < p.V - nv * N) ends[k * E + e] = row_at(b, t)[e < head ? e : nv * N + e];
       }
     }
+    __syncwarp();  // the ends
+    return q;
+  };
+
+  // a row is summed and written by G lanes, of which this is number l
+  const int i = lane / G, l = lane % G;
+  auto work = [&](const LaneRow& q) {
+    const int rows = __popc(__ballot_sync(0xffffffffu, q.mine));
+    const unsigned keeps = __ballot_sync(0xffffffffu, q.keep);
+    Base my_base{};
+    F my_S = 0;
+    if (keeps) {
+      const int nv = of(q.nv, i), singles = p.V - nv * N;
+      const bool keep = keeps >> i & 1;
+      const Vec<T>* const v = place + i * row_vecs;
+      const T* const ends = sh.ends[warp] + i * E;
+      // over the row's lanes
+      auto all_max = [](float x) {
+#pragma unroll
+        for (int k = G / 2; k > 0; k >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
+        return x;
+      };
+      auto all_sum = [](F x) {
+#pragma unroll
+        for (int k = G / 2; k > 0; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
+        return x;
+      };
+      auto ends_max = [&] {
+        float m = -INFINITY;
+        if (keep)
+          for (int e = l; e < singles; e += G) m = fmaxf(m, to_f32(ends[e]));
+        return m;
+      };
+      float m = ends_max();
+      if (keep && l < nv) m = fmaxf(m, vec_max(v[l]));
+      Base base = base_at(fmaxf(all_max(m), of(q.at_token, i)), p.c_hi);
+      auto sum = [&](auto known, bool sums) {
+        Sum s2{0.f, 0.f};
+        if (sums) {
+#pragma unroll 4
+          for (int j = l; j < nv; j += G) {
+            if constexpr (decltype(known)::value) add_any<!POLICY>(s2, v[j], base, p.c_hi, p.c_lo);
+            else add_vec<false, !POLICY>(s2, v[j], base, p.c_hi, p.c_lo);
+          }
+          for (int e = l; e < singles; e += G) s2.a += exp_one<!POLICY>(to_f32(ends[e]), base, p.c_hi, p.c_lo);
+        }
+        return all_sum((F)s2.total());
+      };
+      F S = sum(std::false_type{}, keep);
+      const bool again = keep && (base.far || !in_range((float)S));
+      if (__any_sync(0xffffffffu, again)) {
+        // rare: the row's true maximum, then its sum
+        m = ends_max();
+        if (again)
+          for (int j = l; j < nv; j += G) m = fmaxf(m, vec_max(v[j]));
+        m = all_max(m);
+        if (again) base = base_at(m, p.c_hi);
+        const F y = sum(std::true_type{}, again);
+        if (again) S = y;
+      }
+      // to the row's lane
+      const int from = lane * G & 31;
+      my_base = Base{of(base.m, from), of(base.k, from), of((int)base.far, from) != 0};
+      my_S = of(S, from);
+    }
+    GradRow gr{};
+    if (q.keep) {
+      gr = finish_row<POLICY>(p, a, w, o, q.x, q.r, q.at_token, q.tok, my_base, my_S, true);
+    } else if (q.mine) {
+      skip_row<POLICY>(o, w, q.r);
+    }
+    if constexpr (POLICY) {
+      if (!o.dlogits) return;
+      const int b = of(q.b, i), t = of(q.t, i);
+      T* const drow = static_cast<T*>(o.dlogits) + b * o.dsb + t * o.dst;
+      const GradRow y{Base{of(gr.base.m, i), of(gr.base.k, i), of((int)gr.base.far, i) != 0}, of(gr.g, i), of(gr.inv, i),
+                      of(gr.tok, i), of(gr.at, i), of(gr.kg, i), of((int)gr.negative, i) != 0,
+                      of((int)gr.folded, i) != 0};
+      RowCut c;
+      c.head = of(q.head, i);
+      c.nv = of(q.nv, i);
+      c.tail0 = c.head + c.nv * N;
+      if (i >= rows) return;
+      if (y.g == 0.f) {  // a position that does not count among them
+        fill<T>(drow, 0, p.V, l, G, from_f32<T>(0.f));
+        return;
+      }
+      const Vec<T>* const v = place + i * row_vecs;
+      put_vecs<T>(l, c.nv, G, 0, drow, c, y, same_boundary(drow, c), p.c_hi, p.c_lo, [&](int j) { return v[j]; });
+      put_token(drow, c, y, 0, c.nv, l, G, p.c_hi, p.c_lo);
+      for (int e = l; e < p.V - c.nv * N; e += G) {
+        const int j = e < c.head ? e : c.nv * N + e;
+        drow[j] = one_grad<T>(to_f32(sh.ends[warp][i * E + e]), y, j == y.tok ? 1.f : 0.f, p.c_hi, p.c_lo);
+      }
+    }
+  };
+
+  const int batches = (int)((p.R + each - 1) / each), warps = gridDim.x * W;
+  int batch = blockIdx.x * W + warp;
+  if (batch >= batches) return;
+  for (uint32_t n = 0;; ++n) {
+    const LaneRow q = fetch(batch);
+    if (!wait_warp(&sh.full[warp], n & 1, &sh.dead)) {
+      sm100::mbar_wait(&sh.full[warp], n & 1, kWaitLimit);  // copies in flight end before the CTA does
+      return;
+    }
+    work(q);
+    __syncwarp();  // all have read the place
+    if (batch >= batches - warps) return;
+    batch += warps;
   }
 }
 
@@ -1251,6 +1391,11 @@ __global__ void __launch_bounds__(kGradThreads, 4)
   }
 }
 
+// Positions are counted in 32 bits, and a kernel's stride is added to them.
+int check_rows(const TokenRows& p) {
+  return p.R > INT32_MAX / 2 - 4096 ? fail(M3_ERR_UNSUPPORTED, "token rows: too many positions") : M3_OK;
+}
+
 // How the rows are laid over the device.
 struct RowPlan {
   int C, threads;
@@ -1335,14 +1480,38 @@ int launch_grad_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w,
   return launch_clusters(kernel, plan, p.R, &cache, (size_t)plan.slot_vecs * 16, s, p, a, w, o, pieces);
 }
 
+template <typename T, bool POLICY, int G>
+int launch_warp_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o, cudaStream_t s) {
+  constexpr int W = kWarpThreads / 32, each = 32 / G;
+  int sms = 0;
+  M3_TRY(device_sm_count(&sms));
+  const int row_vecs = (int)(((int64_t)p.V * (int64_t)sizeof(T) + 15) / 16);
+  const size_t smem = (size_t)W * each * row_vecs * 16;
+  // 1 KB of each CTA is the system's
+  const int64_t fit = kSmSmem / (int64_t)(smem + sizeof(WarpRowsShared<T, G>) + 1024);
+  const int64_t most = sms * std::min<int64_t>(kWarpCtas<POLICY>, fit);
+  if constexpr (G < 32)  // few rows: more lanes for each
+    if (p.R < most * W * each) return launch_warp_rows<T, POLICY, 2 * G>(p, a, w, o, s);
+  auto kernel = token_warp_rows_kernel<T, POLICY, G>;
+  static std::atomic<bool> done[kMaxDevices];
+  M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), (size_t)W * kWarpRow, done));
+  const int64_t batches = (p.R + each - 1) / each;
+  kernel<<<(unsigned)std::min(most, (batches + W - 1) / W), kWarpThreads, smem, s>>>(p, a, w, o, row_vecs);
+  return check_launch("token_warp_rows_kernel");
+}
+
 template <typename T, bool POLICY>
 int launch_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, const RowOut& o, cudaStream_t s) {
   if (p.R == 0) return M3_OK;
-  if ((int64_t)p.V * (int64_t)sizeof(T) <= kShortBytes) {
-    const int64_t per = kShortThreads / 32;
-    token_short_rows_kernel<T, POLICY><<<(unsigned)((p.R + per - 1) / per), kShortThreads, 0, s>>>(p, a, w, o);
-    return check_launch("token_short_rows_kernel");
-  }
+  M3_TRY(check_rows(p));
+  const int64_t bytes = (int64_t)p.V * (int64_t)sizeof(T);
+  // Lanes of a row, so that a warp's rows are 5 to 24 KB (without a gradient, TB/s, of 4, 8, 16
+  // and 32 lanes: 300 bf16 logits 2.7, 2.0, 1.8, 1.3; 1000 4.6, 4.4, 3.2, 2.9; 2047 -, 4.4, 4.0,
+  // 3.0; 4096 -, -, 5.4, 4.8; 600 fp32 logits 5.9, 6.4, 5.3, 5.2; 2500 -, -, 6.5, 6.9).
+  if (bytes <= 1280) return launch_warp_rows<T, POLICY, 4>(p, a, w, o, s);
+  if (bytes <= 4096) return launch_warp_rows<T, POLICY, 8>(p, a, w, o, s);
+  if (bytes <= kWarpRow / 2) return launch_warp_rows<T, POLICY, 16>(p, a, w, o, s);
+  if (bytes <= kWarpRow) return launch_warp_rows<T, POLICY, 32>(p, a, w, o, s);
   RowPlan plan;
   M3_TRY(plan_rows(p, (int64_t)sizeof(T), POLICY, &plan));
   if constexpr (POLICY) {
@@ -1352,7 +1521,6 @@ int launch_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w, cons
       return launch_grad_rows<T, 512>(p, a, w, o, plan, s);
     }
   }
-  if (p.R > INT32_MAX / plan.C) return fail(M3_ERR_UNSUPPORTED, "token rows: too many positions");
   if constexpr (POLICY) {
     if (plan.threads == 512) return launch_clusters(token_rows_kernel<T, POLICY, 512>, plan, p.R, nullptr, 0, s, p, a, w, o);
     if (plan.threads == 256) return launch_clusters(token_rows_kernel<T, POLICY, 256>, plan, p.R, nullptr, 0, s, p, a, w, o);
@@ -1403,6 +1571,7 @@ int launch_token_logprobs(const TokenRows& p, int dtype, float* logp, float2* st
 
 int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64_t batch, float* loss, float* kl,
                        float* clipped, float* logp, void* dlogits, int64_t dsb, int64_t dst, void* ws, cudaStream_t s) {
+  M3_TRY(check_rows(p));
   size_t bytes = 0;
   const PolicyWs w = policy_ws(ws, batch, p.R, &bytes);
   cudaError_t e = cudaMemsetAsync(w.head, 0, w.zeroed, s);
@@ -1417,6 +1586,7 @@ int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64
 
 int launch_preference_loss(const TokenRows& p, int dtype, Map2<const float> ref, double beta, double smoothing,
                            int64_t pairs, float* loss, float* rewards, float* logp, void* ws, cudaStream_t s) {
+  M3_TRY(check_rows(p));
   size_t bytes = 0;
   const PrefWs w = pref_ws(ws, 2 * pairs, p.R, &bytes);
   cudaError_t e = cudaMemsetAsync(w.done, 0, sizeof(unsigned), s);
@@ -1442,14 +1612,27 @@ template <typename T>
 static int launch_grad(const TokenRows& p, const float2* stats, Map2<const float> coef, const float* up,
                        bool keep_if_one, void* dlogits, int64_t dsb, int64_t dst, cudaStream_t s) {
   int sms = 0;
+  M3_TRY(check_rows(p));
   M3_TRY(device_sm_count(&sms));
   const int64_t bytes = (int64_t)p.V * (int64_t)sizeof(T), ctas = (int64_t)sms * 4;
   T* const d = static_cast<T*>(dlogits);
   // where the kernel may find nothing to do its grid is small, else as large as the work
-  if (bytes <= 8192) {  // a warp per row
-    const int64_t need = (p.R + kGradThreads / 32 - 1) / (kGradThreads / 32);
-    token_grad_kernel<T, 32><<<(unsigned)(keep_if_one ? std::min(need, ctas) : need), kGradThreads, 0, s>>>(
+  auto by_rows = [&](auto lanes) {
+    constexpr int G = decltype(lanes)::value;
+    const int64_t need = (p.R + kGradThreads / G - 1) / (kGradThreads / G);
+    token_grad_kernel<T, G><<<(unsigned)(keep_if_one ? std::min(need, ctas) : need), kGradThreads, 0, s>>>(
         p, stats, coef, up, keep_if_one, d, dsb, dst, 1, (int)p.R);
+  };
+  if (bytes <= 8192 || (bytes <= 24576 && p.R >= 8 * ctas)) {
+    // Lanes of a row: short rows leave a warp's idle, and each has its position to find (bf16, of
+    // 4, 8, 16 and 32 lanes: 300 logits 5.0, 4.5, 2.5, 1.6 TB/s; 1000 5.1, 5.9, 5.2, 3.7; 2047 5.2,
+    // 6.1, 6.4, 5.7; 4096 logits 6.8 with 32). Few rows: as many lanes as keep the device's busy.
+    int g = bytes <= 1024 ? 4 : bytes <= 2560 ? 8 : bytes <= 6144 ? 16 : 32;
+    while (g < 32 && p.R * g < ctas * kGradThreads) g *= 2;
+    if (g == 4) by_rows(std::integral_constant<int, 4>{});
+    else if (g == 8) by_rows(std::integral_constant<int, 8>{});
+    else if (g == 16) by_rows(std::integral_constant<int, 16>{});
+    else by_rows(std::integral_constant<int, 32>{});
   } else {
     // a CTA per row, or per part of a row (16 KB or more) where there are few rows
     int64_t parts = 1;

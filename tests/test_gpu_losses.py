@@ -795,3 +795,62 @@ def test_misleading_rows_without_grad_have_the_same_bits(V, dtype):
     r = policy_loss(x.requires_grad_(True), tokens, old, adv)
     for a, b in zip(plain, r):
         assert torch.equal(a, b.detach())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["contiguous", "cut"])
+@pytest.mark.parametrize("T,V", [(1000, 257), (1000, 300), (390, 1000), (154, 2500), (154, 5999), (61, 12000)])
+def test_many_short_rows(T, V, layout, dtype):
+    """So many rows that several share a warp and each warp takes several turns. Among them, in
+    every order: positions that do not count, rows whose first elements and token lie far below
+    the rest, excluded elements, a type's lowest value."""
+    from mamba3_ssm import _lib, policy_loss, token_logprobs
+    B = 41
+    x, tokens = _inputs((B, T, V), dtype, 110, layout)
+    g = _gen(111)
+    few = min(300, V // 2)
+    kind = torch.randint(0, 10, (B, T), device=DEV, generator=g)
+    low = torch.finfo(dtype).min
+    tokens = torch.where(kind < 3, tokens % few, tokens)
+    x[..., :few].masked_fill_((kind == 0).unsqueeze(-1), -150.0)
+    x[..., 1:].masked_fill_((kind == 1).unsqueeze(-1), float("-inf"))
+    tokens.masked_fill_(kind == 1, 0)
+    x.masked_fill_((kind == 2).unsqueeze(-1), low)
+    x[..., :-1].masked_fill_((kind == 3).unsqueeze(-1), low)
+    tokens.masked_fill_(kind == 3, V - 1)
+    keep = torch.rand(B, T, device=DEV, generator=g) < 0.7
+    keep[5] = False
+    logp = torch.stack([_logp64(x[b], tokens[b]) for b in range(B)])
+    old = (logp - 0.1).float()
+    adv = torch.randn(B, 1, device=DEV, generator=g)
+    dout = torch.randn(B, T, device=DEV, generator=g)
+    n = keep.sum().item()
+    leaf = x.detach().requires_grad_(True)
+    out = token_logprobs(leaf, tokens, mask=keep)
+    _assert_logp(out.detach()[keep], logp[keep])
+    assert (out.detach()[~keep] == 0).all()
+    d, = torch.autograd.grad(out, leaf, dout)
+    r = policy_loss(leaf, tokens, old, adv, mask=keep, clip_low=0.5, clip_high=0.5)
+    dp, = torch.autograd.grad(r.loss, leaf)
+    plain = policy_loss(x, tokens, old, adv, mask=keep, clip_low=0.5, clip_high=0.5)
+    for a, b in zip(plain, r):
+        assert torch.equal(a, b.detach())
+    # the scale's rounding to 32 bits, the base's and their product's: 2^-22 of a logit's distance
+    loose = LOGP_TOL + 2.0 ** -22 * logp.abs()
+    assert ((r.logprobs.double() - logp).abs() <= loose)[keep].all()
+    ratio = (logp - old.double()).exp()
+    per = torch.where(keep, ratio * adv.double(), torch.zeros_like(ratio)) / n
+    assert abs(r.loss.item() + per.sum().item()) <= (per.abs() * (loose + 2.0 ** -22)).sum().item() + 1e-12
+    u = torch.finfo(dtype).eps / 2
+    least = 2.0 ** -25 if dtype == torch.float16 else 1e-37
+    for b in range(B):
+        one = slice(b, b + 1)
+        _assert_grad(d[one], x[one], tokens[one], torch.where(keep, dout, torch.zeros_like(dout))[one].double())
+        p = torch.softmax(x[one].double(), -1)
+        hot = torch.zeros_like(p).scatter_(-1, tokens[one].unsqueeze(-1), 1.0)
+        gg = -per[one].unsqueeze(-1)
+        exact = gg * (hot - p)
+        tol = exact.abs() * (u * 1.001 + loose[one].unsqueeze(-1) + 2.0 ** -20) + gg.abs() * (2.0 ** -18 * p + 2.0 ** -23)
+        assert ((dp[one].double() - exact).abs() <= tol + least).all()
+    assert (dp[~keep] == 0).all() and (d[~keep] == 0).all()
+    assert _lib.device_timeouts() == 0
