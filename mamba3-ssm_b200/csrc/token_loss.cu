@@ -286,11 +286,16 @@ inline PolicyWs policy_ws(void* ws, int64_t batch, int64_t rows, size_t* bytes) 
 // Positions that count, by sequence and in all, and the rows' order: those first, so that
 // they spread evenly whatever the mask. A warp takes 256 positions and adds its (whole) numbers
 // to counters that are zero at the start, so the counts do not depend on the schedule. The
-// order within the two groups does, but no result depends on it.
-constexpr int kCountThreads = 128, kCountRows = 256;
+// order within the two groups does, but no result depends on it. A single CTA, which few
+// positions need, zeroes the counters itself.
+constexpr int kCountThreads = 256, kCountRows = 256;
 __global__ void __launch_bounds__(kCountThreads) policy_count_kernel(TokenRows p, bool by_sequence, PolicyWs w) {
   const int lane = threadIdx.x & 31, R = (int)p.R;
   const int r0 = ((blockIdx.x * kCountThreads + threadIdx.x) >> 5) * kCountRows;
+  if (gridDim.x == 1) {
+    for (int i = threadIdx.x; i < (int)(w.zeroed / 4); i += kCountThreads) reinterpret_cast<int*>(w.head)[i] = 0;
+    __syncthreads();
+  }
   if (r0 >= R) return;
   unsigned flags = 0;  // bit k: position r0 + 32 k + lane
 #pragma unroll
@@ -390,6 +395,7 @@ struct RowOut {
   float* coef;
   void* dlogits;
   int64_t dsb, dst;
+  unsigned* clear;  // zero for the kernel that follows; may be null
 };
 
 // The gradient of one row: g (one-hot - softmax). tok < 0: no element is the token's.
@@ -647,6 +653,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_rows_kernel(TokenRows p, 
   const int64_t b = r / p.T, t = r - b * p.T;
   constexpr int nt = NT;
   const int tid = threadIdx.x, lane = tid & 31;
+  if constexpr (!POLICY)
+    if (o.clear && blockIdx.x == 0 && threadIdx.x == 0) *o.clear = 0;
   const T* row = static_cast<const T*>(p.logits) + b * p.sb + t * p.st;
   T* drow = nullptr;
   if constexpr (POLICY)
@@ -1056,6 +1064,8 @@ __global__ void __launch_bounds__(kWarpThreads, kWarpCtas<POLICY>)
   __shared__ WarpRowsShared<T, G> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Vec<T>* const place = reinterpret_cast<Vec<T>*>(places_raw) + (size_t)warp * each * row_vecs;
+  if constexpr (!POLICY)
+    if (o.clear && blockIdx.x == 0 && threadIdx.x == 0) *o.clear = 0;
   if (threadIdx.x == 0) {
     for (int k = 0; k < W; ++k) sm100::mbar_init(&sh.full[k], 1);
     sh.dead = 0;
@@ -1566,7 +1576,7 @@ size_t preference_workspace_bytes(int64_t batch, int64_t rows) {
 }
 
 int launch_token_logprobs(const TokenRows& p, int dtype, float* logp, float2* stats, cudaStream_t s) {
-  return launch_rows_of<false>(p, dtype, PolicyArgs{}, PolicyWs{}, RowOut{logp, nullptr, stats, nullptr, nullptr, 0, 0}, s);
+  return launch_rows_of<false>(p, dtype, PolicyArgs{}, PolicyWs{}, RowOut{logp, nullptr, stats, nullptr, nullptr, 0, 0, nullptr}, s);
 }
 
 int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64_t batch, float* loss, float* kl,
@@ -1574,12 +1584,15 @@ int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64
   M3_TRY(check_rows(p));
   size_t bytes = 0;
   const PolicyWs w = policy_ws(ws, batch, p.R, &bytes);
-  cudaError_t e = cudaMemsetAsync(w.head, 0, w.zeroed, s);
-  if (e != cudaSuccess) return fail(M3_ERR_CUDA, std::string("policy loss: ") + cudaGetErrorString(e));
   const int64_t warps = (p.R + kCountRows - 1) / kCountRows, per = kCountThreads / 32;
-  policy_count_kernel<<<(unsigned)((warps + per - 1) / per), kCountThreads, 0, s>>>(p, a.by_sequence != 0, w);
+  const int64_t ctas = std::max<int64_t>(1, (warps + per - 1) / per);
+  if (ctas > 1) {
+    cudaError_t e = cudaMemsetAsync(w.head, 0, w.zeroed, s);
+    if (e != cudaSuccess) return fail(M3_ERR_CUDA, std::string("policy loss: ") + cudaGetErrorString(e));
+  }
+  policy_count_kernel<<<(unsigned)ctas, kCountThreads, 0, s>>>(p, a.by_sequence != 0, w);
   M3_TRY(check_launch("policy_count_kernel"));
-  M3_TRY(launch_rows_of<true>(p, dtype, a, w, RowOut{logp, nullptr, w.stats, w.coef, dlogits, dsb, dst}, s));
+  M3_TRY(launch_rows_of<true>(p, dtype, a, w, RowOut{logp, nullptr, w.stats, w.coef, dlogits, dsb, dst, nullptr}, s));
   policy_sum_kernel<<<(unsigned)((p.R + kSumRows - 1) / kSumRows), kSumThreads, 0, s>>>(p.R, w, loss, kl, clipped);
   return check_launch("policy_sum_kernel");
 }
@@ -1589,10 +1602,12 @@ int launch_preference_loss(const TokenRows& p, int dtype, Map2<const float> ref,
   M3_TRY(check_rows(p));
   size_t bytes = 0;
   const PrefWs w = pref_ws(ws, 2 * pairs, p.R, &bytes);
-  cudaError_t e = cudaMemsetAsync(w.done, 0, sizeof(unsigned), s);
-  if (e != cudaSuccess) return fail(M3_ERR_CUDA, std::string("preference loss: ") + cudaGetErrorString(e));
+  if (p.R == 0) {  // else the rows' kernel does it
+    cudaError_t e = cudaMemsetAsync(w.done, 0, sizeof(unsigned), s);
+    if (e != cudaSuccess) return fail(M3_ERR_CUDA, std::string("preference loss: ") + cudaGetErrorString(e));
+  }
   M3_TRY(launch_rows_of<false>(p, dtype, PolicyArgs{}, PolicyWs{},
-                               RowOut{logp, w.logp, w.stats, nullptr, nullptr, 0, 0}, s));
+                               RowOut{logp, w.logp, w.stats, nullptr, nullptr, 0, 0, w.done}, s));
   preference_pairs_kernel<<<(unsigned)(2 * pairs), kSumThreads, 0, s>>>(p, ref, beta, smoothing, (int)pairs, w, loss,
                                                                        rewards);
   return check_launch("preference_pairs_kernel");

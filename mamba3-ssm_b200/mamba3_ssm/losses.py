@@ -215,6 +215,7 @@ class _PolicyLossFn(torch.autograd.Function):
             ctx.held = (ws, temperature, ignore_index)
             ctx.dlogits = dlogits
             ctx.mark_non_differentiable(logp, means)
+            ctx.set_materialize_grads(False)  # no zeros for the outputs without a gradient
         return loss, logp, means
 
     @staticmethod
@@ -261,6 +262,7 @@ class _PreferenceLossFn(torch.autograd.Function):
             ctx.save_for_backward(logits, tokens, mask)
             ctx.held = (ws, temperature, ignore_index)
             ctx.mark_non_differentiable(rewards, logp)
+            ctx.set_materialize_grads(False)  # no zeros for the outputs without a gradient
         return loss, rewards, logp
 
     @staticmethod

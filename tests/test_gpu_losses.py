@@ -854,3 +854,30 @@ def test_many_short_rows(T, V, layout, dtype):
         assert ((dp[one].double() - exact).abs() <= tol + least).all()
     assert (dp[~keep] == 0).all() and (d[~keep] == 0).all()
     assert _lib.device_timeouts() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [1, 2, 7, 9, 31, 70])
+def test_many_rows_of_a_few_logits(V, dtype):
+    """Rows with few or no whole vectors, on every boundary, several to a warp."""
+    from mamba3_ssm import policy_loss, token_logprobs
+    x, tokens = _inputs((41, 1000, V), dtype, 120)
+    logp = _logp64(x, tokens)
+    leaf = x.detach().requires_grad_(True)
+    dout = torch.randn(41, 1000, device=DEV, generator=_gen(121))
+    out = token_logprobs(leaf, tokens)
+    _assert_logp(out.detach(), logp)
+    d, = torch.autograd.grad(out, leaf, dout)
+    _assert_grad(d, x, tokens, dout.double())
+    old = (logp - 0.1).float()
+    r = policy_loss(leaf, tokens, old, dout, clip_low=0.5, clip_high=0.5)
+    _assert_logp(r.logprobs, logp)
+    dp, = torch.autograd.grad(r.loss, leaf)
+    p = torch.softmax(x.double(), -1)
+    hot = torch.zeros_like(p).scatter_(-1, tokens.unsqueeze(-1), 1.0)
+    gg = -((logp - old.double()).exp() * dout.double() / 41000).unsqueeze(-1)
+    exact = gg * (hot - p)
+    # the ratio carries the log-probability's tolerance, p its own
+    tol = exact.abs() * (torch.finfo(dtype).eps / 2 * 1.001 + 2.0 ** -18) + gg.abs() * (2.0 ** -18 * p + 2.0 ** -23)
+    tol = tol + (2.0 ** -25 if dtype == torch.float16 else 1e-37)
+    assert ((dp.double() - exact).abs() <= tol).all()
