@@ -1424,8 +1424,16 @@ int plan_rows(const TokenRows& p, int64_t elem, bool policy, RowPlan* out) {
     while (C < 8 && bytes / C > kPlaceBytes) C *= 2;
   out->C = C;
   // small CTAs stream best (1200 rows of 100 KB: 24.9 us with 128 threads, 25.4 with 256, 31.7
-  // with 512); a CTA that keeps its part needs warps enough for the whole of it
-  out->threads = !policy || bytes / C <= 16 * 1024 ? 128 : bytes / C <= 52 * 1024 ? 256 : 512;
+  // with 512); a CTA that keeps its part needs warps enough for the whole of it. 16-bit rows want
+  // as many bytes of an SM's shared memory in use as there are (six, four to three, or two CTAs;
+  // bf16 loss and gradient read and written, with the limits of wide rows and with these: rows of
+  // 16384 logits 5.0, 5.3 TB/s, of 32000 4.7, 5.25, of 131072 4.4, 5.0); 32-bit rows, whose
+  // arithmetic is half as much a byte, do better with less of it (17000 logits with 512 threads
+  // twice 6.2 TB/s, with 256 three times 5.6) unless larger clusters wait for one another (57000
+  // logits: 4.9, 6.2). Few rows: more threads to each.
+  const int64_t part = bytes / C;
+  const bool wide = (elem == 4 && C < 4) || p.R * C < 4 * (int64_t)sms;
+  out->threads = !policy || part <= (wide ? 16 : 34) * 1024 ? 128 : part <= (wide ? 52 : 72) * 1024 ? 256 : 512;
   out->slot_vecs = bytes / C <= kPlaceBytes ? (int)(bytes / C / 16 + 2) : 0;
   return M3_OK;
 }
@@ -1487,7 +1495,13 @@ int launch_grad_rows(const TokenRows& p, const PolicyArgs& a, const PolicyWs& w,
   if (pieces > kPieces) return fail(M3_ERR_UNSUPPORTED, "token rows: row too long");
   plan.threads = NT + 32;
   static ClusterCache cache;
-  return launch_clusters(kernel, plan, p.R, &cache, (size_t)plan.slot_vecs * 16, s, p, a, w, o, pieces);
+  int sms = 0;
+  M3_TRY(device_sm_count(&sms));
+  const size_t smem = (size_t)plan.slot_vecs * 16;
+  // 32-bit rows: up to 144 KB of an SM in use (rows of 10000 logits: three CTAs 6.17 TB/s, four
+  // 5.6; of 11000: three 6.17, two 5.3)
+  const int64_t some = sizeof(T) == 4 && plan.C == 1 ? sms * std::max<int64_t>(2, 144 * 1024 / (int64_t)smem) : p.R;
+  return launch_clusters(kernel, plan, std::min(some, p.R), &cache, smem, s, p, a, w, o, pieces);
 }
 
 template <typename T, bool POLICY, int G>
