@@ -640,9 +640,10 @@ __device__ __forceinline__ void join_row(const TokenRows& p, const PolicyArgs& a
 
 // One cluster of CTAs (of one CTA where there are rows enough) per row. A policy gradient of
 // rows too long for token_grad_rows_kernel is written from a second reading.
-// Bound by the memory: 676 MB (6720 rows of 50280 bf16 logits that count, of 11200) in 117 us,
-// 5.8 TB/s, 88% of a copy's rate; 1200 such rows of 2000 in 25 us (4.8 TB/s: the last rows run
-// beside few others). Eight loads in flight per thread: with four 29 us.
+// Bound by the memory: 7952 rows of 50277 bf16 logits in 126 us, 6.3 TB/s, 97% of a copy's rate;
+// 1200 such rows of 2000 in 25 us (4.9 TB/s: the last rows run beside few others). Eight loads in
+// flight per thread, the first while the base is found and the last, which do not fill a turn,
+// all at once as well: with those one by one rows of 24000 logits had 4.8 TB/s instead of 6.1.
 template <typename T, bool POLICY, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) token_rows_kernel(TokenRows p, PolicyArgs a, PolicyWs w, RowOut o) {
   constexpr int U = 8;  // loads in flight per thread
@@ -673,17 +674,26 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_rows_kernel(TokenRows p, 
   TokenOps x{};
   if constexpr (POLICY)
     if (tid == 0) x = token_ops(a, w, b, t, even_weight(a, w));
+  Vec<T> v[U];
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j0 + tid + u * nt < n) v[u] = mine[j0 + tid + u * nt];
+  };
+  load(0);  // while the base is found
   const Base base = base_at(fmaxf(warp_max(first_max(row, p.V, c, lane)), at_token), p.c_hi);
   Sum s2{0.f, 0.f};
-  int j = tid;
-  for (; j + (U - 1) * nt < n; j += U * nt) {
-    Vec<T> v[U];
+  for (int j0 = 0; j0 < n; j0 += U * nt) {
+    if (j0 > 0) load(j0);
+    if (j0 + U * nt <= n) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = mine[j + u * nt];
+      for (int u = 0; u < U; ++u) add_vec<false, !POLICY>(s2, v[u], base, p.c_hi, p.c_lo);
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) add_vec<false, !POLICY>(s2, v[u], base, p.c_hi, p.c_lo);
+      for (int u = 0; u < U; ++u)
+        if (j0 + tid + u * nt < n) add_vec<false, !POLICY>(s2, v[u], base, p.c_hi, p.c_lo);
+    }
   }
-  for (; j < n; j += nt) add_vec<false, !POLICY>(s2, mine[j], base, p.c_hi, p.c_lo);
   float s = s2.total();
   if (rank == 0) {
     for (int i = tid; i < c.head; i += nt) s += exp_one<!POLICY>(to_f32(row[i]), base, p.c_hi, p.c_lo);
@@ -1344,7 +1354,8 @@ __global__ void __launch_bounds__(kSumThreads)
 // The gradient of the logits from the rows' (m, S). A group of G threads takes a part of a row
 // at a time, parts from the end (the forward read the end last, so some of it is still in the
 // L2 cache; the stores are marked to leave it there). Bound by the memory: 11200 rows of 50280
-// bf16 logits, 0.6 of them counting, 1.80 GB in 0.28 ms, 6.4 TB/s.
+// bf16 logits, 0.6 of them counting, 1.80 GB in 0.28 ms, 6.4 TB/s. The last loads of a thread,
+// fewer than kGradU, are in flight together too (rows of 6000 logits 6.55 TB/s, 6.0 one by one).
 constexpr int kGradThreads = 256;
 constexpr int kGradU = 4;  // loads in flight per thread
 template <typename T, int G>
@@ -1377,24 +1388,28 @@ __global__ void __launch_bounds__(kGradThreads, 4)
     uint4* const to = reinterpret_cast<uint4*>(out + c.head);
     const bool same = same_boundary(out, c);
     const int kind = !same || gr.base.far ? 3 : sizeof(T) == 2 && gr.folded ? 1 : 2;
-    int j = v0 + tid;
-    if (kind != 3) {
-      for (; j + (kGradU - 1) * G < v1; j += kGradU * G) {
-        Vec<T> v[kGradU];
+    for (int j = v0 + tid; j < v1; j += kGradU * G) {
+      Vec<T> v[kGradU];
+      const bool full = j + (kGradU - 1) * G < v1;
 #pragma unroll
-        for (int k = 0; k < kGradU; ++k) v[k] = rv[j + k * G];
-        if (kind == 1) {
-          if constexpr (sizeof(T) == 2) {
+      for (int k = 0; k < kGradU; ++k)
+        if (full || j + k * G < v1) v[k] = rv[j + k * G];
+      if (kind == 1) {
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-            for (int k = 0; k < kGradU; ++k) __stcs(to + j + k * G, vec_grad_folded(v[k], gr.kg, gr.negative, p.c_hi).u);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < kGradU; ++k) __stcs(to + j + k * G, vec_grad<false>(v[k], gr, p.c_hi, p.c_lo).u);
+          for (int k = 0; k < kGradU; ++k)
+            if (full || j + k * G < v1) __stcs(to + j + k * G, vec_grad_folded(v[k], gr.kg, gr.negative, p.c_hi).u);
         }
+      } else if (kind == 2) {
+#pragma unroll
+        for (int k = 0; k < kGradU; ++k)
+          if (full || j + k * G < v1) __stcs(to + j + k * G, vec_grad<false>(v[k], gr, p.c_hi, p.c_lo).u);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kGradU; ++k)
+          if (full || j + k * G < v1) put_grad(v[k], j + k * G, out, c, gr, same, p.c_hi, p.c_lo);
       }
     }
-    for (; j < v1; j += G) put_grad(rv[j], j, out, c, gr, same, p.c_hi, p.c_lo);
     if (gr.tok >= 0) gr.at = to_f32(row[gr.tok]);  // a row's loads need not wait for it
     put_token(out, c, gr, v0, v1, tid, G, p.c_hi, p.c_lo);
     if (part == 0) put_ends(row, out, p.V, c, gr, tid, G, p.c_hi, p.c_lo);
@@ -1652,10 +1667,12 @@ static int launch_grad(const TokenRows& p, const float2* stats, Map2<const float
     token_grad_kernel<T, G><<<(unsigned)(keep_if_one ? std::min(need, ctas) : need), kGradThreads, 0, s>>>(
         p, stats, coef, up, keep_if_one, d, dsb, dst, 1, (int)p.R);
   };
-  if (bytes <= 8192 || (bytes <= 24576 && p.R >= 8 * ctas)) {
+  // a warp or less per row: up to 40 KB where there are rows for all warps (13000 bf16 logits 6.3
+  // TB/s, 5.4 with a CTA per row; 20000 6.2, 6.0; 24000 6.2, 6.4)
+  if (bytes <= 8192 || (bytes <= 40960 && p.R >= 8 * ctas)) {
     // Lanes of a row: short rows leave a warp's idle, and each has its position to find (bf16, of
     // 4, 8, 16 and 32 lanes: 300 logits 5.0, 4.5, 2.5, 1.6 TB/s; 1000 5.1, 5.9, 5.2, 3.7; 2047 5.2,
-    // 6.1, 6.4, 5.7; 4096 logits 6.8 with 32). Few rows: as many lanes as keep the device's busy.
+    // 6.1, 6.4, 5.7; 4096 6.7 with 32). Few rows: as many lanes as keep the device's busy.
     int g = bytes <= 1024 ? 4 : bytes <= 2560 ? 8 : bytes <= 6144 ? 16 : 32;
     while (g < 32 && p.R * g < ctas * kGradThreads) g *= 2;
     if (g == 4) by_rows(std::integral_constant<int, 4>{});
