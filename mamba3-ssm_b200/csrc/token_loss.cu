@@ -169,10 +169,18 @@ __device__ __forceinline__ void add_vec(Sum& s, const Vec<T>& v, const Base& b, 
   constexpr int N = Vec<T>::N;
   float l[N];
   unpack(v, l);
+  if constexpr (N == 8) {
+    // a vector's terms first: as many additions, a quarter of them to a large sum
 #pragma unroll
-  for (int k = 0; k < N; k += 2) {
-    s.a += exp2_approx(exponent<FAR, FINE>(l[k], b, c_hi, c_lo));
-    s.b += exp2_approx(exponent<FAR, FINE>(l[k + 1], b, c_hi, c_lo));
+    for (int k = 0; k < N; ++k) l[k] = exp2_approx(exponent<FAR, FINE>(l[k], b, c_hi, c_lo));
+    s.a += (l[0] + l[2]) + (l[4] + l[6]);
+    s.b += (l[1] + l[3]) + (l[5] + l[7]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      s.a += exp2_approx(exponent<FAR, FINE>(l[k], b, c_hi, c_lo));
+      s.b += exp2_approx(exponent<FAR, FINE>(l[k + 1], b, c_hi, c_lo));
+    }
   }
 }
 template <bool FINE, typename T>
