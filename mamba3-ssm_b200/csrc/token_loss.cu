@@ -6,8 +6,8 @@
 //   d logp / d l[v] = s (1[v = tok] - 2^(c (l[v] - m)) / S)
 // m is the largest of the row's first elements and the token's own (a likely one, in earnest):
 // every warp finds the same m by itself, sums of all warps (and CTAs) join by addition, and no
-// element passes through a second rounding exponential. Where S then leaves 2^-60 .. 2^100 the
-// row is done again with its true maximum.
+// element passes through a second rounding exponential. Where S then leaves 2^-60 .. 2^20 the
+// row is done again with its true maximum (in_range says why).
 // c is held in two floats: one float's rounding (up to 3e-8 of c) would move every
 // log-probability of a sequence the same way, and the preference loss sums them.
 // The element work runs in 32 bits; log-probabilities and their differences, once a row, in 64.
@@ -568,8 +568,12 @@ __device__ __forceinline__ GradRow finish_row(const TokenRows& p, const PolicyAr
   return grad_row(base, (float)((double)coef * p.scale), Sn, tok, at_token);
 }
 
-// Whether a sum over an assumed base can be trusted (false for NaN too).
-__device__ __forceinline__ bool in_range(float S) { return S > 8.673617e-19f && S < 1.2676506e30f; }  // 2^-60, 2^100
+// Whether a sum over an assumed base can be trusted (false for NaN too). Logits up to log2 S above
+// the base have exponents that large, whose roundings (three of half a step) and lacking lower half
+// of c (2^-23 of the exponent) move p by ln 2 (3 * 2^-20 + 20 * 2^-23) = 2^-18 at S = 2^20. Far above
+// that p loses more, and the gradient's factor g / S leaves the normal numbers where g is small.
+// Logits that are all alike have S = V, so that the bound has to be above a vocabulary's size.
+__device__ __forceinline__ bool in_range(float S) { return S > 8.673617e-19f && S < 1048576.f; }  // 2^-60, 2^20
 
 template <bool POLICY>
 struct RowShared {

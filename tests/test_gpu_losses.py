@@ -881,3 +881,39 @@ def test_many_rows_of_a_few_logits(V, dtype):
     tol = exact.abs() * (torch.finfo(dtype).eps / 2 * 1.001 + 2.0 ** -18) + gg.abs() * (2.0 ** -18 * p + 2.0 ** -23)
     tol = tol + (2.0 ** -25 if dtype == torch.float16 else 1e-37)
     assert ((dp.double() - exact).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("gap", [49.0, 65.0])
+@pytest.mark.parametrize("V", [2000, 30000, 140000])
+def test_small_gradients_of_misleading_rows(V, gap):
+    """A base far below the maximum makes the sum large and the upstream gradient over it small:
+    it must not leave the normal numbers (dlogp 1e-14 with the maximum 65 above the base would)."""
+    from mamba3_ssm import policy_loss, token_logprobs
+    x = torch.zeros(1, 3, V, device=DEV)
+    tokens = torch.zeros(1, 3, dtype=torch.long, device=DEV)
+    x[0, :, V - 9] = gap
+    x.requires_grad_(True)
+    dout = torch.full((1, 3), 1e-14, device=DEV)
+    d, = torch.autograd.grad(token_logprobs(x, tokens), x, dout)
+    _assert_grad(d, x.detach(), tokens, dout.double())
+    r = policy_loss(x, tokens, _logp64(x.detach(), tokens).float(), dout)
+    d, = torch.autograd.grad(r.loss, x)
+    # ratios of 1, off by old's rounding (2^-24 of up to 65) and the tolerance of a log-probability
+    exact = -dout.double() / 3
+    top = -exact * torch.softmax(x.detach().double(), -1)[..., V - 9]
+    assert ((d[..., V - 9].double() - top).abs() <= 2.0 ** -17 * top.abs()).all()
+    assert ((d[..., 0].double() - exact).abs() <= 2.0 ** -17 * exact.abs()).all()
+
+
+@pytest.mark.parametrize("V", [700, 9000, 60001, 140000])
+def test_gradients_where_the_maximum_is_far_above_the_first_elements(V):
+    """A low temperature spreads the scaled logits over hundreds: the first elements' maximum is
+    tens below the row's, and the tolerances are those of any row."""
+    from mamba3_ssm import token_logprobs
+    x, tokens = _inputs((2, 40, V), torch.float32, 117)
+    x.requires_grad_(True)
+    dout = torch.randn(2, 40, device=DEV, generator=_gen(118))
+    out = token_logprobs(x, tokens, temperature=0.1)
+    _assert_logp(out.detach(), _logp64(x.detach(), tokens, 0.1))
+    d, = torch.autograd.grad(out, x, dout)
+    _assert_grad(d, x.detach(), tokens, dout.double(), 0.1)
