@@ -1142,9 +1142,9 @@ int aligned(const m3_tensor* t, const char* name, size_t bytes) {
   return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": address not aligned to " + std::to_string(bytes) + " bytes");
 }
 
-// The rows that every token loss reads; *empty: there is no position.
+// The rows that every token loss reads; *empty: there is no position. policy: its scale is one float.
 int token_rows(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor* mask, double temperature,
-               int64_t ignore_index, TokenRows* p, bool* empty) {
+               int64_t ignore_index, bool policy, TokenRows* p, bool* empty) {
   if (!present(logits)) return fail(M3_ERR_INVALID_ARGUMENT, "logits: missing");
   if (logits->ndim != 3) return fail(M3_ERR_INVALID_ARGUMENT, "logits: expected (batch, seqlen, vocabulary)");
   const int64_t* sh = logits->shape;
@@ -1163,12 +1163,13 @@ int token_rows(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor
   p->R = sh[0] * sh[1]; p->T = (int)sh[1]; p->V = (int)sh[2];
   p->ignore = ignore_index;
   p->scale = 1.0 / temperature;
-  // c in two floats, the upper one rounded down so that the lower one is positive
+  // c in two floats, the upper one rounded down so that the lower one is positive, or in one,
+  // rounded to the nearest
   const double c = p->scale * 1.44269504088896340736;
   float hi = (float)c;
-  if ((double)hi >= c) hi = std::nextafterf(hi, 0.f);
+  if (!policy && (double)hi >= c) hi = std::nextafterf(hi, 0.f);
   p->c_hi = hi;
-  p->c_lo = (float)(c - (double)hi);
+  p->c_lo = policy ? 0.f : (float)(c - (double)hi);
   return M3_OK;
 }
 
@@ -1194,7 +1195,7 @@ int m3_token_logprobs(const m3_tensor* logits, const m3_tensor* tokens, const m3
                       int64_t ignore_index, m3_tensor* logprobs, m3_tensor* stats, void* stream) {
   TokenRows p{};
   bool empty = false;
-  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, false, &p, &empty));
   const int64_t bt[3] = {logits->shape[0], logits->shape[1], 2};
   M3_TRY(check(logprobs, "logprobs", 2, bt, kF32, true, false, !empty));
   M3_TRY(check(stats, "stats", 3, bt, kF32, true, true, !empty));
@@ -1216,7 +1217,7 @@ int m3_policy_loss(const m3_tensor* logits, const m3_tensor* tokens, const m3_te
                    m3_tensor* dlogits, void* workspace, size_t workspace_bytes, void* stream) {
   TokenRows p{};
   bool empty = false;
-  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, true, &p, &empty));
   const int64_t* sh = logits->shape;
   const int64_t bt[2] = {sh[0], sh[1]};
   if (!(clip_low >= 0 && clip_low <= 1)) return fail(M3_ERR_INVALID_ARGUMENT, "clip_low: expected a number from 0 to 1");
@@ -1258,7 +1259,7 @@ int m3_preference_loss(const m3_tensor* logits, const m3_tensor* tokens, const m
                        void* workspace, size_t workspace_bytes, void* stream) {
   TokenRows p{};
   bool empty = false;
-  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, false, &p, &empty));
   const int64_t* sh = logits->shape;
   if (sh[0] % 2 != 0 || sh[0] == 0)
     return fail(M3_ERR_INVALID_ARGUMENT, "logits: an even number of sequences expected, chosen before rejected");
@@ -1284,7 +1285,7 @@ int loss_grad(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor*
               size_t workspace_bytes, bool policy, cudaStream_t s) {
   TokenRows p{};
   bool empty = false;
-  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, policy, &p, &empty));
   const int64_t* sh = logits->shape;
   M3_TRY(check(dlogits, "dlogits", 3, sh, 1u << logits->dtype, false, false, !empty));
   if (!empty) M3_TRY(aligned(dlogits, "dlogits", dtype_size(logits->dtype)));
@@ -1319,7 +1320,7 @@ int m3_token_logprobs_grad(const m3_tensor* logits, const m3_tensor* tokens, con
                            int64_t ignore_index, m3_tensor* dlogits, void* stream) {
   TokenRows p{};
   bool empty = false;
-  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, &p, &empty));
+  M3_TRY(token_rows(logits, tokens, mask, temperature, ignore_index, false, &p, &empty));
   const int64_t* sh = logits->shape;
   const int64_t bt[3] = {sh[0], sh[1], 2};
   Map2<const float> c;

@@ -8,8 +8,9 @@
 // every warp finds the same m by itself, sums of all warps (and CTAs) join by addition, and no
 // element passes through a second rounding exponential. Where S then leaves 2^-60 .. 2^20 the
 // row is done again with its true maximum (in_range says why).
-// c is held in two floats: one float's rounding (up to 3e-8 of c) would move every
-// log-probability of a sequence the same way, and the preference loss sums them.
+// c is held in two floats: one float's rounding (up to 6e-8 of c) would move every
+// log-probability of a sequence the same way, and the preference loss sums them. The policy loss
+// takes c rounded to the nearest float.
 // The element work runs in 32 bits; log-probabilities and their differences, once a row, in 64.
 //
 // What bounds it: every logit is read once (twice where the gradient has to wait for other rows,
@@ -136,12 +137,14 @@ __device__ __forceinline__ Base base_at(float m, float c_hi) {
 
 // The exponent of a logit. FINE: with c's lower half too (c_lo is positive, so that l = -inf
 // stays -inf); it then carries m c_lo, which norm_sum takes off the sum. The policy loss does
-// without: 1 / temperature is then off by 3e-8 of itself at most, for S and for the token alike.
+// without, c_hi being the float nearest to c: scale is then off by 2^-24 of itself at most, for
+// S and for the token alike, which moves a log-probability by 2^-24 s (l[tok] - mean of l under
+// p), at most half a step of the 32-bit result of an unlikely token.
 template <bool FAR, bool FINE>
 __device__ __forceinline__ float exponent(float l, const Base& b, float c_hi, float c_lo) {
   if constexpr (FAR) {
     const float d = l - b.m;
-    return fmaf(d, c_hi, d * c_lo);
+    return FINE ? fmaf(d, c_hi, d * c_lo) : d * c_hi;
   } else if constexpr (FINE) {
     return fmaf(l, c_lo, fmaf(l, c_hi, b.k));
   } else {
@@ -547,7 +550,7 @@ __device__ __forceinline__ GradRow finish_row(const TokenRows& p, const PolicyAr
                                               const TokenOps& x, int64_t r, float at_token, int tok, const Base& base,
                                               Joined<POLICY> S, bool lead) {
   // the token's exponent exactly as the sum's elements have theirs
-  const double c = POLICY && !base.far ? (double)p.c_hi : (double)p.c_hi + (double)p.c_lo;
+  const double c = POLICY ? (double)p.c_hi : (double)p.c_hi + (double)p.c_lo;
   const double at = base.far ? ((double)at_token - (double)base.m) * c : fma((double)at_token, c, (double)base.k);
   const double logp = at * kLn2 - log_sum(S);
   float coef = 0.f;

@@ -304,7 +304,8 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
     ``kl_coef`` must be 0); with them ``kl`` is reported also for kl_coef 0.
     Where the logits need a gradient it is formed in the forward pass, so that they are read
     once; a loss that is scaled before backward() costs a second pass over them.
-    Returns PolicyLoss(loss, logprobs, kl, clip_fraction)."""
+    Returns PolicyLoss(loss, logprobs, kl, clip_fraction). ``logprobs`` are within a few roundings
+    of token_logprobs' (1 / temperature is held in one float here, in two there), not its bits."""
     name = "policy_loss"
     if reduction not in ("token", "sequence"):
         raise ValueError(f"{name}: reduction is 'token' or 'sequence', got {reduction!r}")

@@ -917,3 +917,28 @@ def test_gradients_where_the_maximum_is_far_above_the_first_elements(V):
     _assert_logp(out.detach(), _logp64(x.detach(), tokens, 0.1))
     d, = torch.autograd.grad(out, x, dout)
     _assert_grad(d, x.detach(), tokens, dout.double(), 0.1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V", [(4096, 5001), (600, 30011)])
+@pytest.mark.parametrize("temperature", [0.7, 0.8, 2.88])
+def test_policy_logprobs_of_unlikely_tokens(temperature, rows, V, dtype):
+    """The policy loss holds scale = log2(e) / temperature in one float, rounded to the nearest: a
+    log-probability is off by that rounding times scale (l[token] - mean of l under p), the same
+    way in every row. Mean error of the rows: that, the sums' (LOGP_TOL), and what is left of
+    the results' own rounding, evenly spread over a step (six standard deviations)."""
+    from mamba3_ssm import policy_loss
+    x, tokens = _inputs((1, rows, V), dtype, 114)
+    x.scatter_(-1, tokens.unsqueeze(-1), -100.0 * temperature)
+    ref = _logp64(x, tokens, temperature)
+    zero = torch.zeros(1, rows, device=DEV)
+    got = policy_loss(x, tokens, old_logprobs=ref.float(), advantages=zero + 1, temperature=temperature).logprobs
+    mean = (torch.softmax(x.double() / temperature, -1) * x.double()).sum(-1)
+    c = 1.0 / math.log(2.0) / temperature
+    rounding = abs(torch.tensor(c, dtype=torch.float64).float().item() / c - 1.0)
+    assert rounding <= 2.0 ** -24
+    moved = rounding * ((x.double().gather(-1, tokens.unsqueeze(-1)).squeeze(-1) - mean) / temperature).abs().max().item()
+    step = 2.0 ** -17  # of results between 64 and 128
+    assert ((ref < -64) & (ref > -128)).all()
+    left = 6 * step / math.sqrt(12 * rows)
+    assert abs((got.double() - ref).mean().item()) <= moved + LOGP_TOL + left
