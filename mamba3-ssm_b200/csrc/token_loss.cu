@@ -122,16 +122,17 @@ __device__ __forceinline__ RowCut cut_row(const T* row, int V) {
   return c;
 }
 
-// What comes off a row's logits before the exponential. `far`: so large (masked entries at a
-// type's lowest value in a row that has no others, or an infinity) that c * base could
-// overflow; the difference is then formed first.
+// What comes off a row's logits before the exponential. `far`: so large (a mask's constant in a
+// row that has nothing else, or an infinity) that the rounding of c * base, which every exponent
+// of the row has in common, could leave an exponent's range; the difference is then formed first.
+// Below 2^20 that rounding is 2^-5 at most, and base * c_lo 2^-3.
 struct Base {
   float m, k;  // the base and -c_hi * base
   bool far;
 };
 __device__ __forceinline__ Base base_at(float m, float c_hi) {
   if (m == -INFINITY) m = 0.f;
-  const bool far = !(fabsf(m) < 1e30f);
+  const bool far = !(fabsf(m) * c_hi < 1048576.f);
   return Base{m, far ? 0.f : -(m * c_hi), far};
 }
 

@@ -942,3 +942,55 @@ def test_policy_logprobs_of_unlikely_tokens(temperature, rows, V, dtype):
     assert ((ref < -64) & (ref > -128)).all()
     left = 6 * step / math.sqrt(12 * rows)
     assert abs((got.double() - ref).mean().item()) <= moved + LOGP_TOL + left
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value", [-1e9, -1e10, 1e12, -1e20, 3e29, -726000.0, -727500.0, 43000.0])
+@pytest.mark.parametrize("V", [300, 9000, 60001, 140000, 900001])
+def test_rows_far_from_zero(V, value, dtype):
+    """Rows that hold one mask's constant alone, two of them, or a spread around it, at scaled
+    magnitudes where the rounding of base times scale leaves the exponents' range (and on either
+    side of 2^20, from which the difference to the base is formed first), beside ordinary ones.
+    Tolerances as in test_rows_whose_first_elements_mislead; the policy's scale is one float,
+    2^-24 of the log-probability. LOGP_TOL and 2^-18 of p are of up to 131072 logits: beyond, a
+    thread's chains of additions, and with them their bound, grow with V."""
+    from mamba3_ssm import _lib, policy_loss, preference_loss, token_logprobs
+    B, T = 2, 4
+    x, tokens = _inputs((B, T, V), dtype, 110)
+    x[:, 0] = value
+    x[:, 1] = value
+    x[:, 1, V // 2:] = value - abs(value) / 32
+    tokens[:, 1] %= V // 2
+    x[:, 2] += value
+    dout = torch.randn(B, T, device=DEV, generator=_gen(111))
+    leaf = x.clone().requires_grad_(True)
+    long = max(1.0, V / 131072)
+    sums, u = LOGP_TOL * long, torch.finfo(dtype).eps / 2
+    for temperature in (1.0, 0.7, 0.6, 0.1):
+        ref = _logp64(x, tokens, temperature)
+        p = torch.softmax(x.double() / temperature, -1)
+        hot = torch.zeros_like(p).scatter_(-1, tokens.unsqueeze(-1), 1.0)
+        out = token_logprobs(leaf, tokens, temperature=temperature)
+        assert ((out.double() - ref).abs() <= sums + 2.0 ** -24 * ref.abs()).all()
+        d, = torch.autograd.grad(out, leaf, dout)
+        g = (dout.double() / temperature).unsqueeze(-1)
+        exact = g * (hot - p)
+        of_p = long * 2.0 ** -18 * p + 2.0 ** -23
+        assert ((d.double() - exact).abs() <= g.abs() * of_p + u * exact.abs() * (1 + 2.0 ** -10) + 1e-37).all()
+        old = ref.float()  # ratios of 1
+        r = policy_loss(leaf, tokens, old, dout, temperature=temperature)
+        bare = policy_loss(x, tokens, old, dout, temperature=temperature)
+        assert torch.equal(r.loss.detach(), bare.loss) and torch.equal(r.logprobs, bare.logprobs)
+        slack = (dout.double().abs() * (sums + 2.0 ** -22 * ref.abs())).mean()
+        assert abs(r.loss.item() + dout.double().mean().item()) <= slack.item() + 1e-6 * abs(dout.double().mean().item())
+        g, exact = -g / (B * T), -exact / (B * T)
+        tol = exact.abs() * ((sums + 2.0 ** -22 * ref.abs()).unsqueeze(-1) + u * 1.001) + g.abs() * of_p + 1e-37
+        for up in (1.0, 3.0):
+            d, = torch.autograd.grad(r.loss * up, leaf, retain_graph=True)
+            assert ((d.double() - up * exact).abs() <= up * tol).all()
+        q = preference_loss(leaf, tokens, old, temperature=temperature)
+        reward_tol = 0.1 * (sums + 2.0 ** -24 * ref.abs()).sum(1) + 1e-12  # old's rounding
+        assert (q.rewards.double().abs() <= reward_tol).all()
+        assert abs(q.loss.item() - math.log(2.0)) <= reward_tol.sum().item() + 2.0 ** -23
+        assert torch.isfinite(torch.autograd.grad(q.loss, leaf)[0]).all()
+    assert _lib.device_timeouts() == 0
