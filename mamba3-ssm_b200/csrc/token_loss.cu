@@ -363,8 +363,9 @@ __device__ __forceinline__ TokenOps token_ops(const PolicyArgs& a, const PolicyW
 }
 
 // exp(d) - 1 - d without the cancellation of a small d: the series to d^9 below 1/2 (its
-// remainder is 2^-30 of the result), the difference above.
+// remainder is 2^-30 of the result), the difference above (infinite for an infinite d).
 __device__ __forceinline__ float kl_term(float d) {
+  if (d == INFINITY) return d;
   if (fabsf(d) >= 0.5f) return expm1f(d) - d;
   float q = 1.f / 362880.f;
   q = fmaf(q, d, 1.f / 40320.f);
@@ -393,8 +394,10 @@ __device__ __forceinline__ TokenLoss policy_token(const PolicyArgs& a, const Tok
   if (a.ref.p != nullptr) {
     const float d = (float)((double)x.ref - logp), k = (float)a.kl_coef;
     o.kl = kl_term(d);
-    o.loss = fmaf(k, o.kl, o.loss);
-    o.dlogp = fmaf(-k, expm1f(d), o.dlogp);
+    if (k != 0.f) {  // else it is only reported, also where it overflows
+      o.loss = fmaf(k, o.kl, o.loss);
+      o.dlogp = fmaf(-k, expm1f(d), o.dlogp);
+    }
   }
   return o;
 }

@@ -994,3 +994,25 @@ def test_rows_far_from_zero(V, value, dtype):
         assert abs(q.loss.item() - math.log(2.0)) <= reward_tol.sum().item() + 2.0 ** -23
         assert torch.isfinite(torch.autograd.grad(q.loss, leaf)[0]).all()
     assert _lib.device_timeouts() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [50, 30000])
+def test_kl_that_is_only_reported(V, dtype):
+    """kl_coef 0 with reference log-probabilities: the loss and its gradient are those of the call
+    without them, also where the KL term overflows (a token that is excluded or all but)."""
+    from mamba3_ssm import policy_loss
+    x, tokens = _inputs((2, 40, V), dtype, 112)
+    old = _logp64(x, tokens).float()
+    x[0, 3, int(tokens[0, 3])] = float("-inf")
+    x[1, 5, int(tokens[1, 5])] = -200.0
+    adv = torch.randn(2, 40, device=DEV, generator=_gen(113))
+    leaf = x.requires_grad_(True)
+    want = policy_loss(leaf, tokens, old, adv)
+    r = policy_loss(leaf, tokens, old, adv, ref_logprobs=old - 0.1)
+    assert r.loss.isfinite() and torch.equal(r.loss, want.loss) and torch.equal(r.logprobs, want.logprobs)
+    assert r.kl.item() == math.inf and want.kl.item() == 0.0
+    for up in (1.0, 2.0):
+        d, = torch.autograd.grad(r.loss * up, leaf, retain_graph=True)
+        assert d.isfinite().all() and torch.equal(d, torch.autograd.grad(want.loss * up, leaf, retain_graph=True)[0])
+    assert (d[0, 3] == 0).all() and (d[1, 4] != 0).any()
