@@ -4,6 +4,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdio>
+#include <limits>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -1163,13 +1164,14 @@ int token_rows(const m3_tensor* logits, const m3_tensor* tokens, const m3_tensor
   p->R = sh[0] * sh[1]; p->T = (int)sh[1]; p->V = (int)sh[2];
   p->ignore = ignore_index;
   p->scale = 1.0 / temperature;
-  // c in two floats, the upper one rounded down so that the lower one is positive, or in one,
-  // rounded to the nearest
+  // c in two floats, the upper one rounded down so that the lower one is positive; or in one,
+  // rounded to the nearest, the lower one then the smallest number that keeps -inf from NaN (with
+  // a product less in the kernels instead, one of them needs more registers than it has)
   const double c = p->scale * 1.44269504088896340736;
   float hi = (float)c;
   if (!policy && (double)hi >= c) hi = std::nextafterf(hi, 0.f);
   p->c_hi = hi;
-  p->c_lo = policy ? 0.f : (float)(c - (double)hi);
+  p->c_lo = policy ? std::numeric_limits<float>::min() : (float)(c - (double)hi);
   return M3_OK;
 }
 

@@ -145,7 +145,7 @@ template <bool FAR, bool FINE>
 __device__ __forceinline__ float exponent(float l, const Base& b, float c_hi, float c_lo) {
   if constexpr (FAR) {
     const float d = l - b.m;
-    return FINE ? fmaf(d, c_hi, d * c_lo) : d * c_hi;
+    return fmaf(d, c_hi, d * c_lo);
   } else if constexpr (FINE) {
     return fmaf(l, c_lo, fmaf(l, c_hi, b.k));
   } else {

@@ -24,7 +24,7 @@ struct TokenRows {
   Map2<const uint8_t> mask;  // p may be null: every position counts
   int64_t ignore;      // token id of positions that do not count
   double scale;        // 1 / temperature
-  float c_hi, c_lo;    // scale * log2(e) in two floats; of the policy loss the nearest one, and 0
+  float c_hi, c_lo;    // scale * log2(e) in two floats; of the policy loss the nearest one, and next to nothing
 };
 
 struct PolicyArgs {
