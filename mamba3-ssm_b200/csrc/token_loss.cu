@@ -1360,9 +1360,11 @@ __global__ void __launch_bounds__(kSumThreads)
   s = 0.0;
   for (int i = threadIdx.x; i < pairs; i += kSumThreads) {
     const double z = rw[i] - rw[pairs + i];
-    const double l = log1p(exp(-fabs(z)));  // softplus(-|z|)
+    const double q = exp(-fabs(z)), l = log1p(q);  // softplus(-|z|)
     s += (1.0 - smoothing) * (l + fmax(-z, 0.0)) + smoothing * (l + fmax(z, 0.0));
-    const double dz = (1.0 / (1.0 + exp(-z)) - (1.0 - smoothing)) * beta / pairs;
+    // e sigma(z) - (1 - e) sigma(-z): sigma(z) - (1 - e) would lose sigma(-z) in the 1
+    const double less = q / (1.0 + q), more = 1.0 / (1.0 + q);  // sigma(-|z|), sigma(|z|)
+    const double dz = (smoothing * (z < 0.0 ? less : more) - (1.0 - smoothing) * (z < 0.0 ? more : less)) * beta / pairs;
     w.coef[i] = (float)dz;
     w.coef[pairs + i] = (float)-dz;
   }

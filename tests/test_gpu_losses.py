@@ -1016,3 +1016,31 @@ def test_kl_that_is_only_reported(V, dtype):
         d, = torch.autograd.grad(r.loss * up, leaf, retain_graph=True)
         assert d.isfinite().all() and torch.equal(d, torch.autograd.grad(want.loss * up, leaf, retain_graph=True)[0])
     assert (d[0, 3] == 0).all() and (d[1, 4] != 0).any()
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_preference_gradient_of_pairs_that_are_told_apart(smoothing):
+    """-(1 - e) sigma(-z) + e sigma(z), also where sigma(z) is 1 to the last bit: a margin's error
+    is a relative one of sigma(-z); 4 tokens an answer, each with LOGP_TOL."""
+    from mamba3_ssm import preference_loss
+    N, T, V = 6, 4, 50
+    x, tokens = _inputs((2 * N, T, V), torch.float32, 115)
+    logp = _logp64(x, tokens)
+    margin = torch.tensor([5.0, 20.0, 30.0, 45.0, 60.0, 70.0], device=DEV, dtype=torch.float64)
+    ref = logp.clone()
+    ref[:N] -= margin[:, None] / T
+    ref = ref.float()
+    z = (logp - ref.double()).sum(1)
+    z = z[:N] - z[N:]
+    x.requires_grad_(True)
+    r = preference_loss(x, tokens, ref, beta=1.0, label_smoothing=smoothing)
+    d, = torch.autograd.grad(r.loss, x)
+    dz = (smoothing * torch.sigmoid(z) - (1 - smoothing) * torch.sigmoid(-z)) / N
+    dz = torch.cat([dz, -dz])[:, None, None]
+    p = torch.softmax(x.detach().double(), -1)
+    hot = torch.zeros_like(p).scatter_(-1, tokens.unsqueeze(-1), 1.0)
+    exact = dz * (hot - p)
+    moved = 2 * T * LOGP_TOL * (torch.sigmoid(-z) / N)  # d^2 loss / d z^2 <= sigma(-z) / N
+    tol = moved.repeat(2)[:, None, None] * (hot - p).abs() + dz.abs() * (2.0 ** -18 * p + 2.0 ** -22) + 1e-37
+    assert ((d.double() - exact).abs() <= tol).all()
+    assert (d != 0).all()
