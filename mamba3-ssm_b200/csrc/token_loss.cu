@@ -1361,7 +1361,9 @@ __global__ void __launch_bounds__(kSumThreads)
   for (int i = threadIdx.x; i < pairs; i += kSumThreads) {
     const double z = rw[i] - rw[pairs + i];
     const double q = exp(-fabs(z)), l = log1p(q);  // softplus(-|z|)
-    s += (1.0 - smoothing) * (l + fmax(-z, 0.0)) + smoothing * (l + fmax(z, 0.0));
+    // a side without weight counts nothing, also where it is infinite
+    if (smoothing < 1.0) s += (1.0 - smoothing) * (l + fmax(-z, 0.0));
+    if (smoothing > 0.0) s += smoothing * (l + fmax(z, 0.0));
     // e sigma(z) - (1 - e) sigma(-z): sigma(z) - (1 - e) would lose sigma(-z) in the 1
     const double less = q / (1.0 + q), more = 1.0 / (1.0 + q);  // sigma(-|z|), sigma(|z|)
     const double dz = (smoothing * (z < 0.0 ? less : more) - (1.0 - smoothing) * (z < 0.0 ? more : less)) * beta / pairs;

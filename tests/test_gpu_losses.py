@@ -1044,3 +1044,23 @@ def test_preference_gradient_of_pairs_that_are_told_apart(smoothing):
     tol = moved.repeat(2)[:, None, None] * (hot - p).abs() + dz.abs() * (2.0 ** -18 * p + 2.0 ** -22) + 1e-37
     assert ((d.double() - exact).abs() <= tol).all()
     assert (d != 0).all()
+
+
+def test_preference_loss_with_an_excluded_token():
+    """A rejected answer with a token of logit -inf has the reward -inf: the pair costs nothing and
+    has no gradient, whatever the other pairs; with smoothing, or as the chosen one, it costs
+    infinitely much."""
+    from mamba3_ssm import preference_loss
+    x, tokens = _inputs((4, 6, 50), torch.float32, 119)
+    want = preference_loss(x[1::2], tokens[1::2], beta=1.0)
+    x[2, 3, int(tokens[2, 3])] = float("-inf")
+    x.requires_grad_(True)
+    r = preference_loss(x, tokens, beta=1.0)
+    assert r.rewards[2].item() == -math.inf
+    assert abs(r.loss.item() - want.loss.item() / 2) <= 2.0 ** -23 * want.loss.item()
+    d, = torch.autograd.grad(r.loss, x)
+    assert (d[::2] == 0).all() and d.isfinite().all() and (d[1::2] != 0).any()
+    assert preference_loss(x, tokens, beta=1.0, label_smoothing=0.1).loss.item() == math.inf
+    swapped = torch.cat([x[2:], x[:2]]), torch.cat([tokens[2:], tokens[:2]])
+    assert preference_loss(*swapped, beta=1.0).loss.item() == math.inf
+    assert preference_loss(*swapped, beta=1.0, label_smoothing=1.0).loss.isfinite()
