@@ -442,7 +442,8 @@ int m3_preference_loss_grad(const m3_tensor* logits, const m3_tensor* tokens, co
  * counts and m3_dtype (f32 / bf16 / f16). outs NULL: in place, and nothing is written where
  * scale is 1 and nothing is clipped. out_dtypes: the gradient's own or M3_FLOAT32. Tensors
  * that are written must not overlap one another or another gradient. max_norm infinite: no
- * clipping. A NaN gradient makes the norm and every scaled gradient NaN.
+ * clipping, and with scale 1 and outs NULL the norm alone. A NaN gradient makes the norm and
+ * everything that is written NaN, as does an infinite one with an infinite max_norm.
  *   norm (1) f32. workspace: m3_clip_grads_workspace_size(count) bytes, 16-byte aligned.
  * ------------------------------------------------------------------------------- */
 size_t m3_clip_grads_workspace_size(int64_t count);

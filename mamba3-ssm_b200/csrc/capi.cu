@@ -1347,9 +1347,14 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
   if (largest != 0 && largest != 1) return fail(M3_ERR_INVALID_ARGUMENT, "largest: expected 0 or 1");
   if (!(max_norm >= 0)) return fail(M3_ERR_INVALID_ARGUMENT, "max_norm: expected a number from 0 on");
   if (!(scale > 0 && std::isfinite(scale))) return fail(M3_ERR_INVALID_ARGUMENT, "scale: expected a positive finite number");
-  // what is written (and, with outs, what is read) as address ranges, to find overlaps
+  bool in_place = true;  // outs that are the gradients themselves count as that too
+  if (outs)
+    for (int64_t i = 0; i < count && in_place; ++i) in_place = outs[i] == grads[i] && out_dtypes[i] == dtypes[i];
+  const bool norm_alone = !outs && scale == 1.0 && std::isinf(max_norm);
+  // what is written (and, with outs, what is read) as address ranges, to find overlaps; in place
+  // with scale 1 and no bound nothing but NaN is written, to all of the gradients
   struct Range { uintptr_t lo, hi; bool written; int64_t index; };
-  const bool writes = outs || scale != 1.0 || !std::isinf(max_norm);
+  const bool writes = !in_place || scale != 1.0 || !std::isinf(max_norm);
   int64_t first = -1;  // tensor with elements
   std::vector<Range> ranges;
   if (writes) ranges.reserve((size_t)count * (outs ? 2 : 1));
@@ -1386,7 +1391,8 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
   }
   M3_TRY(scalar_out(norm, "norm", false));
   if (count > 0) M3_TRY(workspace_ok(workspace, workspace_bytes, clip_grads_workspace_bytes(count), "clip_grads"));
-  ClipArgs a{count, grads, numel, dtypes, outs, out_dtypes, largest != 0, max_norm, scale, fptr<float>(norm)};
+  ClipArgs a{count, grads, numel, dtypes, outs, out_dtypes, largest != 0, max_norm, scale, in_place, norm_alone,
+             fptr<float>(norm)};
   return launch_clip_grads(a, workspace, reinterpret_cast<cudaStream_t>(stream));
 } catch (const std::exception& e) {
   return fail(M3_ERR_INVALID_ARGUMENT, std::string("clip_grads: ") + e.what());

@@ -1,7 +1,8 @@
 // Global gradient norm over many tensors, with scaling and clipping:
 //   n = scale * sqrt(sum_i sum_j g_ij^2)   (or scale * max |g_ij|)
 //   f = scale * min(1, max_norm / (n + 1e-6)),   g <- f g  (or out <- f g)
-// A NaN among the gradients makes n and every scaled gradient NaN; an infinite n makes f 0.
+// A NaN among the gradients makes n and everything that is written NaN; an infinite n makes f 0, or
+// NaN where max_norm is infinite too. In place with scale 1 and max_norm infinite only n is formed.
 // Two launches: partial norms of fixed parts, then every CTA adds the partial norms in the
 // same order (so all agree on f, and the result does not depend on the schedule) and scales
 // its parts. The tensors' table travels in the kernel's parameters, so a captured graph holds
@@ -189,7 +190,7 @@ __device__ __forceinline__ void scale_part(const T* g, O* o, int n, float f) {
 template <int K, bool LARGEST>
 __global__ void __launch_bounds__(kThreads)
     grad_scale_kernel(const __grid_constant__ Table<K> t, const double* partial, int partials, double max_norm,
-                      double scale, bool in_place, float* norm) {
+                      double scale, bool in_place, bool norm_alone, float* norm) {
   __shared__ double sh[kThreads / 32];
   double sum = 0.0;
   float mx = 0.f;
@@ -200,7 +201,8 @@ __global__ void __launch_bounds__(kThreads)
   const double all = block_join<LARGEST>(sum, mx, sh);
   const double n = scale * (LARGEST ? all : sqrt(all));
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-  double c = isinf(max_norm) ? 1.0 : max_norm / (n + 1e-6);
+  if (norm_alone) return;
+  double c = max_norm / (n + 1e-6);
   if (c > 1.0) c = 1.0;  // a NaN stays
   if (in_place && c == 1.0 && scale == 1.0) return;
   const float f = (float)(c * scale);
@@ -280,11 +282,12 @@ int run(const ClipArgs& a, double* partial, cudaStream_t s) {
     i = fill(i);
     if (t.parts == 0 && norm == nullptr) continue;
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(t.parts, ctas));
-    const bool in_place = a.outs == nullptr;
     if (a.largest)
-      grad_scale_kernel<K, true><<<grid, kThreads, 0, s>>>(t, partial, partials, a.max_norm, a.scale, in_place, norm);
+      grad_scale_kernel<K, true><<<grid, kThreads, 0, s>>>(t, partial, partials, a.max_norm, a.scale, a.in_place,
+                                                           a.norm_alone, norm);
     else
-      grad_scale_kernel<K, false><<<grid, kThreads, 0, s>>>(t, partial, partials, a.max_norm, a.scale, in_place, norm);
+      grad_scale_kernel<K, false><<<grid, kThreads, 0, s>>>(t, partial, partials, a.max_norm, a.scale, a.in_place,
+                                                            a.norm_alone, norm);
     M3_TRY(check_launch("grad_scale_kernel"));
     norm = nullptr;  // the first launch writes it
   }

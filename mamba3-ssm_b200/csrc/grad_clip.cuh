@@ -16,6 +16,8 @@ struct ClipArgs {
   const int32_t* out_dtypes;
   bool largest;                // the largest magnitude in place of the 2-norm
   double max_norm, scale;
+  bool in_place;               // outs are null or the gradients themselves
+  bool norm_alone;             // nothing is written but the norm
   float* norm;                 // device, one value
 };
 

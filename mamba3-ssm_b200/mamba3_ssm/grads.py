@@ -50,10 +50,12 @@ def clip_grads_(grads, max_norm, norm_type=2.0, *, scale=1.0, out=None):
     magnitude), multiplies every gradient by scale * min(1, max_norm / (n + 1e-6)) and returns n
     (fp32, 0-d, on the device; nothing waits for it).
 
-    ``max_norm`` inf scales without clipping; with scale 1 that is the norm alone. ``out``: as
+    ``max_norm`` inf scales without clipping; in place with scale 1 that is the norm alone, and
+    nothing is written. ``out``: as
     many tensors of the same shapes and strides that receive the result in place of the
     gradients, fp32 or the gradient's dtype. The gradients may be of mixed dtypes, each
-    dense in memory, and must not share memory. A NaN among them makes n and all results NaN."""
+    dense in memory, and must not share memory. A NaN among them makes n and all that is written
+    NaN; so does an infinite n with an infinite ``max_norm``."""
     if isinstance(grads, torch.Tensor):
         grads = [grads]
         out = [out] if isinstance(out, torch.Tensor) else out
@@ -124,4 +126,5 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         if not torch.isfinite(norm):
             raise RuntimeError(f"clip_grad_norm_: the total norm of order {float(norm_type)} is {norm.item()}, so the "
                                "gradients cannot be clipped")
-    return clip_grads_(grads, max_norm, norm_type)
+    # without a bound clip_grads_ would form the norm alone, and a NaN would not spread
+    return clip_grads_(grads, max_norm, norm_type, out=grads if max_norm == math.inf else None)

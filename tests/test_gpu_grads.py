@@ -249,3 +249,60 @@ def test_refusals():
     with pytest.raises(TypeError, match="sparse"):
         clip_grad_norm_([p], 1.0)
     assert (a == 1).all()
+
+
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_without_a_bound_a_nan_still_spreads(dtype, bad, norm_type):
+    """max_norm inf: min(1, inf / n) is NaN for an n that is NaN or infinite, in all that is
+    written. The norm alone (in place with scale 1) writes nothing."""
+    from mamba3_ssm import clip_grad_norm_, clip_grads_
+
+    def make():
+        g = torch.ones(9999, device=DEV, dtype=dtype)
+        g[3000] = bad
+        return [torch.ones(10, device=DEV, dtype=dtype), g]
+
+    def same(n):
+        return n.isnan() if math.isnan(bad) else n == math.inf
+
+    a = make()
+    assert same(clip_grads_(a, math.inf, norm_type, scale=0.5))
+    assert all(t.isnan().all() for t in a)
+    for scale in (1.0, 0.5):
+        a = make()
+        out = [torch.zeros(t.shape, device=DEV) for t in a]
+        assert same(clip_grads_(a, math.inf, norm_type, scale=scale, out=out))
+        assert all(t.isnan().all() for t in out)
+        assert all(torch.equal(t, o) or math.isnan(bad) for t, o in zip(a, make()))
+    a = make()
+    assert same(clip_grads_(a, math.inf, norm_type))
+    assert (a[0] == 1).all() and (a[1][:3000] == 1).all()
+    # as torch.nn.utils.clip_grad_norm_ has it
+    ps, qs = ([torch.nn.Parameter(torch.zeros(t.shape, device=DEV, dtype=dtype)) for t in a] for _ in range(2))
+    for p, q, g in zip(ps, qs, a):
+        p.grad, q.grad = g.clone(), g.clone()
+    assert same(clip_grad_norm_(ps, math.inf, norm_type))
+    torch.nn.utils.clip_grad_norm_(qs, math.inf, norm_type)
+    for p, q in zip(ps, qs):
+        assert torch.equal(p.grad.isnan(), q.grad.isnan()) and p.grad.isnan().all()
+    with pytest.raises(RuntimeError, match="cannot be clipped"):
+        clip_grad_norm_(_with_grads(make()), math.inf, norm_type, error_if_nonfinite=True)
+
+
+def _with_grads(ts):
+    ps = [torch.nn.Parameter(torch.zeros(t.shape, device=DEV, dtype=t.dtype)) for t in ts]
+    for p, t in zip(ps, ts):
+        p.grad = t
+    return ps
+
+
+def test_without_a_bound_nothing_changes():
+    """clip_grad_norm_ with max_norm inf leaves gradients of a finite norm as they are."""
+    from mamba3_ssm import clip_grad_norm_
+    src = _grads(SHAPES["odd"], DTYPES, 9)
+    ps = _with_grads([t.clone() for t in src])
+    n = clip_grad_norm_(ps, math.inf)
+    assert abs(n.item() - _norm64(src)) <= NORM_TOL * n.item()
+    assert all(torch.equal(p.grad, t) for p, t in zip(ps, src))
