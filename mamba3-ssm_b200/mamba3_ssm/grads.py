@@ -1,7 +1,8 @@
 """Global norm of a model's gradients, and their scaling and clipping, on m3_clip_grads (two
 kernel launches for up to a thousand tensors, no host synchronisation, deterministic).
 
-``clip_grad_norm_`` takes parameters, with the arguments of torch.nn.utils.clip_grad_norm_;
+``clip_grad_norm_`` takes parameters, with the arguments of torch.nn.utils.clip_grad_norm_ (norm
+types, dtypes and devices: see there);
 ``clip_grads_`` takes the gradients themselves and can also unscale them (loss scaling,
 accumulated micro-batches) and write fp32 gradients for an optimiser from 16-bit ones. No
 counterpart in the reference's package.
@@ -111,11 +112,12 @@ def clip_grads_(grads, max_norm, norm_type=2.0, *, scale=1.0, out=None):
     return norm
 
 
-def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
-    """torch.nn.utils.clip_grad_norm_ for norm_type 2 or inf: clips the ``.grad`` of the
-    parameters in place to a global norm of ``max_norm`` and returns the norm they had. A
-    parameter given twice counts once. ``error_if_nonfinite`` waits for the norm and raises,
-    with the gradients as they were."""
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
+    """torch.nn.utils.clip_grad_norm_ for norm_type 2 or inf and float32, bfloat16 or float16
+    gradients on one device: clips the ``.grad`` of the parameters in place to a global norm of
+    ``max_norm`` and returns the norm they had. A parameter given twice counts once (torch: twice).
+    ``error_if_nonfinite`` waits for the norm and raises, with the gradients as they were.
+    ``foreach`` has no effect: there is one way here."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [p.grad for p in dict.fromkeys(parameters) if p.grad is not None]

@@ -292,3 +292,25 @@ def test_policy_derivative_against_differences():
             got = (0.0 if clipped else -r * A) - k * math.expm1(ref - lp)
             h = 1e-5
             assert abs((loss(lp + h) - loss(lp - h)) / (2 * h) - got) < 1e-6
+
+
+def test_clip_grad_norm_takes_the_arguments_of_torch():
+    import inspect
+    from mamba3_ssm import clip_grad_norm_
+    ours, theirs = (inspect.signature(f).parameters.values() for f in (clip_grad_norm_, torch.nn.utils.clip_grad_norm_))
+    assert [(p.name, p.default) for p in ours] == [(p.name, p.default) for p in theirs]
+    p = torch.nn.Parameter(torch.zeros(3))
+    for foreach in (None, True, False):
+        assert clip_grad_norm_([p], 1.0, foreach=foreach).item() == 0.0
+
+
+def test_clip_grads_without_a_bound_reads_shared_memory(lib):
+    """Nothing but NaN to all of them can be written then, through ``outs`` too; with a scale the
+    gradients are written."""
+    f32 = _codes()[0]
+    a = (4096, 100, f32)
+    for outs in (None, [a, a]):
+        rc, msg = _clip(lib, [a, a], outs=outs, max_norm=math.inf)
+        assert rc != 0 and "shares" not in msg
+        rc, msg = _clip(lib, [a, a], outs=outs, max_norm=math.inf, scale=0.5)
+        assert rc == 1 and "shares memory" in msg
