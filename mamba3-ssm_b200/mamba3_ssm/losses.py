@@ -12,13 +12,15 @@ giving the last position ``ignore_index`` also spares autograd the padding of th
 Positions with mask 0 or the token ``ignore_index`` do not count: their logits are not read,
 their log-probability is 0 and their gradient is 0, whatever is stored there. A token id
 outside the vocabulary that is not ``ignore_index`` makes its position NaN. Gradients flow to
-the logits alone; old and reference log-probabilities, advantages and masks are constants.
+the logits alone, once and backwards (no second derivatives, no forward mode); old and reference
+log-probabilities, advantages and masks are constants.
 No counterpart in the reference's package.
 """
 
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -49,6 +51,8 @@ class PreferenceLoss(NamedTuple):
 def _rows(name, logits, tokens):
     """Logits as (batch, length, V) and tokens as (batch, length), without a copy where the
     strides allow."""
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise NotImplementedError(f"{name}: no forward-mode derivative, but the logits carry a tangent")
     if not (logits.is_cuda and tokens.is_cuda):
         _require_cuda(name, logits, tokens)
     if logits.dtype not in _LOGIT_DTYPES:

@@ -1064,3 +1064,26 @@ def test_preference_loss_with_an_excluded_token():
     swapped = torch.cat([x[2:], x[:2]]), torch.cat([tokens[2:], tokens[:2]])
     assert preference_loss(*swapped, beta=1.0).loss.item() == math.inf
     assert preference_loss(*swapped, beta=1.0, label_smoothing=1.0).loss.isfinite()
+
+
+def test_forward_mode_tangents_are_refused():
+    """There is no forward-mode derivative: a tangent of the logits must not be lost silently,
+    with or without a gradient."""
+    import torch.autograd.forward_ad as fwd
+    from mamba3_ssm import policy_loss, preference_loss, token_logprobs
+    x, tokens = _inputs((2, 4, 100), torch.float32, 116)
+    z = torch.zeros(2, 4, device=DEV)
+    calls = (lambda y: token_logprobs(y, tokens), lambda y: policy_loss(y, tokens, z, z + 1),
+             lambda y: preference_loss(y, tokens))
+    with fwd.dual_level():
+        for leaf in (x, x.clone().requires_grad_(True)):
+            dual = fwd.make_dual(leaf, torch.ones_like(x))
+            for call in calls:
+                with pytest.raises(NotImplementedError):
+                    call(dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError):
+                    call(dual)
+        for call in calls:
+            call(x)  # no tangent: as ever
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(calls[0], (x,), (torch.ones_like(x),))

@@ -314,3 +314,19 @@ def test_clip_grads_without_a_bound_reads_shared_memory(lib):
         assert rc != 0 and "shares" not in msg
         rc, msg = _clip(lib, [a, a], outs=outs, max_norm=math.inf, scale=0.5)
         assert rc == 1 and "shares memory" in msg
+
+
+def test_forward_mode_tangents_are_refused():
+    """Before anything else: the losses have no forward-mode derivative to lose."""
+    import torch.autograd.forward_ad as fwd
+    from mamba3_ssm import policy_loss, preference_loss, token_logprobs
+    x, t, z = torch.randn(2, 3, 8), torch.zeros(2, 3, dtype=torch.long), torch.zeros(2, 3)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for f in (lambda: token_logprobs(dual, t), lambda: policy_loss(dual, t, z, z), lambda: preference_loss(dual, t)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            token_logprobs(x, t)
