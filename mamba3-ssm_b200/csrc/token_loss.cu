@@ -35,6 +35,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "copy_rounds.cuh"
 #include "m3_common.cuh"
 #include "sm100.cuh"
 #include "token_loss.cuh"
@@ -847,7 +848,7 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
   if (warp == W) {
     // ------------------------------------------------------------------ the copying warp
     const double even = even_weight(a, w);
-    uint32_t round = 0, issued = 0;  // issued: pieces whose copy of the current round is under way
+    CopyRounds rounds;  // lane 0 issues
     bool ok = true;
     // zeros to a position that does not count, this CTA's part of the row
     auto skip = [&](int i) {
@@ -869,7 +870,8 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
     const int mine = cid < kept_rows ? (kept_rows - cid + ncl - 1) / ncl : 0;  // rows that count
     const int rest = p.R - kept_rows, skips = cid < rest ? (int)(rest - cid + ncl - 1) / ncl : 0;
     int skipped = 0;
-    for (int i = cid; i < kept_rows; i += ncl, ++round) {
+    for (int i = cid; i < kept_rows; i += ncl, rounds.next()) {
+      const uint32_t round = rounds.round;
       const int slot = round & 1;
       if (round >= 2 && !(ok = wait_warp(&sh.info_empty[slot], ((round >> 1) - 1) & 1, &sh.dead))) break;
       RowInfo<T> q;
@@ -890,13 +892,12 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
         sh.info[slot] = q;
         sm100::mbar_arrive(&sh.info_full[slot]);
         const Vec<T>* src = reinterpret_cast<const Vec<T>*>(q.row + q.c.head) + q.v0;
-        issued = 0;
         for (int k = 0; k < pieces; ++k) {
           if (round >= 1 && !(ok = wait_one(&sh.empty[k], (round - 1) & 1, &sh.dead))) break;
           const int n = min(kPiece, q.n - k * kPiece);
           sm100::mbar_expect_tx(&sh.full[k], n > 0 ? (uint32_t)n * 16u : 0u);
           if (n > 0) sm100::bulk_load(kept + k * kPiece, src + k * kPiece, (uint32_t)n * 16u, &sh.full[k]);
-          issued |= 1u << k;
+          rounds.issue(k);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -906,12 +907,10 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
         skip(kept_rows + cid + skipped * ncl);
     }
     for (; ok && skipped < skips; ++skipped) skip(kept_rows + cid + skipped * ncl);
-    if (!ok && lane == 0) {
-      // copies in flight end before the CTA does
-      for (int k = 0; k < pieces; ++k) {
-        const uint32_t phase = (issued >> k & 1) ? round & 1 : (round + 1) & 1;
-        if (round > 0 || (issued >> k & 1)) sm100::mbar_wait(&sh.full[k], phase, kWaitLimit);
-      }
+    if (lane == 0) {
+      // copies in flight end before the CTA does, also where the others have given up on them
+      for (int k = 0; k < pieces; ++k)
+        if (rounds.copied(k)) sm100::mbar_wait(&sh.full[k], rounds.last_phase(k), kWaitLimit);
     }
     sm100::bulk_wait0();
   } else {

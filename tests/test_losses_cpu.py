@@ -330,3 +330,47 @@ def test_forward_mode_tangents_are_refused():
                 f()
         with pytest.raises(RuntimeError, match="no CPU path"):
             token_logprobs(x, t)
+
+
+_COPY_ROUNDS = r"""
+#include "copy_rounds.cuh"
+// A copying warp as in the policy loss's kernel: `rows` rows of `pieces` pieces; before row r it
+// waits for a place (from the third row on), before piece k of it for the piece to be read (from
+// the second row on). Wait number `fails` gives up (-1: none does). What the last copy of each
+// piece is, and what is waited for at the end, as parities; -1: nothing.
+extern "C" void run(int rows, int pieces, int fails, int* last, int* waited) {
+  m3::CopyRounds c;
+  int waits = 0;
+  bool ok = true;
+  for (int k = 0; k < pieces; ++k) last[k] = waited[k] = -1;
+  for (int i = 0; i < rows && ok; ++i, c.next()) {
+    if (c.round >= 2 && waits++ == fails) { ok = false; break; }
+    for (int k = 0; k < pieces; ++k) {
+      if (c.round >= 1 && waits++ == fails) { ok = false; break; }
+      last[k] = i & 1;
+      c.issue(k);
+    }
+    if (!ok) break;
+  }
+  for (int k = 0; k < pieces; ++k)
+    if (c.copied(k)) waited[k] = (int)c.last_phase(k);
+}
+"""
+
+
+def test_copies_in_flight_are_waited_for(tmp_path):
+    """Wherever the copying warp of the policy loss gives up, and where it does not, it waits for
+    the phase that each piece's last copy completes, before its CTA's shared memory is released."""
+    import os
+    import subprocess
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mamba3-ssm_b200", "csrc")
+    cpp, so = tmp_path / "rounds.cpp", tmp_path / "rounds.so"
+    cpp.write_text(_COPY_ROUNDS)
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", src, str(cpp), "-o", str(so)], check=True)
+    run = ctypes.CDLL(str(so)).run
+    for rows in range(6):
+        for pieces in range(1, 6):
+            for fails in range(-1, rows * (pieces + 1)):
+                last, waited = (ctypes.c_int * pieces)(), (ctypes.c_int * pieces)()
+                run(rows, pieces, fails, last, waited)
+                assert list(last) == list(waited), (rows, pieces, fails)
