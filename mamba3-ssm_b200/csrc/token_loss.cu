@@ -1132,13 +1132,13 @@ __global__ void __launch_bounds__(kWarpThreads, kWarpCtas<POLICY>)
       if (pos.known) q.at_token = to_f32(row[pos.tok]);
       if constexpr (POLICY) q.x = token_ops(a, w, q.b, q.t, even);
     }
-    if (__any_sync(0xffffffffu, q.keep && p.V != c.nv * N)) {
+    if (const unsigned need = __ballot_sync(0xffffffffu, q.keep && p.V != c.nv * N)) {
       T* const ends = sh.ends[warp];
 #pragma unroll
       for (int k0 = 0; k0 < each; k0 += 32 / E) {
         const int k = k0 + lane / E, e = lane % E;
         const int head = of(q.head, k), nv = of(q.nv, k), b = of(q.b, k), t = of(q.t, k);
-        if (k < rows && e < p.V - nv * N) ends[k * E + e] = row_at(b, t)[e < head ? e : nv * N + e];
+        if ((need >> k & 1) && e < p.V - nv * N) ends[k * E + e] = row_at(b, t)[e < head ? e : nv * N + e];
       }
     }
     __syncwarp();  // the ends
