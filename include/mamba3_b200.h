@@ -395,7 +395,9 @@ int m3_silu_gate_bwd(const m3_tensor* y, const m3_tensor* z, const m3_tensor* do
  *   not ignore_index. Other positions are not read: their logp and gradient rows are 0. A
  *   token outside [0, V) that is not ignore_index makes its position's results NaN.
  *   old_logprobs, advantages, ref_logprobs, dlogprobs (batch, seqlen) f32, any strides (0 where
- *   one value serves a sequence); ref_logprobs optional (absent: no KL term / reference 0).
+ *   one value serves a sequence); ref_logprobs optional (absent: no KL term / reference 0). With
+ *   kl_coef 0 the KL term is only reported, with label_smoothing 0 or 1 one side of the pairs' loss
+ *   does not count, also where they are infinite.
  *   logprobs (batch, seqlen) f32 contiguous. temperature: between 1e-6 and 1e6.
  *   m3_token_logprobs: stats (batch, seqlen, 2) f32 contiguous, optional: what
  *   m3_token_logprobs_grad needs of each row.

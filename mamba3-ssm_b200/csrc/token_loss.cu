@@ -1057,8 +1057,10 @@ __global__ void __launch_bounds__(NT + 32, NT == 128 ? 6 : 1024 / NT)
 // is a row where a row's few numbers are concerned: its token, logarithm, loss and gradient's
 // factor cost a warp as much for one row as for eight. No warp waits for another, and none copies
 // ahead: twice the warps hide a copy better than a second place each (4096 bf16 logits a row, loss
-// and gradient: 5.1 TB/s read and written against 4.3). What bounds it: with 24 and more warps of
-// an SM in flight the instructions per logit in 16 bits and per row in short rows, the memory else.
+// and gradient: 5.1 TB/s read and written against 4.3). What bounds it: in short 16-bit rows the
+// latency of loads that depend on one another (position, token's logit, ends; at 300 logits 57% of
+// the issue slots are busy, at 1000 50-66% of the exponential's unit, with 30-42% of the warps
+// active), the memory else.
 // 400 million logits, at most 262144 rows, TB/s, without a gradient | with the policy's:
 //   bf16, rows of 300, 1000, 2500, 4096, 8192: 2.9 4.3 4.7 5.5 5.7 | 2.8 4.2 4.7 5.4 5.4
 //   fp32, rows of 300, 1000, 2500, 4096, 6000: 5.8 6.5 6.6 6.9 6.6 | 4.5 5.4 5.6 5.6 6.1

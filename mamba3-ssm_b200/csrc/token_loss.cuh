@@ -42,7 +42,7 @@ int token_error_word(bool reset, int* out);
 size_t policy_workspace_bytes(int64_t batch, int64_t rows);
 size_t preference_workspace_bytes(int64_t batch, int64_t rows);
 
-// logp (R) and, where given, stats (R) = (maximum, sum) of each row
+// logp (R) and, where given, stats (R) = (base, sum over it) of each row
 int launch_token_logprobs(const TokenRows& p, int dtype, float* logp, float2* stats, cudaStream_t s);
 // loss, mean KL, share of clipped tokens; dlogits where given
 int launch_policy_loss(const TokenRows& p, int dtype, const PolicyArgs& a, int64_t batch, float* loss, float* kl,

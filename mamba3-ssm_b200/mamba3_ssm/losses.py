@@ -305,9 +305,11 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
     the sequences (last dimension of tokens) that have any, of each one's mean. 0 where no
     position counts. ``advantages`` may be per token or broadcast (e.g. (batch, 1)).
     ``clip_high`` defaults to ``clip_low``. Without ``ref_logprobs`` there is no KL term (and
-    ``kl_coef`` must be 0); with them ``kl`` is reported also for kl_coef 0.
+    ``kl_coef`` must be 0); with them ``kl`` is reported also for kl_coef 0, where the
+    loss is the one without them.
     Where the logits need a gradient it is formed in the forward pass, so that they are read
-    once; a loss that is scaled before backward() costs a second pass over them.
+    once; a loss that is scaled before backward() costs a second pass over them. That gradient is
+    kept until backward outside of autograd's saved tensors, where their hooks do not see it.
     Returns PolicyLoss(loss, logprobs, kl, clip_fraction). ``logprobs`` are within a few roundings
     of token_logprobs' (1 / temperature is held in one float here, in two there), not its bits."""
     name = "policy_loss"
