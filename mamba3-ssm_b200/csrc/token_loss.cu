@@ -141,7 +141,8 @@ __device__ __forceinline__ Base base_at(float m, float c_hi) {
 // stays -inf); it then carries m c_lo, which norm_sum takes off the sum. The policy loss does
 // without, c_hi being the float nearest to c: scale is then off by 2^-24 of itself at most, for
 // S and for the token alike, which moves a log-probability by 2^-24 s (l[tok] - mean of l under
-// p), at most half a step of the 32-bit result of an unlikely token.
+// p). By -logp = entropy of p - s (l[tok] - mean) that is at most 2^-24 of an unlikely token's own
+// value, and 2^-24 ln V of a likely one's.
 template <bool FAR, bool FINE>
 __device__ __forceinline__ float exponent(float l, const Base& b, float c_hi, float c_lo) {
   if constexpr (FAR) {
