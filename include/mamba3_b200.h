@@ -454,6 +454,84 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
                   m3_tensor* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * Selective state space scan and its short causal convolution, for sequences and single
+ * steps (no counterpart in the reference's package). E channels, N states a channel.
+ * m3_causal_conv:  pre[t] = bias + sum_k weight[:, k] x[t - K + 1 + k], y = pre, or
+ *   pre * sigmoid(pre) with silu = 1; K = 2, 3 or 4. Rows in front of the first are those of
+ *   initial, absent = zeros.
+ *   x (batch, seqlen, E), weight (E, K) and bias (E, optional) of f32 or x's dtype, initial
+ *   (batch, K - 1, E, optional) of x's dtype; y as x; last (batch, K - 1, E, optional), contiguous,
+ *   x's dtype: the last K - 1 rows, what the next call takes as initial or m3_causal_conv_step as state.
+ * m3_causal_conv_bwd: dx, dweight, dbias, dinitial (the last two optional) from dy and dlast
+ *   (optional); dweight, dbias of weight's dtype, contiguous.
+ * m3_causal_conv_step: one row; state (batch, K - 1, E) moves on in place. x, y (batch, E).
+ * m3_selective_scan:  dt = delta + delta_bias, with softplus = 1 log(1 + exp(.)) of it;
+ *   h[t] = exp(dt A) h[t - 1] + dt u B[t];  y = (sum_n C[t] h[t] + D u) (z sigmoid(z))
+ *   u (batch, seqlen, E); delta the same, u's dtype or f32; z as u, optional (no gate); B, C
+ *   (batch, seqlen, G, N), u's dtype or f32 both, E a multiple of G; N <= 128; A (E, N), D (E,
+ *   optional), delta_bias (E, optional) f32 contiguous; initial, last (batch, E, N, optional) f32
+ *   contiguous; y as u. states, optional: m3_selective_scan_states_size bytes that keep what
+ *   m3_selective_scan_bwd needs. workspace: m3_selective_scan_workspace_size bytes.
+ * m3_selective_scan_bwd: all gradients from dy and dlast (optional); dA, dD, ddelta_bias f32, dB
+ *   and dC contiguous of B's dtype, dinitial optional.
+ * m3_selective_step: one row; state (batch, E, N) f32 in place, each sequence's part contiguous.
+ * lengths (batch) i64, optional: positions from lengths[b] on are padding. They are not read, y and
+ *   the gradients are 0 there, and last is the state in front of them. Values are cut to 0 .. seqlen.
+ * Workspaces are 16-byte aligned. dtypes f32 / bf16 / f16, innermost strides 1.
+ * ------------------------------------------------------------------------------- */
+int m3_causal_conv(const m3_tensor* x, const m3_tensor* weight, const m3_tensor* bias, const m3_tensor* initial,
+                   const m3_tensor* lengths, int silu, m3_tensor* y, m3_tensor* last, void* stream);
+size_t m3_causal_conv_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t channels, int64_t taps);
+int m3_causal_conv_bwd(const m3_tensor* x, const m3_tensor* weight, const m3_tensor* bias, const m3_tensor* initial,
+                       const m3_tensor* lengths, int silu, const m3_tensor* dy, const m3_tensor* dlast, m3_tensor* dx,
+                       m3_tensor* dweight, m3_tensor* dbias, m3_tensor* dinitial, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int m3_causal_conv_step(m3_tensor* state, const m3_tensor* x, const m3_tensor* weight, const m3_tensor* bias, int silu,
+                        m3_tensor* y, void* stream);
+size_t m3_selective_scan_workspace_size(int64_t batch, int64_t seqlen, int64_t channels, int64_t d_state, int64_t groups);
+size_t m3_selective_scan_states_size(int64_t batch, int64_t seqlen, int64_t channels, int64_t d_state);
+int m3_selective_scan(const m3_tensor* u, const m3_tensor* delta, const m3_tensor* A, const m3_tensor* B,
+                      const m3_tensor* C, const m3_tensor* D, const m3_tensor* z, const m3_tensor* delta_bias,
+                      const m3_tensor* initial, const m3_tensor* lengths, int softplus, m3_tensor* y, m3_tensor* last,
+                      void* states, size_t states_bytes, void* workspace, size_t workspace_bytes, void* stream);
+size_t m3_selective_scan_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t channels, int64_t d_state,
+                                            int64_t groups);
+int m3_selective_scan_bwd(const m3_tensor* u, const m3_tensor* delta, const m3_tensor* A, const m3_tensor* B,
+                          const m3_tensor* C, const m3_tensor* D, const m3_tensor* z, const m3_tensor* delta_bias,
+                          const m3_tensor* initial, const m3_tensor* lengths, int softplus, const m3_tensor* dy,
+                          const m3_tensor* dlast, m3_tensor* du, m3_tensor* ddelta, m3_tensor* dA, m3_tensor* dB,
+                          m3_tensor* dC, m3_tensor* dD, m3_tensor* dz, m3_tensor* ddelta_bias, m3_tensor* dinitial,
+                          const void* states, size_t states_bytes, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int m3_selective_step(m3_tensor* state, const m3_tensor* u, const m3_tensor* delta, const m3_tensor* A,
+                      const m3_tensor* B, const m3_tensor* C, const m3_tensor* D, const m3_tensor* z,
+                      const m3_tensor* delta_bias, int softplus, m3_tensor* y, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Beam search (no counterpart in the reference's package).
+ * m3_beam_select: of each prompt, the num largest of scores[j] + logits[j, v] - log sum exp
+ *   logits[j, :] over its beams j and tokens v, largest first, formed and compared in 64 bits; ties to the
+ *   lowest (j, v). A finished beam offers end_token alone, at no cost (its logits are not read);
+ *   a beam with score -inf, or all of whose logits are -inf, offers -inf; one with a NaN or +inf
+ *   among its logits, or as its score, offers NaN, which ranks first.
+ *   logits (batch, beams, V), beams <= 32, V <= 2^24; scores (batch, beams) f32; finished (batch,
+ *   beams) u8, optional; out_scores f32, parents (j) and tokens (v) i64: (batch, num) contiguous,
+ *   num <= 64. workspace: m3_beam_select_workspace_size bytes, 16-byte aligned.
+ * m3_reorder_states: row b T + j of every tensor becomes its row b S + parents[b, j], zeros where
+ *   the parent is outside [0, S). parents (batch, T) i64. Tensors are given as host arrays: device
+ *   addresses of (batch S) rows of row_bytes bytes, their pitches, and those of the (batch T) rows that receive
+ *   them; dst NULL: in place, then S = T <= 32. Rows that are written must not overlap other
+ *   tensors of the call.
+ * ------------------------------------------------------------------------------- */
+size_t m3_beam_select_workspace_size(int64_t batch, int64_t beams, int64_t vocabulary, int64_t num, int dtype);
+int m3_beam_select(const m3_tensor* logits, const m3_tensor* scores, const m3_tensor* finished, int64_t end_token,
+                   m3_tensor* out_scores, m3_tensor* parents, m3_tensor* tokens, void* workspace,
+                   size_t workspace_bytes, void* stream);
+int m3_reorder_states(int64_t count, const void* const* src, void* const* dst, const int64_t* row_bytes,
+                      const int64_t* src_pitch, const int64_t* dst_pitch, int64_t source_rows, const m3_tensor* parents,
+                      void* stream);
+
+/* ---------------------------------------------------------------------------------
  * Health word of the warp-specialised kernels and of the single-pass MIMO forward on the
  * current device: *flag_out is nonzero once any bounded wait (between warps, on a TMA
  * box, or on an earlier chunk's published state) gave up (the kernel then drained and its

@@ -10,12 +10,15 @@
 #include <vector>
 
 #include "argmax.cuh"
+#include "beam.cuh"
+#include "causal_conv.cuh"
 #include "decode_step.cuh"
 #include "grad_clip.cuh"
 #include "m3_common.cuh"
 #include "mimo_scan.cuh"
 #include "prologue.cuh"
 #include "rmsnorm.cuh"
+#include "selective_scan.cuh"
 #include "siso_chunk.cuh"
 #include "siso_scan.cuh"
 #include "token_loss.cuh"
@@ -1396,6 +1399,440 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
   return launch_clip_grads(a, workspace, reinterpret_cast<cudaStream_t>(stream));
 } catch (const std::exception& e) {
   return fail(M3_ERR_INVALID_ARGUMENT, std::string("clip_grads: ") + e.what());
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------
+// selective scan, causal convolution
+// ------------------------------------------------------------------------------------
+namespace m3 {
+namespace {
+
+constexpr int64_t kMaxGrid = 65535;
+
+// Multiprocessors of the current device; 148 where there is none (workspace sizes asked for on a host).
+int sms_here() {
+  int n = 0;
+  if (device_sm_count(&n) != M3_OK) {
+    cudaGetLastError();
+    n = 148;
+  }
+  return n;
+}
+
+// What a tensor of the call's other float type may be: u's own dtype or fp32.
+unsigned own_or_f32(const m3_tensor* t) { return (1u << t->dtype) | kF32; }
+
+int flag(int v, const char* name) {
+  return v == 0 || v == 1 ? M3_OK : fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": expected 0 or 1");
+}
+
+int elem_aligned(const m3_tensor* t, const char* name) {
+  if (!present(t)) return M3_OK;
+  return aligned(t, name, t->dtype == M3_INT64 ? 8 : dtype_size(t->dtype));
+}
+
+// check() with the address on a boundary of its elements
+int operand(const m3_tensor* t, const char* name, int ndim, const int64_t* shape, unsigned mask, bool contig, bool optional,
+            bool devcheck) {
+  M3_TRY(check(t, name, ndim, shape, mask, contig, optional, devcheck));
+  return devcheck ? elem_aligned(t, name) : M3_OK;
+}
+
+// An optional (batch) i64 tensor, contiguous.
+int lengths_ok(const m3_tensor* t, int64_t batch, bool devcheck, const int64_t** out) {
+  *out = nullptr;
+  if (!present(t)) return M3_OK;
+  if (t->ndim != 1 || t->shape[0] != batch || t->dtype != M3_INT64 || (batch > 1 && t->stride[0] != 1))
+    return fail(M3_ERR_INVALID_ARGUMENT, "lengths: expected (batch) int64, contiguous");
+  if (devcheck) {
+    M3_TRY(check_device_ptr(t->data, "lengths"));
+    M3_TRY(elem_aligned(t, "lengths"));
+  }
+  *out = static_cast<const int64_t*>(t->data);
+  return M3_OK;
+}
+
+int conv_operands(const m3_tensor* x, int xdims, const m3_tensor* weight, const m3_tensor* bias, int silu, int64_t* taps) {
+  if (!present(x) || x->ndim != xdims)
+    return fail(M3_ERR_INVALID_ARGUMENT, xdims == 3 ? "x: expected (batch, seqlen, channels)" : "x: expected (batch, channels)");
+  const int64_t E = x->shape[xdims - 1], batch = x->shape[0], L = xdims == 3 ? x->shape[1] : 1;
+  if (batch < 0 || L < 0 || E < 0) return fail(M3_ERR_INVALID_ARGUMENT, "x: negative extent");
+  if (L > INT32_MAX / 2 || E > INT32_MAX / 8 || (xdims == 3 && batch > kMaxGrid))
+    return fail(M3_ERR_UNSUPPORTED, "x: dimension too large");
+  M3_TRY(operand(x, "x", xdims, x->shape, kAnyFloat, false, false, batch * L * E > 0));
+  if (!present(weight) || weight->ndim != 2) return fail(M3_ERR_INVALID_ARGUMENT, "weight: expected (channels, taps)");
+  *taps = weight->shape[1];
+  if (*taps < 2 || *taps > 4) return fail(M3_ERR_UNSUPPORTED, "weight: 2, 3 or 4 taps expected, got " + std::to_string(*taps));
+  const int64_t ws[2] = {E, *taps};
+  M3_TRY(operand(weight, "weight", 2, ws, own_or_f32(x), false, false, E > 0));
+  M3_TRY(operand(bias, "bias", 1, ws, 1u << weight->dtype, true, true, E > 0));
+  return flag(silu, "silu");
+}
+
+int conv_params(const m3_tensor* x, const m3_tensor* weight, const m3_tensor* bias, const m3_tensor* initial,
+                const m3_tensor* lengths, int silu, ConvParams* p, int64_t* taps) {
+  M3_TRY(conv_operands(x, 3, weight, bias, silu, taps));
+  const int64_t batch = x->shape[0], L = x->shape[1], E = x->shape[2], is[3] = {batch, *taps - 1, E};
+  M3_TRY(operand(initial, "initial", 3, is, 1u << x->dtype, false, true, batch * E > 0));
+  M3_TRY(lengths_ok(lengths, batch, batch > 0, &p->lengths));
+  p->x = x->data; p->xb = x->stride[0]; p->xl = x->stride[1];
+  p->w = weight->data; p->we = weight->stride[0];
+  p->bias = fptr<const void>(bias);
+  p->w_f32 = weight->dtype == M3_FLOAT32;
+  p->init = fptr<const void>(initial);
+  p->ib = present(initial) ? initial->stride[0] : 0; p->il = present(initial) ? initial->stride[1] : 0;
+  p->silu = silu != 0;
+  p->batch = (int)batch; p->L = (int)L; p->E = (int)E;
+  return M3_OK;
+}
+
+Seq seq(const m3_tensor* t) { return present(t) ? Seq{t->data, t->stride[0], t->stride[1]} : Seq{nullptr, 0, 0}; }
+
+// Everything that the scan's forward and backward read; *empty: no channel of any sequence.
+int selective_params(const m3_tensor* u, const m3_tensor* delta, const m3_tensor* A, const m3_tensor* B, const m3_tensor* C,
+                     const m3_tensor* D, const m3_tensor* z, const m3_tensor* delta_bias, const m3_tensor* initial,
+                     const m3_tensor* lengths, int softplus, SelScanParams* p, bool* empty) {
+  if (!present(u) || u->ndim != 3) return fail(M3_ERR_INVALID_ARGUMENT, "u: expected (batch, seqlen, channels)");
+  const int64_t batch = u->shape[0], L = u->shape[1], E = u->shape[2];
+  if (batch < 0 || L < 0 || E < 0) return fail(M3_ERR_INVALID_ARGUMENT, "u: negative extent");
+  const bool some = batch * L * E > 0;
+  *empty = batch * E == 0;
+  M3_TRY(operand(u, "u", 3, u->shape, kAnyFloat, false, false, some));
+  M3_TRY(operand(delta, "delta", 3, u->shape, own_or_f32(u), false, false, some));
+  M3_TRY(operand(z, "z", 3, u->shape, 1u << u->dtype, false, true, some));
+  if (!present(A) || A->ndim != 2) return fail(M3_ERR_INVALID_ARGUMENT, "A: expected (channels, d_state)");
+  const int64_t N = A->shape[1], an[2] = {E, N};
+  if (N < 1) return fail(M3_ERR_INVALID_ARGUMENT, "A: d_state must be positive");
+  if (N > kSelMaxStates) return fail(M3_ERR_UNSUPPORTED, "A: d_state above " + std::to_string(kSelMaxStates));
+  M3_TRY(operand(A, "A", 2, an, kF32, true, false, E > 0));
+  if (!present(B) || B->ndim != 4) return fail(M3_ERR_INVALID_ARGUMENT, "B: expected (batch, seqlen, groups, d_state)");
+  const int64_t G = B->shape[2], bs[4] = {batch, L, G, N};
+  if (G < 1 || E % G != 0) return fail(M3_ERR_INVALID_ARGUMENT, "B: the channels must divide into its groups");
+  M3_TRY(operand(B, "B", 4, bs, own_or_f32(u), false, false, batch * L > 0));
+  M3_TRY(operand(C, "C", 4, bs, 1u << B->dtype, false, false, batch * L > 0));
+  M3_TRY(operand(D, "D", 1, an, kF32, true, true, E > 0));
+  M3_TRY(operand(delta_bias, "delta_bias", 1, an, kF32, true, true, E > 0));
+  const int64_t hs[3] = {batch, E, N};
+  M3_TRY(operand(initial, "initial", 3, hs, kF32, true, true, !*empty));
+  M3_TRY(lengths_ok(lengths, batch, batch > 0, &p->lengths));
+  M3_TRY(flag(softplus, "softplus"));
+  if (batch > kMaxGrid || L > INT32_MAX / 2 || E > INT32_MAX / (2 * kSelMaxStates) || batch * L * G > INT64_C(1) << 36)
+    return fail(M3_ERR_UNSUPPORTED, "u: dimension too large");
+  p->u = seq(u); p->delta = seq(delta); p->z = seq(z); p->B = seq(B); p->C = seq(C);
+  p->Bg = B->stride[2]; p->Cg = C->stride[2];
+  p->delta_f32 = delta->dtype == M3_FLOAT32; p->bc_f32 = B->dtype == M3_FLOAT32;
+  p->A = fptr<const float>(A); p->D = fptr<const float>(D); p->bias = fptr<const float>(delta_bias);
+  p->softplus = softplus != 0;
+  p->h0 = fptr<const float>(initial);
+  p->batch = (int)batch; p->L = (int)L; p->E = (int)E; p->N = (int)N; p->G = (int)G;
+  return M3_OK;
+}
+
+SelScanParams selective_sizes(int64_t batch, int64_t seqlen, int64_t channels, int64_t d_state, int64_t groups) {
+  SelScanParams p{};
+  p.batch = (int)batch; p.L = (int)seqlen; p.E = (int)channels; p.N = (int)d_state; p.G = (int)groups;
+  return p;
+}
+
+bool selective_sizes_ok(int64_t batch, int64_t seqlen, int64_t channels, int64_t d_state, int64_t groups) {
+  return batch >= 0 && seqlen >= 0 && channels >= 0 && d_state >= 1 && d_state <= kSelMaxStates && groups >= 1 &&
+         batch <= kMaxGrid && seqlen <= INT32_MAX / 2 && channels <= INT32_MAX / (2 * kSelMaxStates);
+}
+
+}  // namespace
+}  // namespace m3
+
+extern "C" {
+
+int m3_causal_conv(const m3_tensor* x, const m3_tensor* weight, const m3_tensor* bias, const m3_tensor* initial,
+                   const m3_tensor* lengths, int silu, m3_tensor* y, m3_tensor* last, void* stream) {
+  ConvParams p{};
+  int64_t taps = 0;
+  M3_TRY(conv_params(x, weight, bias, initial, lengths, silu, &p, &taps));
+  const int64_t ls[3] = {p.batch, taps - 1, p.E};
+  const bool some = (int64_t)p.batch * p.E > 0;
+  M3_TRY(operand(y, "y", 3, x->shape, 1u << x->dtype, false, false, some && p.L > 0));
+  M3_TRY(operand(last, "last", 3, ls, 1u << x->dtype, true, true, some));
+  if (!some) return M3_OK;
+  p.y = y->data; p.yb = y->stride[0]; p.yl = y->stride[1];
+  p.last = fptr<void>(last);
+  return launch_conv_fwd(p, (int)taps, x->dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t m3_causal_conv_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t channels, int64_t taps) {
+  if (batch < 0 || seqlen < 0 || channels < 0 || taps < 2 || taps > 4) return 0;
+  return conv_bwd_workspace(batch, seqlen, channels, (int)taps);
+}
+
+int m3_causal_conv_bwd(const m3_tensor* x, const m3_tensor* weight, const m3_tensor* bias, const m3_tensor* initial,
+                       const m3_tensor* lengths, int silu, const m3_tensor* dy, const m3_tensor* dlast, m3_tensor* dx,
+                       m3_tensor* dweight, m3_tensor* dbias, m3_tensor* dinitial, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  ConvParams p{};
+  ConvGrads g{};
+  int64_t taps = 0;
+  M3_TRY(conv_params(x, weight, bias, initial, lengths, silu, &p, &taps));
+  const int64_t ls[3] = {p.batch, taps - 1, p.E}, wsz[2] = {p.E, taps};
+  const bool some = (int64_t)p.batch * p.E > 0;
+  const unsigned xt = 1u << x->dtype, wt = 1u << weight->dtype;
+  M3_TRY(operand(dy, "dy", 3, x->shape, xt, false, false, some && p.L > 0));
+  M3_TRY(operand(dx, "dx", 3, x->shape, xt, false, false, some && p.L > 0));
+  M3_TRY(operand(dlast, "dlast", 3, ls, xt, false, true, some));
+  M3_TRY(operand(dweight, "dweight", 2, wsz, wt, true, false, p.E > 0));
+  M3_TRY(operand(dbias, "dbias", 1, wsz, wt, true, true, p.E > 0));
+  M3_TRY(operand(dinitial, "dinitial", 3, ls, xt, true, true, some));
+  if (p.E == 0) return M3_OK;
+  const size_t need = conv_bwd_workspace(p.batch, p.L, p.E, (int)taps);
+  if (need > 0) M3_TRY(workspace_ok(workspace, workspace_bytes, need, "causal_conv_bwd"));
+  g.dy = dy->data; g.dyb = dy->stride[0]; g.dyl = dy->stride[1];
+  g.dlast = fptr<const void>(dlast);
+  g.dlb = present(dlast) ? dlast->stride[0] : 0; g.dll = present(dlast) ? dlast->stride[1] : 0;
+  g.dx = dx->data; g.dxb = dx->stride[0]; g.dxl = dx->stride[1];
+  g.dw = dweight->data;
+  g.dbias = fptr<void>(dbias);
+  g.dinit = fptr<void>(dinitial);
+  return launch_conv_bwd(p, g, (int)taps, x->dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int m3_causal_conv_step(m3_tensor* state, const m3_tensor* x, const m3_tensor* weight, const m3_tensor* bias, int silu,
+                        m3_tensor* y, void* stream) {
+  int64_t taps = 0;
+  M3_TRY(conv_operands(x, 2, weight, bias, silu, &taps));
+  const int64_t batch = x->shape[0], E = x->shape[1], ss[3] = {batch, taps - 1, E};
+  const bool some = batch * E > 0;
+  M3_TRY(operand(state, "state", 3, ss, 1u << x->dtype, false, false, some));
+  M3_TRY(operand(y, "y", 2, x->shape, 1u << x->dtype, true, false, some));
+  if (!some) return M3_OK;
+  ConvStepParams p{state->data, state->stride[0], state->stride[1], x->data, x->stride[0], weight->data, weight->stride[0],
+                   fptr<const void>(bias), weight->dtype == M3_FLOAT32, silu != 0, y->data, batch, (int)E};
+  return launch_conv_step(p, (int)taps, x->dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t m3_selective_scan_workspace_size(int64_t batch, int64_t seqlen, int64_t channels, int64_t d_state, int64_t groups) {
+  if (!selective_sizes_ok(batch, seqlen, channels, d_state, groups)) return 0;
+  return sel_scan_fwd_workspace(selective_sizes(batch, seqlen, channels, d_state, groups), sms_here());
+}
+
+size_t m3_selective_scan_states_size(int64_t batch, int64_t seqlen, int64_t channels, int64_t d_state) {
+  if (!selective_sizes_ok(batch, seqlen, channels, d_state, 1)) return 0;
+  return sel_scan_save_bytes(batch, seqlen, channels, (int)d_state);
+}
+
+size_t m3_selective_scan_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t channels, int64_t d_state, int64_t groups) {
+  if (!selective_sizes_ok(batch, seqlen, channels, d_state, groups)) return 0;
+  return sel_scan_bwd_workspace(selective_sizes(batch, seqlen, channels, d_state, groups), sms_here());
+}
+
+int m3_selective_scan(const m3_tensor* u, const m3_tensor* delta, const m3_tensor* A, const m3_tensor* B, const m3_tensor* C,
+                      const m3_tensor* D, const m3_tensor* z, const m3_tensor* delta_bias, const m3_tensor* initial,
+                      const m3_tensor* lengths, int softplus, m3_tensor* y, m3_tensor* last, void* states,
+                      size_t states_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  SelScanParams p{};
+  bool empty = false;
+  M3_TRY(selective_params(u, delta, A, B, C, D, z, delta_bias, initial, lengths, softplus, &p, &empty));
+  const int64_t hs[3] = {p.batch, p.E, p.N};
+  M3_TRY(operand(y, "y", 3, u->shape, 1u << u->dtype, false, false, !empty && p.L > 0));
+  M3_TRY(operand(last, "last", 3, hs, kF32, true, true, !empty));
+  if (empty) return M3_OK;
+  const size_t need = sel_scan_fwd_workspace(p, sms_here());
+  if (need > 0) M3_TRY(workspace_ok(workspace, workspace_bytes, need, "selective_scan"));
+  if (states != nullptr)
+    M3_TRY(workspace_ok(states, states_bytes, sel_scan_save_bytes(p.batch, p.L, p.E, p.N), "selective_scan states"));
+  p.y = seq(y);
+  p.h_last = fptr<float>(last);
+  p.save = static_cast<float*>(states);
+  return launch_sel_scan_fwd(p, u->dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int m3_selective_scan_bwd(const m3_tensor* u, const m3_tensor* delta, const m3_tensor* A, const m3_tensor* B,
+                          const m3_tensor* C, const m3_tensor* D, const m3_tensor* z, const m3_tensor* delta_bias,
+                          const m3_tensor* initial, const m3_tensor* lengths, int softplus, const m3_tensor* dy,
+                          const m3_tensor* dlast, m3_tensor* du, m3_tensor* ddelta, m3_tensor* dA, m3_tensor* dB,
+                          m3_tensor* dC, m3_tensor* dD, m3_tensor* dz, m3_tensor* ddelta_bias, m3_tensor* dinitial,
+                          const void* states, size_t states_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  SelScanParams p{};
+  SelScanGrads g{};
+  bool empty = false;
+  M3_TRY(selective_params(u, delta, A, B, C, D, z, delta_bias, initial, lengths, softplus, &p, &empty));
+  const bool some = !empty && p.L > 0;
+  const unsigned ut = 1u << u->dtype;
+  const int64_t hs[3] = {p.batch, p.E, p.N}, an[2] = {p.E, p.N};
+  M3_TRY(operand(dy, "dy", 3, u->shape, ut, false, false, some));
+  M3_TRY(operand(dlast, "dlast", 3, hs, kF32, true, true, !empty));
+  M3_TRY(operand(du, "du", 3, u->shape, ut, false, false, some));
+  M3_TRY(operand(ddelta, "ddelta", 3, u->shape, 1u << delta->dtype, false, false, some));
+  M3_TRY(operand(dz, "dz", 3, u->shape, ut, false, !present(z), some));
+  M3_TRY(operand(dA, "dA", 2, an, kF32, true, false, p.E > 0));
+  M3_TRY(operand(dB, "dB", 4, B->shape, 1u << B->dtype, true, false, some));
+  M3_TRY(operand(dC, "dC", 4, B->shape, 1u << B->dtype, true, false, some));
+  M3_TRY(operand(dD, "dD", 1, an, kF32, true, true, p.E > 0));
+  M3_TRY(operand(ddelta_bias, "ddelta_bias", 1, an, kF32, true, true, p.E > 0));
+  M3_TRY(operand(dinitial, "dinitial", 3, hs, kF32, true, true, !empty));
+  if (p.E == 0) return M3_OK;
+  if (some) M3_TRY(workspace_ok(states, states_bytes, sel_scan_save_bytes(p.batch, p.L, p.E, p.N), "selective_scan states"));
+  const size_t need = sel_scan_bwd_workspace(p, sms_here());
+  if (need > 0) M3_TRY(workspace_ok(workspace, workspace_bytes, need, "selective_scan_bwd"));
+  p.save = static_cast<float*>(const_cast<void*>(states));
+  g.dy = seq(dy); g.du = seq(du); g.ddelta = seq(ddelta); g.dz = seq(dz);
+  g.dstate = fptr<const float>(dlast);
+  g.dA = fptr<float>(dA); g.dD = fptr<float>(dD); g.dbias = fptr<float>(ddelta_bias);
+  g.dB = dB->data; g.dC = dC->data;
+  g.dh0 = fptr<float>(dinitial);
+  return launch_sel_scan_bwd(p, g, u->dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int m3_selective_step(m3_tensor* state, const m3_tensor* u, const m3_tensor* delta, const m3_tensor* A, const m3_tensor* B,
+                      const m3_tensor* C, const m3_tensor* D, const m3_tensor* z, const m3_tensor* delta_bias, int softplus,
+                      m3_tensor* y, void* stream) {
+  if (!present(u) || u->ndim != 2) return fail(M3_ERR_INVALID_ARGUMENT, "u: expected (batch, channels)");
+  const int64_t batch = u->shape[0], E = u->shape[1];
+  if (batch < 0 || E < 0) return fail(M3_ERR_INVALID_ARGUMENT, "u: negative extent");
+  const bool some = batch * E > 0;
+  M3_TRY(operand(u, "u", 2, u->shape, kAnyFloat, false, false, some));
+  M3_TRY(operand(delta, "delta", 2, u->shape, own_or_f32(u), false, false, some));
+  M3_TRY(operand(z, "z", 2, u->shape, 1u << u->dtype, false, true, some));
+  if (!present(A) || A->ndim != 2) return fail(M3_ERR_INVALID_ARGUMENT, "A: expected (channels, d_state)");
+  const int64_t N = A->shape[1], an[2] = {E, N}, hs[3] = {batch, E, N};
+  if (N < 1) return fail(M3_ERR_INVALID_ARGUMENT, "A: d_state must be positive");
+  if (N > kSelMaxStates) return fail(M3_ERR_UNSUPPORTED, "A: d_state above " + std::to_string(kSelMaxStates));
+  M3_TRY(operand(A, "A", 2, an, kF32, true, false, some));
+  if (!present(B) || B->ndim != 3) return fail(M3_ERR_INVALID_ARGUMENT, "B: expected (batch, groups, d_state)");
+  const int64_t G = B->shape[1], bs[3] = {batch, G, N};
+  if (G < 1 || E % G != 0) return fail(M3_ERR_INVALID_ARGUMENT, "B: the channels must divide into its groups");
+  M3_TRY(operand(B, "B", 3, bs, own_or_f32(u), false, false, some));
+  M3_TRY(operand(C, "C", 3, bs, 1u << B->dtype, false, false, some));
+  M3_TRY(operand(D, "D", 1, an, kF32, true, true, some));
+  M3_TRY(operand(delta_bias, "delta_bias", 1, an, kF32, true, true, some));
+  M3_TRY(operand(state, "state", 3, hs, kF32, false, false, some));
+  if (some && E > 1 && state->stride[1] != N)
+    return fail(M3_ERR_INVALID_ARGUMENT, "state: each sequence's part must be contiguous");
+  M3_TRY(operand(y, "y", 2, u->shape, 1u << u->dtype, false, false, some));
+  M3_TRY(flag(softplus, "softplus"));
+  if (E > INT32_MAX / (2 * kSelMaxStates) || batch > (INT64_C(1) << 36) / std::max<int64_t>(1, E))
+    return fail(M3_ERR_UNSUPPORTED, "u: dimension too large");
+  if (!some) return M3_OK;
+  SelStepParams p{};
+  p.u = u->data; p.delta = delta->data; p.z = fptr<const void>(z); p.B = B->data; p.C = C->data; p.y = y->data;
+  p.su = u->stride[0]; p.sd = delta->stride[0]; p.sz = present(z) ? z->stride[0] : 0;
+  p.sB = B->stride[0]; p.sC = C->stride[0]; p.sBg = B->stride[1]; p.sCg = C->stride[1]; p.sy = y->stride[0];
+  p.delta_f32 = delta->dtype == M3_FLOAT32; p.bc_f32 = B->dtype == M3_FLOAT32;
+  p.A = fptr<const float>(A); p.D = fptr<const float>(D); p.bias = fptr<const float>(delta_bias);
+  p.softplus = softplus != 0;
+  p.state = fptr<float>(state); p.sstate = state->stride[0];
+  p.batch = batch; p.E = (int)E; p.N = (int)N; p.G = (int)G;
+  return launch_sel_step(p, u->dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+// ------------------------------------------------------------------------------------
+// beam search
+// ------------------------------------------------------------------------------------
+size_t m3_beam_select_workspace_size(int64_t batch, int64_t beams, int64_t vocabulary, int64_t num, int dtype) {
+  if (batch < 0 || beams < 1 || beams > kMaxBeams || vocabulary < 1 || vocabulary > kMaxVocab || num < 1 ||
+      num > kMaxCandidates || dtype < 0 || dtype > M3_FLOAT16)
+    return 0;
+  return beam_workspace_bytes(batch, (int)beams, (int)vocabulary, (int)num, dtype, sms_here());
+}
+
+int m3_beam_select(const m3_tensor* logits, const m3_tensor* scores, const m3_tensor* finished, int64_t end_token,
+                   m3_tensor* out_scores, m3_tensor* parents, m3_tensor* tokens, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+  if (!present(logits) || logits->ndim != 3) return fail(M3_ERR_INVALID_ARGUMENT, "logits: expected (batch, beams, vocabulary)");
+  const int64_t batch = logits->shape[0], K = logits->shape[1], V = logits->shape[2];
+  if (batch < 0 || K < 1 || V < 1) return fail(M3_ERR_INVALID_ARGUMENT, "logits: no beam or no token");
+  if (K > kMaxBeams) return fail(M3_ERR_UNSUPPORTED, "logits: more than " + std::to_string(kMaxBeams) + " beams");
+  if (V > kMaxVocab || batch * K > kMaxGrid) return fail(M3_ERR_UNSUPPORTED, "logits: dimension too large");
+  M3_TRY(operand(logits, "logits", 3, logits->shape, kAnyFloat, false, false, batch > 0));
+  Map2<const float> sc;
+  Map2<const uint8_t> fin;
+  M3_TRY(map2(scores, "scores", M3_FLOAT32, logits->shape, false, batch > 0, &sc));
+  M3_TRY(map2(finished, "finished", M3_UINT8, logits->shape, true, batch > 0, &fin));
+  if (end_token < 0 || end_token >= V) return fail(M3_ERR_INVALID_ARGUMENT, "end_token: outside the vocabulary");
+  if (!present(out_scores) || out_scores->ndim != 2) return fail(M3_ERR_INVALID_ARGUMENT, "out_scores: expected (batch, num)");
+  const int64_t num = out_scores->shape[1], os[2] = {batch, num};
+  if (num < 1 || num > K * V) return fail(M3_ERR_INVALID_ARGUMENT, "out_scores: 1 to beams * vocabulary candidates expected");
+  if (num > kMaxCandidates) return fail(M3_ERR_UNSUPPORTED, "out_scores: more than " + std::to_string(kMaxCandidates) + " candidates");
+  M3_TRY(operand(out_scores, "out_scores", 2, os, kF32, true, false, batch > 0));
+  for (const m3_tensor* t : {static_cast<const m3_tensor*>(parents), static_cast<const m3_tensor*>(tokens)}) {
+    const char* name = t == parents ? "parents" : "tokens";
+    if (!present(t) || t->dtype != M3_INT64 || t->ndim != 2 || t->shape[0] != batch || t->shape[1] != num ||
+        (num > 1 && t->stride[1] != 1) || (batch > 1 && t->stride[0] != num))
+      return fail(M3_ERR_INVALID_ARGUMENT, std::string(name) + ": expected (batch, num) int64, contiguous");
+    if (batch > 0) {
+      M3_TRY(check_device_ptr(t->data, name));
+      M3_TRY(elem_aligned(t, name));
+    }
+  }
+  if (batch == 0) return M3_OK;
+  M3_TRY(workspace_ok(workspace, workspace_bytes,
+                      beam_workspace_bytes(batch, (int)K, (int)V, (int)num, logits->dtype, sms_here()), "beam_select"));
+  BeamParams p{};
+  p.logits = logits->data; p.lb = logits->stride[0]; p.lk = logits->stride[1];
+  p.scores = sc.p; p.sb = sc.sb; p.sk = sc.st;
+  p.finished = fin.p; p.fb = fin.sb; p.fk = fin.st;
+  p.batch = batch; p.beams = (int)K; p.V = (int)V; p.num = (int)num; p.end_token = (int)end_token;
+  p.out_scores = fptr<float>(out_scores); p.parents = fptr<int64_t>(parents); p.tokens = fptr<int64_t>(tokens);
+  return launch_beam_select(p, logits->dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int m3_reorder_states(int64_t count, const void* const* src, void* const* dst, const int64_t* row_bytes,
+                      const int64_t* src_pitch, const int64_t* dst_pitch, int64_t source_rows, const m3_tensor* parents,
+                      void* stream) try {
+  if (count < 0 || (count > 0 && (!src || !row_bytes || !src_pitch || (dst && !dst_pitch))))
+    return fail(M3_ERR_INVALID_ARGUMENT, "states: missing");
+  if (!present(parents) || parents->ndim != 2 || parents->dtype != M3_INT64)
+    return fail(M3_ERR_INVALID_ARGUMENT, "parents: expected (batch, rows) int64");
+  const int64_t batch = parents->shape[0], T = parents->shape[1], S = source_rows;
+  if (parents->stride[0] < 0 || parents->stride[1] < 0) return fail(M3_ERR_INVALID_ARGUMENT, "parents: negative stride");
+  if (S < 0 || batch < 0 || T < 0 || S > INT32_MAX || batch > INT32_MAX || T > INT32_MAX)
+    return fail(M3_ERR_INVALID_ARGUMENT, "parents: sizes out of range");
+  if (!dst && S != T) return fail(M3_ERR_INVALID_ARGUMENT, "parents: in place, as many rows as the source has expected");
+  if (!dst && T > kMaxBeams)
+    return fail(M3_ERR_UNSUPPORTED, "parents: more than " + std::to_string(kMaxBeams) + " rows of a group in place");
+  // what is read and written: rows of `bytes` every `pitch` bytes from lo to hi
+  struct Range { uintptr_t lo, hi; int64_t bytes, pitch, index; bool written; };
+  std::vector<Range> ranges, open;
+  ranges.reserve((size_t)count * (dst ? 2 : 1));
+  const bool some = batch > 0 && T > 0;
+  int64_t first = -1;
+  for (int64_t i = 0; i < count; ++i) {
+    auto name = [&](const char* what) { return std::string(what) + "[" + std::to_string(i) + "]"; };
+    if (row_bytes[i] < 0) return fail(M3_ERR_INVALID_ARGUMENT, name("row_bytes") + ": negative");
+    if (row_bytes[i] == 0 || !some) continue;
+    auto add = [&](const void* p, int64_t pitch, int64_t rows, bool written, const char* what) {
+      if (!p) return fail(M3_ERR_INVALID_ARGUMENT, name(what) + ": missing");
+      if (rows > 1 && pitch < row_bytes[i]) return fail(M3_ERR_INVALID_ARGUMENT, name(what) + ": rows overlap");
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+      ranges.push_back(Range{lo, lo + (uintptr_t)((rows - 1) * pitch + row_bytes[i]), row_bytes[i], pitch, i, written});
+      return (int)M3_OK;
+    };
+    if (S > 0) M3_TRY(add(src[i], src_pitch[i], batch * S, dst == nullptr, "states"));
+    if (dst) M3_TRY(add(dst[i], dst_pitch[i], batch * T, true, "out"));
+    if (first < 0) first = i;
+  }
+  // ranges that meet may still be rows of one pitch that lie between each other, as views of a pool do
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
+  for (const Range& r : ranges) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Range& o) { return o.hi <= r.lo; }), open.end());
+    for (const Range& o : open) {
+      if (!o.written && !r.written) continue;
+      const uintptr_t d = o.pitch > 0 ? (r.lo - o.lo) % (uintptr_t)o.pitch : 0;
+      if (o.pitch != r.pitch || d < (uintptr_t)o.bytes || d + (uintptr_t)r.bytes > (uintptr_t)o.pitch)
+        return fail(M3_ERR_INVALID_ARGUMENT, "states[" + std::to_string(r.index) + "]: shares memory with another tensor of the call");
+    }
+    open.push_back(r);
+  }
+  if (first < 0) return M3_OK;
+  M3_TRY(check_device_ptr(parents->data, "parents"));
+  M3_TRY(elem_aligned(parents, "parents"));
+  if (S > 0) M3_TRY(check_device_ptr(src[first], "states"));
+  if (dst) M3_TRY(check_device_ptr(dst[first], "out"));
+  ReorderArgs a{count, src, dst ? dst : const_cast<void* const*>(src), row_bytes, src_pitch, dst ? dst_pitch : src_pitch, static_cast<const int64_t*>(parents->data),
+                parents->stride[0], parents->stride[1], batch, S, T, dst == nullptr};
+  return launch_reorder_states(a, reinterpret_cast<cudaStream_t>(stream));
+} catch (const std::exception& e) {
+  return fail(M3_ERR_INVALID_ARGUMENT, std::string("reorder_states: ") + e.what());
 }
 
 }  // extern "C"

@@ -21,7 +21,7 @@ M3_FLOAT32, M3_BFLOAT16, M3_FLOAT16 = 0, 1, 2
 M3_OK, M3_ERR_INVALID_ARGUMENT, M3_ERR_UNSUPPORTED, M3_ERR_CUDA, M3_ERR_WORKSPACE = 0, 1, 2, 3, 4
 M3_INT64, M3_UINT8 = 3, 4
 _DTYPE_CODE = {torch.float32: M3_FLOAT32, torch.bfloat16: M3_BFLOAT16, torch.float16: M3_FLOAT16,
-               torch.int64: M3_INT64}
+               torch.int64: M3_INT64, torch.uint8: M3_UINT8}
 _STATUS = {1: "invalid argument", 2: "unsupported", 3: "CUDA error", 4: "workspace"}
 
 
@@ -103,6 +103,23 @@ _SIGS = {
     "m3_clip_grads_workspace_size": ([ctypes.c_int64], ctypes.c_size_t),
     "m3_clip_grads": ([ctypes.c_int64] + [ctypes.c_void_p] * 5 + [ctypes.c_int, ctypes.c_double, ctypes.c_double, _P,
                        ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
+    "m3_causal_conv": ([_P] * 5 + [ctypes.c_int] + [_P] * 2 + [ctypes.c_void_p], ctypes.c_int),
+    "m3_causal_conv_bwd_workspace_size": ([ctypes.c_int64] * 4, ctypes.c_size_t),
+    "m3_causal_conv_bwd": ([_P] * 5 + [ctypes.c_int] + [_P] * 6 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+                           ctypes.c_int),
+    "m3_causal_conv_step": ([_P] * 4 + [ctypes.c_int, _P, ctypes.c_void_p], ctypes.c_int),
+    "m3_selective_scan_workspace_size": ([ctypes.c_int64] * 5, ctypes.c_size_t),
+    "m3_selective_scan_states_size": ([ctypes.c_int64] * 4, ctypes.c_size_t),
+    "m3_selective_scan": ([_P] * 10 + [ctypes.c_int] + [_P] * 2 + [ctypes.c_void_p, ctypes.c_size_t] * 2 +
+                          [ctypes.c_void_p], ctypes.c_int),
+    "m3_selective_scan_bwd_workspace_size": ([ctypes.c_int64] * 5, ctypes.c_size_t),
+    "m3_selective_scan_bwd": ([_P] * 10 + [ctypes.c_int] + [_P] * 11 + [ctypes.c_void_p, ctypes.c_size_t] * 2 +
+                              [ctypes.c_void_p], ctypes.c_int),
+    "m3_selective_step": ([_P] * 9 + [ctypes.c_int, _P, ctypes.c_void_p], ctypes.c_int),
+    "m3_beam_select_workspace_size": ([ctypes.c_int64] * 4 + [ctypes.c_int], ctypes.c_size_t),
+    "m3_beam_select": ([_P] * 3 + [ctypes.c_int64] + [_P] * 3 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+                       ctypes.c_int),
+    "m3_reorder_states": ([ctypes.c_int64] + [ctypes.c_void_p] * 5 + [ctypes.c_int64, _P, ctypes.c_void_p], ctypes.c_int),
 }
 
 _lib = None
