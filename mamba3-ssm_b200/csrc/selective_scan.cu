@@ -6,6 +6,7 @@
 // channel's lanes are formed for several steps together by halving exchanges, and y leaves
 // through shared memory in whole rows. The next tile's operands are loaded while this one is scanned.
 #include <algorithm>
+#include <type_traits>
 
 #include "selective_scan.cuh"
 
@@ -13,169 +14,256 @@ namespace m3 {
 namespace {
 
 constexpr int TT = kSelTile;
-constexpr int TS = TT + 4;  // row pitch: rows that a warp reads together start on different banks
+constexpr int TS = kSelPitch;
+
+// states of a lane whose decays the FMA pipe forms
+#ifndef M3_POLY
+#define M3_POLY 0
+#endif
+template <int K> constexpr int kPolyStates() { return K >= 4 ? M3_POLY : 0; }
 
 // steps whose sums over the lanes are formed together
 template <int P> constexpr int group_steps() { return P < 4 ? 4 : P; }
 
-template <int K, int P, int NT>
+template <int K, int P, int M, int NT>
 struct FwdSmem {
-  static constexpr int NP = K * P, EC = NT / P;
+  static constexpr int NP = K * P, EC = NT / P * M;
   float dt[EC][TS], dx[EC][TS];
   float B[NP][TS], C[NP][TS];
   float y[TT][EC + 8];
 };
 
+template <int NT>
+__device__ __forceinline__ void tile_sync() {
+  if constexpr (NT == 32) __syncwarp();
+  else __syncthreads();
+}
+
 // OUT: the scan proper. Else only the state that a piece of the sequence leaves, from zero, and
-// the sum of its step sizes.
-template <typename T, int K, int P, int NT, bool OUT>
+// the sum of its step sizes. FAST: every operand is of u's type and read two elements at a time.
+template <typename T, int K, int P, int M, int NT, bool OUT, bool FAST>
 __global__ void __launch_bounds__(NT) sel_scan_kernel(const SelScanParams p) {
-  using S = FwdSmem<K, P, NT>;
-  constexpr int NP = S::NP, EC = S::EC, JN = TT * EC / NT, JB = (TT * NP + NT - 1) / NT, GS = group_steps<P>();
+  using S = FwdSmem<K, P, M, NT>;
+  constexpr int NP = S::NP, EC = S::EC, GS = group_steps<P>();
+  constexpr int R = TT * M / (2 * P) > 0 ? TT * M / (2 * P) : 1;  // steps of a pair of channels that a thread brings
+  constexpr bool kAhead = BcTile<T, K, P, NT, FAST>::J <= 2;      // B and C of the next tile are loaded ahead too
   extern __shared__ __align__(16) unsigned char smem_raw[];
   S& sh = *reinterpret_cast<S*>(smem_raw);
-  const int tid = threadIdx.x, q = tid % P, el = tid / P;
+  const int tid = threadIdx.x, q = tid % P, el = tid / P;  // channels el, el + NT / P, ..
   const int Eg = p.E / p.G, tiles = (Eg + EC - 1) / EC;
   const int g = blockIdx.x / tiles, e_first = g * Eg + (blockIdx.x % tiles) * EC, e_end = (g + 1) * Eg;
   const int b = blockIdx.z, c = blockIdx.y;
   const int beg = c * p.chunk, end = min(p.L, beg + p.chunk);
   const int len = seq_len(p.lengths, b, p.L);
-  const int e = e_first + el;
-  const bool live = e < e_end;
-  const int ec = live ? e : e_end - 1;
-  // element (t, le) of a tile that this thread brings and stores
-  const int le = tid % EC, lt = tid / EC;
-  const int lec = min(e_first + le, e_end - 1);
-  const bool lelive = e_first + le < e_end;
+  // channels (le, le + 1) at steps lt .. lt + R - 1 of a tile: what this thread brings and stores. A pair
+  // behind the last channel reads the tile's first one instead, which lies on a pair's boundary too.
+  const int le = tid % (EC / 2) * 2, lt = tid / (EC / 2) * R;
+  const bool brings = TT * EC / 2 >= NT * R || lt < TT;
+  const int l0 = e_first + le < e_end ? e_first + le : e_first, second = l0 + 1 < e_end ? 1 : 0;
+  const bool lelive = brings && e_first + le < e_end;
+  const bool vu = FAST || p.vec_u, vd = FAST || p.vec_d, vz = FAST || p.vec_z, vy = FAST || p.vec_y;
 
-  float A2[K], h[K];
+  float A2[M][K], h[M][K], dts[M];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int n = q * K + k;
-    A2[k] = n < p.N ? p.A[(int64_t)ec * p.N + n] * kLog2e : 0.f;
-    h[k] = 0.f;
-    if (OUT) {
-      if (p.nchunk > 1) h[k] = p.states[(((int64_t)b * p.nchunk + c) * p.E + ec) * NP + n];
-      else if (p.h0 != nullptr && n < p.N) h[k] = p.h0[((int64_t)b * p.E + ec) * p.N + n];
+  for (int m = 0; m < M; ++m) {
+    const int ec = min(e_first + el + m * (NT / P), e_end - 1);
+    dts[m] = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int n = q * K + k;
+      A2[m][k] = n < p.N ? p.A[(int64_t)ec * p.N + n] * kLog2e : 0.f;
+      h[m][k] = 0.f;
+      if (OUT) {
+        if (p.nchunk > 1) h[m][k] = p.states[(((int64_t)b * p.nchunk + c) * p.E + ec) * NP + n];
+        else if (p.h0 != nullptr && n < p.N) h[m][k] = p.h0[((int64_t)b * p.E + ec) * p.N + n];
+      }
     }
   }
-  const float bias = p.bias != nullptr ? p.bias[lec] : 0.f;
-  const float Dv = OUT && p.D != nullptr ? p.D[lec] : 0.f;
-  float dts = 0.f;
+  const float bias0 = p.bias != nullptr ? p.bias[l0] : 0.f, bias1 = p.bias != nullptr ? p.bias[l0 + second] : 0.f;
+  const float D0 = OUT && p.D != nullptr ? p.D[l0] : 0.f, D1 = OUT && p.D != nullptr ? p.D[l0 + second] : 0.f;
 
-  const T* up = static_cast<const T*>(p.u.p) + (int64_t)b * p.u.sb + lec;
-  const T* zp = OUT && p.z.p != nullptr ? static_cast<const T*>(p.z.p) + (int64_t)b * p.z.sb + lec : nullptr;
-  T* yp = OUT ? static_cast<T*>(const_cast<void*>(p.y.p)) + (int64_t)b * p.y.sb + lec : nullptr;
-  const int64_t doff = (int64_t)b * p.delta.sb + lec;
+  const T* up = static_cast<const T*>(p.u.p) + (int64_t)b * p.u.sb + l0;
+  const T* zp = OUT && p.z.p != nullptr ? static_cast<const T*>(p.z.p) + (int64_t)b * p.z.sb + l0 : nullptr;
+  T* yp = OUT ? static_cast<T*>(const_cast<void*>(p.y.p)) + (int64_t)b * p.y.sb + l0 : nullptr;
+  const int64_t doff = (int64_t)b * p.delta.sb + l0;
   const int64_t boff = (int64_t)b * p.B.sb + g * p.Bg, coff = (int64_t)b * p.C.sb + g * p.Cg;
 
-  float ru[JN], rd[JN];
+  // loads of rows behind the sequence's end read its last one; nothing is made of them
+  Raw2<T> ru[R];
+  std::conditional_t<FAST, Raw2<T>, RawAny<T>> rd[R];
+  BcTile<T, K, P, NT, FAST> tb, tc;
   auto fetch = [&](int t0) {
+    if (brings) {
 #pragma unroll
-    for (int j = 0; j < JN; ++j) {
-      const int t = t0 + lt + j * (NT / EC);
-      ru[j] = rd[j] = 0.f;
-      if (t < len) {
-        ru[j] = ld(up + (int64_t)t * p.u.sl);
-        rd[j] = ld_any<T>(p.delta.p, p.delta_f32, doff + (int64_t)t * p.delta.sl);
+      for (int j = 0; j < R; ++j) {
+        const int64_t t = min(t0 + lt + j, len - 1);
+        ru[j] = load2<T>(up + t * p.u.sl, vu, second);
+        load2_any<T>(rd[j], p.delta.p, p.delta_f32, doff + t * p.delta.sl, vd, second);
       }
     }
   };
-  if (beg < len) fetch(beg);
-  int t0 = beg;
-  for (; t0 < end && t0 < len; t0 += TT) {
+  auto fetch_bc = [&](int t0) {
+    tb.fetch(p.B.p, p.bc_f32, boff, p.B.sl, p.vec_B, p.N, t0, len, tid);
+    if (OUT) tc.fetch(p.C.p, p.bc_f32, coff, p.C.sl, p.vec_C, p.N, t0, len, tid);
+  };
+  if (beg < len) {
+    fetch(beg);
+    if (kAhead) fetch_bc(beg);
+  }
+  for (int t0 = beg; t0 < end && t0 < len; t0 += TT) {
+    if (!kAhead) fetch_bc(t0);
+    Raw2<T> zu[R], zz[R];
+    if (brings) {
+      float d0[R], d1[R], x0[R], x1[R];
 #pragma unroll
-    for (int j = 0; j < JN; ++j) {
-      const int t = lt + j * (NT / EC);
-      const float dt = t0 + t < len ? step_size(rd[j] + bias, p.softplus) : 0.f;
-      sh.dt[le][t] = dt;
-      sh.dx[le][t] = dt * ru[j];
-    }
-#pragma unroll 4
-    for (int j = 0; j < JB; ++j) {
-      const int i = tid + j * NT, n = i % NP, t = i / NP;
-      if (t < TT) {
-        const bool in = n < p.N && t0 + t < len;
-        const int row = (n % K) * P + n / K;
-        sh.B[row][t] = in ? ld_any<T>(p.B.p, p.bc_f32, boff + (int64_t)(t0 + t) * p.B.sl + n) : 0.f;
-        if (OUT) sh.C[row][t] = in ? ld_any<T>(p.C.p, p.bc_f32, coff + (int64_t)(t0 + t) * p.C.sl + n) : 0.f;
-      }
-    }
-    __syncthreads();
-    float zu[JN], zz[JN];
-    if (OUT) {
-#pragma unroll
-      for (int j = 0; j < JN; ++j) {
-        const int t = t0 + lt + j * (NT / EC);
+      for (int j = 0; j < R; ++j) {
+        const float2 r = value2<T>(rd[j], p.delta_f32), u = value2(ru[j]);
+        const float2 d = step_size2(make_float2(r.x + bias0, r.y + bias1), p.softplus);
+        const bool in = t0 + lt + j < len;
+        d0[j] = in ? d.x : 0.f;
+        d1[j] = in ? d.y : 0.f;
+        x0[j] = in ? d.x * u.x : 0.f;
+        x1[j] = in ? d.y * u.y : 0.f;
         zu[j] = ru[j];
-        zz[j] = zp != nullptr && t < len ? ld(zp + (int64_t)t * p.z.sl) : 0.f;
       }
+      put_steps<R>(&sh.dt[le][lt], d0);
+      put_steps<R>(&sh.dt[le + 1][lt], d1);
+      put_steps<R>(&sh.dx[le][lt], x0);
+      put_steps<R>(&sh.dx[le + 1][lt], x1);
     }
-    if (t0 + TT < end && t0 + TT < len) fetch(t0 + TT);
-#pragma unroll 1
-    for (int tg = 0; tg < TT; tg += GS) {
-      float yv[GS];
+    tb.put(sh.B, p.bc_f32, p.N, t0, len, tid);
+    if (OUT) tc.put(sh.C, p.bc_f32, p.N, t0, len, tid);
+    tile_sync<NT>();
+    if (OUT && zp != nullptr && brings) {
 #pragma unroll
-      for (int i = 0; i < GS; ++i) yv[i] = 0.f;
+      for (int j = 0; j < R; ++j) zz[j] = load2<T>(zp + (int64_t)min(t0 + lt + j, len - 1) * p.z.sl, vz, second);
+    }
+    if (t0 + TT < end && t0 + TT < len) {
+      fetch(t0 + TT);
+      if (kAhead) fetch_bc(t0 + TT);
+    }
+    constexpr int BS = GS < kSelSub ? kSelSub : GS;  // steps between two looks at whether states are kept
+#pragma unroll 1
+    for (int tb8 = 0; tb8 < TT; tb8 += BS) {
+#pragma unroll
+    for (int tg = tb8; tg < tb8 + BS; tg += GS) {
+      float yv[M][GS];
 #pragma unroll
       for (int i4 = 0; i4 < GS; i4 += 4) {
-        if (OUT && p.save != nullptr && (tg + i4) % kSelSub == 0 && live && t0 + tg + i4 < len) {
-          float* sv = p.save + (((int64_t)b * ((p.L + kSelSub - 1) / kSelSub) + (t0 + tg + i4) / kSelSub) * p.E + e) * NP + q * K;
+        if (OUT && (GS < kSelSub ? tg == tb8 : i4 % kSelSub == 0) && p.save != nullptr && t0 + tg + i4 < len) {
+          float* sv = p.save + (((int64_t)b * ((p.L + kSelSub - 1) / kSelSub) + (t0 + tg + i4) / kSelSub) * p.E + e_first + el) * NP + q * K;
 #pragma unroll
-          for (int k = 0; k < K; ++k) sv[k] = h[k];
+          for (int m = 0; m < M; ++m)
+            if (e_first + el + m * (NT / P) < e_end) {
+              float* at = sv + (int64_t)m * (NT / P) * NP;
+              if constexpr (K == 4) *reinterpret_cast<float4*>(at) = make_float4(h[m][0], h[m][1], h[m][2], h[m][3]);
+              else {
+#pragma unroll
+                for (int k = 0; k < K; ++k) at[k] = h[m][k];
+              }
+            }
         }
-        const float4 d4 = *reinterpret_cast<const float4*>(&sh.dt[el][tg + i4]);
-        const float4 x4 = *reinterpret_cast<const float4*>(&sh.dx[el][tg + i4]);
-        const float dv[4] = {d4.x, d4.y, d4.z, d4.w}, xv[4] = {x4.x, x4.y, x4.z, x4.w};
-        if (!OUT) dts += (dv[0] + dv[1]) + (dv[2] + dv[3]);
+        ulonglong2 d4[M], x4[M];
+        f2 ya[M], yb[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          d4[m] = *reinterpret_cast<const ulonglong2*>(&sh.dt[el + m * (NT / P)][tg + i4]);
+          x4[m] = *reinterpret_cast<const ulonglong2*>(&sh.dx[el + m * (NT / P)][tg + i4]);
+          ya[m] = yb[m] = 0;
+          if (!OUT) {
+            float s0, s1;
+            unpack2(add2(d4[m].x, d4[m].y), s0, s1);
+            dts[m] += s0 + s1;
+          }
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          const float4 b4 = *reinterpret_cast<const float4*>(&sh.B[k * P + q][tg + i4]);
-          const float bv[4] = {b4.x, b4.y, b4.z, b4.w};
-          float cv[4];
-          if (OUT) {
-            const float4 c4 = *reinterpret_cast<const float4*>(&sh.C[k * P + q][tg + i4]);
-            cv[0] = c4.x; cv[1] = c4.y; cv[2] = c4.z; cv[3] = c4.w;
-          }
+          const ulonglong2 b4 = *reinterpret_cast<const ulonglong2*>(&sh.B[k * P + q][tg + i4]);
+          ulonglong2 c4{0, 0};
+          if (OUT) c4 = *reinterpret_cast<const ulonglong2*>(&sh.C[k * P + q][tg + i4]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            h[k] = fmaf(ex2(dv[i] * A2[k]), h[k], xv[i] * bv[i]);
-            if (OUT) yv[i4 + i] = fmaf(h[k], cv[i], yv[i4 + i]);
+          for (int m = 0; m < M; ++m) {
+            const f2 A2k = pack2(A2[m][k], A2[m][k]), mean = pack2(kEx2Mean, kEx2Mean);
+            float a[4], x[4], hv[4];
+            if (k < kPolyStates<K>()) {
+              unpack2(ex2_poly2(mul2(d4[m].x, A2k)), a[0], a[1]);
+              unpack2(ex2_poly2(mul2(d4[m].y, A2k)), a[2], a[3]);
+            } else {
+              unpack2(fma2(d4[m].x, A2k, mean), a[0], a[1]);
+              unpack2(fma2(d4[m].y, A2k, mean), a[2], a[3]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) a[i] = ex2(a[i]);
+            }
+            unpack2(mul2(x4[m].x, b4.x), x[0], x[1]);
+            unpack2(mul2(x4[m].y, b4.y), x[2], x[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) hv[i] = h[m][k] = fmaf(a[i], h[m][k], x[i]);
+            if (OUT) {
+              ya[m] = fma2(pack2(hv[0], hv[1]), c4.x, ya[m]);
+              yb[m] = fma2(pack2(hv[2], hv[3]), c4.y, yb[m]);
+            }
           }
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          unpack2(ya[m], yv[m][i4], yv[m][i4 + 1]);
+          unpack2(yb[m], yv[m][i4 + 2], yv[m][i4 + 3]);
         }
       }
       if (OUT) {
-        const int at = spread_sum<GS, P>(yv, q);
 #pragma unroll
-        for (int j = 0; j < GS / P; ++j) sh.y[tg + at + j][el] = yv[j];
+        for (int m = 0; m < M; ++m) {
+          const int at = spread_sum<GS, P>(yv[m], q);
+#pragma unroll
+          for (int j = 0; j < GS / P; ++j) sh.y[tg + at + j][el + m * (NT / P)] = yv[m][j];
+        }
       }
     }
-    __syncthreads();
-    if (OUT) {
+    }
+    tile_sync<NT>();
+    if (OUT && lelive) {
 #pragma unroll
-      for (int j = 0; j < JN; ++j) {
-        const int t = lt + j * (NT / EC);
-        if (lelive && t0 + t < end) {
-          float v = fmaf(Dv, zu[j], sh.y[t][le]);
-          if (zp != nullptr) v *= zz[j] * fast_sigmoid(zz[j]);
-          st(yp + (int64_t)(t0 + t) * p.y.sl, t0 + t < len ? v : 0.f);
+      for (int j = 0; j < R; ++j) {
+        const int t = t0 + lt + j;
+        if (t < end) {
+          const float2 u = value2(zu[j]), y2 = *reinterpret_cast<const float2*>(&sh.y[lt + j][le]);
+          float v0 = fmaf(D0, u.x, y2.x), v1 = fmaf(D1, u.y, y2.y);
+          if (zp != nullptr) {
+            const float2 z = value2(zz[j]);
+            v0 *= z.x * fast_sigmoid(z.x);
+            v1 *= z.y * fast_sigmoid(z.y);
+          }
+          store2<T>(yp + (int64_t)t * p.y.sl, vy, second, t < len ? v0 : 0.f, t < len ? v1 : 0.f);
         }
       }
     }
   }
   if (OUT) {
-    for (int t = t0 + lt; t < end; t += NT / EC)  // padding
-      if (lelive) st(yp + (int64_t)t * p.y.sl, 0.f);
-    if (p.h_last != nullptr && c == p.nchunk - 1 && live) {
+    // padding behind the last tile with a position that counts
+    const int from = len > beg ? beg + (min(len, end) - beg + TT - 1) / TT * TT : beg;
+    for (int t0 = from; t0 < end; t0 += TT) {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (q * K + k < p.N) p.h_last[((int64_t)b * p.E + e) * p.N + q * K + k] = h[k];
+      for (int j = 0; j < R; ++j)
+        if (lelive && t0 + lt + j < end) store2<T>(yp + (int64_t)(t0 + lt + j) * p.y.sl, vy, second, 0.f, 0.f);
     }
-  } else if (live) {
-    const int64_t at = ((int64_t)b * p.nchunk + c) * p.E + e;
+  }
 #pragma unroll
-    for (int k = 0; k < K; ++k) p.states[at * NP + q * K + k] = h[k];
-    if (q == 0) p.dtsum[at] = dts;
+  for (int m = 0; m < M; ++m) {
+    const int e = e_first + el + m * (NT / P);
+    if (e < e_end) {
+      if (OUT) {
+        if (p.h_last != nullptr && c == p.nchunk - 1) {
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if (q * K + k < p.N) p.h_last[((int64_t)b * p.E + e) * p.N + q * K + k] = h[m][k];
+        }
+      } else {
+        const int64_t at = ((int64_t)b * p.nchunk + c) * p.E + e;
+#pragma unroll
+        for (int k = 0; k < K; ++k) p.states[at * NP + q * K + k] = h[m][k];
+        if (q == 0) p.dtsum[at] = dts[m];
+      }
+    }
   }
 }
 
@@ -190,11 +278,12 @@ __global__ void __launch_bounds__(256) sel_carry_kernel(const SelScanParams p, i
   float* st = p.states + (int64_t)b * p.nchunk * pitch + i;
   const float* ds = p.dtsum + (int64_t)b * p.nchunk * p.E + e;
 #pragma unroll 4
-  for (int c = 0; c < p.nchunk; ++c) {
+  for (int c = 0; c < p.nchunk - 1; ++c) {
     const float local = st[c * pitch], a = ex2(A2 * ds[(int64_t)c * p.E]);
     st[c * pitch] = h;
     h = fmaf(a, h, local);
   }
+  st[(p.nchunk - 1) * pitch] = h;
 }
 
 // One step: y and the state in place. P lanes a channel, K states each.
@@ -262,17 +351,30 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
+#ifndef M3_M
+#define M3_M 1
+#endif
+#ifndef M3_NT
+#define M3_NT 64
+#endif
 template <typename T, int K, int P, bool OUT>
 int launch_pass(const SelScanParams& p, cudaStream_t s) {
-  constexpr int NT = 128;
-  using S = FwdSmem<K, P, NT>;
-  static std::atomic<bool> done[kMaxDevices];
-  const void* kernel = reinterpret_cast<const void*>(&sel_scan_kernel<T, K, P, NT, OUT>);
-  M3_TRY(ensure_dynamic_smem(kernel, sizeof(S), done));
+  constexpr int M = P >= 4 ? M3_M : 1, NT = P >= 16 ? 128 : M3_NT;
+  using S = FwdSmem<K, P, M, NT>;
   const int Eg = p.E / p.G;
-  const dim3 grid((unsigned)(p.G * ((Eg + S::EC - 1) / S::EC)), (unsigned)p.nchunk, (unsigned)p.batch);
-  sel_scan_kernel<T, K, P, NT, OUT><<<grid, NT, sizeof(S), s>>>(p);
-  return check_launch("sel_scan_kernel");
+  // what the last piece leaves enters no other
+  const dim3 grid((unsigned)(p.G * ((Eg + S::EC - 1) / S::EC)), (unsigned)(OUT ? p.nchunk : p.nchunk - 1), (unsigned)p.batch);
+  auto go = [&](auto fast) {
+    static std::atomic<bool> done[kMaxDevices];
+    constexpr bool FAST = decltype(fast)::value;
+    M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(&sel_scan_kernel<T, K, P, M, NT, OUT, FAST>), sizeof(S), done));
+    sel_scan_kernel<T, K, P, M, NT, OUT, FAST><<<grid, NT, sizeof(S), s>>>(p);
+    return check_launch("sel_scan_kernel");
+  };
+  const bool f32 = sizeof(T) == 4;
+  const bool fast = p.vec_u && p.vec_d && (p.vec_z || p.z.p == nullptr) && p.vec_y && p.vec_B && p.vec_C &&
+                    (f32 || (!p.delta_f32 && !p.bc_f32));
+  return fast ? go(std::true_type{}) : go(std::false_type{});
 }
 
 // f(K, P) as types: lanes and states a lane by the padded number of states
@@ -280,7 +382,7 @@ template <int K, int P> struct KP { static constexpr int k = K, p = P; };
 template <typename F>
 int by_states(int n, F&& f) {
   switch (sel_padded_states(n)) {
-    case 4: return f(KP<4, 1>{});
+    case 4: return f(KP<2, 2>{});
     case 8: return f(KP<4, 2>{});
     case 16: return f(KP<4, 4>{});
     case 32: return f(KP<4, 8>{});
@@ -290,6 +392,8 @@ int by_states(int n, F&& f) {
 }
 
 }  // namespace
+
+static int sel_lanes(int np) { return std::max(2, np / 4); }
 
 // Pieces that the sequence is cut into: one, unless the channels alone leave most of the GPU idle. A
 // piece's state has to be formed ahead (about as much work again), so cutting begins where
@@ -305,13 +409,29 @@ int sel_pieces(const SelScanParams& p, int lanes, int sms, int* chunk) {
   return std::max<int>(1, (int)((p.L + *chunk - 1) / *chunk));
 }
 
+// Whether two neighbouring elements of the rows may be moved at once: pairs begin on even channels of each group.
+static bool pairs(const Seq& s, int64_t inner, int es) {
+  return s.p != nullptr && inner % 2 == 0 && s.sb % 2 == 0 && s.sl % 2 == 0 &&
+         (reinterpret_cast<uintptr_t>(s.p) & (2 * es - 1)) == 0;
+}
+
+void sel_pair_flags(SelScanParams* p, int dtype) {
+  const int es = (int)dtype_size(dtype), Eg = p->E / p->G;
+  p->vec_u = pairs(p->u, Eg, es);
+  p->vec_d = pairs(p->delta, Eg, p->delta_f32 ? 4 : es);
+  p->vec_z = pairs(p->z, Eg, es);
+  p->vec_y = pairs(p->y, Eg, es);
+  p->vec_B = pairs(p->B, p->N, p->bc_f32 ? 4 : es) && p->Bg % 2 == 0;
+  p->vec_C = pairs(p->C, p->N, p->bc_f32 ? 4 : es) && p->Cg % 2 == 0;
+}
+
 size_t sel_scan_save_bytes(int64_t batch, int64_t L, int64_t E, int N) {
   return (size_t)batch * ((L + kSelSub - 1) / kSelSub) * E * sel_padded_states(N) * sizeof(float);
 }
 
 size_t sel_scan_fwd_workspace(const SelScanParams& p, int sms) {
   int chunk = 0;
-  const int np = sel_padded_states(p.N), n = sel_pieces(p, np / 4, sms, &chunk);
+  const int np = sel_padded_states(p.N), n = sel_pieces(p, sel_lanes(np), sms, &chunk);
   return n == 1 ? 0 : (size_t)p.batch * n * p.E * (np + 1) * sizeof(float);
 }
 
@@ -319,7 +439,8 @@ int launch_sel_scan_fwd(SelScanParams p, int dtype, void* ws, cudaStream_t s) {
   int sms = 0;
   M3_TRY(device_sm_count(&sms));
   const int np = sel_padded_states(p.N);
-  p.nchunk = sel_pieces(p, np / 4, sms, &p.chunk);
+  sel_pair_flags(&p, dtype);
+  p.nchunk = sel_pieces(p, sel_lanes(np), sms, &p.chunk);
   if (p.nchunk > 1) {
     p.states = static_cast<float*>(ws);
     p.dtsum = p.states + (int64_t)p.batch * p.nchunk * p.E * np;

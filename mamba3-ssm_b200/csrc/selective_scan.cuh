@@ -3,6 +3,8 @@
 // the device functions they share.
 #pragma once
 
+#include <type_traits>
+
 #include "m3_common.cuh"
 
 namespace m3 {
@@ -17,6 +19,7 @@ struct SelScanParams {
   Seq u, delta, z, B, C, y;      // z.p may be null; B, C: (batch, length, G, N) with rows of G * N
   int64_t Bg, Cg;                // stride of the groups of B and C
   bool delta_f32, bc_f32;        // else u's type
+  bool vec_u, vec_d, vec_z, vec_y, vec_B, vec_C;  // rows that may be read or written two elements at a time
   const float* A;                // (E, N) contiguous
   const float* D;                // (E), may be null
   const float* bias;             // (E), may be null
@@ -34,6 +37,7 @@ struct SelScanParams {
 
 struct SelScanGrads {
   Seq dy, du, ddelta, dz;        // dy: gradient of the output (after the gate), u's type
+  bool vec_du, vec_dd, vec_dz;   // rows that may be written two elements at a time
   const float* dstate;           // (batch, E, N): gradient of the last state, may be null
   float* dA;                     // (E, N)
   float* dD;                     // (E), may be null
@@ -72,11 +76,16 @@ size_t sel_scan_save_bytes(int64_t batch, int64_t L, int64_t E, int N);
 size_t sel_scan_bwd_workspace(const SelScanParams& p, int sms);
 int launch_sel_scan_bwd(SelScanParams p, SelScanGrads g, int dtype, void* ws, cudaStream_t s);
 int launch_sel_step(const SelStepParams& p, int dtype, cudaStream_t s);
+void sel_pair_flags(SelScanParams* p, int dtype);
 // the piece-wise passes that the forward and the backward share
 int sel_pieces(const SelScanParams& p, int lanes, int sms, int* chunk);
 
 #ifdef __CUDACC__
 constexpr float kLog2e = 1.4426950408889634f;
+// The hardware's 2^x is 2e-8 too small on average between -1/2 and -1/500 and 5e-9 closer to 0 (measured); a decay
+// that is wrong by that in each of the many steps a slow state remembers shows in the state. Added to the
+// exponent in the product's own rounding, this halves it where it is largest and keeps 2^0 = 1.
+constexpr float kEx2Mean = 1.5e-8f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -84,22 +93,144 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// log(1 + e^x) = max(x, 0) + log1p(w), w = e^-|x|, with log1p(w) = 2 atanh(s), s = w / (2 + w) <= 1/3,
-// by its series up to s^13 (the rest is below 2e-8 of it): relative error a few 1e-7 everywhere, which
-// a logarithm of 1 + w would not have for the small step sizes that matter most.
-__device__ __forceinline__ float softplus_series(float x) {
-  const float w = ex2(-fabsf(x) * kLog2e);
-  const float s = __fdividef(w, 2.f + w), q = s * s;
-  float r = fmaf(q, 1.f / 13, 1.f / 11);
-  r = fmaf(q, r, 1.f / 9);
-  r = fmaf(q, r, 1.f / 7);
-  r = fmaf(q, r, 1.f / 5);
-  r = fmaf(q, r, 1.f / 3);
-  r = fmaf(q * r, s, s);
-  return fmaxf(x, 0.f) + 2.f * r;
+// two floats in one register pair, for the instructions that work on both
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+  f2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void unpack2(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
 }
 
-__device__ __forceinline__ float step_size(float raw, bool softplus) { return softplus ? softplus_series(raw) : raw; }
+// 2^x of two numbers on the FMA and integer pipes, for a share of the decays: the exponential's own unit does 16 a
+// clock and SM, which would bound the scan. x = n + f with n the nearest whole number (by adding 1.5 2^23), 2^f by
+// a polynomial of degree 5 on [-1/2, 1/2] that is 1 at 0, fitted here for the smallest relative error (1.7e-7 at
+// most with its roundings, 7e-8 rms), n added to the exponent's bits. From -126 down the result is 2^-126, from 128 up infinite.
+__device__ __forceinline__ f2 ex2_poly2(f2 x) {
+  float x0, x1, t0, t1, p0, p1;
+  unpack2(x, x0, x1);
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x0));
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x1));
+  asm("min.NaN.f32 %0, %0, 0f43000000;" : "+f"(x0));
+  asm("min.NaN.f32 %0, %0, 0f43000000;" : "+f"(x1));
+  x = pack2(x0, x1);
+  const f2 magic = pack2(12582912.f, 12582912.f), less = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f);
+  const f2 t = add2(x, magic), f = fma2(add2(t, less), minus, x);
+  f2 p = fma2(pack2(1.3264728050203965e-3f, 1.3264728050203965e-3f), f, pack2(9.671513139367519e-3f, 9.671513139367519e-3f));
+  p = fma2(p, f, pack2(5.550733745779106e-2f, 5.550733745779106e-2f));
+  p = fma2(p, f, pack2(2.4022242077762193e-1f, 2.4022242077762193e-1f));
+  p = fma2(p, f, pack2(6.931469775948809e-1f, 6.931469775948809e-1f));
+  p = fma2(p, f, pack2(1.f, 1.f));
+  unpack2(t, t0, t1);
+  unpack2(p, p0, p1);
+  return pack2(__int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23)),
+               __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)));
+}
+
+// Two neighbouring elements of a row as they lie in memory, converted when they are used, so that loads can
+// stay in flight. W32: the row is fp32 whatever T is.
+template <typename T> struct Raw2 { uint32_t v; };
+template <> struct Raw2<float> { float2 v; };
+__device__ __forceinline__ float2 value2(Raw2<float> r) { return r.v; }
+__device__ __forceinline__ float2 value2(Raw2<__nv_bfloat16> r) {
+  return make_float2(__uint_as_float(r.v << 16), __uint_as_float(r.v & 0xffff0000u));
+}
+__device__ __forceinline__ float2 value2(Raw2<__half> r) { return __half22float2(*reinterpret_cast<__half2*>(&r.v)); }
+// vec: both at once (the address is on a boundary of the pair); else one by one, the second at `second`
+template <typename T>
+__device__ __forceinline__ Raw2<T> load2(const T* p, bool vec, int second) {
+  Raw2<T> r;
+  if constexpr (sizeof(T) == 4) {
+    if (vec) r.v = *reinterpret_cast<const float2*>(p);
+    else r.v = make_float2(p[0], p[second]);
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    if (vec) r.v = *reinterpret_cast<const uint32_t*>(p);
+    else r.v = (uint32_t)h[0] | (uint32_t)h[second] << 16;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store2(T* p, bool vec, bool both, float a, float b) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(a, b);
+    else {
+      T v[2] = {from_f32<T>(a), from_f32<T>(b)};
+      *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(v);
+    }
+  } else {
+    st(p, a);
+    if (both) st(p + 1, b);
+  }
+}
+// a row that is either T or fp32
+template <typename T>
+struct RawAny { uint32_t a, b; };
+template <typename T>
+__device__ __forceinline__ float2 value2(Raw2<T> r, bool) { return value2(r); }
+template <typename T>
+__device__ __forceinline__ float2 value2(RawAny<T> r, bool f32) {
+  if (f32) return make_float2(__uint_as_float(r.a), __uint_as_float(r.b));
+  if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(r.a), __uint_as_float(r.b));
+  else return value2(Raw2<T>{r.a});
+}
+template <typename T>
+__device__ __forceinline__ void load2_any(Raw2<T>& r, const void* p, bool, int64_t i, bool, int) {
+  r = load2<T>(static_cast<const T*>(p) + i, true, 1);
+}
+template <typename T>
+__device__ __forceinline__ void load2_any(RawAny<T>& r, const void* p, bool f32, int64_t i, bool vec, int second) {
+  if (sizeof(T) == 4 || f32) {
+    const float2 v = load2<float>(static_cast<const float*>(p) + i, vec, second).v;
+    r.a = __float_as_uint(v.x);
+    r.b = __float_as_uint(v.y);
+  } else {
+    if constexpr (sizeof(T) == 2) r.a = load2<T>(static_cast<const T*>(p) + i, vec, second).v;
+    r.b = 0;
+  }
+}
+
+// log(1 + e^x) = max(x, 0) + log1p(w), w = e^-|x| in [0, 1], log1p(w) / w by a polynomial of degree 8 that is 1 at 0, fitted
+// here for the smallest relative error (3.3e-8; 1.1e-7 with its roundings), which also holds for the small
+// step sizes that matter most, where a logarithm of 1 + w would lose their digits. Two numbers at once.
+__device__ __forceinline__ f2 softplus2(float x0, float x1) {
+  const f2 w = pack2(ex2(-fabsf(x0) * kLog2e), ex2(-fabsf(x1) * kLog2e));
+  auto c = [](float v) { return pack2(v, v); };
+  f2 r = fma2(w, c(0.005364825617334684f), c(-0.030065797599842133f));
+  r = fma2(w, r, c(0.07920454444779973f));
+  r = fma2(w, r, c(-0.1375380311293698f));
+  r = fma2(w, r, c(0.19153655310223328f));
+  r = fma2(w, r, c(-0.24857163763289894f));
+  r = fma2(w, r, c(0.33321322629882966f));
+  r = fma2(w, r, c(-0.49999647963987515f));
+  r = fma2(w, r, c(1.f));
+  return fma2(w, r, pack2(fmaxf(x0, 0.f), fmaxf(x1, 0.f)));
+}
+
+// 1 / (1 + e^-x) of two numbers, from the hardware's 2^x and reciprocal (relative error a few 1e-7).
+__device__ __forceinline__ float2 sigmoid2(float2 x) { return make_float2(fast_sigmoid(x.x), fast_sigmoid(x.y)); }
+
+// dt of two raw step sizes
+__device__ __forceinline__ float2 step_size2(float2 raw, bool softplus) {
+  if (softplus) unpack2(softplus2(raw.x, raw.y), raw.x, raw.y);
+  return raw;
+}
+__device__ __forceinline__ float step_size(float raw, bool softplus) { return step_size2(make_float2(raw, raw), softplus).x; }
 
 template <typename T>
 __device__ __forceinline__ float ld_any(const void* p, bool f32, int64_t i) {
@@ -138,6 +269,60 @@ __device__ __forceinline__ int spread_sum(float (&v)[V], int lane) {
   }
   return at;
 }
+
+constexpr int kSelPitch = kSelTile + 4;  // of a tile's rows: those that a warp reads together start on different banks
+
+// Four (or R < 4) steps of one row of a tile in shared memory.
+template <int R>
+__device__ __forceinline__ void put_steps(float* row, const float (&v)[R]) {
+  if constexpr (R % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < R; i += 4) *reinterpret_cast<float4*>(row + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  } else if constexpr (R == 2) {
+    *reinterpret_cast<float2*>(row) = make_float2(v[0], v[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) row[i] = v[i];
+  }
+}
+
+// B or C of a tile: a task is two neighbouring states at four steps. Rows behind the sequence's end
+// read its last one, and put() writes zeros in their place.
+template <typename T, int K, int P, int NT, bool FAST>
+struct BcTile {
+  static constexpr int NP = K * P, TASKS = NP / 2 * (kSelTile / 4), J = (TASKS + NT - 1) / NT;
+  std::conditional_t<FAST, Raw2<T>, RawAny<T>> r[J][4];
+  __device__ __forceinline__ void fetch(const void* p, bool f32, int64_t off, int64_t sl, bool vec, int N, int t0, int len, int tid) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int i = tid + j * NT, n0 = i % (NP / 2) * 2, n = n0 < N ? n0 : 0, t = t0 + i / (NP / 2) * 4;
+      if (TASKS % NT == 0 || i < TASKS) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          load2_any<T>(r[j][u], p, f32, off + (int64_t)min(t + u, len - 1) * sl + n, vec, n + 1 < N ? 1 : 0);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(float (*rows)[kSelPitch], bool f32, int N, int t0, int len, int tid) const {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int i = tid + j * NT, n = i % (NP / 2) * 2, t = i / (NP / 2) * 4;
+      if (TASKS % NT == 0 || i < TASKS) {
+        float a[4], b[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float2 v = value2<T>(r[j][u], f32);
+          const bool in = t0 + t + u < len;
+          a[u] = in && n < N ? v.x : 0.f;
+          b[u] = in && n + 1 < N ? v.y : 0.f;
+        }
+        put_steps<4>(&rows[n % K * P + n / K][t], a);
+        put_steps<4>(&rows[(n + 1) % K * P + (n + 1) / K][t], b);
+      }
+    }
+  }
+};
+
 #endif
 
 }  // namespace m3

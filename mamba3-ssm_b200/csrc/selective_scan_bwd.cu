@@ -15,24 +15,31 @@
 namespace m3 {
 namespace {
 
-constexpr int TT = kSelTile, TS = TT + 4, SUB = kSelSub;
+constexpr int TT = kSelTile, TS = kSelPitch, SUB = kSelSub;
 
 template <int K, int P, int M, int NT>
 struct BwdSmem {
   static constexpr int NP = K * P, EC = NT / P * M, W = NT / 32;
-  float dt[EC][TS], dx[EC][TS], dy[EC][TS];
+  // (channel, step): dt, dy, u; and what becomes a gradient in its place: dt u -> du, the softplus's slope ->
+  // ddelta, dout silu'(z) -> dz
+  float dt[EC][TS], dy[EC][TS], u[EC][TS], du[EC][TS], dd[EC][TS], dz[EC][TS];
   float B[NP][TS], C[NP][TS];
-  float s0[TT][EC + 1], s1[TT][EC + 1], s2[TT][EC + 1];  // sums over the states: C h, g B, A w
   float red[W][2 * SUB * NP];
-  double ends[2][NT];
 };
 
-template <typename T, int K, int P, int M, int NT>
+__device__ __forceinline__ void lds4(const float* p, f2& a, f2& b) {
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+  a = v.x;
+  b = v.y;
+}
+
+template <typename T, int K, int P, int M, int NT, bool FAST>
 __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, const SelScanGrads g) {
   using S = BwdSmem<K, P, M, NT>;
   constexpr int NP = S::NP, EC = S::EC, W = S::W, Q = 32 / P;
-  constexpr int JN = TT * EC / NT, JB = (TT * NP + NT - 1) / NT;
-  static_assert(NT % EC == 0, "a thread brings and stores one channel");
+  constexpr int R = TT * EC / 2 / NT > 0 ? TT * EC / 2 / NT : 1;  // steps of a pair of channels that a thread brings and stores
+  constexpr int RR = R < 4 ? R : 4;                               // of them at a time
+  constexpr int SP = SUB / P > 0 ? SUB / P : 1;                   // steps of a channel whose sums a lane ends up with
   extern __shared__ __align__(16) unsigned char smem_raw[];
   S& sh = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, q = tid % P, lane = tid & 31, warp = tid >> 5;
@@ -43,184 +50,257 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
   const int beg = c * p.chunk, end = min(p.L, beg + p.chunk);
   const int len = seq_len(p.lengths, b, p.L);
   const int nsave = (p.L + SUB - 1) / SUB;
-  const int le = tid % EC, lt = tid / EC;
-  const int lec = min(e_first + le, e_end - 1);
-  const bool lelive = e_first + le < e_end;
+  const int le = tid % (EC / 2) * 2, lt = tid / (EC / 2) * R;
+  const bool brings = TT * EC / 2 >= NT * R || lt < TT;
+  const int l0 = e_first + le < e_end ? e_first + le : e_first, second = l0 + 1 < e_end ? 1 : 0;
+  const bool lelive = brings && e_first + le < e_end, lelive1 = brings && e_first + le + 1 < e_end;
+  const bool vu = FAST || p.vec_u, vd = FAST || p.vec_d, vz = FAST || p.vec_z, vy = FAST || p.vec_y;
 
-  int el[M], ec[M];
-  float A[M][K], gv[M][K];
-  double dA[M][K];
+  float A[M][K], gv[M][K], hn[M][K];
+  double dA[M][K], sumD[M], sumbias[M];
+  const float* save[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
-    el[m] = m * (NT / P) + tid / P;
-    ec[m] = min(e_first + el[m], e_end - 1);
+    const int e = e_first + m * (NT / P) + tid / P, ec = min(e, e_end - 1);
+    save[m] = p.save + ((int64_t)b * nsave * p.E + ec) * NP + q * K;
+    sumD[m] = sumbias[m] = 0.0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int n = q * K + k;
-      A[m][k] = n < p.N ? p.A[(int64_t)ec[m] * p.N + n] : 0.f;
+      A[m][k] = n < p.N ? p.A[(int64_t)ec * p.N + n] : 0.f;
       dA[m][k] = 0.0;
       gv[m][k] = 0.f;
-      if (p.nchunk > 1) gv[m][k] = p.states[(((int64_t)b * p.nchunk + c) * p.E + ec[m]) * NP + n];
-      else if (g.dstate != nullptr && n < p.N) gv[m][k] = g.dstate[((int64_t)b * p.E + ec[m]) * p.N + n];
-      if (e_first + el[m] >= e_end) gv[m][k] = 0.f;
+      if (e < e_end) {
+        if (p.nchunk > 1) gv[m][k] = p.states[(((int64_t)b * p.nchunk + c) * p.E + ec) * NP + n];
+        else if (g.dstate != nullptr && n < p.N) gv[m][k] = g.dstate[((int64_t)b * p.E + ec) * p.N + n];
+      }
     }
   }
-  const float bias = p.bias != nullptr ? p.bias[lec] : 0.f;
-  const float Dv = p.D != nullptr ? p.D[lec] : 0.f;
-  double sumD = 0.0, sumbias = 0.0;
+  const float bias0 = p.bias != nullptr ? p.bias[l0] : 0.f, bias1 = p.bias != nullptr ? p.bias[l0 + second] : 0.f;
+  float Dv[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) Dv[m] = p.D != nullptr ? p.D[min(e_first + m * (NT / P) + tid / P, e_end - 1)] : 0.f;
 
-  const T* up = static_cast<const T*>(p.u.p) + (int64_t)b * p.u.sb + lec;
-  const T* zp = p.z.p != nullptr ? static_cast<const T*>(p.z.p) + (int64_t)b * p.z.sb + lec : nullptr;
-  const T* yp = static_cast<const T*>(g.dy.p) + (int64_t)b * g.dy.sb + lec;
-  T* dup = static_cast<T*>(const_cast<void*>(g.du.p)) + (int64_t)b * g.du.sb + lec;
-  T* dzp = zp != nullptr ? static_cast<T*>(const_cast<void*>(g.dz.p)) + (int64_t)b * g.dz.sb + lec : nullptr;
-  const int64_t doff = (int64_t)b * p.delta.sb + lec, ddoff = (int64_t)b * g.ddelta.sb + lec;
+  const bool has_z = p.z.p != nullptr;
+  const T* up = static_cast<const T*>(p.u.p) + (int64_t)b * p.u.sb + l0;
+  const T* zp = has_z ? static_cast<const T*>(p.z.p) + (int64_t)b * p.z.sb + l0 : nullptr;
+  const T* yp = static_cast<const T*>(g.dy.p) + (int64_t)b * g.dy.sb + l0;
+  T* dup = static_cast<T*>(const_cast<void*>(g.du.p)) + (int64_t)b * g.du.sb + l0;
+  T* dzp = has_z ? static_cast<T*>(const_cast<void*>(g.dz.p)) + (int64_t)b * g.dz.sb + l0 : nullptr;
+  const int64_t doff = (int64_t)b * p.delta.sb + l0, ddoff = (int64_t)b * g.ddelta.sb + l0;
   const int64_t boff = (int64_t)b * p.B.sb + gr * p.Bg, coff = (int64_t)b * p.C.sb + gr * p.Cg;
-  auto put_ddelta = [&](int t, float v) {
+  auto put_ddelta = [&](int t, float v0, float v1) {
     const int64_t i = ddoff + (int64_t)t * g.ddelta.sl;
     void* d = const_cast<void*>(g.ddelta.p);
-    if (p.delta_f32) static_cast<float*>(d)[i] = v;
-    else st(static_cast<T*>(d) + i, v);
+    if (!FAST && p.delta_f32) store2<float>(static_cast<float*>(d) + i, g.vec_dd, second, v0, v1);
+    else store2<T>(static_cast<T*>(d) + i, FAST || g.vec_dd, second, v0, v1);
   };
 
   // padding behind the sequence: gradients of zero
-  const int first_pad = max(beg, len);
-  for (int t = first_pad + lt; t < end; t += NT / EC)
-    if (lelive) {
-      st(dup + (int64_t)t * g.du.sl, 0.f);
-      put_ddelta(t, 0.f);
-      if (zp != nullptr) st(dzp + (int64_t)t * g.dz.sl, 0.f);
+  if (lelive)
+    for (int t = max(beg, len) + (R == 1 ? lt : lt / R); t < end; t += NT / (EC / 2)) {
+      store2<T>(dup + (int64_t)t * g.du.sl, FAST || g.vec_du, second, 0.f, 0.f);
+      put_ddelta(t, 0.f, 0.f);
+      if (has_z) store2<T>(dzp + (int64_t)t * g.dz.sl, FAST || g.vec_dz, second, 0.f, 0.f);
     }
 
   const int last = min(end, len);
   for (int t0 = last > beg ? beg + (last - 1 - beg) / TT * TT : beg - TT; t0 >= beg; t0 -= TT) {
+    const int top = min(TT, last - t0);  // steps of the tile that count
+    {
+      const int s = (t0 + top - 1) / SUB;
 #pragma unroll
-    for (int j = 0; j < JN; ++j) {
-      const int t = lt + j * (NT / EC);
-      float dt = 0.f, u = 0.f, dy = 0.f;
-      if (t0 + t < len && lelive) {
-        u = ld(up + (int64_t)(t0 + t) * p.u.sl);
-        dt = step_size(ld_any<T>(p.delta.p, p.delta_f32, doff + (int64_t)(t0 + t) * p.delta.sl) + bias, p.softplus);
-        dy = ld(yp + (int64_t)(t0 + t) * g.dy.sl);
-        if (zp != nullptr) {
-          const float z = ld(zp + (int64_t)(t0 + t) * p.z.sl);
-          dy *= z * fast_sigmoid(z);
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int k = 0; k < K; ++k) hn[m][k] = save[m][(int64_t)s * p.E * NP + k];
+    }
+    if (brings) {
+#pragma unroll 1
+      for (int j0 = 0; j0 < R; j0 += RR) {
+        Raw2<T> ru[RR], rz[RR], ry[RR];
+        std::conditional_t<FAST, Raw2<T>, RawAny<T>> rd[RR];
+#pragma unroll
+        for (int j = 0; j < RR; ++j) {  // rows behind the end read the last one; nothing is made of them
+          const int64_t t = min(t0 + lt + j0 + j, len - 1);
+          ru[j] = load2<T>(up + t * p.u.sl, vu, second);
+          load2_any<T>(rd[j], p.delta.p, p.delta_f32, doff + t * p.delta.sl, vd, second);
+          ry[j] = load2<T>(yp + t * g.dy.sl, vy, second);
+          if (has_z) rz[j] = load2<T>(zp + t * p.z.sl, vz, second);
+        }
+        float v[6][2][RR];
+#pragma unroll
+        for (int j = 0; j < RR; ++j) {
+          const float2 r = value2<T>(rd[j], p.delta_f32), raw = make_float2(r.x + bias0, r.y + bias1);
+          float2 dt = step_size2(raw, p.softplus), sl = p.softplus ? sigmoid2(raw) : make_float2(1.f, 1.f);
+          float2 u = value2(ru[j]), dy = value2(ry[j]), zf = make_float2(0.f, 0.f);
+          if (has_z) {
+            const float2 z = value2(rz[j]), sg = sigmoid2(z);
+            zf.x = dy.x * (sg.x * fmaf(z.x, 1.f - sg.x, 1.f));
+            zf.y = dy.y * (sg.y * fmaf(z.y, 1.f - sg.y, 1.f));
+            dy.x *= z.x * sg.x;
+            dy.y *= z.y * sg.y;
+          }
+          const bool in0 = t0 + lt + j0 + j < len && lelive, in1 = in0 && lelive1;
+          v[0][0][j] = in0 ? dt.x : 0.f; v[0][1][j] = in1 ? dt.y : 0.f;
+          v[1][0][j] = in0 ? dy.x : 0.f; v[1][1][j] = in1 ? dy.y : 0.f;
+          v[2][0][j] = in0 ? u.x : 0.f; v[2][1][j] = in1 ? u.y : 0.f;
+          v[3][0][j] = v[0][0][j] * v[2][0][j]; v[3][1][j] = v[0][1][j] * v[2][1][j];
+          v[4][0][j] = in0 ? sl.x : 0.f; v[4][1][j] = in1 ? sl.y : 0.f;
+          v[5][0][j] = zf.x; v[5][1][j] = zf.y;
+        }
+        const int t = lt + j0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          put_steps<RR>(&sh.dt[le + i][t], v[0][i]);
+          put_steps<RR>(&sh.dy[le + i][t], v[1][i]);
+          put_steps<RR>(&sh.u[le + i][t], v[2][i]);
+          put_steps<RR>(&sh.du[le + i][t], v[3][i]);
+          put_steps<RR>(&sh.dd[le + i][t], v[4][i]);
+          if (has_z) put_steps<RR>(&sh.dz[le + i][t], v[5][i]);
         }
       }
-      sh.dt[le][t] = dt;
-      sh.dx[le][t] = dt * u;
-      sh.dy[le][t] = dy;
     }
-#pragma unroll 4
-    for (int j = 0; j < JB; ++j) {
-      const int i = tid + j * NT, n = i % NP, t = i / NP;
-      if (t < TT) {
-        const bool in = n < p.N && t0 + t < len;
-        const int row = (n % K) * P + n / K;
-        sh.B[row][t] = in ? ld_any<T>(p.B.p, p.bc_f32, boff + (int64_t)(t0 + t) * p.B.sl + n) : 0.f;
-        sh.C[row][t] = in ? ld_any<T>(p.C.p, p.bc_f32, coff + (int64_t)(t0 + t) * p.C.sl + n) : 0.f;
-      }
+    {
+      BcTile<T, K, P, NT, FAST> tb;
+      tb.fetch(p.B.p, p.bc_f32, boff, p.B.sl, p.vec_B, p.N, t0, len, tid);
+      tb.put(sh.B, p.bc_f32, p.N, t0, len, tid);
+      tb.fetch(p.C.p, p.bc_f32, coff, p.C.sl, p.vec_C, p.N, t0, len, tid);
+      tb.put(sh.C, p.bc_f32, p.N, t0, len, tid);
     }
     __syncthreads();
 #pragma unroll 1
-    for (int ts = TT - SUB; ts >= 0; ts -= SUB) {
-      if (t0 + ts >= len) continue;  // the same for the whole CTA
-      float acc[2 * SUB * K];  // dB, then dC: (step, k)
+    for (int ts = (top - 1) / SUB * SUB; ts >= 0; ts -= SUB) {
+      f2 acc[2][K][SUB / 2];  // dB, dC
 #pragma unroll
-      for (int i = 0; i < 2 * SUB * K; ++i) acc[i] = 0.f;
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < SUB / 2; ++j) acc[i][k][j] = 0;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        float dt[SUB], dx[SUB], dy[SUB], S0[SUB], S1[SUB], S2[SUB];
+        const int el = m * (NT / P) + tid / P;
+        f2 dt[SUB / 2], dx[SUB / 2], dy[SUB / 2], S0[SUB / 2], S1[SUB / 2], S2[SUB / 2];
 #pragma unroll
-        for (int i = 0; i < SUB; i += 4) {
-          const float4 a = *reinterpret_cast<const float4*>(&sh.dt[el[m]][ts + i]);
-          const float4 x = *reinterpret_cast<const float4*>(&sh.dx[el[m]][ts + i]);
-          const float4 y = *reinterpret_cast<const float4*>(&sh.dy[el[m]][ts + i]);
-          dt[i] = a.x; dt[i + 1] = a.y; dt[i + 2] = a.z; dt[i + 3] = a.w;
-          dx[i] = x.x; dx[i + 1] = x.y; dx[i + 2] = x.z; dx[i + 3] = x.w;
-          dy[i] = y.x; dy[i + 1] = y.y; dy[i + 2] = y.z; dy[i + 3] = y.w;
+        for (int j = 0; j < SUB / 2; j += 2) {
+          lds4(&sh.dt[el][ts + 2 * j], dt[j], dt[j + 1]);
+          lds4(&sh.du[el][ts + 2 * j], dx[j], dx[j + 1]);
+          lds4(&sh.dy[el][ts + 2 * j], dy[j], dy[j + 1]);
         }
 #pragma unroll
-        for (int i = 0; i < SUB; ++i) S0[i] = S1[i] = S2[i] = 0.f;
-        const float* sv = p.save + (((int64_t)b * nsave + (t0 + ts) / SUB) * p.E + ec[m]) * NP + q * K;
+        for (int j = 0; j < SUB / 2; ++j) S0[j] = S1[j] = S2[j] = 0;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          const float h_in = sv[k], A2 = A[m][k] * kLog2e;
-          float bv[SUB], cv[SUB], av[SUB], hv[SUB];
+          const float A2 = A[m][k] * kLog2e, h_in = hn[m][k];
+          const f2 A2k = pack2(A2, A2), Ak = pack2(A[m][k], A[m][k]), mean = pack2(kEx2Mean, kEx2Mean);
+          f2 bv[SUB / 2], cv[SUB / 2];
+          float av[SUB], hv[SUB];
 #pragma unroll
-          for (int i = 0; i < SUB; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(&sh.B[k * P + q][ts + i]);
-            const float4 y = *reinterpret_cast<const float4*>(&sh.C[k * P + q][ts + i]);
-            bv[i] = x.x; bv[i + 1] = x.y; bv[i + 2] = x.z; bv[i + 3] = x.w;
-            cv[i] = y.x; cv[i + 1] = y.y; cv[i + 2] = y.z; cv[i + 3] = y.w;
+          for (int j = 0; j < SUB / 2; j += 2) {
+            lds4(&sh.B[k * P + q][ts + 2 * j], bv[j], bv[j + 1]);
+            lds4(&sh.C[k * P + q][ts + 2 * j], cv[j], cv[j + 1]);
           }
           float h = h_in;
 #pragma unroll
-          for (int i = 0; i < SUB; ++i) {
-            av[i] = ex2(dt[i] * A2);
-            h = fmaf(av[i], h, dx[i] * bv[i]);
-            hv[i] = h;
-            S0[i] = fmaf(cv[i], h, S0[i]);
+          for (int j = 0; j < SUB / 2; ++j) {
+            float x0, x1;
+            unpack2(fma2(dt[j], A2k, mean), av[2 * j], av[2 * j + 1]);
+            av[2 * j] = ex2(av[2 * j]);
+            av[2 * j + 1] = ex2(av[2 * j + 1]);
+            unpack2(mul2(dx[j], bv[j]), x0, x1);
+            hv[2 * j] = fmaf(av[2 * j], h, x0);
+            h = hv[2 * j + 1] = fmaf(av[2 * j + 1], hv[2 * j], x1);
+            const f2 hh = pack2(hv[2 * j], hv[2 * j + 1]);
+            S0[j] = fma2(cv[j], hh, S0[j]);
+            acc[1][k][j] = fma2(dy[j], hh, acc[1][k][j]);
           }
-          float gk = gv[m][k], da = 0.f;
+          float gk = gv[m][k];
+          f2 da = 0;
 #pragma unroll
-          for (int i = SUB - 1; i >= 0; --i) {
-            gk = fmaf(cv[i], dy[i], gk);
-            acc[i * K + k] = fmaf(gk, dx[i], acc[i * K + k]);
-            acc[(SUB + i) * K + k] = fmaf(dy[i], hv[i], acc[(SUB + i) * K + k]);
-            S1[i] = fmaf(gk, bv[i], S1[i]);
-            gk *= av[i];
-            const float w = gk * (i > 0 ? hv[i - 1] : h_in);
-            S2[i] = fmaf(A[m][k], w, S2[i]);
-            da = fmaf(dt[i], w, da);
+          for (int j = SUB / 2 - 1; j >= 0; --j) {
+            float c0, c1, y0, y1;
+            unpack2(cv[j], c0, c1);
+            unpack2(dy[j], y0, y1);
+            const float g1 = fmaf(c1, y1, gk), a1 = g1 * av[2 * j + 1];
+            const float g0 = fmaf(c0, y0, a1);
+            gk = g0 * av[2 * j];
+            const f2 gg = pack2(g0, g1);
+            const f2 w = pack2(gk * (j > 0 ? hv[2 * j - 1] : h_in), a1 * hv[2 * j]);
+            acc[0][k][j] = fma2(gg, dx[j], acc[0][k][j]);
+            S1[j] = fma2(gg, bv[j], S1[j]);
+            S2[j] = fma2(Ak, w, S2[j]);
+            da = fma2(dt[j], w, da);
           }
           gv[m][k] = gk;
-          dA[m][k] += (double)da;
+          float d0, d1;
+          unpack2(da, d0, d1);
+          dA[m][k] += (double)(d0 + d1);
         }
-        int at = spread_sum<SUB, P>(S0, q);
-        spread_sum<SUB, P>(S1, q);
-        spread_sum<SUB, P>(S2, q);
+        if (ts > 0) {  // the states for the eight steps in front of these
 #pragma unroll
-        for (int j = 0; j < (SUB > P ? SUB / P : 1); ++j) {
-          sh.s0[ts + at + j][el[m]] = S0[j];
-          sh.s1[ts + at + j][el[m]] = S1[j];
-          sh.s2[ts + at + j][el[m]] = S2[j];
+          for (int k = 0; k < K; ++k) hn[m][k] = save[m][(int64_t)((t0 + ts) / SUB - 1) * p.E * NP + k];
+        }
+        float s0[SUB], s1[SUB], s2[SUB];
+#pragma unroll
+        for (int j = 0; j < SUB / 2; ++j) {
+          unpack2(S0[j], s0[2 * j], s0[2 * j + 1]);
+          unpack2(S1[j], s1[2 * j], s1[2 * j + 1]);
+          unpack2(S2[j], s2[2 * j], s2[2 * j + 1]);
+        }
+        if (has_z) spread_sum<SUB, P>(s0, q);
+        spread_sum<SUB, P>(s1, q);
+        const int at = spread_sum<SUB, P>(s2, q);
+        __syncwarp();  // the channel's lanes have read dt u
+        if (P <= SUB || q % (P > SUB ? P / SUB : 1) == 0) {
+#pragma unroll
+          for (int j = 0; j < SP; ++j) {
+            const int t = ts + at + j;
+            const float u = sh.u[el][t], d = sh.dt[el][t], y = sh.dy[el][t];
+            sh.du[el][t] = fmaf(d, s1[j], Dv[m] * y);
+            const float dd = fmaf(u, s1[j], s2[j]) * sh.dd[el][t];
+            sh.dd[el][t] = dd;
+            if (has_z) sh.dz[el][t] *= fmaf(Dv[m], u, s0[j]);
+            sumD[m] += (double)(y * u);
+            sumbias[m] += (double)dd;
+          }
         }
       }
       // over the warp's channels: lanes q, q + P, ... ; then over the warps
-      const int at = spread_sum<2 * SUB * K, Q, P>(acc, lane / P);
+      float v[2 * SUB * K];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < SUB / 2; ++j) unpack2(acc[i][k][j], v[(i * K + k) * SUB + 2 * j], v[(i * K + k) * SUB + 2 * j + 1]);
+      const int at = spread_sum<2 * SUB * K, Q, P>(v, lane / P);
 #pragma unroll
       for (int j = 0; j < 2 * SUB * K / Q; ++j) {
-        const int i = at + j, w = i / (SUB * K), t = i / K % SUB, k = i % K;
-        sh.red[warp][(t * 2 + w) * NP + q * K + k] = acc[j];
+        const int i = at + j, w = i / (SUB * K), k = i / SUB % K, t = i % SUB;
+        sh.red[warp][(t * 2 + w) * NP + q * K + k] = v[j];
       }
       __syncthreads();
       for (int i = tid; i < 2 * SUB * NP; i += NT) {
-        float v = 0.f;
+        float r = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) v += sh.red[w][i];
+        for (int w = 0; w < W; ++w) r += sh.red[w][i];
         const int t = t0 + ts + i / (2 * NP);
-        if (t < len) g.part_bc[((((int64_t)b * p.L + t) * p.G + gr) * tiles + tile) * 2 * NP + i % (2 * NP)] = v;
+        if (t < len) g.part_bc[((((int64_t)b * p.L + t) * p.G + gr) * tiles + tile) * 2 * NP + i % (2 * NP)] = r;
       }
       __syncthreads();
     }
+    if (lelive) {
+#pragma unroll 1
+      for (int j0 = 0; j0 < R; j0 += RR) {
 #pragma unroll
-    for (int j = 0; j < JN; ++j) {
-      const int t = lt + j * (NT / EC);
-      if (t0 + t < len && lelive) {
-        const float u = ld(up + (int64_t)(t0 + t) * p.u.sl);
-        const float dt = sh.dt[le][t], dy = sh.dy[le][t], s1 = sh.s1[t][le];
-        st(dup + (int64_t)(t0 + t) * g.du.sl, fmaf(dt, s1, Dv * dy));
-        float dd = fmaf(u, s1, sh.s2[t][le]);
-        if (p.softplus)
-          dd *= fast_sigmoid(ld_any<T>(p.delta.p, p.delta_f32, doff + (int64_t)(t0 + t) * p.delta.sl) + bias);
-        put_ddelta(t0 + t, dd);
-        sumbias += (double)dd;
-        sumD += (double)(dy * u);
-        if (zp != nullptr) {
-          const float z = ld(zp + (int64_t)(t0 + t) * p.z.sl), dout = ld(yp + (int64_t)(t0 + t) * g.dy.sl);
-          const float sg = fast_sigmoid(z);
-          st(dzp + (int64_t)(t0 + t) * g.dz.sl, dout * fmaf(Dv, u, sh.s0[t][le]) * (sg * fmaf(z, 1.f - sg, 1.f)));
+        for (int j = 0; j < RR; ++j) {
+          const int t = t0 + lt + j0 + j;
+          if (t < last) {
+            const int l = lt + j0 + j;
+            store2<T>(dup + (int64_t)t * g.du.sl, FAST || g.vec_du, second, sh.du[le][l], sh.du[le + 1][l]);
+            put_ddelta(t, sh.dd[le][l], sh.dd[le + 1][l]);
+            if (has_z) store2<T>(dzp + (int64_t)t * g.dz.sl, FAST || g.vec_dz, second, sh.dz[le][l], sh.dz[le + 1][l]);
+          }
         }
       }
     }
@@ -230,23 +310,23 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
   float* pa = g.part_a + ((int64_t)b * p.nchunk + c) * p.E * (NP + 2);
 #pragma unroll
   for (int m = 0; m < M; ++m) {
-    if (e_first + el[m] < e_end) {
+    const int e = e_first + m * (NT / P) + tid / P;
+#pragma unroll
+    for (int o = P / 2; o >= 1; o /= 2) {
+      sumD[m] += __shfl_xor_sync(0xffffffffu, sumD[m], o);
+      sumbias[m] += __shfl_xor_sync(0xffffffffu, sumbias[m], o);
+    }
+    if (e < e_end) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        pa[(int64_t)ec[m] * (NP + 2) + q * K + k] = (float)dA[m][k];
-        if (g.dh0 != nullptr && c == 0 && q * K + k < p.N) g.dh0[((int64_t)b * p.E + ec[m]) * p.N + q * K + k] = gv[m][k];
+        pa[(int64_t)e * (NP + 2) + q * K + k] = (float)dA[m][k];
+        if (g.dh0 != nullptr && c == 0 && q * K + k < p.N) g.dh0[((int64_t)b * p.E + e) * p.N + q * K + k] = gv[m][k];
+      }
+      if (q == 0) {
+        pa[(int64_t)e * (NP + 2) + NP] = (float)sumD[m];
+        pa[(int64_t)e * (NP + 2) + NP + 1] = (float)sumbias[m];
       }
     }
-  }
-  sh.ends[0][tid] = sumD;
-  sh.ends[1][tid] = sumbias;
-  __syncthreads();
-  if (tid < EC && lelive) {
-    double sd = 0.0, sb = 0.0;
-#pragma unroll
-    for (int j = 0; j < NT / EC; ++j) { sd += sh.ends[0][tid + j * EC]; sb += sh.ends[1][tid + j * EC]; }
-    pa[(int64_t)lec * (NP + 2) + NP] = (float)sd;
-    pa[(int64_t)lec * (NP + 2) + NP + 1] = (float)sb;
   }
 }
 
@@ -381,21 +461,27 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
+#ifndef M3_BM
+#define M3_BM 2
+#endif
+#ifndef M3_BNT
+#define M3_BNT 128
+#endif
 // states a lane, lanes, channels a lane by the padded number of states
 template <int K, int P, int M> struct KPM { static constexpr int k = K, p = P, m = M; };
 template <typename F>
 int by_states(int n, F&& f) {
   switch (sel_padded_states(n)) {
-    case 4: return f(KPM<2, 2, 2>{});
-    case 8: return f(KPM<2, 4, 2>{});
-    case 16: return f(KPM<2, 8, 2>{});
-    case 32: return f(KPM<2, 16, 2>{});
-    case 64: return f(KPM<2, 32, 2>{});
-    default: return f(KPM<4, 32, 1>{});
+    case 4: return f(KPM<2, 2, 1>{});
+    case 8: return f(KPM<4, 2, 1>{});
+    case 16: return f(KPM<4, 4, M3_BM>{});
+    case 32: return f(KPM<4, 8, 2>{});
+    case 64: return f(KPM<4, 16, 2>{});
+    default: return f(KPM<4, 32, 2>{});
   }
 }
 
-constexpr int kBwdThreads = 128;
+constexpr int kBwdThreads = M3_BNT;
 
 struct BwdPlan {
   int np, tiles, nchunk, chunk;
@@ -436,6 +522,12 @@ int launch_sel_scan_bwd(SelScanParams p, SelScanGrads g, int dtype, void* ws, cu
   p.dtsum = p.states + w.states;
   p.nchunk = w.nchunk;
   p.chunk = w.chunk;
+  p.y = g.dy;  // the flags of y are those of its gradient here
+  sel_pair_flags(&p, dtype);
+  SelScanParams o = p;
+  o.u = g.du; o.delta = g.ddelta; o.z = g.dz;
+  sel_pair_flags(&o, dtype);
+  g.vec_du = o.vec_u; g.vec_dd = o.vec_d; g.vec_dz = o.vec_z;
   const int Eg = p.E / p.G;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -453,11 +545,17 @@ int launch_sel_scan_bwd(SelScanParams p, SelScanGrads g, int dtype, void* ws, cu
         M3_TRY(check_launch("sel_bwd_carry_kernel"));
       }
       using S = BwdSmem<K, P, M, NT>;
-      static std::atomic<bool> done[kMaxDevices];
-      M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(&sel_bwd_kernel<T, K, P, M, NT>), sizeof(S), done));
       const dim3 grid((unsigned)(p.G * w.tiles), (unsigned)p.nchunk, (unsigned)p.batch);
-      sel_bwd_kernel<T, K, P, M, NT><<<grid, NT, sizeof(S), s>>>(p, g);
-      return check_launch("sel_bwd_kernel");
+      auto go = [&](auto fast) {
+        constexpr bool FAST = decltype(fast)::value;
+        static std::atomic<bool> done[kMaxDevices];
+        M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(&sel_bwd_kernel<T, K, P, M, NT, FAST>), sizeof(S), done));
+        sel_bwd_kernel<T, K, P, M, NT, FAST><<<grid, NT, sizeof(S), s>>>(p, g);
+        return check_launch("sel_bwd_kernel");
+      };
+      const bool fast = p.vec_u && p.vec_d && (p.vec_z || p.z.p == nullptr) && p.vec_y && p.vec_B && p.vec_C && g.vec_du &&
+                        g.vec_dd && (g.vec_dz || p.z.p == nullptr) && (sizeof(T) == 4 || (!p.delta_f32 && !p.bc_f32));
+      return fast ? go(std::true_type{}) : go(std::false_type{});
     }));
     const int64_t rows = (int64_t)p.batch * p.L * p.G;
     const unsigned bc_ctas = (unsigned)((rows * 2 * w.np + 255) / 256);
