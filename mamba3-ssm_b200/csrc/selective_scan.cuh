@@ -286,6 +286,23 @@ __device__ __forceinline__ void put_steps(float* row, const float (&v)[R]) {
   }
 }
 
+template <int R>
+__device__ __forceinline__ void get_steps(const float* row, float (&v)[R]) {
+  if constexpr (R % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < R; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(row + i);
+      v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+    }
+  } else if constexpr (R == 2) {
+    const float2 x = *reinterpret_cast<const float2*>(row);
+    v[0] = x.x; v[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] = row[i];
+  }
+}
+
 // B or C of a tile: a task is two neighbouring states at four steps. Rows behind the sequence's end
 // read its last one, and put() writes zeros in their place.
 template <typename T, int K, int P, int NT, bool FAST>

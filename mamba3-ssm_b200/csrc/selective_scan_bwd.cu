@@ -25,7 +25,21 @@ struct BwdSmem {
   float dt[EC][TS], dy[EC][TS], u[EC][TS], du[EC][TS], dd[EC][TS], dz[EC][TS];
   float B[NP][TS], C[NP][TS];
   float red[W][2 * SUB * NP];
+  float h[2][M][NT][K];  // the states in front of these eight steps and of the next eight (earlier) ones, by thread
+  // sums over the tiles so far, by thread: those of one tile are formed in 32 bits
+  double dA[M * K][NT], dD[M][NT], dbias[M][NT];
 };
+
+// Copies 16 bytes (or K floats) into shared memory without passing registers.
+template <int K>
+__device__ __forceinline__ void copy_ahead(float* to, const float* from) {
+  const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
+  if constexpr (K == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from));
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(from), "n"(K * 4));
+}
+__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 __device__ __forceinline__ void lds4(const float* p, f2& a, f2& b) {
   const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
@@ -34,7 +48,10 @@ __device__ __forceinline__ void lds4(const float* p, f2& a, f2& b) {
 }
 
 template <typename T, int K, int P, int M, int NT, bool FAST>
-__global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, const SelScanGrads g) {
+#ifndef M3_BMIN
+#define M3_BMIN 1
+#endif
+__global__ void __launch_bounds__(NT, M3_BMIN) sel_bwd_kernel(const SelScanParams p, const SelScanGrads g) {
   using S = BwdSmem<K, P, M, NT>;
   constexpr int NP = S::NP, EC = S::EC, W = S::W, Q = 32 / P;
   constexpr int R = TT * EC / 2 / NT > 0 ? TT * EC / 2 / NT : 1;  // steps of a pair of channels that a thread brings and stores
@@ -43,6 +60,10 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
   extern __shared__ __align__(16) unsigned char smem_raw[];
   S& sh = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, q = tid % P, lane = tid & 31, warp = tid >> 5;
+  // register k of a lane holds state q K + (k ^ flip): neighbouring channels of a warp hold them in orders in which
+  // what one gives to the other when dB and dC are summed stands in the same registers, without selecting
+  constexpr int FLIP = K < Q ? K : Q;  // orders
+  const int flip = lane / P % FLIP;
   const int Eg = p.E / p.G, tiles = (Eg + EC - 1) / EC;
   const int gr = blockIdx.x / tiles, tile = blockIdx.x % tiles;
   const int e_first = gr * Eg + tile * EC, e_end = (gr + 1) * Eg;
@@ -56,19 +77,24 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
   const bool lelive = brings && e_first + le < e_end, lelive1 = brings && e_first + le + 1 < e_end;
   const bool vu = FAST || p.vec_u, vd = FAST || p.vec_d, vz = FAST || p.vec_z, vy = FAST || p.vec_y;
 
-  float A[M][K], gv[M][K], hn[M][K];
-  double dA[M][K], sumD[M], sumbias[M];
+  int nk[K], row[K];  // states, and their rows among B and C
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    nk[k] = q * K + (k ^ flip);
+    row[k] = (k ^ flip) * P + q;
+  }
+  float A2[M][K], gv[M][K];
   const float* save[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     const int e = e_first + m * (NT / P) + tid / P, ec = min(e, e_end - 1);
     save[m] = p.save + ((int64_t)b * nsave * p.E + ec) * NP + q * K;
-    sumD[m] = sumbias[m] = 0.0;
+    sh.dD[m][tid] = sh.dbias[m][tid] = 0.0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int n = q * K + k;
-      A[m][k] = n < p.N ? p.A[(int64_t)ec * p.N + n] : 0.f;
-      dA[m][k] = 0.0;
+      const int n = nk[k];
+      A2[m][k] = n < p.N ? p.A[(int64_t)ec * p.N + n] * kLog2e : 0.f;
+      sh.dA[m * K + k][tid] = 0.0;
       gv[m][k] = 0.f;
       if (e < e_end) {
         if (p.nchunk > 1) gv[m][k] = p.states[(((int64_t)b * p.nchunk + c) * p.E + ec) * NP + n];
@@ -105,14 +131,24 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
     }
 
   const int last = min(end, len);
+  // the states in front of the eight steps that begin at 8 s, or nothing in front of this piece; a thread reads what it copied itself
+  auto copy_states = [&](int s, int half) {
+    if (s * SUB >= beg) {
+#pragma unroll
+      for (int m = 0; m < M; ++m) copy_ahead<K>(sh.h[half][m][tid], save[m] + (int64_t)s * p.E * NP);
+    }
+    copies_sent();
+  };
+  int half = 0;
+  if (last > beg) copy_states((last - 1) / SUB, 0);
   for (int t0 = last > beg ? beg + (last - 1 - beg) / TT * TT : beg - TT; t0 >= beg; t0 -= TT) {
     const int top = min(TT, last - t0);  // steps of the tile that count
-    {
-      const int s = (t0 + top - 1) / SUB;
+    float dA[M][K], sumD[M], sumbias[M];
 #pragma unroll
-      for (int m = 0; m < M; ++m)
+    for (int m = 0; m < M; ++m) {
+      sumD[m] = sumbias[m] = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) hn[m][k] = save[m][(int64_t)s * p.E * NP + k];
+      for (int k = 0; k < K; ++k) dA[m][k] = 0.f;
     }
     if (brings) {
 #pragma unroll 1
@@ -170,6 +206,8 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
     __syncthreads();
 #pragma unroll 1
     for (int ts = (top - 1) / SUB * SUB; ts >= 0; ts -= SUB) {
+      copy_states((t0 + ts) / SUB - 1, half ^ 1);
+      copies_done<1>();
       f2 acc[2][K][SUB / 2];  // dB, dC
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -191,14 +229,14 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
         for (int j = 0; j < SUB / 2; ++j) S0[j] = S1[j] = S2[j] = 0;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          const float A2 = A[m][k] * kLog2e, h_in = hn[m][k];
-          const f2 A2k = pack2(A2, A2), Ak = pack2(A[m][k], A[m][k]), mean = pack2(kEx2Mean, kEx2Mean);
+          const float h_in = sh.h[half][m][tid][k ^ flip];
+          const f2 A2k = pack2(A2[m][k], A2[m][k]), mean = pack2(kEx2Mean, kEx2Mean);
           f2 bv[SUB / 2], cv[SUB / 2];
           float av[SUB], hv[SUB];
 #pragma unroll
           for (int j = 0; j < SUB / 2; j += 2) {
-            lds4(&sh.B[k * P + q][ts + 2 * j], bv[j], bv[j + 1]);
-            lds4(&sh.C[k * P + q][ts + 2 * j], cv[j], cv[j + 1]);
+            lds4(&sh.B[row[k]][ts + 2 * j], bv[j], bv[j + 1]);
+            lds4(&sh.C[row[k]][ts + 2 * j], cv[j], cv[j + 1]);
           }
           float h = h_in;
 #pragma unroll
@@ -228,17 +266,13 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
             const f2 w = pack2(gk * (j > 0 ? hv[2 * j - 1] : h_in), a1 * hv[2 * j]);
             acc[0][k][j] = fma2(gg, dx[j], acc[0][k][j]);
             S1[j] = fma2(gg, bv[j], S1[j]);
-            S2[j] = fma2(Ak, w, S2[j]);
+            S2[j] = fma2(A2k, w, S2[j]);  // times log2(e)
             da = fma2(dt[j], w, da);
           }
           gv[m][k] = gk;
           float d0, d1;
           unpack2(da, d0, d1);
-          dA[m][k] += (double)(d0 + d1);
-        }
-        if (ts > 0) {  // the states for the eight steps in front of these
-#pragma unroll
-          for (int k = 0; k < K; ++k) hn[m][k] = save[m][(int64_t)((t0 + ts) / SUB - 1) * p.E * NP + k];
+          dA[m][k] += d0 + d1;
         }
         float s0[SUB], s1[SUB], s2[SUB];
 #pragma unroll
@@ -252,32 +286,55 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
         const int at = spread_sum<SUB, P>(s2, q);
         __syncwarp();  // the channel's lanes have read dt u
         if (P <= SUB || q % (P > SUB ? P / SUB : 1) == 0) {
+          const int t = ts + at;
+          float u[SP], d[SP], y[SP], sl[SP], zf[SP], du[SP];
+          get_steps<SP>(&sh.u[el][t], u);
+          get_steps<SP>(&sh.dt[el][t], d);
+          get_steps<SP>(&sh.dy[el][t], y);
+          get_steps<SP>(&sh.dd[el][t], sl);
+          if (has_z) get_steps<SP>(&sh.dz[el][t], zf);
+          float sD = 0.f, sb = 0.f;
 #pragma unroll
           for (int j = 0; j < SP; ++j) {
-            const int t = ts + at + j;
-            const float u = sh.u[el][t], d = sh.dt[el][t], y = sh.dy[el][t];
-            sh.du[el][t] = fmaf(d, s1[j], Dv[m] * y);
-            const float dd = fmaf(u, s1[j], s2[j]) * sh.dd[el][t];
-            sh.dd[el][t] = dd;
-            if (has_z) sh.dz[el][t] *= fmaf(Dv[m], u, s0[j]);
-            sumD[m] += (double)(y * u);
-            sumbias[m] += (double)dd;
+            du[j] = fmaf(d[j], s1[j], Dv[m] * y[j]);
+            sl[j] *= fmaf(u[j], s1[j], 0.6931471805599453f * s2[j]);
+            if (has_z) zf[j] *= fmaf(Dv[m], u[j], s0[j]);
+            sD = fmaf(y[j], u[j], sD);
+            sb += sl[j];
           }
+          put_steps<SP>(&sh.du[el][t], du);
+          put_steps<SP>(&sh.dd[el][t], sl);
+          if (has_z) put_steps<SP>(&sh.dz[el][t], zf);
+          sumD[m] += sD;
+          sumbias[m] += sb;
         }
       }
-      // over the warp's channels: lanes q, q + P, ... ; then over the warps
-      float v[2 * SUB * K];
+      // over the warp's channels: lanes q, q + P, ..; exchanges of registers k and k ^ o first, then of steps; then over the warps
+      float v[K][2 * SUB];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < SUB / 2; ++j) unpack2(acc[i][k][j], v[k][i * SUB + 2 * j], v[k][i * SUB + 2 * j + 1]);
+      constexpr int KL = K / FLIP;  // registers k that are left
+#pragma unroll
+      for (int o = FLIP / 2; o >= 1; o /= 2)
 #pragma unroll
         for (int k = 0; k < K; ++k)
+          if ((k & (FLIP - 1)) < o) {
 #pragma unroll
-          for (int j = 0; j < SUB / 2; ++j) unpack2(acc[i][k][j], v[(i * K + k) * SUB + 2 * j], v[(i * K + k) * SUB + 2 * j + 1]);
-      const int at = spread_sum<2 * SUB * K, Q, P>(v, lane / P);
+            for (int i = 0; i < 2 * SUB; ++i) v[k][i] += __shfl_xor_sync(0xffffffffu, v[k + o][i], o * P);
+          }
 #pragma unroll
-      for (int j = 0; j < 2 * SUB * K / Q; ++j) {
-        const int i = at + j, w = i / (SUB * K), k = i / SUB % K, t = i % SUB;
-        sh.red[warp][(t * 2 + w) * NP + q * K + k] = v[j];
+      for (int kl = 0; kl < KL; ++kl) {
+        const int k = kl * FLIP;
+        const int at = spread_sum<2 * SUB, Q / FLIP, P * FLIP>(v[k], lane / (P * FLIP));
+#pragma unroll
+        for (int j = 0; j < 2 * SUB / (Q / FLIP); ++j) {
+          const int i = at + j, w = i / SUB, t = i % SUB;
+          sh.red[warp][(t * 2 + w) * NP + nk[k]] = v[k][j];
+        }
       }
       __syncthreads();
       for (int i = tid; i < 2 * SUB * NP; i += NT) {
@@ -288,18 +345,32 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
         if (t < len) g.part_bc[((((int64_t)b * p.L + t) * p.G + gr) * tiles + tile) * 2 * NP + i % (2 * NP)] = r;
       }
       __syncthreads();
+      half ^= 1;
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      sh.dD[m][tid] += (double)sumD[m];
+      sh.dbias[m][tid] += (double)sumbias[m];
+#pragma unroll
+      for (int k = 0; k < K; ++k) sh.dA[m * K + k][tid] += (double)dA[m][k];
     }
     if (lelive) {
 #pragma unroll 1
       for (int j0 = 0; j0 < R; j0 += RR) {
+        float v[3][2][RR];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          get_steps<RR>(&sh.du[le + i][lt + j0], v[0][i]);
+          get_steps<RR>(&sh.dd[le + i][lt + j0], v[1][i]);
+          if (has_z) get_steps<RR>(&sh.dz[le + i][lt + j0], v[2][i]);
+        }
 #pragma unroll
         for (int j = 0; j < RR; ++j) {
           const int t = t0 + lt + j0 + j;
           if (t < last) {
-            const int l = lt + j0 + j;
-            store2<T>(dup + (int64_t)t * g.du.sl, FAST || g.vec_du, second, sh.du[le][l], sh.du[le + 1][l]);
-            put_ddelta(t, sh.dd[le][l], sh.dd[le + 1][l]);
-            if (has_z) store2<T>(dzp + (int64_t)t * g.dz.sl, FAST || g.vec_dz, second, sh.dz[le][l], sh.dz[le + 1][l]);
+            store2<T>(dup + (int64_t)t * g.du.sl, FAST || g.vec_du, second, v[0][0][j], v[0][1][j]);
+            put_ddelta(t, v[1][0][j], v[1][1][j]);
+            if (has_z) store2<T>(dzp + (int64_t)t * g.dz.sl, FAST || g.vec_dz, second, v[2][0][j], v[2][1][j]);
           }
         }
       }
@@ -311,20 +382,21 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     const int e = e_first + m * (NT / P) + tid / P;
+    double sumD = sh.dD[m][tid], sumbias = sh.dbias[m][tid];
 #pragma unroll
     for (int o = P / 2; o >= 1; o /= 2) {
-      sumD[m] += __shfl_xor_sync(0xffffffffu, sumD[m], o);
-      sumbias[m] += __shfl_xor_sync(0xffffffffu, sumbias[m], o);
+      sumD += __shfl_xor_sync(0xffffffffu, sumD, o);
+      sumbias += __shfl_xor_sync(0xffffffffu, sumbias, o);
     }
     if (e < e_end) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        pa[(int64_t)e * (NP + 2) + q * K + k] = (float)dA[m][k];
-        if (g.dh0 != nullptr && c == 0 && q * K + k < p.N) g.dh0[((int64_t)b * p.E + e) * p.N + q * K + k] = gv[m][k];
+        pa[(int64_t)e * (NP + 2) + nk[k]] = (float)sh.dA[m * K + k][tid];
+        if (g.dh0 != nullptr && c == 0 && nk[k] < p.N) g.dh0[((int64_t)b * p.E + e) * p.N + nk[k]] = gv[m][k];
       }
       if (q == 0) {
-        pa[(int64_t)e * (NP + 2) + NP] = (float)sumD[m];
-        pa[(int64_t)e * (NP + 2) + NP + 1] = (float)sumbias[m];
+        pa[(int64_t)e * (NP + 2) + NP] = (float)sumD;
+        pa[(int64_t)e * (NP + 2) + NP + 1] = (float)sumbias;
       }
     }
   }
@@ -461,6 +533,9 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
+#ifndef M3_BK
+#define M3_BK 4
+#endif
 #ifndef M3_BM
 #define M3_BM 2
 #endif
@@ -474,7 +549,7 @@ int by_states(int n, F&& f) {
   switch (sel_padded_states(n)) {
     case 4: return f(KPM<2, 2, 1>{});
     case 8: return f(KPM<4, 2, 1>{});
-    case 16: return f(KPM<4, 4, M3_BM>{});
+    case 16: return f(KPM<M3_BK, 16 / M3_BK, M3_BM>{});
     case 32: return f(KPM<4, 8, 2>{});
     case 64: return f(KPM<4, 16, 2>{});
     default: return f(KPM<4, 32, 2>{});
