@@ -1606,7 +1606,7 @@ int m3_causal_conv_step(m3_tensor* state, const m3_tensor* x, const m3_tensor* w
   M3_TRY(operand(y, "y", 2, x->shape, 1u << x->dtype, true, false, some));
   if (!some) return M3_OK;
   ConvStepParams p{state->data, state->stride[0], state->stride[1], x->data, x->stride[0], weight->data, weight->stride[0],
-                   fptr<const void>(bias), weight->dtype == M3_FLOAT32, silu != 0, y->data, batch, (int)E};
+                   fptr<const void>(bias), weight->dtype == M3_FLOAT32, silu != 0, y->data, batch, (int)E, false};
   return launch_conv_step(p, (int)taps, x->dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 

@@ -8,35 +8,63 @@
 
 #include "causal_conv.cuh"
 #include "m3_common.cuh"
+#include "pairs.cuh"
 
 namespace m3 {
 namespace {
 
-constexpr int kRun = 16;        // rows that a warp walks
 constexpr int kWarps = 8;
 
-template <typename T, int V>
-struct alignas(V * sizeof(T)) Pack { T e[V]; };
+// A row's 2 NV neighbouring channels of a lane as they lie in memory; converted when they are used, so that loads
+// stay in flight.
+template <typename T, int NV> struct RawRow;
+template <> struct RawRow<float, 2> { float4 v; };
+template <> struct RawRow<__nv_bfloat16, 2> { uint2 v; };
+template <> struct RawRow<__half, 2> { uint2 v; };
+template <typename T> struct RawRow<T, 1> { Raw2<T> v; };
 
-template <typename T, int V>
-__device__ __forceinline__ void load(const T* p, float (&v)[V]) {
-  const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(p);
+template <typename T, int NV>
+struct Chan {  // how a lane reaches its channels: all at once, or (NV = 1) one by one, the second one `second` further
+  bool vec;
+  int second;
+  __device__ __forceinline__ RawRow<T, NV> load(const T* p) const {
+    RawRow<T, NV> r;
+    if constexpr (NV == 2) r = *reinterpret_cast<const RawRow<T, 2>*>(p);
+    else r.v = load2<T>(p, vec, second);
+    return r;
+  }
+  __device__ __forceinline__ void store(T* p, const f2 (&v)[NV]) const {
+    float a[2 * NV];
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = to_f32(x.e[i]);
+    for (int i = 0; i < NV; ++i) unpack2(v[i], a[2 * i], a[2 * i + 1]);
+    if constexpr (NV == 2) {
+      alignas(16) T o[4] = {from_f32<T>(a[0]), from_f32<T>(a[1]), from_f32<T>(a[2]), from_f32<T>(a[3])};
+      *reinterpret_cast<RawRow<T, 2>*>(p) = *reinterpret_cast<const RawRow<T, 2>*>(o);
+    } else {
+      store2<T>(p, vec, second, a[0], a[1]);
+    }
+  }
+};
+
+template <typename T, int NV>
+__device__ __forceinline__ void values(const RawRow<T, NV>& r, f2 (&v)[NV]) {
+  if constexpr (NV == 1) {
+    const float2 x = value2(r.v);
+    v[0] = pack2(x.x, x.y);
+  } else if constexpr (sizeof(T) == 4) {
+    v[0] = pack2(r.v.x, r.v.y);
+    v[1] = pack2(r.v.z, r.v.w);
+  } else {
+    const float2 x = value2(Raw2<T>{r.v.x}), y = value2(Raw2<T>{r.v.y});
+    v[0] = pack2(x.x, x.y);
+    v[1] = pack2(y.x, y.y);
+  }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
-  Pack<T, V> x;
+template <int NV>
+__device__ __forceinline__ void zero(f2 (&v)[NV]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) x.e[i] = from_f32<T>(v[i]);
-  *reinterpret_cast<Pack<T, V>*>(p) = x;
-}
-
-template <int V>
-__device__ __forceinline__ void zero(float (&v)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = 0.f;
+  for (int i = 0; i < NV; ++i) v[i] = 0;
 }
 
 template <typename T>
@@ -50,143 +78,154 @@ __device__ __forceinline__ int row_count(const int64_t* lengths, int b, int L) {
   return n < 0 ? 0 : n > L ? L : (int)n;
 }
 
-template <typename T, int V, int K>
+template <typename T, int NV, int K>
 struct Lane {  // a lane's channels of one sequence
   const ConvParams& p;
+  Chan<T, NV> ch;
   const T* x;
   const T* init;
-  int e;
-  float w[K][V], bias[V];
+  f2 w[K][NV], bias[NV];
 
-  __device__ __forceinline__ Lane(const ConvParams& q, int b, int e_) : p(q), e(e_) {
+  __device__ __forceinline__ Lane(const ConvParams& q, int b, int e) : p(q), ch{q.vec, e + 1 < q.E ? 1 : 0} {
     x = static_cast<const T*>(p.x) + (int64_t)b * p.xb + e;
     init = p.init != nullptr ? static_cast<const T*>(p.init) + (int64_t)b * p.ib + e : nullptr;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < NV; ++i) {
+      const int e0 = e + 2 * i, e1 = e0 + ch.second;
 #pragma unroll
-      for (int k = 0; k < K; ++k) w[k][i] = weight<T>(p.w, p.w_f32, (int64_t)(e + i) * p.we + k);
-      bias[i] = p.bias != nullptr ? weight<T>(p.bias, p.w_f32, e + i) : 0.f;
+      for (int k = 0; k < K; ++k)
+        w[k][i] = pack2(weight<T>(p.w, p.w_f32, (int64_t)e0 * p.we + k), weight<T>(p.w, p.w_f32, (int64_t)e1 * p.we + k));
+      bias[i] = p.bias != nullptr ? pack2(weight<T>(p.bias, p.w_f32, e0), weight<T>(p.bias, p.w_f32, e1)) : 0;
     }
   }
   // row t of the sequence with its state in front of it, -(K - 1) <= t < count
-  __device__ __forceinline__ void row(int t, float (&v)[V]) const {
-    if (t >= 0) load<T, V>(x + (int64_t)t * p.xl, v);
-    else if (init != nullptr) load<T, V>(init + (int64_t)(t + K - 1) * p.il, v);
+  __device__ __forceinline__ void row(int t, f2 (&v)[NV]) const {
+    if (t >= 0) values<T, NV>(ch.load(x + (int64_t)t * p.xl), v);
+    else if (init != nullptr) values<T, NV>(ch.load(init + (int64_t)(t + K - 1) * p.il), v);
     else zero(v);
   }
-  __device__ __forceinline__ void pre(const float (&win)[K][V], float (&v)[V]) const {
+  __device__ __forceinline__ void pre(const f2 (&win)[K][NV], f2 (&v)[NV]) const {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < NV; ++i) {
       v[i] = bias[i];
 #pragma unroll
-      for (int k = 0; k < K; ++k) v[i] = fmaf(w[k][i], win[k][i], v[i]);
+      for (int k = 0; k < K; ++k) v[i] = fma2(w[k][i], win[k][i], v[i]);
     }
   }
 };
 
-template <int K, int V>
-__device__ __forceinline__ void shift(float (&win)[K][V]) {
+template <int K, int NV>
+__device__ __forceinline__ void shift(f2 (&win)[K][NV]) {
 #pragma unroll
   for (int k = 0; k + 1 < K; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+    for (int i = 0; i < NV; ++i) win[k][i] = win[k + 1][i];
 }
 
-template <typename T, int V, int K>
+template <typename T, int NV, int K>
 __global__ void __launch_bounds__(32 * kWarps) conv_fwd_kernel(const ConvParams p) {
-  const int e = (blockIdx.x * 32 + threadIdx.x) * V, b = blockIdx.z;
-  const int t0 = (blockIdx.y * kWarps + threadIdx.y) * kRun;
+  const int e = (blockIdx.x * 32 + threadIdx.x) * 2 * NV, b = blockIdx.z;
+  const int t0 = (blockIdx.y * kWarps + threadIdx.y) * p.run;
   if (e >= p.E) return;
   const int n = row_count(p.lengths, b, p.L);
-  const Lane<T, V, K> ln(p, b, e);
+  const Lane<T, NV, K> ln(p, b, e);
   if (t0 == 0 && p.last != nullptr) {
     T* last = static_cast<T*>(p.last) + (int64_t)b * (K - 1) * p.E + e;
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
-      float v[V];
+      f2 v[NV];
       ln.row(n - (K - 1) + k, v);
-      store<T, V>(last + (int64_t)k * p.E, v);
+      ln.ch.store(last + (int64_t)k * p.E, v);
     }
   }
-  const int t1 = min(t0 + kRun, p.L);
+  const int t1 = min(t0 + p.run, p.L);
   if (t0 >= t1) return;
   T* y = static_cast<T*>(p.y) + (int64_t)b * p.yb + e;
-  float win[K][V];
+  f2 win[K][NV];
+#pragma unroll
+  for (int k = 0; k < K; ++k) zero(win[k]);
   if (t0 < n) {
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) ln.row(t0 - (K - 1) + k, win[k + 1]);
   }
   constexpr int U = 8;
+  const int end = min(t1, n);
 #pragma unroll 1
-  for (int t = t0; t < t1; t += U) {
-    float in[U][V];
+  for (int t = t0; t < end; t += U) {
+    RawRow<T, NV> in[U];
+    if (t + U <= end) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (t + u < min(t1, n)) load<T, V>(ln.x + (int64_t)(t + u) * p.xl, in[u]);
-      else zero(in[u]);
+      for (int u = 0; u < U; ++u) in[u] = ln.ch.load(ln.x + (int64_t)(t + u) * p.xl);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) in[u] = ln.ch.load(ln.x + (int64_t)min(t + u, end - 1) * p.xl);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float v[V];
-      shift(win);
+      if (t + u < end) {
+        f2 v[NV];
+        shift(win);
+        values<T, NV>(in[u], win[K - 1]);
+        ln.pre(win, v);
+        if (p.silu) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[K - 1][i] = in[u][i];
-      ln.pre(win, v);
-      if (t + u < t1) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (p.silu) v[i] *= fast_sigmoid(v[i]);
-          if (t + u >= n) v[i] = 0.f;
+          for (int i = 0; i < NV; ++i) v[i] = mul2(v[i], sigmoid2(v[i]));
         }
-        store<T, V>(y + (int64_t)(t + u) * p.yl, v);
+        ln.ch.store(y + (int64_t)(t + u) * p.yl, v);
       }
     }
   }
+  f2 none[NV];
+  zero(none);
+  for (int t = max(t0, n); t < t1; ++t) ln.ch.store(y + (int64_t)t * p.yl, none);  // padding
 }
 
 // d[t] from the window that ends at t
-template <typename T, int V, int K>
-__device__ __forceinline__ void slope(const Lane<T, V, K>& ln, const float (&win)[K][V], float (&d)[V]) {
+template <typename T, int NV, int K>
+__device__ __forceinline__ void slope(const Lane<T, NV, K>& ln, const f2 (&win)[K][NV], f2 (&d)[NV]) {
   if (!ln.p.silu) return;
-  float v[V];
+  f2 v[NV];
   ln.pre(win, v);
+  const f2 one = pack2(1.f, 1.f), minus = pack2(-1.f, -1.f);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float s = fast_sigmoid(v[i]);
-    d[i] *= s * fmaf(v[i], 1.f - s, 1.f);
+  for (int i = 0; i < NV; ++i) {
+    const f2 s = sigmoid2(v[i]);
+    d[i] = mul2(d[i], mul2(s, fma2(v[i], fma2(s, minus, one), one)));
   }
 }
 
 // Gradient of the last rows that falls on row t (of the sequence with its state in front of it).
-template <typename T, int V, int K>
-__device__ __forceinline__ void add_last(const ConvParams& p, const ConvGrads& g, int b, int e, int n, int t, float (&v)[V]) {
+template <typename T, int NV, int K>
+__device__ __forceinline__ void add_last(const Lane<T, NV, K>& ln, const ConvGrads& g, int b, int e, int n, int t, f2 (&v)[NV]) {
   const int i = t - n + K - 1;
   if (g.dlast == nullptr || i < 0 || i >= K - 1) return;
-  float d[V];
-  load<T, V>(static_cast<const T*>(g.dlast) + (int64_t)b * g.dlb + (int64_t)i * g.dll + e, d);
+  f2 d[NV];
+  values<T, NV>(ln.ch.load(static_cast<const T*>(g.dlast) + (int64_t)b * g.dlb + (int64_t)i * g.dll + e), d);
 #pragma unroll
-  for (int j = 0; j < V; ++j) v[j] += d[j];
+  for (int j = 0; j < NV; ++j) v[j] = add2(v[j], d[j]);
 }
 
-template <typename T, int V, int K>
+template <typename T, int NV, int K>
 __global__ void __launch_bounds__(32 * kWarps) conv_bwd_kernel(const ConvParams p, const ConvGrads g) {
-  __shared__ float sums[kWarps][K + 1][32 * V];
-  const int e = (blockIdx.x * 32 + threadIdx.x) * V, b = blockIdx.z;
-  const int t0 = (blockIdx.y * kWarps + threadIdx.y) * kRun, t1 = min(t0 + kRun, p.L);
+  __shared__ f2 sums[kWarps][K + 1][32 * NV];
+  const int e = (blockIdx.x * 32 + threadIdx.x) * 2 * NV, b = blockIdx.z;
+  const int t0 = (blockIdx.y * kWarps + threadIdx.y) * p.run, t1 = min(t0 + p.run, p.L);
   const bool live = e < p.E;
-  float dw[K + 1][V];  // dw, then dbias
+  f2 dw[K + 1][NV];  // dw, then dbias
 #pragma unroll
   for (int k = 0; k <= K; ++k) zero(dw[k]);
   if (live) {
     const int n = row_count(p.lengths, b, p.L);
-    const Lane<T, V, K> ln(p, b, e);
+    const Lane<T, NV, K> ln(p, b, e);
     const T* dy = static_cast<const T*>(g.dy) + (int64_t)b * g.dyb + e;
     T* dx = static_cast<T*>(g.dx) + (int64_t)b * g.dxb + e;
-    float win[K][V], dwin[K][V];  // rows t - K + 1 .. t of x, and of d
+    f2 win[K][NV], dwin[K][NV];  // rows t - K + 1 .. t of x, and of d
+#pragma unroll
+    for (int k = 0; k < K; ++k) { zero(win[k]); zero(dwin[k]); }
     if (t0 == 0 && g.dinit != nullptr) {
       // the rows in front of the first take part in the first K - 1 outputs only
       T* di = static_cast<T*>(g.dinit) + (int64_t)b * (K - 1) * p.E + e;
-      float out[K][V];
+      f2 out[K][NV];
 #pragma unroll
       for (int k = 0; k < K; ++k) zero(out[k]);
 #pragma unroll
@@ -194,90 +233,93 @@ __global__ void __launch_bounds__(32 * kWarps) conv_bwd_kernel(const ConvParams 
 #pragma unroll
       for (int t = 0; t < K - 1; ++t) {
         if (t < n) {
-          float d[V];
+          f2 d[NV];
           shift(win);
           ln.row(t, win[K - 1]);
-          load<T, V>(dy + (int64_t)t * g.dyl, d);
+          values<T, NV>(ln.ch.load(dy + (int64_t)t * g.dyl), d);
           slope(ln, win, d);
           // row t - K + 1 + k has index t + k among the state's rows
 #pragma unroll
           for (int k = 0; k < K - 1 - t; ++k)
 #pragma unroll
-            for (int i = 0; i < V; ++i) out[t + k][i] = fmaf(ln.w[k][i], d[i], out[t + k][i]);
+            for (int i = 0; i < NV; ++i) out[t + k][i] = fma2(ln.w[k][i], d[i], out[t + k][i]);
         }
       }
 #pragma unroll
       for (int k = 0; k < K - 1; ++k) {
-        add_last<T, V, K>(p, g, b, e, n, k - (K - 1), out[k]);
-        store<T, V>(di + (int64_t)k * p.E, out[k]);
+        add_last<T, NV, K>(ln, g, b, e, n, k - (K - 1), out[k]);
+        ln.ch.store(di + (int64_t)k * p.E, out[k]);
       }
     }
-    if (t0 < t1) {
+    const int end = min(t1, n);  // rows of this run that count
+    if (t0 < end) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) { zero(win[k]); zero(dwin[k]); }
-      if (t0 < n) {
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k) ln.row(t0 - (K - 1) + k, win[k + 1]);
-      }
+      for (int k = 0; k < K - 1; ++k) ln.row(t0 - (K - 1) + k, win[k + 1]);
       constexpr int U = 4;
+      const int ahead = min(end + K - 1, n);  // rows whose d this run needs
 #pragma unroll 1
-      for (int t = t0; t < t1 + K - 1; t += U) {
-        float in[U][V], din[U][V];
+      for (int t = t0; t < end + K - 1; t += U) {
+        RawRow<T, NV> in[U], din[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (t + u < min(t1 + K - 1, n)) {
-            load<T, V>(ln.x + (int64_t)(t + u) * p.xl, in[u]);
-            load<T, V>(dy + (int64_t)(t + u) * g.dyl, din[u]);
-          } else {
-            zero(in[u]);
-            zero(din[u]);
-          }
+          const int64_t r = min(t + u, ahead - 1);
+          in[u] = ln.ch.load(ln.x + r * p.xl);
+          din[u] = ln.ch.load(dy + r * g.dyl);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           shift(win);
           shift(dwin);
+          if (t + u < ahead) {
+            values<T, NV>(in[u], win[K - 1]);
+            values<T, NV>(din[u], dwin[K - 1]);
+            slope(ln, win, dwin[K - 1]);
+          } else {
+            zero(dwin[K - 1]);
+          }
+          if (t + u < end) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) { win[K - 1][i] = in[u][i]; dwin[K - 1][i] = din[u][i]; }
-          if (t + u < n) slope(ln, win, dwin[K - 1]);
-          if (t + u < min(t1, n)) {
+            for (int i = 0; i < NV; ++i) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-#pragma unroll
-              for (int k = 0; k < K; ++k) dw[k][i] = fmaf(dwin[K - 1][i], win[k][i], dw[k][i]);
-              dw[K][i] += dwin[K - 1][i];
+              for (int k = 0; k < K; ++k) dw[k][i] = fma2(dwin[K - 1][i], win[k][i], dw[k][i]);
+              dw[K][i] = add2(dw[K][i], dwin[K - 1][i]);
             }
           }
           const int at = t + u - (K - 1);  // all of d[at ..  at + K - 1] is at hand
-          if (at >= t0 && at < t1) {
-            float v[V];
+          if (at >= t0 && at < end) {
+            f2 v[NV];
             zero(v);
-            if (at < n) {
 #pragma unroll
-              for (int i = 0; i < V; ++i)
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int k = 0; k < K; ++k) v[i] = fmaf(ln.w[k][i], dwin[K - 1 - k][i], v[i]);
-              add_last<T, V, K>(p, g, b, e, n, at, v);
-            }
-            store<T, V>(dx + (int64_t)at * g.dxl, v);
+              for (int k = 0; k < K; ++k) v[i] = fma2(ln.w[k][i], dwin[K - 1 - k][i], v[i]);
+            add_last<T, NV, K>(ln, g, b, e, n, at, v);
+            ln.ch.store(dx + (int64_t)at * g.dxl, v);
           }
         }
       }
     }
+    f2 none[NV];
+    zero(none);
+    for (int t = max(t0, n); t < t1; ++t) ln.ch.store(dx + (int64_t)t * g.dxl, none);  // padding
   }
 #pragma unroll
   for (int k = 0; k <= K; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) sums[threadIdx.y][k][threadIdx.x * V + i] = dw[k][i];
+    for (int i = 0; i < NV; ++i) sums[threadIdx.y][k][threadIdx.x * NV + i] = dw[k][i];
   __syncthreads();
   const int64_t part = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
-  for (int i = threadIdx.y * 32 + threadIdx.x; i < (K + 1) * 32 * V; i += 32 * kWarps) {
-    const int k = i / (32 * V), c = i % (32 * V), ch = blockIdx.x * 32 * V + c;
-    if (ch < p.E) {
-      float v = 0.f;
+  for (int i = threadIdx.y * 32 + threadIdx.x; i < (K + 1) * 32 * NV; i += 32 * kWarps) {
+    const int k = i / (32 * NV), c = i % (32 * NV), to = (blockIdx.x * 32 * NV + c) * 2;
+    if (to < p.E) {
+      f2 v = 0;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += sums[w][k][c];
-      g.part[(part * (K + 1) + k) * p.E + ch] = v;
+      for (int w = 0; w < kWarps; ++w) v = add2(v, sums[w][k][c]);
+      float a, d;
+      unpack2(v, a, d);
+      float* out = g.part + (part * (K + 1) + k) * p.E + to;
+      out[0] = a;
+      if (to + 1 < p.E) out[1] = d;
     }
   }
 }
@@ -308,28 +350,41 @@ __global__ void __launch_bounds__(256) conv_bwd_join_kernel(const float* part, i
 }
 
 // One step: the window moves on by one row, in place.
-template <typename T, int V, int K>
+template <typename T, int NV, int K>
 __global__ void __launch_bounds__(128) conv_step_kernel(const ConvStepParams p) {
+  const int per = (p.E + 2 * NV - 1) / (2 * NV);
   const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-  const int per = p.E / V;
   if (i >= p.batch * per) return;
   const int64_t b = i / per;
-  const int e = (int)(i % per) * V;
+  const int e = (int)(i % per) * 2 * NV;
+  const Chan<T, NV> ch{p.vec, e + 1 < p.E ? 1 : 0};
   T* state = static_cast<T*>(p.state) + b * p.sb + e;
-  float win[K][V], v[V];
+  RawRow<T, NV> raw[K];
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) load<T, V>(state + k * p.sl, win[k]);
-  load<T, V>(static_cast<const T*>(p.x) + b * p.xb + e, win[K - 1]);
+  for (int k = 0; k < K - 1; ++k) raw[k] = ch.load(state + k * p.sl);
+  raw[K - 1] = ch.load(static_cast<const T*>(p.x) + b * p.xb + e);
+  f2 v[NV];
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) store<T, V>(state + k * p.sl, win[k + 1]);
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    v[j] = p.bias != nullptr ? weight<T>(p.bias, p.w_f32, e + j) : 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[j] = fmaf(weight<T>(p.w, p.w_f32, (int64_t)(e + j) * p.we + k), win[k][j], v[j]);
-    if (p.silu) v[j] *= fast_sigmoid(v[j]);
+  for (int j = 0; j < NV; ++j) {
+    const int e0 = e + 2 * j, e1 = e0 + ch.second;
+    v[j] = p.bias != nullptr ? pack2(weight<T>(p.bias, p.w_f32, e0), weight<T>(p.bias, p.w_f32, e1)) : 0;
   }
-  store<T, V>(static_cast<T*>(p.y) + b * p.E + e, v);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    f2 x[NV];
+    values<T, NV>(raw[k], x);
+    if (k > 0) ch.store(state + (k - 1) * p.sl, x);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = e + 2 * j, e1 = e0 + ch.second;
+      v[j] = fma2(pack2(weight<T>(p.w, p.w_f32, (int64_t)e0 * p.we + k), weight<T>(p.w, p.w_f32, (int64_t)e1 * p.we + k)), x[j], v[j]);
+    }
+  }
+  if (p.silu) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = mul2(v[j], sigmoid2(v[j]));
+  }
+  ch.store(static_cast<T*>(p.y) + b * p.E + e, v);
 }
 
 bool fits(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -339,13 +394,13 @@ bool rows_fit(const void* p, int64_t s0, int64_t s1, int v, int es) {
   return p == nullptr || (fits(p, (int64_t)v * es) && s0 % v == 0 && s1 % v == 0);
 }
 
-// f(V) with the channels that a lane takes: as many as fill `most` bytes, where base addresses and
-// pitches allow it; else 4 bytes' worth; else one.
-template <typename T, int MOST, typename Fits, typename F>
-int by_vector(Fits&& ok, F&& f) {
-  constexpr int es = sizeof(T), V0 = MOST / es, V1 = 4 / es;
-  if (ok(V0)) return f(std::integral_constant<int, V0>{});
-  if (V1 > 1 && ok(V1)) return f(std::integral_constant<int, V1>{});
+// f(pairs of channels that a lane takes): two where addresses and pitches let a row's four be moved at once, else one, whose two
+// channels go at once or one by one (*vec).
+template <typename Fits, typename F>
+int by_vector(Fits&& ok, bool* vec, F&& f) {
+  *vec = true;
+  if (ok(4)) return f(std::integral_constant<int, 2>{});
+  *vec = ok(2);
   return f(std::integral_constant<int, 1>{});
 }
 
@@ -363,22 +418,29 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
-unsigned runs(int64_t L) { return (unsigned)((L + kRun * kWarps - 1) / (kRun * kWarps)); }
+// Rows that a warp walks: 32, fewer where that leaves less than about two CTAs an SM (rows between two runs are read twice).
+int run_rows(int64_t batch, int64_t L, int64_t E) {
+  int run = 32;
+  while (run > 8 && batch * ((E + 127) / 128) * ((L + run * kWarps - 1) / (run * kWarps)) < 296) run /= 2;
+  return run;
+}
+unsigned runs(int64_t L, int run) { return (unsigned)std::max<int64_t>(1, (L + run * kWarps - 1) / (run * kWarps)); }
 
 }  // namespace
 
-int launch_conv_fwd(const ConvParams& p, int taps, int dtype, cudaStream_t s) {
+int launch_conv_fwd(ConvParams p, int taps, int dtype, cudaStream_t s) {
+  p.run = run_rows(p.batch, p.L, p.E);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto ok = [&](int v) {
       return p.E % v == 0 && rows_fit(p.x, p.xb, p.xl, v, sizeof(T)) && rows_fit(p.y, p.yb, p.yl, v, sizeof(T)) &&
              rows_fit(p.init, p.ib, p.il, v, sizeof(T)) && fits(p.last, v * sizeof(T));
     };
-    return by_vector<T, 16>(ok, [&](auto v) {
+    return by_vector(ok, &p.vec, [&](auto nv) {
       return by_taps(taps, [&](auto k) {
-        const int per = 32 * v;
-        const dim3 grid((unsigned)((p.E + per - 1) / per), std::max(1u, runs(p.L)), (unsigned)p.batch);
-        conv_fwd_kernel<T, decltype(v)::value, decltype(k)::value><<<grid, dim3(32, kWarps), 0, s>>>(p);
+        const int per = 64 * nv;
+        const dim3 grid((unsigned)((p.E + per - 1) / per), runs(p.L, p.run), (unsigned)p.batch);
+        conv_fwd_kernel<T, decltype(nv)::value, decltype(k)::value><<<grid, dim3(32, kWarps), 0, s>>>(p);
         return check_launch("conv_fwd_kernel");
       });
     });
@@ -386,11 +448,12 @@ int launch_conv_fwd(const ConvParams& p, int taps, int dtype, cudaStream_t s) {
 }
 
 size_t conv_bwd_workspace(int64_t batch, int64_t L, int64_t E, int taps) {
-  return (size_t)batch * std::max(1u, runs(L)) * E * (taps + 1) * sizeof(float);
+  return (size_t)batch * runs(L, run_rows(batch, L, E)) * E * (taps + 1) * sizeof(float);
 }
 
-int launch_conv_bwd(const ConvParams& p, ConvGrads g, int taps, int dtype, void* ws, cudaStream_t s) {
+int launch_conv_bwd(ConvParams p, ConvGrads g, int taps, int dtype, void* ws, cudaStream_t s) {
   g.part = static_cast<float*>(ws);
+  p.run = run_rows(p.batch, p.L, p.E);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int es = sizeof(T);
@@ -399,12 +462,12 @@ int launch_conv_bwd(const ConvParams& p, ConvGrads g, int taps, int dtype, void*
              rows_fit(g.dx, g.dxb, g.dxl, v, es) && rows_fit(p.init, p.ib, p.il, v, es) &&
              rows_fit(g.dlast, g.dlb, g.dll, v, es) && fits(g.dinit, v * es);
     };
-    const unsigned ny = std::max(1u, runs(p.L));
-    if (p.batch > 0) M3_TRY((by_vector<T, es == 4 ? 16 : 8>(ok, [&](auto v) {
+    const unsigned ny = runs(p.L, p.run);
+    if (p.batch > 0) M3_TRY((by_vector(ok, &p.vec, [&](auto nv) {
       return by_taps(taps, [&](auto k) {
-        const int per = 32 * v;
+        const int per = 64 * nv;
         const dim3 grid((unsigned)((p.E + per - 1) / per), ny, (unsigned)p.batch);
-        conv_bwd_kernel<T, decltype(v)::value, decltype(k)::value><<<grid, dim3(32, kWarps), 0, s>>>(p, g);
+        conv_bwd_kernel<T, decltype(nv)::value, decltype(k)::value><<<grid, dim3(32, kWarps), 0, s>>>(p, g);
         return check_launch("conv_bwd_kernel");
       });
     })));
@@ -415,17 +478,17 @@ int launch_conv_bwd(const ConvParams& p, ConvGrads g, int taps, int dtype, void*
   });
 }
 
-int launch_conv_step(const ConvStepParams& p, int taps, int dtype, cudaStream_t s) {
+int launch_conv_step(ConvStepParams p, int taps, int dtype, cudaStream_t s) {
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int es = sizeof(T);
     auto ok = [&](int v) {
       return p.E % v == 0 && rows_fit(p.state, p.sb, p.sl, v, es) && rows_fit(p.x, p.xb, 0, v, es) && fits(p.y, v * es);
     };
-    return by_vector<T, es == 4 ? 16 : 8>(ok, [&](auto v) {
+    return by_vector(ok, &p.vec, [&](auto nv) {
       return by_taps(taps, [&](auto k) {
-        const int64_t n = p.batch * (p.E / v);
-        conv_step_kernel<T, decltype(v)::value, decltype(k)::value><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
+        const int64_t n = p.batch * ((p.E + 2 * nv - 1) / (2 * nv));
+        conv_step_kernel<T, decltype(nv)::value, decltype(k)::value><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
         return check_launch("conv_step_kernel");
       });
     });

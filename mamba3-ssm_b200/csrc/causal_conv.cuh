@@ -18,6 +18,8 @@ struct ConvParams {
   void* y; int64_t yb, yl;
   void* last;                           // (batch, taps - 1, E) contiguous: the last rows; may be null
   int batch, L, E;
+  int run;                              // rows that a warp walks
+  bool vec;                             // a lane's channels are moved at once
 };
 
 struct ConvGrads {
@@ -38,11 +40,12 @@ struct ConvStepParams {
   bool w_f32, silu;
   void* y;                              // (batch, E) contiguous
   int64_t batch; int E;
+  bool vec;                             // a lane's channels are moved at once
 };
 
-int launch_conv_fwd(const ConvParams& p, int taps, int dtype, cudaStream_t s);
+int launch_conv_fwd(ConvParams p, int taps, int dtype, cudaStream_t s);
 size_t conv_bwd_workspace(int64_t batch, int64_t L, int64_t E, int taps);
-int launch_conv_bwd(const ConvParams& p, ConvGrads g, int taps, int dtype, void* ws, cudaStream_t s);
-int launch_conv_step(const ConvStepParams& p, int taps, int dtype, cudaStream_t s);
+int launch_conv_bwd(ConvParams p, ConvGrads g, int taps, int dtype, void* ws, cudaStream_t s);
+int launch_conv_step(ConvStepParams p, int taps, int dtype, cudaStream_t s);
 
 }  // namespace m3

@@ -230,8 +230,9 @@ __global__ void __launch_bounds__(NT) sel_scan_kernel(const SelScanParams p) {
           float v0 = fmaf(D0, u.x, y2.x), v1 = fmaf(D1, u.y, y2.y);
           if (zp != nullptr) {
             const float2 z = value2(zz[j]);
-            v0 *= z.x * fast_sigmoid(z.x);
-            v1 *= z.y * fast_sigmoid(z.y);
+            const float2 sg = sigmoid2(z);
+            v0 *= z.x * sg.x;
+            v1 *= z.y * sg.y;
           }
           store2<T>(yp + (int64_t)t * p.y.sl, vy, second, t < len ? v0 : 0.f, t < len ? v1 : 0.f);
         }
@@ -286,61 +287,95 @@ __global__ void __launch_bounds__(256) sel_carry_kernel(const SelScanParams p, i
   st[(p.nchunk - 1) * pitch] = h;
 }
 
-// One step: y and the state in place. P lanes a channel, K states each.
-template <typename T, int K, int P>
-__global__ void __launch_bounds__(256) sel_step_kernel(const SelStepParams p, bool vec) {
+// Four values of a row from element i on, as fp32; vec: the address is on a boundary of the four.
+template <typename T>
+__device__ __forceinline__ void load4(const void* p, bool f32, int64_t i, bool vec, int n, float (&v)[4]) {
+  if (vec) {
+    if (sizeof(T) == 4 || f32) {
+      const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+      if constexpr (sizeof(T) == 2) {
+        const float2 lo = value2(Raw2<T>{x.x}), hi = value2(Raw2<T>{x.y});
+        v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = k < n ? ld_any<T>(p, f32, i + k) : 0.f;
+  }
+}
+
+// One step: y and the state in place. P lanes share a channel with four states each and take RB sequences, so that
+// A and the channel's parameters are loaded once, a step size is formed by one lane, and loads of RB states are in flight.
+template <typename T, int P, int RB>
+__global__ void __launch_bounds__(256) sel_step_kernel(const SelStepParams p, bool vec, bool vec_bc) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t ch = i / P;
-  const int q = (int)(i % P);
-  const bool live = ch < p.batch * p.E;
-  const int64_t b = live ? ch / p.E : 0;
+  const int q = (int)(i % P), n = q * 4;
+  const int64_t b0 = ch / p.E * RB;
+  const bool live = b0 < p.batch;
+  const int rows = live ? (int)min((int64_t)RB, p.batch - b0) : 0;
   const int e = live ? (int)(ch % p.E) : 0;
-  const int g = e / (p.E / p.G);
-  float raw = ld_any<T>(p.delta, p.delta_f32, b * p.sd + e);
-  const float u = ld(static_cast<const T*>(p.u) + b * p.su + e);
-  if (p.bias != nullptr) raw += p.bias[e];
-  float* st_ = p.state + b * p.sstate + (int64_t)e * p.N;
-  float h[K], y = 0.f;
-  if (vec) {
+  const int g = e / (p.E / p.G), mine = p.N - n;  // states from this lane on
+  float h[RB][4], A2[4], y[RB];
 #pragma unroll
-    for (int k = 0; k < K; k += 4) {
-      const int n = q * K + k;
-      const float4 v = live && n < p.N ? *reinterpret_cast<const float4*>(st_ + n) : make_float4(0.f, 0.f, 0.f, 0.f);
-      h[k] = v.x; h[k + 1] = v.y; h[k + 2] = v.z; h[k + 3] = v.w;
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < K; ++k) h[k] = live && q * K + k < p.N ? st_[q * K + k] : 0.f;
+  for (int r = 0; r < RB; ++r) {
+    if (r < rows && mine > 0) load4<float>(p.state + (b0 + r) * p.sstate + (int64_t)e * p.N, true, n, vec, mine, h[r]);
+    else h[r][0] = h[r][1] = h[r][2] = h[r][3] = 0.f;
   }
-  const float dt = step_size(raw, p.softplus), dx = dt * u;
+  // step size and input of the sequences: one a lane where there are lanes enough
+  constexpr int OWN = P < RB ? RB : 1;
+  float dt[OWN], u[OWN];
+  const float bias = p.bias != nullptr ? p.bias[e] : 0.f;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int n = q * K + k;
-    if (n < p.N) {
-      const float a = ex2(dt * (p.A[(int64_t)e * p.N + n] * kLog2e));
-      h[k] = fmaf(a, h[k], dx * ld_any<T>(p.B, p.bc_f32, b * p.sB + g * p.sBg + n));
-      y = fmaf(h[k], ld_any<T>(p.C, p.bc_f32, b * p.sC + g * p.sCg + n), y);
-    }
+  for (int r = 0; r < OWN; ++r) {
+    const int64_t b = b0 + min(OWN == 1 ? q % RB : r, max(rows - 1, 0));
+    dt[r] = live ? step_size(ld_any<T>(p.delta, p.delta_f32, b * p.sd + e) + bias, p.softplus) : 0.f;
+    u[r] = live ? ld(static_cast<const T*>(p.u) + b * p.su + e) : 0.f;
   }
 #pragma unroll
-  for (int m = P / 2; m >= 1; m /= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
-  if (!live) return;
-  if (vec) {
+  for (int k = 0; k < 4; ++k) A2[k] = k < mine ? p.A[(int64_t)e * p.N + n + k] * kLog2e : 0.f;
 #pragma unroll
-    for (int k = 0; k < K; k += 4)
-      if (q * K + k < p.N) *reinterpret_cast<float4*>(st_ + q * K + k) = make_float4(h[k], h[k + 1], h[k + 2], h[k + 3]);
-  } else {
+  for (int r = 0; r < RB; ++r) {
+    const float d = OWN == 1 ? __shfl_sync(0xffffffffu, dt[0], r, P) : dt[OWN == 1 ? 0 : r];
+    const float x = d * (OWN == 1 ? __shfl_sync(0xffffffffu, u[0], r, P) : u[OWN == 1 ? 0 : r]);
+    y[r] = 0.f;
+    if (r < rows && mine > 0) {
+      float B[4], C[4];
+      load4<T>(p.B, p.bc_f32, (b0 + r) * p.sB + g * p.sBg + n, vec_bc, mine, B);
+      load4<T>(p.C, p.bc_f32, (b0 + r) * p.sC + g * p.sCg + n, vec_bc, mine, C);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (q * K + k < p.N) st_[q * K + k] = h[k];
-  }
-  if (q == 0) {
-    if (p.D != nullptr) y = fmaf(p.D[e], u, y);
-    if (p.z != nullptr) {
-      const float z = ld(static_cast<const T*>(p.z) + b * p.sz + e);
-      y *= z * fast_sigmoid(z);
+      for (int k = 0; k < 4; ++k) {
+        h[r][k] = fmaf(ex2(fmaf(d, A2[k], kEx2Mean)), h[r][k], x * B[k]);
+        y[r] = fmaf(h[r][k], C[k], y[r]);
+      }
+      float* to = p.state + (b0 + r) * p.sstate + (int64_t)e * p.N + n;
+      if (vec) *reinterpret_cast<float4*>(to) = make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
+      else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < mine) to[k] = h[r][k];
+      }
     }
-    st(static_cast<T*>(p.y) + b * p.sy + e, y);
+  }
+  const int at = spread_sum<RB, P>(y, q);
+  constexpr int LEFT = RB / P > 0 ? RB / P : 1;
+  if (P > RB && q % (P > RB ? P / RB : 1) != 0) return;  // lanes with the same sums
+#pragma unroll
+  for (int j = 0; j < LEFT; ++j) {
+    const int r = at + j;
+    if (r < rows) {
+      const int64_t b = b0 + r;
+      float v = y[j];
+      if (p.D != nullptr) v = fmaf(p.D[e], ld(static_cast<const T*>(p.u) + b * p.su + e), v);
+      if (p.z != nullptr) {
+        const float z = ld(static_cast<const T*>(p.z) + b * p.sz + e);
+        v *= z * fast_sigmoid(z);
+      }
+      st(static_cast<T*>(p.y) + b * p.sy + e, v);
+    }
   }
 }
 
@@ -461,15 +496,30 @@ int launch_sel_scan_fwd(SelScanParams p, int dtype, void* ws, cudaStream_t s) {
 }
 
 int launch_sel_step(const SelStepParams& p, int dtype, cudaStream_t s) {
-  return by_type(dtype, [&](auto t) {
+  const bool vec = p.N % 4 == 0 && p.sstate % 4 == 0 && (reinterpret_cast<uintptr_t>(p.state) & 15) == 0;
+  auto go = [&](auto t, auto lanes) {
     using T = decltype(t);
-    return by_states(p.N, [&](auto kp) {
-      using L_ = decltype(kp);
-      const int64_t threads = p.batch * p.E * L_::p;
-      const bool vec = p.N % 4 == 0 && p.sstate % 4 == 0 && (reinterpret_cast<uintptr_t>(p.state) & 15) == 0;
-      sel_step_kernel<T, L_::k, L_::p><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(p, vec);
-      return check_launch("sel_step_kernel");
-    });
+    constexpr int P = decltype(lanes)::value;
+    const int es = sizeof(T) == 4 || p.bc_f32 ? 4 : 2;
+    const bool vec_bc = p.N % 4 == 0 && p.sB % 4 == 0 && p.sC % 4 == 0 && p.sBg % 4 == 0 && p.sCg % 4 == 0 &&
+                        ((reinterpret_cast<uintptr_t>(p.B) | reinterpret_cast<uintptr_t>(p.C)) & (4 * es - 1)) == 0;
+    // four sequences a thread where that leaves some warps for every SM
+    const bool four = p.batch >= 4 && p.batch * p.E * P >= 4 * 128 * 1024;
+    const int64_t threads = (four ? (p.batch + 3) / 4 : p.batch) * p.E * P;
+    const unsigned grid = (unsigned)((threads + 255) / 256);
+    if (four) sel_step_kernel<T, P, 4><<<grid, 256, 0, s>>>(p, vec, vec_bc);
+    else sel_step_kernel<T, P, 1><<<grid, 256, 0, s>>>(p, vec, vec_bc);
+    return check_launch("sel_step_kernel");
+  };
+  return by_type(dtype, [&](auto t) {
+    switch (sel_padded_states(p.N)) {
+      case 4: return go(t, std::integral_constant<int, 1>{});
+      case 8: return go(t, std::integral_constant<int, 2>{});
+      case 16: return go(t, std::integral_constant<int, 4>{});
+      case 32: return go(t, std::integral_constant<int, 8>{});
+      case 64: return go(t, std::integral_constant<int, 16>{});
+      default: return go(t, std::integral_constant<int, 32>{});
+    }
   });
 }
 
