@@ -128,6 +128,16 @@ __global__ void __launch_bounds__(32 * kWarps) conv_fwd_kernel(const ConvParams 
   const int t0 = (blockIdx.y * kWarps + threadIdx.y) * p.run;
   if (e >= p.E) return;
   const int n = row_count(p.lengths, b, p.L);
+  const int t1 = min(t0 + p.run, p.L), end = min(t1, n);
+  constexpr int U = 4;
+  RawRow<T, NV> in[U];  // the next rows, on their way while those before them are worked on
+  auto fetch = [&](int t) {
+    const Chan<T, NV> ch{p.vec, e + 1 < p.E ? 1 : 0};
+    const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.xb + e;
+#pragma unroll
+    for (int u = 0; u < U; ++u) in[u] = ch.load(x + (int64_t)min(t + u, end - 1) * p.xl);
+  };
+  if (t0 < end) fetch(t0);
   const Lane<T, NV, K> ln(p, b, e);
   if (t0 == 0 && p.last != nullptr) {
     T* last = static_cast<T*>(p.last) + (int64_t)b * (K - 1) * p.E + e;
@@ -138,7 +148,6 @@ __global__ void __launch_bounds__(32 * kWarps) conv_fwd_kernel(const ConvParams 
       ln.ch.store(last + (int64_t)k * p.E, v);
     }
   }
-  const int t1 = min(t0 + p.run, p.L);
   if (t0 >= t1) return;
   T* y = static_cast<T*>(p.y) + (int64_t)b * p.yb + e;
   f2 win[K][NV];
@@ -148,24 +157,18 @@ __global__ void __launch_bounds__(32 * kWarps) conv_fwd_kernel(const ConvParams 
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) ln.row(t0 - (K - 1) + k, win[k + 1]);
   }
-  constexpr int U = 8;
-  const int end = min(t1, n);
 #pragma unroll 1
   for (int t = t0; t < end; t += U) {
-    RawRow<T, NV> in[U];
-    if (t + U <= end) {
+    RawRow<T, NV> now[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) in[u] = ln.ch.load(ln.x + (int64_t)(t + u) * p.xl);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) in[u] = ln.ch.load(ln.x + (int64_t)min(t + u, end - 1) * p.xl);
-    }
+    for (int u = 0; u < U; ++u) now[u] = in[u];
+    if (t + U < end) fetch(t + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (t + u < end) {
         f2 v[NV];
         shift(win);
-        values<T, NV>(in[u], win[K - 1]);
+        values<T, NV>(now[u], win[K - 1]);
         ln.pre(win, v);
         if (p.silu) {
 #pragma unroll
@@ -257,15 +260,25 @@ __global__ void __launch_bounds__(32 * kWarps) conv_bwd_kernel(const ConvParams 
       for (int k = 0; k < K - 1; ++k) ln.row(t0 - (K - 1) + k, win[k + 1]);
       constexpr int U = 4;
       const int ahead = min(end + K - 1, n);  // rows whose d this run needs
+      RawRow<T, NV> xn[U], dn[U];             // the next rows, on their way while those before them are worked on
+      auto fetch = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t r = min(t + u, ahead - 1);
+          xn[u] = ln.ch.load(ln.x + r * p.xl);
+          dn[u] = ln.ch.load(dy + r * g.dyl);
+        }
+      };
+      fetch(t0);
 #pragma unroll 1
       for (int t = t0; t < end + K - 1; t += U) {
         RawRow<T, NV> in[U], din[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int64_t r = min(t + u, ahead - 1);
-          in[u] = ln.ch.load(ln.x + r * p.xl);
-          din[u] = ln.ch.load(dy + r * g.dyl);
+          in[u] = xn[u];
+          din[u] = dn[u];
         }
+        if (t + U < ahead) fetch(t + U);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           shift(win);

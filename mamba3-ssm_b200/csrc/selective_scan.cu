@@ -436,7 +436,7 @@ static int sel_lanes(int np) { return std::max(2, np / 4); }
 int sel_pieces(const SelScanParams& p, int lanes, int sms, int* chunk) {
   const int64_t warps = (int64_t)p.batch * p.E * lanes / 32 + 1, want = (int64_t)sms * 16;
   int n = 1;
-  if (warps * 4 <= want) n = (int)std::min<int64_t>(want / warps, (p.L + 4 * kSelTile - 1) / (4 * kSelTile));
+  if (warps * 4 <= want) n = (int)std::min<int64_t>(want / warps, p.L / (8 * kSelTile));
   n = std::max(1, std::min(n, 4096));
   int64_t len = (p.L + n - 1) / n;
   len = (len + kSelTile - 1) / kSelTile * kSelTile;

@@ -245,6 +245,26 @@ def rec3(t, code, a, b, c):
     return (t.data_ptr() or 1, code, 3, a, b, c, 0, 0, 0, *t.stride(), 0, 0, 0)
 
 
+def rec1(t, code, a):
+    return (t.data_ptr() or 1, code, 1, a, 0, 0, 0, 0, 0, *t.stride(), 0, 0, 0, 0, 0)
+
+
+def rec4(t, code, a, b, c, d):
+    return (t.data_ptr() or 1, code, 4, a, b, c, d, 0, 0, *t.stride(), 0, 0)
+
+
+def rec4_of3(t, code, a, b, d):
+    """The record of a three-dimensional (a, b, d) tensor as (a, b, 1, d)."""
+    s = t.stride()
+    return (t.data_ptr() or 1, code, 4, a, b, 1, d, 0, 0, s[0], s[1], d, s[2], 0, 0)
+
+
+def rec3_of2(t, code, a, d):
+    """The record of a two-dimensional (a, d) tensor as (a, 1, d)."""
+    s = t.stride()
+    return (t.data_ptr() or 1, code, 3, a, 1, d, 0, 0, 0, s[0], d, s[1], 0, 0, 0)
+
+
 def rec0(ptr, code):
     """The record of one value at an address."""
     return (ptr, code, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)

@@ -101,19 +101,23 @@ def _flat(states):
     return [t for s in states for t in ((s,) if isinstance(s, torch.Tensor) else _flat(s))]
 
 
-def _pitches(what, ts, rows, device):
-    """Addresses and row pitches in bytes; each tensor has that many rows, each row dense."""
-    pitches = []
+def _pitches(what, ts, rows, index):
+    """Addresses, row pitches and row sizes in bytes; each tensor has that many rows, each row dense."""
+    if not all([t.get_device() == index for t in ts]):
+        raise RuntimeError(f"reorder_states_: {what} must be CUDA tensors of the parents' device (no CPU path)")
+    pitches, sizes = [], []
     for t in ts:
-        if t.get_device() != device.index:
-            raise RuntimeError(f"reorder_states_: {what} must be CUDA tensors of the parents' device (no CPU path)")
-        if t.dim() == 0 or t.shape[0] != rows:
-            raise ValueError(f"reorder_states_: {what} of {rows} rows expected, got {tuple(t.shape)}")
-        if not t.is_contiguous() and t.numel() and not t[0].is_contiguous():
+        shape = t.shape
+        if not shape or shape[0] != rows:
+            raise ValueError(f"reorder_states_: {what} of {rows} rows expected, got {tuple(shape)}")
+        n = t.numel()
+        if not t.is_contiguous() and n and not t[0].is_contiguous():
             raise ValueError(f"reorder_states_: rows of {what} must be dense in memory, got strides {t.stride()} for "
-                             f"{tuple(t.shape)}")
-        pitches.append(t.stride(0) * t.element_size())
-    return [t.data_ptr() for t in ts], pitches
+                             f"{tuple(shape)}")
+        es = t.element_size()
+        pitches.append(t.stride(0) * es)
+        sizes.append(n // rows * es if rows else 0)
+    return [t.data_ptr() for t in ts], pitches, sizes
 
 
 def reorder_states_(states, parents, *, out=None):
@@ -139,12 +143,12 @@ def reorder_states_(states, parents, *, out=None):
     given = out if out is not None else states
     if not n:
         return given
-    if src[0].dim() == 0 or (batch and src[0].shape[0] % batch):
-        raise ValueError(f"{name}: states of {tuple(src[0].shape)} for a batch of {batch}")
-    source = src[0].shape[0] // batch if batch else 0
+    first = src[0].shape
+    if not first or (batch and first[0] % batch):
+        raise ValueError(f"{name}: states of {tuple(first)} for a batch of {batch}")
+    source = first[0] // batch if batch else 0
     dev = parents.device
-    ptrs, pitch = _pitches("states", src, source * batch, dev)
-    size = [t.numel() // t.shape[0] * t.element_size() if t.shape[0] else 0 for t in src]
+    ptrs, pitch, size = _pitches("states", src, source * batch, dev.index)
     dst = src
     if out is None:
         if source != rows:
@@ -156,13 +160,13 @@ def reorder_states_(states, parents, *, out=None):
         dst = _flat(out)
         if len(dst) != n:
             raise ValueError(f"{name}: {n} states but {len(dst)} outputs")
-        outs, opitch = _pitches("out", dst, rows * batch, dev)
+        outs, opitch, osize = _pitches("out", dst, rows * batch, dev.index)
         for t, o in zip(src, dst):
             if t.shape[1:] != o.shape[1:] or t.dtype is not o.dtype:
                 raise ValueError(f"{name}: output of rows {tuple(o.shape[1:])} {o.dtype} for rows {tuple(t.shape[1:])} {t.dtype}")
         if not source:
-            size = [o.numel() // o.shape[0] * o.element_size() if o.shape[0] else 0 for o in dst]
-    if torch.is_grad_enabled() and any([t.requires_grad for t in src] + [t.requires_grad for t in dst]):
+            size = osize
+    if torch.is_grad_enabled() and (any([t.requires_grad for t in src]) or (out is not None and any([t.requires_grad for t in dst]))):
         raise RuntimeError(f"{name}: works without gradients; call it under torch.no_grad()")
     lib = L.load()
     # one block of host memory: addresses, row sizes and pitches

@@ -30,36 +30,46 @@ __all__ = ["causal_conv", "causal_conv_step_", "ssm_scan_selective", "ssm_step_s
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _check(name, main, **others):
+_CODE = L._DTYPE_CODE
+_F32 = torch.float32
+
+
+def _check(name, what, t, names, others):
     """Dtype of the main operand; one CUDA device for all that are given; no forward-mode tangents."""
-    what, t = main
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: {what} must be a tensor")
-    _require_cuda(name, t)
+    if not t.is_cuda:
+        _require_cuda(name, t)
     if t.dtype not in _FLOATS:
         raise TypeError(f"{name}: {what} must be float32, bfloat16 or float16, got {t.dtype}")
     at = t.get_device()
-    for k, v in others.items():
-        if v is not None:
-            if not isinstance(v, torch.Tensor):
+    try:
+        same = all([v is None or v.get_device() == at for v in others])
+    except AttributeError:
+        same = False
+    if not same:
+        for k, v in zip(names, others):
+            if v is not None and not isinstance(v, torch.Tensor):
                 raise TypeError(f"{name}: {k} must be a tensor")
-            if v.get_device() != at:
+            if v is not None and v.get_device() != at:
                 raise RuntimeError(f"{name}: {k} is on {v.device}, {what} on {t.device}")
     if getattr(forward_ad, "_current_level", 0) >= 0:
-        for k, v in (main, *others.items()):
+        for k, v in ((what, t), *zip(names, others)):
             if v is not None and forward_ad.unpack_dual(v).tangent is not None:
                 raise NotImplementedError(f"{name}: no forward-mode derivative, but {k} carries a tangent")
 
 
-def _shape(name, what, t, *shape):
-    if t is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name}: {what} of shape {tuple(t.shape)}, expected {shape}")
+def _shape(name, what, t, shape):
+    if t is not None and t.shape != shape:
+        raise ValueError(f"{name}: {what} of shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _silu(name, activation):
-    if activation not in (None, "silu"):
+    if activation is None:
+        return 0
+    if activation != "silu":
         raise ValueError(f"{name}: activation is None or 'silu', got {activation!r}")
-    return int(activation == "silu")
+    return 1
 
 
 def _lengths(name, lengths, batch):
@@ -67,12 +77,32 @@ def _lengths(name, lengths, batch):
         return None
     if lengths.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{name}: lengths must be int64 or int32, got {lengths.dtype}")
-    _shape(name, "lengths", lengths, batch)
-    return lengths.long().contiguous()
+    _shape(name, "lengths", lengths, (batch,))
+    return _dense(lengths if lengths.dtype is torch.int64 else lengths.long())
 
 
-def _no_grad_only(name, *ts):
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in ts]):
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _param(t):
+    """A parameter of the channels as the kernels read it: fp32, contiguous."""
+    if t is None:
+        return None
+    return _dense(t if t.dtype is _F32 else t.float())
+
+
+def _needs_grad(ts):
+    if not torch.is_grad_enabled():
+        return False
+    for t in ts:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def _no_grad_only(name, ts):
+    if _needs_grad(ts):
         raise RuntimeError(f"{name}: works in place, without gradients; call it under torch.no_grad()")
 
 
@@ -81,26 +111,47 @@ def _written(t):
         torch.autograd.graph.increment_version(t)
 
 
-def _needs_grad(*ts):
-    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in ts])
+# Records of the operands (see _lib.Records), for which the shapes are known by then: a call has up to two
+# dozen operands, and finding out each one's shape again would cost more than the launches.
+def _r1(t, a):
+    return L.NO_RECORD if t is None else L.rec1(t, _CODE[t.dtype], a)
 
 
-def _new(t, *shape, dtype=None):
-    return torch.empty(shape, dtype=dtype or t.dtype, device=t.device)
+def _r2(t, a, b):
+    return L.NO_RECORD if t is None else L.rec2(t, _CODE[t.dtype], a, b)
+
+
+def _r3(t, a, b, c):
+    return L.NO_RECORD if t is None else L.rec3(t, _CODE[t.dtype], a, b, c)
+
+
+def _at(base, vals, i):
+    """Address of record i, None where its operand is absent."""
+    return base + 112 * i if vals[15 * i] else None
 
 
 # ------------------------------------------------------------------------------------------
 # convolution
 # ------------------------------------------------------------------------------------------
+def _conv_vals(x, weight, bias, initial, lengths, b, n, e, k):
+    return [*_r3(x, b, n, e), *_r2(weight, e, k), *_r1(bias, e), *_r3(initial, b, k - 1, e), *_r1(lengths, b)]
+
+
 def _conv_forward(x, weight, bias, initial, lengths, silu, want):
     b, n, e = x.shape
-    y = _new(x, b, n, e)
-    last = _new(x, b, weight.shape[1] - 1, e) if want else None
-    a = L.pack(x, weight, bias, initial, lengths, y, last)
-    p = a.ptrs
-    with L.on_device(x.device):
-        rc = L.load().m3_causal_conv(p[0], p[1], p[2], p[3], p[4], silu, p[5], p[6], L.stream_ptr(x.device))
-    L.check(rc, "m3_causal_conv")
+    k = weight.shape[1]
+    dev = x.device
+    y = torch.empty((b, n, e), dtype=x.dtype, device=dev)
+    last = torch.empty((b, k - 1, e), dtype=x.dtype, device=dev) if want else None
+    vals = _conv_vals(x, weight, bias, initial, lengths, b, n, e, k)
+    vals += _r3(y, b, n, e)
+    vals += _r3(last, b, k - 1, e)
+    a = L.Records(vals)
+    p = [_at(a.base, vals, i) for i in range(7)]
+    with L.on_device(dev):
+        rc = L.load().m3_causal_conv(p[0], p[1], p[2], p[3], p[4], silu, p[5], p[6], L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "m3_causal_conv")
     return y, last
 
 
@@ -119,20 +170,28 @@ class _CausalConvFn(torch.autograd.Function):
         if dy is None and dlast is None:
             return (None,) * 7
         b, n, e = x.shape
-        dy = torch.zeros_like(x) if dy is None else _inner(dy)
+        k = weight.shape[1]
+        dev = x.device
+        dy = torch.zeros((b, n, e), dtype=x.dtype, device=dev) if dy is None else _inner(dy)
         dlast = None if dlast is None else _inner(dlast)
-        dx = _new(x, b, n, e)
-        dw = _new(weight, *weight.shape)
-        db = None if bias is None else _new(bias, e)
-        di = _new(x, *initial.shape) if initial is not None and ctx.needs_input_grad[3] else None
+        dx = torch.empty_like(x)
+        dw = torch.empty((e, k), dtype=weight.dtype, device=dev)
+        db = None if bias is None else torch.empty_like(bias)
+        di = None
+        if initial is not None and ctx.needs_input_grad[3]:
+            di = torch.empty((b, k - 1, e), dtype=x.dtype, device=dev)
+        vals = _conv_vals(x, weight, bias, initial, lengths, b, n, e, k)
+        vals += (*_r3(dy, b, n, e), *_r3(dlast, b, k - 1, e), *_r3(dx, b, n, e), *_r2(dw, e, k), *_r1(db, e),
+                 *_r3(di, b, k - 1, e))
+        a = L.Records(vals)
+        p = [_at(a.base, vals, i) for i in range(11)]
         lib = L.load()
-        nbytes = lib.m3_causal_conv_bwd_workspace_size(b, n, e, weight.shape[1])
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        p = (a := L.pack(x, weight, bias, initial, lengths, dy, dlast, dx, dw, db, di)).ptrs
-        with L.on_device(x.device):
-            rc = lib.m3_causal_conv_bwd(*p[:5], ctx.silu, *p[5:], ws.data_ptr(), nbytes, L.stream_ptr(x.device))
-        L.check(rc, "m3_causal_conv_bwd")
-        del a
+        with L.on_device(dev):
+            nbytes = lib.m3_causal_conv_bwd_workspace_size(b, n, e, k)
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            rc = lib.m3_causal_conv_bwd(*p[:5], ctx.silu, *p[5:], ws.data_ptr(), nbytes, L.stream_ptr(dev))
+        if rc:
+            L.check(rc, "m3_causal_conv_bwd")
         return dx, dw, db, di, None, None, None
 
 
@@ -141,12 +200,12 @@ def _conv_weights(name, x, weight, bias, e):
         raise ValueError(f"{name}: weight of shape {tuple(weight.shape)}, expected ({e}, taps)")
     if not 2 <= weight.shape[1] <= 4:
         raise ValueError(f"{name}: 2, 3 or 4 taps, got {weight.shape[1]}")
-    _shape(name, "bias", bias, e)
-    if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
+    _shape(name, "bias", bias, (e,))
+    if weight.dtype is not x.dtype and weight.dtype is not _F32:
         weight = weight.float()
     if bias is not None and bias.dtype is not weight.dtype:
         bias = bias.to(weight.dtype)
-    return _inner(weight), bias if bias is None else bias.contiguous()
+    return _inner(weight), _dense(bias)
 
 
 def causal_conv(x, weight, bias=None, *, activation=None, initial_state=None, lengths=None, return_state=False):
@@ -158,19 +217,19 @@ def causal_conv(x, weight, bias=None, *, activation=None, initial_state=None, le
     (zeros without it). With ``return_state`` returns (y, state), the last K - 1 rows in that layout: the
     initial state of a following piece, or the state of ``causal_conv_step_``. ``lengths``: see above."""
     name = "causal_conv"
-    _check(name, ("x", x), weight=weight, bias=bias, initial_state=initial_state, lengths=lengths)
+    _check(name, "x", x, ("weight", "bias", "initial_state", "lengths"), (weight, bias, initial_state, lengths))
     if x.dim() != 3:
         raise ValueError(f"{name}: x is (batch, length, channels), got {tuple(x.shape)}")
     b, _, e = x.shape
     silu = _silu(name, activation)
     weight, bias = _conv_weights(name, x, weight, bias, e)
     if initial_state is not None:
-        _shape(name, "initial_state", initial_state, b, weight.shape[1] - 1, e)
+        _shape(name, "initial_state", initial_state, (b, weight.shape[1] - 1, e))
         if initial_state.dtype is not x.dtype:
             raise TypeError(f"{name}: initial_state must be of x's dtype {x.dtype}, got {initial_state.dtype}")
         initial_state = _inner(initial_state)
     args = (_inner(x), weight, bias, initial_state, _lengths(name, lengths, b), silu, bool(return_state))
-    y, last = (_CausalConvFn.apply if _needs_grad(x, weight, bias, initial_state) else _conv_forward)(*args)
+    y, last = (_CausalConvFn.apply if _needs_grad(args[:4]) else _conv_forward)(*args)
     return (y, last) if return_state else y
 
 
@@ -178,23 +237,28 @@ def causal_conv_step_(state, x, weight, bias=None, *, activation=None):
     """``causal_conv`` for one more row x (batch, channels): returns y (batch, channels) and moves
     ``state`` (batch, K - 1, channels, x's dtype) on by one row, in place. Without gradients."""
     name = "causal_conv_step_"
-    _check(name, ("x", x), state=state, weight=weight, bias=bias)
+    _check(name, "x", x, ("state", "weight", "bias"), (state, weight, bias))
     if x.dim() != 2:
         raise ValueError(f"{name}: x is (batch, channels), got {tuple(x.shape)}")
-    _no_grad_only(name, x, state, weight, bias)
+    _no_grad_only(name, (x, state, weight, bias))
     b, e = x.shape
     silu = _silu(name, activation)
     weight, bias = _conv_weights(name, x, weight, bias, e)
-    _shape(name, "state", state, b, weight.shape[1] - 1, e)
+    k = weight.shape[1]
+    _shape(name, "state", state, (b, k - 1, e))
     if state.dtype is not x.dtype:
         raise TypeError(f"{name}: state must be of x's dtype {x.dtype}, got {state.dtype}")
     x = _inner(x)
-    y = _new(x, b, e)
-    p = (a := L.pack(state, x, weight, bias, y)).ptrs
-    with L.on_device(x.device):
-        rc = L.load().m3_causal_conv_step(*p[:4], silu, p[4], L.stream_ptr(x.device))
-    L.check(rc, "m3_causal_conv_step")
-    del a
+    dev = x.device
+    y = torch.empty((b, e), dtype=x.dtype, device=dev)
+    vals = [*_r3(state, b, k - 1, e), *_r2(x, b, e), *_r2(weight, e, k), *_r1(bias, e), *_r2(y, b, e)]
+    a = L.Records(vals)
+    at = a.base
+    with L.on_device(dev):
+        rc = L.load().m3_causal_conv_step(at, at + 112, at + 224, None if bias is None else at + 336, silu, at + 448,
+                                          L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "m3_causal_conv_step")
     _written(state)
     return y
 
@@ -202,22 +266,43 @@ def causal_conv_step_(state, x, weight, bias=None, *, activation=None):
 # ------------------------------------------------------------------------------------------
 # scan
 # ------------------------------------------------------------------------------------------
+def _scan_vals(u, delta, A, B, C, D, z, bias, initial, lengths, b, n, e, m):
+    vals = [*_r3(u, b, n, e), *_r3(delta, b, n, e), *_r2(A, e, m)]
+    code = _CODE[B.dtype]
+    if B.dim() == 3:  # one group
+        vals += (*L.rec4_of3(B, code, b, n, m), *L.rec4_of3(C, code, b, n, m))
+    else:
+        g = B.shape[2]
+        vals += (*L.rec4(B, code, b, n, g, m), *L.rec4(C, code, b, n, g, m))
+    vals += (*_r1(D, e), *_r3(z, b, n, e), *_r1(bias, e), *_r3(initial, b, e, m), *_r1(lengths, b))
+    return vals
+
+
+def _groups(B):
+    return 1 if B.dim() == 3 else B.shape[2]
+
+
 def _scan_forward(u, delta, A, B, C, D, z, bias, initial, lengths, softplus, want, keep=False):
     b, n, e = u.shape
     m = A.shape[1]
+    dev = u.device
     lib = L.load()
-    y = _new(u, b, n, e)
-    last = _new(u, b, e, m, dtype=torch.float32) if want else None
-    with L.on_device(u.device):
-        nws = lib.m3_selective_scan_workspace_size(b, n, e, m, B.shape[2])
+    y = torch.empty((b, n, e), dtype=u.dtype, device=dev)
+    last = torch.empty((b, e, m), dtype=_F32, device=dev) if want else None
+    vals = _scan_vals(u, delta, A, B, C, D, z, bias, initial, lengths, b, n, e, m)
+    vals += _r3(y, b, n, e)
+    vals += _r3(last, b, e, m)
+    a = L.Records(vals)
+    p = [_at(a.base, vals, i) for i in range(12)]
+    with L.on_device(dev):
+        nws = lib.m3_selective_scan_workspace_size(b, n, e, m, _groups(B))
         nst = lib.m3_selective_scan_states_size(b, n, e, m) if keep else 0
-        ws = torch.empty(nws, dtype=torch.uint8, device=u.device) if nws else None
-        states = torch.empty(nst, dtype=torch.uint8, device=u.device) if keep else None
-        p = (a := L.pack(u, delta, A, B, C, D, z, bias, initial, lengths, y, last)).ptrs
+        ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws else None
+        states = torch.empty((nst,), dtype=torch.uint8, device=dev) if keep else None
         rc = lib.m3_selective_scan(*p[:10], softplus, *p[10:], states.data_ptr() if nst else None, nst,
-                                   ws.data_ptr() if nws else None, nws, L.stream_ptr(u.device))
-    L.check(rc, "m3_selective_scan")
-    del a
+                                   ws.data_ptr() if nws else None, nws, L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "m3_selective_scan")
     return (y, last, states) if keep else (y, last)
 
 
@@ -238,57 +323,70 @@ class _SelectiveScanFn(torch.autograd.Function):
         if dy is None and dlast is None:
             return (None,) * 12
         b, n, e = u.shape
+        m = A.shape[1]
+        g = _groups(B)
+        dev, empty = u.device, torch.empty
+        dy = torch.zeros((b, n, e), dtype=u.dtype, device=dev) if dy is None else _inner(dy)
+        dlast = _dense(dlast)
+        # (empty_like costs half of empty; it keeps the order of the dimensions in memory, which B's and C's gradients may not)
+        like = torch.empty_like
+        du, ddelta, dA = like(u), like(delta), like(A)
+        dB = like(B) if B.is_contiguous() else empty(B.shape, dtype=B.dtype, device=dev)
+        dC = like(C) if C.is_contiguous() else empty(B.shape, dtype=B.dtype, device=dev)
+        dD = None if D is None else like(D)
+        dz = None if z is None else like(z)
+        dbias = None if bias is None else like(bias)
+        di = empty((b, e, m), dtype=_F32, device=dev) if initial is not None and ctx.needs_input_grad[8] else None
+        vals = _scan_vals(u, delta, A, B, C, D, z, bias, initial, lengths, b, n, e, m)
+        code = _CODE[B.dtype]
+        vals += (*_r3(dy, b, n, e), *_r3(dlast, b, e, m), *_r3(du, b, n, e), *_r3(ddelta, b, n, e), *_r2(dA, e, m))
+        if B.dim() == 3:
+            vals += (*L.rec4_of3(dB, code, b, n, m), *L.rec4_of3(dC, code, b, n, m))
+        else:
+            vals += (*L.rec4(dB, code, b, n, g, m), *L.rec4(dC, code, b, n, g, m))
+        vals += (*_r1(dD, e), *_r3(dz, b, n, e), *_r1(dbias, e), *_r3(di, b, e, m))
+        a = L.Records(vals)
+        p = [_at(a.base, vals, i) for i in range(21)]
         lib = L.load()
-        dy = torch.zeros_like(u) if dy is None else _inner(dy)
-        dlast = None if dlast is None else dlast.contiguous()
-        du, ddelta = _new(u, b, n, e), _new(delta, b, n, e)
-        dA, dB, dC = _new(A, *A.shape), _new(B, *B.shape), _new(C, *C.shape)
-        dD = None if D is None else _new(D, e)
-        dz = None if z is None else _new(z, b, n, e)
-        dbias = None if bias is None else _new(bias, e)
-        di = _new(A, *initial.shape) if initial is not None and ctx.needs_input_grad[8] else None
-        with L.on_device(u.device):
-            nws = lib.m3_selective_scan_bwd_workspace_size(b, n, e, A.shape[1], B.shape[2])
-            ws = torch.empty(nws, dtype=torch.uint8, device=u.device)
-            p = (a := L.pack(u, delta, A, B, C, D, z, bias, initial, lengths, dy, dlast, du, ddelta, dA, dB, dC, dD, dz,
-                             dbias, di)).ptrs
+        with L.on_device(dev):
+            nws = lib.m3_selective_scan_bwd_workspace_size(b, n, e, m, g)
+            ws = empty((nws,), dtype=torch.uint8, device=dev)
             rc = lib.m3_selective_scan_bwd(*p[:10], ctx.softplus, *p[10:], states.data_ptr() or None, states.numel(),
-                                           ws.data_ptr() or None, nws, L.stream_ptr(u.device))
-        L.check(rc, "m3_selective_scan_bwd")
-        del a
+                                           ws.data_ptr() or None, nws, L.stream_ptr(dev))
+        if rc:
+            L.check(rc, "m3_selective_scan_bwd")
         return du, ddelta, dA, dB, dC, dD, dz, dbias, di, None, None, None
 
 
 def _scan_operands(name, u, delta, A, B, C, D, z, bias, lead):
-    """The operands in the layouts and dtypes of the kernels, B and C as (..., groups, states)."""
-    e = u.shape[-1]
-    if A.dim() != 2 or A.shape[0] != e or A.shape[1] == 0:
-        raise ValueError(f"{name}: A of shape {tuple(A.shape)}, expected ({e}, states)")
-    m = A.shape[1]
+    """The operands in the layouts and dtypes of the kernels."""
+    shape, an, bs = u.shape, A.shape, B.shape
+    e = shape[-1]
+    if len(an) != 2 or an[0] != e or an[1] == 0:
+        raise ValueError(f"{name}: A of shape {tuple(an)}, expected ({e}, states)")
+    m = an[1]
     if m > 128:
         raise ValueError(f"{name}: at most 128 states a channel, got {m}")
-    _shape(name, "delta", delta, *u.shape)
-    _shape(name, "z", z, *u.shape)
-    _shape(name, "D", D, e)
-    _shape(name, "delta_bias", bias, e)
-    if B.dim() == len(lead) + 1:
-        B = B.unsqueeze(-2)
-    if C.dim() == len(lead) + 1:
-        C = C.unsqueeze(-2)
-    if B.dim() != len(lead) + 2 or B.shape[:-2] != lead or B.shape[-1] != m or C.shape != B.shape:
-        raise ValueError(f"{name}: B and C are {(*lead, m)} or {(*lead, 'groups', m)}, got {tuple(B.shape)} and "
+    if delta.shape != shape:
+        _shape(name, "delta", delta, shape)
+    if z is not None and z.shape != shape:
+        _shape(name, "z", z, shape)
+    _shape(name, "D", D, (e,))
+    _shape(name, "delta_bias", bias, (e,))
+    if bs != (*lead, m) and (len(bs) != len(lead) + 2 or bs[:-2] != lead or bs[-1] != m) or C.shape != bs:
+        raise ValueError(f"{name}: B and C are {(*lead, m)} or {(*lead, 'groups', m)}, got {tuple(bs)} and "
                          f"{tuple(C.shape)}")
-    if B.shape[-2] == 0 or e % B.shape[-2]:
-        raise ValueError(f"{name}: {e} channels do not divide into {B.shape[-2]} groups")
+    if len(bs) > len(lead) + 1 and (bs[-2] == 0 or e % bs[-2]):
+        raise ValueError(f"{name}: {e} channels do not divide into {bs[-2]} groups")
     if z is not None and z.dtype is not u.dtype:
         raise TypeError(f"{name}: z must be of u's dtype {u.dtype}, got {z.dtype}")
-    if delta.dtype is not u.dtype and delta.dtype is not torch.float32:
+    dtype, dd, bd = u.dtype, delta.dtype, B.dtype
+    if dd is not dtype and dd is not _F32:
         delta = delta.float()
-    if B.dtype is not C.dtype or (B.dtype is not u.dtype and B.dtype is not torch.float32):
+    if bd is not C.dtype or (bd is not dtype and bd is not _F32):
         B, C = B.float(), C.float()
-    return (_inner(u), _inner(delta), A.float().contiguous(), _inner(B), _inner(C),
-            None if D is None else D.float().contiguous(), None if z is None else _inner(z),
-            None if bias is None else bias.float().contiguous())
+    return (_inner(u), _inner(delta), _param(A), _inner(B), _inner(C), _param(D), None if z is None else _inner(z),
+            _param(bias))
 
 
 def ssm_scan_selective(u, delta, A, B_proj, C_proj, D=None, *, z=None, delta_bias=None, delta_softplus=True,
@@ -308,17 +406,17 @@ def ssm_scan_selective(u, delta, A, B_proj, C_proj, D=None, *, z=None, delta_bia
     initial state of a following piece, or the state of ``ssm_step_selective_``. ``lengths``: see above.
     For the backward the call keeps the state in front of every eighth position."""
     name = "ssm_scan_selective"
-    _check(name, ("u", u), delta=delta, A=A, B_proj=B_proj, C_proj=C_proj, D=D, z=z, delta_bias=delta_bias,
-           initial_state=initial_state, lengths=lengths)
+    _check(name, "u", u, ("delta", "A", "B_proj", "C_proj", "D", "z", "delta_bias", "initial_state", "lengths"),
+           (delta, A, B_proj, C_proj, D, z, delta_bias, initial_state, lengths))
     if u.dim() != 3:
         raise ValueError(f"{name}: u is (batch, length, channels), got {tuple(u.shape)}")
-    b, _, e = u.shape
     ops = _scan_operands(name, u, delta, A, B_proj, C_proj, D, z, delta_bias, u.shape[:2])
+    b, _, e = u.shape
     if initial_state is not None:
-        _shape(name, "initial_state", initial_state, b, e, A.shape[1])
-        initial_state = initial_state.float().contiguous()
-    args = (*ops, initial_state, _lengths(name, lengths, b), int(bool(delta_softplus)), bool(return_state))
-    y, last = (_SelectiveScanFn.apply if _needs_grad(*ops, initial_state) else _scan_forward)(*args)
+        _shape(name, "initial_state", initial_state, (b, e, A.shape[1]))
+        initial_state = _param(initial_state)
+    args = (*ops, initial_state, _lengths(name, lengths, b), 1 if delta_softplus else 0, bool(return_state))
+    y, last = (_SelectiveScanFn.apply if _needs_grad(args[:9]) else _scan_forward)(*args)
     return (y, last) if return_state else y
 
 
@@ -327,20 +425,32 @@ def ssm_step_selective_(state, u, delta, A, B_proj, C_proj, D=None, *, z=None, d
     (batch, states) or (batch, groups, states). Returns y (batch, channels) and updates ``state``
     (batch, channels, states) fp32 in place. Without gradients."""
     name = "ssm_step_selective_"
-    _check(name, ("u", u), state=state, delta=delta, A=A, B_proj=B_proj, C_proj=C_proj, D=D, z=z, delta_bias=delta_bias)
+    given = (state, u, delta, A, B_proj, C_proj, D, z, delta_bias)
+    _check(name, "u", u, ("state", "u", "delta", "A", "B_proj", "C_proj", "D", "z", "delta_bias"), given)
     if u.dim() != 2:
         raise ValueError(f"{name}: u is (batch, channels), got {tuple(u.shape)}")
-    _no_grad_only(name, state, u, delta, A, B_proj, C_proj, D, z, delta_bias)
+    _no_grad_only(name, given)
+    u, delta, A, B, C, D, z, bias = _scan_operands(name, u, delta, A, B_proj, C_proj, D, z, delta_bias, u.shape[:1])
     b, e = u.shape
-    ops = _scan_operands(name, u, delta, A, B_proj, C_proj, D, z, delta_bias, u.shape[:1])
-    _shape(name, "state", state, b, e, A.shape[1])
-    if state.dtype is not torch.float32:
+    m = A.shape[1]
+    _shape(name, "state", state, (b, e, m))
+    if state.dtype is not _F32:
         raise TypeError(f"{name}: state must be float32, got {state.dtype}")
-    y = _new(u, b, e)
-    p = (a := L.pack(state, *ops, y)).ptrs
-    with L.on_device(u.device):
-        rc = L.load().m3_selective_step(*p[:9], int(bool(delta_softplus)), p[9], L.stream_ptr(u.device))
-    L.check(rc, "m3_selective_step")
-    del a
+    dev = u.device
+    y = torch.empty((b, e), dtype=u.dtype, device=dev)
+    code = _CODE[B.dtype]
+    vals = [*_r3(state, b, e, m), *_r2(u, b, e), *_r2(delta, b, e), *_r2(A, e, m)]
+    if B.dim() == 2:  # one group
+        vals += (*L.rec3_of2(B, code, b, m), *L.rec3_of2(C, code, b, m))
+    else:
+        g = B.shape[1]
+        vals += (*L.rec3(B, code, b, g, m), *L.rec3(C, code, b, g, m))
+    vals += (*_r1(D, e), *_r2(z, b, e), *_r1(bias, e), *_r2(y, b, e))
+    a = L.Records(vals)
+    p = [_at(a.base, vals, i) for i in range(10)]
+    with L.on_device(dev):
+        rc = L.load().m3_selective_step(*p[:9], 1 if delta_softplus else 0, p[9], L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "m3_selective_step")
     _written(state)
     return y

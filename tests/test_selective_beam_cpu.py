@@ -144,7 +144,9 @@ def test_convolution_refusals(lib):
     _says(lib, step((2, 0), (2, 2, 0)), 1, b"state: shape")
     assert step((2, 0), (2, 3, 0)) == 0
     assert lib.m3_causal_conv_bwd_workspace_size(2, 100, 8, 5) == 0
-    assert lib.m3_causal_conv_bwd_workspace_size(2, 128, 8, 4) == 2 * 8 * 5 * 4
+    # parts of (taps + 1, channels) floats for every sequence: a whole number of them, more for a long one
+    sizes = [lib.m3_causal_conv_bwd_workspace_size(2, n, 8, 4) for n in (0, 64, 65, 100000)]
+    assert all(v > 0 and v % (2 * 8 * 5 * 4) == 0 for v in sizes) and sizes[0] == sizes[1] < sizes[2] < sizes[3]
 
 
 def test_scan_refusals(lib):
