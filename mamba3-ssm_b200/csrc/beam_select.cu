@@ -4,29 +4,24 @@
 // are, offers -inf; one with a NaN or an infinite logit or score offers NaN, which ranks first.
 // beam_rows_kernel reads the logits once: a CTA a part of a row keeps its largest element and the sum of
 // exponentials (32 bits a thread, joined in 64) and the part's `num` largest elements. Those pass a
-// threshold: the num-th largest of the threads' own maxima of the first tile, so that later tiles are mostly
-// dismissed by one comparison a vector. Keys are unique (value, then the lower index), so a
-// tile passes at most num threads' elements whatever the logits are. beam_join_kernel, a CTA a prompt,
+// threshold, at first the num-th largest of the maxima of groups of threads, which rises whenever the list of those that
+// passed has grown, so that later tiles are mostly dismissed by one comparison a vector. Where more pass than the list
+// holds (rising or equal logits), the rest of the tile waits for the risen threshold; keys are unique (value, then the
+// lower index), so that each look lists a full list's worth of them. beam_join_kernel, a CTA a prompt,
 // joins the sums in 64 bits and ranks the parts' elements by their score in 64 bits.
 // Bound by the memory where there are many rows, by latency where there are few.
 #include <algorithm>
 
 #include "beam.cuh"
 #include "m3_common.cuh"
+#include "pairs.cuh"
 
 namespace m3 {
 namespace {
 
 constexpr int NT = 256;
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct Part { double sum; float max; int n; };  // of a row's part: sum of exp(l - max), and listed elements
-
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // floats in the order of unsigned integers; -0 counts as +0
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -48,25 +43,30 @@ __device__ __forceinline__ double unordered64(uint64_t k) {
   return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
 }
 
+constexpr int kGroups = NT / 4;  // threads whose largest elements give the first threshold
+static_assert(kGroups >= kMaxCandidates, "the first threshold is the num-th largest of the groups' maxima");
+
 template <typename T, int U>
 struct Rows {
   static constexpr int VN = 16 / sizeof(T), TILE = NT * U * VN;
-  static constexpr int CAP = kMaxCandidates * U * VN + kMaxCandidates;
-  uint64_t list[CAP], best[kMaxCandidates], thread_max[NT];
+  static constexpr int CAP = 1024;  // listed elements; more of a tile wait until the threshold has risen
+  uint64_t list[CAP], best[kMaxCandidates];
+  uint32_t group[kGroups];
   double sum[NT / 32];
   float max[NT / 32];
-  int total, n;
-  uint64_t tau;
+  int n;
+  uint64_t tau;  // keys above it pass
 };
 
-// Keeps the `num` largest keys of the list, in order, and the last of them as the threshold.
+// Keeps the `num` largest keys of the list, in order, and the last of them as the threshold; returns how many there are.
 template <typename R>
-__device__ __forceinline__ void compact(R& sh, int num) {
+__device__ __forceinline__ int compact(R& sh, int num) {
   __syncthreads();
-  const int n = sh.n;
+  const int n = min(sh.n, R::CAP);
   for (int i = threadIdx.x; i < n; i += NT) {
     const uint64_t k = sh.list[i];
     int r = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) r += sh.list[j] > k;
     if (r < num) sh.best[r] = k;
   }
@@ -78,12 +78,13 @@ __device__ __forceinline__ void compact(R& sh, int num) {
     if (m == num) sh.tau = max(sh.tau, sh.best[num - 1]);
   }
   __syncthreads();
+  return m;
 }
 
 template <typename T, int U>
 __global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part* parts, uint64_t* keys, int seg) {
   using R = Rows<T, U>;
-  constexpr int VN = R::VN;
+  constexpr int VN = R::VN, TILE = R::TILE;
   __shared__ R sh;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.y;
@@ -95,102 +96,158 @@ __global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part*
   const int s0 = blockIdx.x * seg, s1 = min(p.V, s0 + seg);
   // vectors lie on 16-byte boundaries: the first begins up to VN - 1 elements in front of the part
   const int off = (int)((reinterpret_cast<uintptr_t>(x + s0) & 15) / sizeof(T));
-  if (tid == 0) { sh.n = 0; sh.tau = 0; sh.total = 0; }
-  float run = -INFINITY, sum = 0.f;
-  __syncthreads();
-  for (int t0 = s0 - off; t0 < s1; t0 += R::TILE) {
-    float v[U][VN];
-    float tm = -INFINITY;
+  if (tid == 0) { sh.n = 0; sh.tau = 0; }
+  uint4 next[U];
+  auto fetch = [&](int t0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i0 = t0 + (u * NT + tid) * VN;
       if (i0 >= s0 && i0 + VN <= s1) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(x + i0);
-        const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-        for (int k = 0; k < VN; ++k) v[u][k] = to_f32(e[k]);
+        next[u] = *reinterpret_cast<const uint4*>(x + i0);
       } else {
+        alignas(16) T e[VN];
 #pragma unroll
-        for (int k = 0; k < VN; ++k) v[u][k] = i0 + k >= s0 && i0 + k < s1 ? to_f32(x[i0 + k]) : -INFINITY;
+        for (int k = 0; k < VN; ++k) e[k] = i0 + k >= s0 && i0 + k < s1 ? x[i0 + k] : from_f32<T>(-INFINITY);
+        next[u] = *reinterpret_cast<const uint4*>(e);
       }
     }
+  };
+  // Lists the tile's elements above the threshold, of those left; false where some found no place.
+  auto look = [&](const uint4 (&raw)[U], const float (&vm)[U], float tm, int t0, uint32_t& left) {
+    const uint64_t tau = sh.tau;
+    const float tau_v = unordered((uint32_t)((tau + 1) >> 32));  // the lowest value that may pass,
+    const bool ties = key_of(tau_v, max(t0, s0)) > tau;           // and whether it may from this tile on
+    auto may = [&](float v) { return ties ? v >= tau_v : v > tau_v; };
+    const uint32_t all = 0xffffffffu;
+    bool placed = true;
+    if (__any_sync(all, may(tm))) {
+      uint32_t pass = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (__any_sync(all, may(vm[u]))) {
+          const T* e = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+          for (int k = 0; k < VN; ++k)
+            if (may(to_f32(e[k]))) pass |= 1u << (u * VN + k);
+        }
+      pass &= left;
+      while (pass) {
+        const int bit = __ffs(pass) - 1, i = t0 + (bit / VN * NT + tid) * VN + bit % VN;
+        pass &= pass - 1;
+        const uint64_t key = i >= s0 && i < s1 ? key_of(to_f32(x[i]), i) : 0;
+        if (key > tau) {
+          const int at = *const_cast<volatile int*>(&sh.n) < R::CAP ? atomicAdd(&sh.n, 1) : R::CAP;
+          if (at >= R::CAP) {
+            placed = false;
+            break;
+          }
+          sh.list[at] = key;
+        }
+        left &= ~(1u << bit);
+      }
+    }
+    return placed;
+  };
+  // the largest elements of the vectors, and of all of them
+  auto largest = [&](const uint4 (&raw)[U], float (&vm)[U]) {
+    float tm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float m = v[u][0];
+      const T* e = reinterpret_cast<const T*>(&raw[u]);
+      vm[u] = to_f32(e[0]);
 #pragma unroll
-      for (int k = 1; k < VN; ++k) m = fmaxf(m, v[u][k]);
-      if (m > run) {
-        sum *= ex2f((run - m) * kLog2e);
-        run = m;
+      for (int k = 1; k < VN; ++k) vm[u] = fmaxf(vm[u], to_f32(e[k]));
+      tm = fmaxf(tm, vm[u]);
+    }
+    return tm;
+  };
+  const int begin = s0 - off;
+  fetch(begin);
+  float run = -INFINITY, sum = 0.f;
+  int held = 0;  // listed elements at the last barrier
+  __syncthreads();
+  // a few tiles between two barriers, at which the list is cut to its best and the threshold rises
+  constexpr int kTiles = 4;
+#pragma unroll 1
+  for (int g0 = begin; g0 < s1; g0 += kTiles * TILE) {
+    const int g1 = min(g0 + kTiles * TILE, s1);
+    bool placed = true;
+#pragma unroll 1
+    for (int t0 = g0; t0 < g1; t0 += TILE) {
+      uint4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = next[u];
+      if (t0 + TILE < s1) fetch(t0 + TILE);
+      float vm[U];
+      const float tm = largest(raw, vm);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (vm[u] > run) {
+          sum *= ex2((run - vm[u]) * kLog2e);
+          run = vm[u];
+        }
+        // elements of -inf in front of the first finite one: the difference to -inf would be NaN
+        const float base = run == -INFINITY ? 0.f : -run;
+        const f2 less = pack2(base, base), scale = pack2(kLog2e, kLog2e);
+        const T* e = reinterpret_cast<const T*>(&raw[u]);
+        f2 s = 0;
+#pragma unroll
+        for (int k = 0; k < VN; k += 2) {
+          float d0, d1;
+          unpack2(mul2(add2(pack2(to_f32(e[k]), to_f32(e[k + 1])), less), scale), d0, d1);
+          s = add2(s, pack2(ex2(d0), ex2(d1)));
+        }
+        float a0, a1;
+        unpack2(s, a0, a1);
+        sum += a0 + a1;
       }
-      tm = fmaxf(tm, m);
-      // elements of -inf in front of the first finite one: the difference to -inf would be NaN
-      const float base = run == -INFINITY ? 0.f : run;
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < VN; ++k) s += ex2f((v[u][k] - base) * kLog2e);
-      sum += s;
-    }
-    // elements above the threshold
-    const float tau_v = sh.tau == 0 ? -INFINITY : unordered((uint32_t)(sh.tau >> 32));
-    const bool some = tm >= tau_v;
-    if (!__syncthreads_or(some)) continue;
-    auto count = [&]() {
-      const uint64_t tau = sh.tau;
-      int c = 0;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < VN; ++k) {
-          const int i = t0 + (u * NT + tid) * VN + k;
-          c += i >= s0 && i < s1 && key_of(v[u][k], i) > tau;
-        }
-      return c;
-    };
-    int c = some ? count() : 0;
-    if (c) atomicAdd(&sh.total, c);
-    __syncthreads();
-    const int would = sh.n + sh.total;
-    __syncthreads();  // the list grows only once every thread has read its length
-    if (would > R::CAP) {
-      // the num-th largest of the threads' maxima: at most num threads hold elements from there on
-      uint64_t mine = 0;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < VN; ++k) {
-          const int i = t0 + (u * NT + tid) * VN + k;
-          if (i >= s0 && i < s1) mine = max(mine, key_of(v[u][k], i));
-        }
-      sh.thread_max[tid] = mine;
-      compact(sh, p.num);
-      int r = 0;
+      if (t0 == begin) {
+        // the first threshold: just below the num-th largest of the maxima of groups of four threads
+        uint32_t o = ordered(tm);
+        o = max(o, __shfl_xor_sync(0xffffffffu, o, 1));
+        o = max(o, __shfl_xor_sync(0xffffffffu, o, 2));
+        if ((tid & 3) == 0) sh.group[tid >> 2] = o;
+        __syncthreads();
+        if (tid < kGroups) {
+          const uint32_t mine = sh.group[tid];
+          int r = 0;
 #pragma unroll 8
-      for (int i = 0; i < NT; ++i) r += sh.thread_max[i] > mine;
-      if (tid == 0) sh.total = 0;
-      __syncthreads();
-      // keys from the threshold on pass: the threshold itself is that of an element
-      if (r == p.num - 1 && mine != 0 && mine - 1 > sh.tau) sh.tau = mine - 1;
-      __syncthreads();
-      c = count();
-    }
-    if (c) {
-      const uint64_t tau = sh.tau;
-      int at = atomicAdd(&sh.n, c);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < VN; ++k) {
-          const int i = t0 + (u * NT + tid) * VN + k;
-          const uint64_t key = key_of(v[u][k], i);
-          if (i >= s0 && i < s1 && key > tau) sh.list[at++] = key;
+          for (int i = 0; i < kGroups; ++i) r += sh.group[i] > mine || (sh.group[i] == mine && i < tid);
+          if (r == p.num - 1) sh.tau = ((uint64_t)mine << 32) - 1;
         }
+        __syncthreads();
+      }
+      uint32_t left = ~0u;
+      placed &= look(raw, vm, tm, t0, left);
     }
-    __syncthreads();
-    if (tid == 0) sh.total = 0;
+    if (__syncthreads_or(!placed)) {
+      // more passed than the list holds: these tiles again, each as often as it takes, the threshold rising in between
+      if (tid == 0) sh.n = held;
+      __syncthreads();
+#pragma unroll 1
+      for (int t0 = g0; t0 < g1; t0 += TILE) {
+        uint4 keep[U], raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) keep[u] = next[u];
+        fetch(t0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          raw[u] = next[u];
+          next[u] = keep[u];
+        }
+        float vm[U];
+        const float tm = largest(raw, vm);
+        uint32_t left = ~0u;  // of this thread's U VN elements
+        bool again;
+        do {
+          again = __syncthreads_or(!look(raw, vm, tm, t0, left));
+          compact(sh, p.num);
+        } while (again);
+      }
+    }
+    held = compact(sh, p.num);
   }
-  compact(sh, p.num);
-  const int n = sh.n;
+  const int n = held;
   const int64_t part = row * gridDim.x + blockIdx.x;
   if (tid < n) keys[part * p.num + tid] = sh.list[tid];
   // the sum over the CTA, to one base
@@ -225,51 +282,61 @@ __device__ __forceinline__ uint64_t tie_of(int beam, uint32_t logit, int token) 
   return ((uint64_t)(63 - beam) << (32 + kTokenBits)) | ((uint64_t)logit << kTokenBits) | (uint32_t)((1 << kTokenBits) - 1 - token);
 }
 
-constexpr int kCands = kMaxCandidates * kMaxCandidates;
+// Lists that reach into the num best are num at most, with num elements each.
+__host__ __device__ inline int most_candidates(int lists, int num) { return (lists < num ? lists : num) * num; }
 
 __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const Part* parts, const uint64_t* keys, int splits) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  Cand* cand = reinterpret_cast<Cand*>(smem_raw);        // kCands
-  Cand* head = cand + kCands;                            // beams * splits
+  Cand* head = reinterpret_cast<Cand*>(smem_raw);  // beams * splits
+  Cand* cand = head + p.beams * splits;            // most_candidates
   // a logarithm of probability is (l - max) - log(sum): l - (max + log(sum)) would lose the digits of large logits
   __shared__ double s_max[kMaxBeams], s_log[kMaxBeams], s_score[kMaxBeams];
   __shared__ int s_kind[kMaxBeams], s_n;                 // 0 listed, 1 ended, 2 nothing, 3 NaN
   __shared__ Cand s_tau;
-  const int tid = threadIdx.x, K = p.beams, lists = K * splits;
+  const int tid = threadIdx.x, lane = tid & 31, K = p.beams, lists = K * splits;
   const int64_t b = blockIdx.x;
   if (tid == 0) { s_n = 0; s_tau = Cand{0, 0}; }
-  if (tid < K) {
-    const float score = p.scores[b * p.sb + tid * p.sk];
+  // what the first element of this thread's list will need, on its way while the sums are joined (not used where it was not written)
+  const int first_n = tid < lists ? parts[b * lists + tid].n : 0;
+  const uint64_t first_key = tid < lists ? keys[(b * lists + tid) * p.num] : 0;
+  // a warp a beam joins its parts' sums
+  for (int j = tid >> 5; j < K; j += NT / 32) {
+    const float score = p.scores[b * p.sb + j * p.sk];
     int kind = 0;
     double peak = 0.0, logs = 0.0;
     if (score == -INFINITY) kind = 2;
     else if (!(score < INFINITY)) kind = 3;
-    else if (p.finished != nullptr && p.finished[b * p.fb + tid * p.fk] != 0) kind = 1;
+    else if (p.finished != nullptr && p.finished[b * p.fb + j * p.fk] != 0) kind = 1;
     else {
-      const Part* q = parts + (b * K + tid) * splits;
-      float m = -INFINITY;
-      for (int i = 0; i < splits; ++i) m = fmaxf(m, q[i].max);
-      double s = 0.0;
-      for (int i = 0; i < splits; ++i) s += q[i].max == -INFINITY ? q[i].sum : q[i].sum * exp((double)q[i].max - (double)m);
+      const Part* q = parts + (b * K + j) * splits;
+      const Part mine = lane < splits ? q[lane] : Part{0.0, -INFINITY, 0};
+      float m = mine.max;
+      for (int i = lane + 32; i < splits; i += 32) m = fmaxf(m, q[i].max);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      auto part = [&](const Part& x) { return x.max == -INFINITY ? x.sum : x.sum * exp((double)x.max - (double)m); };
+      double s = part(mine);
+      for (int i = lane + 32; i < splits; i += 32) s += part(q[i]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       peak = (double)m;
       logs = log(s);
       if (!(s == s) || m == INFINITY) kind = 3;
       else if (m == -INFINITY) kind = 2;
     }
-    s_kind[tid] = kind;
-    s_max[tid] = peak;
-    s_log[tid] = logs;
-    s_score[tid] = (double)score;
+    if (lane == 0) {
+      s_kind[j] = kind;
+      s_max[j] = peak;
+      s_log[j] = logs;
+      s_score[j] = (double)score;
+    }
   }
   __syncthreads();
-  // element i of list l: false behind its end
-  auto get = [&](int l, int i, Cand* c) {
+  // element i of list l, of n listed ones the one with this key: false behind its end
+  auto make = [&](int l, int i, int n, uint64_t key, Cand* c) {
     const int j = l / splits, kind = s_kind[j];
-    if (i >= p.num) return false;
     if (kind == 0) {
-      const int64_t part = (b * K + j) * splits + l % splits;
-      if (i >= parts[part].n) return false;
-      const uint64_t key = keys[part * p.num + i];
+      if (i >= n) return false;
       const uint32_t o = (uint32_t)(key >> 32);
       *c = Cand{ordered64(s_score[j] + (((double)unordered(o) - s_max[j]) - s_log[j])), tie_of(j, o, (int)~(uint32_t)key)};
       return true;
@@ -283,7 +350,9 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
     *c = Cand{kind == 3 ? ~0ull : ordered64(-(double)INFINITY), tie_of(j, 0, token)};
     return true;
   };
-  for (int l = tid; l < lists; l += NT)
+  auto get = [&](int l, int i, Cand* c) { return make(l, i, parts[b * lists + l].n, keys[(b * lists + l) * p.num + i], c); };
+  if (tid < lists && !make(tid, 0, first_n, first_key, &head[tid])) head[tid] = Cand{0, 0};
+  for (int l = tid + NT; l < lists; l += NT)
     if (!get(l, 0, &head[l])) head[l] = Cand{0, 0};
   __syncthreads();
   // nothing below the num-th best head can be among the num best
@@ -291,21 +360,25 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
     for (int l = tid; l < lists; l += NT) {
       const Cand mine = head[l];
       int r = 0;
+#pragma unroll 4
       for (int i = 0; i < lists; ++i) r += above(head[i], mine);
       if (r == p.num - 1 && mine.tie != 0) s_tau = mine;
     }
     __syncthreads();
   }
   const Cand tau = s_tau;
-  for (int l = tid; l < lists; l += NT) {
+  for (int i = tid; i < lists * p.num; i += NT) {
+    const int l = i / p.num;
+    const Cand h = head[l];
     Cand c;
-    for (int i = 0; get(l, i, &c) && !above(tau, c); ++i) cand[atomicAdd(&s_n, 1)] = c;
+    if (h.tie != 0 && !above(tau, h) && get(l, i % p.num, &c) && !above(tau, c)) cand[atomicAdd(&s_n, 1)] = c;
   }
   __syncthreads();
   const int n = s_n;
   for (int i = tid; i < n; i += NT) {
     const Cand mine = cand[i];
     int r = 0;
+#pragma unroll 4
     for (int k = 0; k < n; ++k) r += above(cand[k], mine);
     if (r < p.num) {
       const int64_t at = b * p.num + r;
@@ -316,6 +389,12 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
   }
 }
 
+#ifndef M3_W
+#define M3_W 4
+#endif
+#ifndef M3_U
+#define M3_U 4
+#endif
 struct BeamPlan { int u, seg, splits; };
 
 // Parts of a row: tiles of four vectors a thread where the rows alone fill the GPU, of one where they do not;
@@ -323,11 +402,11 @@ struct BeamPlan { int u, seg, splits; };
 BeamPlan plan(int64_t rows, int V, int es, int sms) {
   const int vn = 16 / es;
   BeamPlan w;
-  const int64_t big = (V + 4 * NT * vn - 1) / (4 * NT * vn);
-  w.u = rows * big >= 2 * sms ? 4 : 1;
+  const int64_t big = (V + M3_U * NT * vn - 1) / (M3_U * NT * vn);
+  w.u = rows * big >= 2 * sms ? M3_U : 1;
   const int tile = NT * w.u * vn;
   const int64_t tiles = (V + tile - 1) / tile;
-  const int64_t want = std::max<int64_t>(1, (int64_t)4 * sms / std::max<int64_t>(1, rows));
+  const int64_t want = std::max<int64_t>(1, (int64_t)M3_W * sms / std::max<int64_t>(1, rows));
   const int64_t per = (tiles + std::min(want, tiles) - 1) / std::min(want, tiles);
   w.seg = (int)(per * tile);
   w.splits = (int)((V + w.seg - 1) / w.seg);
@@ -355,7 +434,7 @@ int launch_beam_select(const BeamParams& p, int dtype, void* ws, cudaStream_t s)
   const dim3 grid((unsigned)w.splits, (unsigned)rows);
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (w.u == 4) beam_rows_kernel<T, 4><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
+    if (w.u == M3_U) beam_rows_kernel<T, M3_U><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
     else beam_rows_kernel<T, 1><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
     return check_launch("beam_rows_kernel");
   };
@@ -363,9 +442,10 @@ int launch_beam_select(const BeamParams& p, int dtype, void* ws, cudaStream_t s)
   else if (dtype == M3_BFLOAT16) M3_TRY(go(__nv_bfloat16{}));
   else M3_TRY(go(__half{}));
   static std::atomic<bool> done[kMaxDevices];
-  const size_t most = (size_t)(kCands + kMaxLists) * sizeof(Cand);
+  const size_t most = (size_t)(kMaxCandidates * kMaxCandidates + kMaxLists) * sizeof(Cand);
   M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(&beam_join_kernel), most, done));
-  const size_t smem = (size_t)(kCands + p.beams * w.splits) * sizeof(Cand);
+  const int lists = p.beams * w.splits;
+  const size_t smem = (size_t)(lists + most_candidates(lists, p.num)) * sizeof(Cand);
   beam_join_kernel<<<(unsigned)p.batch, NT, smem, s>>>(p, parts, keys, w.splits);
   return check_launch("beam_join_kernel");
 }
