@@ -3,12 +3,12 @@
 // A beam that has ended offers its end token at no cost; one whose score is -inf, or all of whose logits
 // are, offers -inf; one with a NaN or an infinite logit or score offers NaN, which ranks first.
 // beam_rows_kernel reads the logits once: a CTA a part of a row keeps its largest element and the sum of
-// exponentials (32 bits a thread, joined in 64) and the part's `num` largest elements. Those pass a
+// exponentials (one float a thread, two where they join) and the part's `num` largest elements. Those pass a
 // threshold, at first the num-th largest of the maxima of groups of threads, which rises whenever the list of those that
 // passed has grown, so that later tiles are mostly dismissed by one comparison a vector. Where more pass than the list
 // holds (rising or equal logits), the rest of the tile waits for the risen threshold; keys are unique (value, then the
 // lower index), so that each look lists a full list's worth of them. beam_join_kernel, a CTA a prompt,
-// joins the sums in 64 bits and ranks the parts' elements by their score in 64 bits.
+// joins the sums and ranks the parts' elements by their score, both in two floats (about 48 bits).
 // Bound by the memory where there are many rows, by latency where there are few.
 #include <algorithm>
 
@@ -21,7 +21,7 @@ namespace {
 
 constexpr int NT = 256;
 
-struct Part { double sum; float max; int n; };  // of a row's part: sum of exp(l - max), and listed elements
+struct Part { Two sum; float max; int n; };  // of a row's part: sum of exp(l - max), and listed elements
 
 // floats in the order of unsigned integers; -0 counts as +0
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -33,14 +33,52 @@ __device__ __forceinline__ float unordered(uint32_t k) {
 }
 __device__ __forceinline__ uint64_t key_of(float v, int i) { return ((uint64_t)ordered(v) << 32) | (uint32_t)~i; }
 
-__device__ __forceinline__ uint64_t ordered64(double v) {
-  if (v != v) return ~0ull;
-  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
-  return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
+// Scores are held in two floats, hi + lo with |lo| at most half a step of hi: an infinite or NaN hi has lo = 0.
+__device__ __forceinline__ Two two_sum(float a, float b) {
+  Two r{a, 0.f};
+  r.add(b);
+  if (!(fabsf(r.hi) < INFINITY)) r.lo = 0.f;
+  return r;
 }
-__device__ __forceinline__ double unordered64(uint64_t k) {
-  if (k == ~0ull) return __longlong_as_double(0x7ff8000000000000ll);
-  return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
+__device__ __forceinline__ Two plus(const Two& a, const Two& b) {
+  Two r = two_sum(a.hi, b.hi);
+  if (fabsf(r.hi) < INFINITY) {
+    const float l = __fadd_rn(r.lo, __fadd_rn(a.lo, b.lo)), h = __fadd_rn(r.hi, l);
+    r.lo = __fsub_rn(l, __fsub_rn(h, r.hi));
+    r.hi = h;
+  }
+  return r;
+}
+// in the order of unsigned integers, a NaN above all
+__device__ __forceinline__ uint64_t ordered64(const Two& v) {
+  return v.hi != v.hi ? ~0ull : ((uint64_t)ordered(v.hi) << 32) | ordered(v.lo);
+}
+__device__ __forceinline__ float score_of(uint64_t k) {
+  return k == ~0ull ? __int_as_float(0x7fc00000) : __fadd_rn(unordered((uint32_t)(k >> 32)), unordered((uint32_t)k));
+}
+
+// log of a sum s > 0, to a few 1e-9: s = 2^n m with m in [3/4, 3/2), log m = 2 atanh(t), t = (m - 1) / (m + 1), |t| <= 1/5, of which
+// t itself is formed in two floats and the rest of the series, 125 times smaller, in one.
+__device__ __forceinline__ Two log_two(const Two& s) {
+  const float top = __fadd_rn(s.hi, s.lo);
+  if (!(top > 0.f && top < INFINITY)) return Two{logf(top), 0.f};
+  int n = (__float_as_int(top) - 0x3f400000) >> 23;  // of 3/4
+  const float scale = __int_as_float((127 - n) << 23);  // (sums of at most 2^24 terms of at most 1)
+  const float m = s.hi * scale, ml = s.lo * scale;
+  const Two a = two_sum(m, -1.f), b = two_sum(m, 1.f);
+  const float al = a.lo + ml, bl = b.lo + ml;
+  const float th = __fdiv_rn(a.hi, b.hi);
+  // what the quotient leaves: (a - th b) / b
+  const float tl = __fdiv_rn(__fadd_rn(fmaf(-th, b.hi, a.hi), al - th * bl), b.hi);
+  const float q = th * th;
+  float r = fmaf(q, 1.f / 13, 1.f / 11);
+  r = fmaf(q, r, 1.f / 9);
+  r = fmaf(q, r, 1.f / 7);
+  r = fmaf(q, r, 1.f / 5);
+  r = fmaf(q, r, 1.f / 3);
+  const Two logm = two_sum(2.f * th, 2.f * fmaf(q * th, r, tl));
+  // n log 2, log 2 in two parts of which the first has few enough bits for an exact product
+  return plus(plus(Two{n * 0.693145751953125f, 0.f}, Two{n * 1.42860682030941723212e-6f, 0.f}), logm);
 }
 
 constexpr int kGroups = NT / 4;  // threads whose largest elements give the first threshold
@@ -52,7 +90,7 @@ struct Rows {
   static constexpr int CAP = 1024;  // listed elements; more of a tile wait until the threshold has risen
   uint64_t list[CAP], best[kMaxCandidates];
   uint32_t group[kGroups];
-  double sum[NT / 32];
+  Two sum[NT / 32];
   float max[NT / 32];
   int n;
   uint64_t tau;  // keys above it pass
@@ -259,15 +297,14 @@ __global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part*
   m = sh.max[0];
 #pragma unroll
   for (int w = 1; w < NT / 32; ++w) m = fmaxf(m, sh.max[w]);
-  double d = run == -INFINITY ? (double)sum : (double)sum * exp((double)run - (double)m);
+  Two d{run == -INFINITY ? sum : sum * ex2((run - m) * kLog2e), 0.f};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  for (int o = 16; o > 0; o >>= 1) d.add(d.shuffled(o));
   if ((tid & 31) == 0) sh.sum[tid >> 5] = d;
   __syncthreads();
   if (tid == 0) {
-    d = sh.sum[0];
 #pragma unroll
-    for (int w = 1; w < NT / 32; ++w) d += sh.sum[w];
+    for (int w = 1; w < NT / 32; ++w) d.add(sh.sum[w]);
     parts[part] = Part{d, m, n};
   }
 }
@@ -290,7 +327,8 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
   Cand* head = reinterpret_cast<Cand*>(smem_raw);  // beams * splits
   Cand* cand = head + p.beams * splits;            // most_candidates
   // a logarithm of probability is (l - max) - log(sum): l - (max + log(sum)) would lose the digits of large logits
-  __shared__ double s_max[kMaxBeams], s_log[kMaxBeams], s_score[kMaxBeams];
+  __shared__ float s_max[kMaxBeams], s_score[kMaxBeams];
+  __shared__ Two s_log[kMaxBeams];
   __shared__ int s_kind[kMaxBeams], s_n;                 // 0 listed, 1 ended, 2 nothing, 3 NaN
   __shared__ Cand s_tau;
   const int tid = threadIdx.x, lane = tid & 31, K = p.beams, lists = K * splits;
@@ -303,32 +341,37 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
   for (int j = tid >> 5; j < K; j += NT / 32) {
     const float score = p.scores[b * p.sb + j * p.sk];
     int kind = 0;
-    double peak = 0.0, logs = 0.0;
+    float peak = 0.f;
+    Two logs{0.f, 0.f};
     if (score == -INFINITY) kind = 2;
     else if (!(score < INFINITY)) kind = 3;
     else if (p.finished != nullptr && p.finished[b * p.fb + j * p.fk] != 0) kind = 1;
     else {
       const Part* q = parts + (b * K + j) * splits;
-      const Part mine = lane < splits ? q[lane] : Part{0.0, -INFINITY, 0};
+      const Part mine = lane < splits ? q[lane] : Part{Two{0.f, 0.f}, -INFINITY, 0};
       float m = mine.max;
       for (int i = lane + 32; i < splits; i += 32) m = fmaxf(m, q[i].max);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      auto part = [&](const Part& x) { return x.max == -INFINITY ? x.sum : x.sum * exp((double)x.max - (double)m); };
-      double s = part(mine);
-      for (int i = lane + 32; i < splits; i += 32) s += part(q[i]);
+      auto part = [&](const Part& x) {
+        const float f = x.max == m || x.max == -INFINITY ? 1.f : ex2((x.max - m) * kLog2e);
+        return Two{x.sum.hi * f, x.sum.lo * f};
+      };
+      Two s = part(mine);
+      for (int i = lane + 32; i < splits; i += 32) s.add(part(q[i]));
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      peak = (double)m;
-      logs = log(s);
-      if (!(s == s) || m == INFINITY) kind = 3;
+      for (int o = 16; o > 0; o >>= 1) s.add(s.shuffled(o));
+      peak = m;
+      const float total = s.value();
+      if (!(total == total) || m == INFINITY) kind = 3;
       else if (m == -INFINITY) kind = 2;
+      else logs = log_two(s);
     }
     if (lane == 0) {
       s_kind[j] = kind;
       s_max[j] = peak;
-      s_log[j] = logs;
-      s_score[j] = (double)score;
+      s_log[j] = Two{-logs.hi, -logs.lo};
+      s_score[j] = score;
     }
   }
   __syncthreads();
@@ -338,16 +381,17 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
     if (kind == 0) {
       if (i >= n) return false;
       const uint32_t o = (uint32_t)(key >> 32);
-      *c = Cand{ordered64(s_score[j] + (((double)unordered(o) - s_max[j]) - s_log[j])), tie_of(j, o, (int)~(uint32_t)key)};
+      const Two logp = plus(two_sum(unordered(o), -s_max[j]), s_log[j]);
+      *c = Cand{ordered64(plus(Two{s_score[j], 0.f}, logp)), tie_of(j, o, (int)~(uint32_t)key)};
       return true;
     }
     if (l % splits != 0 || i >= p.V) return false;
     if (kind == 1 && i == 0) {
-      *c = Cand{ordered64(s_score[j]), tie_of(j, ~0u, p.end_token)};
+      *c = Cand{ordered64(Two{s_score[j], 0.f}), tie_of(j, ~0u, p.end_token)};
       return true;
     }
     const int token = kind == 1 && i <= p.end_token ? i - 1 : i;
-    *c = Cand{kind == 3 ? ~0ull : ordered64(-(double)INFINITY), tie_of(j, 0, token)};
+    *c = Cand{kind == 3 ? ~0ull : ordered64(Two{-INFINITY, 0.f}), tie_of(j, 0, token)};
     return true;
   };
   auto get = [&](int l, int i, Cand* c) { return make(l, i, parts[b * lists + l].n, keys[(b * lists + l) * p.num + i], c); };
@@ -358,11 +402,15 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
   // nothing below the num-th best head can be among the num best
   if (lists > p.num) {
     for (int l = tid; l < lists; l += NT) {
+      // (equal values in the order of the lists, which is that of their beams)
       const Cand mine = head[l];
       int r = 0;
 #pragma unroll 4
-      for (int i = 0; i < lists; ++i) r += above(head[i], mine);
+      for (int i = 0; i < l; ++i) r += head[i].value >= mine.value;
+#pragma unroll 4
+      for (int i = l + 1; i < lists; ++i) r += head[i].value > mine.value;
       if (r == p.num - 1 && mine.tie != 0) s_tau = mine;
+      if (r >= p.num) head[l].tie = 0;  // the list is left out
     }
     __syncthreads();
   }
@@ -371,18 +419,17 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
     const int l = i / p.num;
     const Cand h = head[l];
     Cand c;
-    if (h.tie != 0 && !above(tau, h) && get(l, i % p.num, &c) && !above(tau, c)) cand[atomicAdd(&s_n, 1)] = c;
+    if (h.tie != 0 && get(l, i % p.num, &c) && !above(tau, c)) cand[atomicAdd(&s_n, 1)] = c;
   }
   __syncthreads();
   const int n = s_n;
-  for (int i = tid; i < n; i += NT) {
+  for (int i = tid >> 5; i < n; i += NT / 32) {  // a warp a candidate: how many are above it
     const Cand mine = cand[i];
     int r = 0;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) r += above(cand[k], mine);
-    if (r < p.num) {
+    for (int k = lane; k - lane < n; k += 32) r += __popc(__ballot_sync(0xffffffffu, k < n && above(cand[k], mine)));
+    if (lane == 0 && r < p.num) {
       const int64_t at = b * p.num + r;
-      p.out_scores[at] = (float)unordered64(mine.value);
+      p.out_scores[at] = score_of(mine.value);
       p.parents[at] = 63 - (int)(mine.tie >> (32 + kTokenBits));
       p.tokens[at] = (1 << kTokenBits) - 1 - (int)(mine.tie & ((1 << kTokenBits) - 1));
     }

@@ -337,29 +337,28 @@ __global__ void __launch_bounds__(32 * kWarps) conv_bwd_kernel(const ConvParams 
   }
 }
 
-// dw and dbias from the CTAs' parts: a warp a value's column of parts in 64 bits, in a fixed order.
+// dw and dbias from the CTAs' parts, in two floats and a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(256) conv_bwd_join_kernel(const float* part, int64_t parts, int E, int taps, void* dw,
                                                           void* dbias, bool f32) {
-  __shared__ double sums[8][32];
+  __shared__ Two sums[8][32];
   const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x, per = (int64_t)E * (taps + 1);
-  double v = 0.0;
+  Two v{0.f, 0.f};
   if (i < per) {
 #pragma unroll 8
-    for (int64_t j = threadIdx.y; j < parts; j += 8) v += (double)part[j * per + i];
+    for (int64_t j = threadIdx.y; j < parts; j += 8) v.add(part[j * per + i]);
   }
   sums[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.y != 0 || i >= per) return;
-  v = 0.0;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) v += sums[w][threadIdx.x];
+  for (int w = 1; w < 8; ++w) v.add(sums[w][threadIdx.x]);
   const int k = (int)(i / E), e = (int)(i % E);
   void* out = k < taps ? dw : dbias;
   if (out == nullptr) return;
   const int64_t at = k < taps ? (int64_t)e * taps + k : e;
-  if (f32) static_cast<float*>(out)[at] = (float)v;
-  else st(static_cast<T*>(out) + at, (float)v);
+  if (f32) static_cast<float*>(out)[at] = v.value();
+  else st(static_cast<T*>(out) + at, v.value());
 }
 
 // One step: the window moves on by one row, in place.

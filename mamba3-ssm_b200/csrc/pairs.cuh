@@ -55,6 +55,25 @@ __device__ __forceinline__ float2 sigmoid2(float2 x) {
   return x;
 }
 
+// A sum in two floats, hi + lo, with what each addition of hi rounds away kept in lo: 48 bits or so, without
+// conversions to 64-bit floats and their few units.
+struct Two {
+  float hi, lo;
+  __device__ __forceinline__ void add(float x) {
+    const float s = __fadd_rn(hi, x), part = __fsub_rn(s, hi);
+    lo = __fadd_rn(lo, __fadd_rn(__fsub_rn(hi, __fsub_rn(s, part)), __fsub_rn(x, part)));
+    hi = s;
+  }
+  __device__ __forceinline__ void add(const Two& o) {
+    add(o.hi);
+    lo = __fadd_rn(lo, o.lo);
+  }
+  __device__ __forceinline__ Two shuffled(int mask) const {
+    return Two{__shfl_xor_sync(0xffffffffu, hi, mask), __shfl_xor_sync(0xffffffffu, lo, mask)};
+  }
+  __device__ __forceinline__ float value() const { return __fadd_rn(hi, lo); }
+};
+
 // Two neighbouring elements of a row as they lie in memory, converted when they are used, so that loads can
 // stay in flight. W32: the row is fp32 whatever T is.
 template <typename T> struct Raw2 { uint32_t v; };

@@ -26,8 +26,8 @@ struct BwdSmem {
   float B[NP][TS], C[NP][TS];
   float red[W][2 * SUB * NP];
   float h[2][M][NT][K];  // the states in front of these eight steps and of the next eight (earlier) ones, by thread
-  // sums over the tiles so far, by thread: those of one tile are formed in 32 bits
-  double dA[M * K][NT], dD[M][NT], dbias[M][NT];
+  // sums over the tiles so far, by thread, in two floats: those of one tile are formed in one
+  Two dA[M * K][NT], dD[M][NT], dbias[M][NT];
 };
 
 // Copies 16 bytes (or K floats) into shared memory without passing registers.
@@ -89,12 +89,12 @@ __global__ void __launch_bounds__(NT, M3_BMIN) sel_bwd_kernel(const SelScanParam
   for (int m = 0; m < M; ++m) {
     const int e = e_first + m * (NT / P) + tid / P, ec = min(e, e_end - 1);
     save[m] = p.save + ((int64_t)b * nsave * p.E + ec) * NP + q * K;
-    sh.dD[m][tid] = sh.dbias[m][tid] = 0.0;
+    sh.dD[m][tid] = sh.dbias[m][tid] = Two{0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int n = nk[k];
       A2[m][k] = n < p.N ? p.A[(int64_t)ec * p.N + n] * kLog2e : 0.f;
-      sh.dA[m * K + k][tid] = 0.0;
+      sh.dA[m * K + k][tid] = Two{0.f, 0.f};
       gv[m][k] = 0.f;
       if (e < e_end) {
         if (p.nchunk > 1) gv[m][k] = p.states[(((int64_t)b * p.nchunk + c) * p.E + ec) * NP + n];
@@ -349,10 +349,10 @@ __global__ void __launch_bounds__(NT, M3_BMIN) sel_bwd_kernel(const SelScanParam
     }
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      sh.dD[m][tid] += (double)sumD[m];
-      sh.dbias[m][tid] += (double)sumbias[m];
+      sh.dD[m][tid].add(sumD[m]);
+      sh.dbias[m][tid].add(sumbias[m]);
 #pragma unroll
-      for (int k = 0; k < K; ++k) sh.dA[m * K + k][tid] += (double)dA[m][k];
+      for (int k = 0; k < K; ++k) sh.dA[m * K + k][tid].add(dA[m][k]);
     }
     if (lelive) {
 #pragma unroll 1
@@ -382,21 +382,21 @@ __global__ void __launch_bounds__(NT, M3_BMIN) sel_bwd_kernel(const SelScanParam
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     const int e = e_first + m * (NT / P) + tid / P;
-    double sumD = sh.dD[m][tid], sumbias = sh.dbias[m][tid];
+    Two sumD = sh.dD[m][tid], sumbias = sh.dbias[m][tid];
 #pragma unroll
     for (int o = P / 2; o >= 1; o /= 2) {
-      sumD += __shfl_xor_sync(0xffffffffu, sumD, o);
-      sumbias += __shfl_xor_sync(0xffffffffu, sumbias, o);
+      sumD.add(sumD.shuffled(o));
+      sumbias.add(sumbias.shuffled(o));
     }
     if (e < e_end) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        pa[(int64_t)e * (NP + 2) + nk[k]] = (float)sh.dA[m * K + k][tid];
+        pa[(int64_t)e * (NP + 2) + nk[k]] = sh.dA[m * K + k][tid].value();
         if (g.dh0 != nullptr && c == 0 && nk[k] < p.N) g.dh0[((int64_t)b * p.E + e) * p.N + nk[k]] = gv[m][k];
       }
       if (q == 0) {
-        pa[(int64_t)e * (NP + 2) + NP] = (float)sumD;
-        pa[(int64_t)e * (NP + 2) + NP + 1] = (float)sumbias;
+        pa[(int64_t)e * (NP + 2) + NP] = sumD.value();
+        pa[(int64_t)e * (NP + 2) + NP + 1] = sumbias.value();
       }
     }
   }
@@ -519,11 +519,13 @@ __global__ void __launch_bounds__(256) sel_bwd_join_kernel(const SelScanParams p
   const int64_t i = (int64_t)(blockIdx.x - bc_ctas) * 256 + threadIdx.x;
   if (i >= (int64_t)p.E * (NP + 2)) return;
   const int e = (int)(i / (NP + 2)), n = (int)(i % (NP + 2));
-  double v = 0.0;
-  for (int j = 0; j < p.batch * p.nchunk; ++j) v += (double)g.part_a[(int64_t)j * p.E * (NP + 2) + i];
-  if (n < p.N) g.dA[(int64_t)e * p.N + n] = (float)v;
-  else if (n == NP && g.dD != nullptr) g.dD[e] = (float)v;
-  else if (n == NP + 1 && g.dbias != nullptr) g.dbias[e] = (float)v;
+  Two sum{0.f, 0.f};
+#pragma unroll 4
+  for (int j = 0; j < p.batch * p.nchunk; ++j) sum.add(g.part_a[(int64_t)j * p.E * (NP + 2) + i]);
+  const float v = sum.value();
+  if (n < p.N) g.dA[(int64_t)e * p.N + n] = v;
+  else if (n == NP && g.dD != nullptr) g.dD[e] = v;
+  else if (n == NP + 1 && g.dbias != nullptr) g.dbias[e] = v;
 }
 
 template <typename F>

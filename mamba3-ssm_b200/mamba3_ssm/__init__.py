@@ -15,7 +15,7 @@ For beam search: the selection (beam_select) and the moves of the states (reorde
 
 from .config import MambaConfig, SSMConfig
 from .layer import Mamba3
-from .block import MambaLMHeadModel, MambaBlock, DecodeGraph
+from .block import MambaLMHeadModel, MambaBlock, DecodeGraph, BeamGraph
 from .ops import RMSNorm, apply_rope, ssm_scan_siso, ssm_scan_mimo
 from .losses import PolicyLoss, PreferenceLoss, policy_loss, preference_loss, token_logprobs
 from .grads import clip_grad_norm_, clip_grads_
@@ -29,6 +29,7 @@ __all__ = [
     "MambaLMHeadModel",
     "MambaBlock",
     "DecodeGraph",
+    "BeamGraph",
     "RMSNorm",
     "apply_rope",
     "ssm_scan_siso",

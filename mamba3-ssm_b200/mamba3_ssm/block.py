@@ -9,6 +9,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .beam import beam_select, reorder_states_
 from .config import MambaConfig
 from .layer import Mamba3
 from .losses import token_logprobs
@@ -140,6 +141,19 @@ class MambaLMHeadModel(nn.Module):
         Not part of the reference interface; step() keeps the reference's semantics."""
         return DecodeGraph(self, batch_size, greedy)
 
+    def beam_graph(self, batch_size: int, num_beams: int, end_token: int = None) -> "BeamGraph":
+        """A CUDA-graph beam search for this model at a fixed number of prompts and beams (see
+        BeamGraph). Not part of the reference interface."""
+        return BeamGraph(self, batch_size, num_beams, end_token)
+
+    def beam_search(self, input_ids: torch.Tensor, num_beams: int, max_new_tokens: int, end_token: int = None,
+                    length_penalty: float = 0.0):
+        """The num_beams best continuations of each prompt (B, L): (tokens (B, num_beams, n), scores
+        (B, num_beams)), the best first; see BeamGraph.search. Captures a graph for this one
+        search: keep a ``beam_graph`` for several."""
+        graph = self.beam_graph(input_ids.shape[0], num_beams, end_token)
+        return graph.search(input_ids, max_new_tokens, length_penalty)
+
 
 class DecodeGraph:
     """Replays one whole decode step (embedding, every layer's norm / in_proj / fused step
@@ -219,3 +233,87 @@ class DecodeGraph:
         """One greedy step on the previous step's argmax; returns the static token buffer."""
         self.graph.replay()
         return self.tokens
+
+
+class BeamGraph(DecodeGraph):
+    """Beam search with one CUDA graph a token: the selection among the previous step's logits
+    (beam.beam_select), the beams' states moved to the beams that continue them
+    (beam.reorder_states_, in place), and the decode step of DecodeGraph for batch_size * num_beams
+    rows.
+
+        g = model.beam_graph(batch, beams, end_token)
+        tokens, scores = g.search(prompt, max_new_tokens)
+    """
+
+    def __init__(self, model: "MambaLMHeadModel", batch_size: int, num_beams: int, end_token: int = None):
+        dev = model.embedding.weight.device
+        if dev.type != "cuda":
+            raise RuntimeError("BeamGraph needs the model on a CUDA device")
+        self.vocabulary = min(model.config.vocab_size, model.vocab_size)  # without the padding of the weights
+        if end_token is not None and not 0 <= end_token < self.vocabulary:
+            raise ValueError(f"BeamGraph: end_token {end_token} is outside the vocabulary of {self.vocabulary}")
+        if batch_size < 1 or not 1 <= num_beams <= 32:
+            raise ValueError(f"BeamGraph: at least one prompt and 1 to 32 beams, got {batch_size} and {num_beams}")
+        self.end_token = end_token
+        shape = (batch_size, num_beams)
+        self.ahead = torch.zeros(*shape, model.vocab_size, dtype=model.lm_head.weight.dtype, device=dev)
+        self.scores = torch.zeros(shape, dtype=torch.float32, device=dev)
+        self.parents = torch.zeros(shape, dtype=torch.int64, device=dev)
+        self.finished = torch.zeros(shape, dtype=torch.bool, device=dev)
+        super().__init__(model, batch_size * num_beams, greedy=False)
+
+    def _body(self):
+        ended = self.end_token is not None
+        sel = beam_select(self.ahead[..., :self.vocabulary], self.scores, finished=self.finished if ended else None,
+                          end_token=self.end_token if ended else 0)
+        self.scores.copy_(sel.scores)
+        self.parents.copy_(sel.parents)
+        self.tokens.copy_(sel.tokens.view(-1))
+        if ended:
+            self.finished.copy_(self.finished.gather(1, sel.parents) | (sel.tokens == self.end_token))
+        reorder_states_(self.cache, self.parents)
+        logits = super()._body()
+        self.ahead.copy_(logits.view_as(self.ahead))
+        return logits
+
+    @torch.no_grad()
+    def search(self, prompt: torch.Tensor, max_new_tokens: int, length_penalty: float = 0.0):
+        """(tokens (B, num_beams, n), scores (B, num_beams)) for prompts (B, L), n <= max_new_tokens, the
+        best first. scores: the sum of the tokens' log-probabilities over their number (up to the
+        end token, which counts) to the power of length_penalty. Behind the end token a row is filled
+        with it; the search ends early once every beam has ended (looked at every 16 tokens)."""
+        b, k = self.scores.shape
+        if prompt.dim() != 2 or prompt.shape[0] != b or prompt.shape[1] == 0:
+            raise ValueError(f"BeamGraph: prompts ({b}, length) expected, got {tuple(prompt.shape)}")
+        if max_new_tokens < 1:
+            raise ValueError(f"BeamGraph: max_new_tokens must be 1 or more, got {max_new_tokens}")
+        dev = self.scores.device
+        logits, cache = self.model.prefill(prompt)
+        # every beam starts from the prompt; all but the first are empty places, so that the first step takes its best tokens
+        reorder_states_(cache, torch.zeros((b, k), dtype=torch.int64, device=dev), out=self.cache)
+        self.ahead.copy_(logits[:, -1:].expand(b, k, logits.shape[-1]))
+        self.scores.fill_(float("-inf"))
+        self.scores[:, 0] = 0.0
+        self.finished.zero_()
+        parents = torch.empty((max_new_tokens, b, k), dtype=torch.int64, device=dev)
+        tokens = torch.empty_like(parents)
+        n = 0
+        while n < max_new_tokens:
+            self.graph.replay()
+            parents[n].copy_(self.parents)
+            tokens[n].copy_(self.tokens.view(b, k))
+            n += 1
+            if self.end_token is not None and n % 16 == 0 and bool(self.finished.all()):
+                break
+        # from the last tokens back through the beams that they continue
+        at = torch.arange(k, device=dev).expand(b, k)
+        out = torch.empty((b, k, n), dtype=torch.int64, device=dev)
+        for t in range(n - 1, -1, -1):
+            out[:, :, t] = tokens[t].gather(1, at)
+            at = parents[t].gather(1, at)
+        scores = self.scores
+        if length_penalty:
+            length = n if self.end_token is None else ((out == self.end_token).cumsum(-1) == 0).sum(-1).add(1).clamp(max=n)
+            scores = scores / (length ** length_penalty if isinstance(length, int) else length.float() ** length_penalty)
+        best, order = scores.sort(dim=1, descending=True, stable=True)
+        return out.gather(1, order.unsqueeze(-1).expand_as(out)), best
