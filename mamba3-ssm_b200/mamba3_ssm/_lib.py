@@ -226,8 +226,8 @@ class Records:
     __slots__ = ("buf", "base")
 
     def __init__(self, vals):
-        self.buf = _records_struct(len(vals) // 15).pack(*vals)
-        self.base = address(self.buf)
+        self.buf = buf = _records_struct(len(vals) // 15).pack(*vals)
+        self.base = address(buf)
 
     def at(self, i):
         return self.base + _REC.size * i
@@ -270,9 +270,21 @@ def rec0(ptr, code):
     return (ptr, code, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
+def _address(b):
+    return ctypes.cast(ctypes.c_char_p(b), ctypes.c_void_p).value
+
+
+# the contents of a bytes object lie behind its header in CPython, which is quicker to add than ctypes is to ask
+_HEADER = bytes.__basicsize__ - 1
+
+
 def address(b):
     """Address of a bytes object's contents; it must stay alive until the call returns."""
-    return ctypes.cast(ctypes.c_char_p(b), ctypes.c_void_p).value
+    return id(b) + _HEADER
+
+
+if any(address(b) != _address(b) for b in (b"x", b"records" * 99)):
+    address = _address  # noqa: F811
 
 
 def ref(m):

@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib as L
-from .ops import _inner, _require_cuda
+from .ops import _require_cuda
 
 __all__ = ["BeamSelection", "beam_select", "reorder_states_"]
 
@@ -46,48 +46,56 @@ def beam_select(logits, scores, num=None, *, finished=None, end_token=0):
     name = "beam_select"
     if not (isinstance(logits, torch.Tensor) and isinstance(scores, torch.Tensor)):
         raise TypeError(f"{name}: logits and scores must be tensors")
-    _require_cuda(name, logits, scores, finished)
+    dev = logits.device
+    if not (logits.is_cuda and scores.is_cuda):
+        _require_cuda(name, logits, scores, finished)
     if logits.dtype not in _FLOATS:
         raise TypeError(f"{name}: logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    if scores.dim() != 2 or scores.shape[1] == 0:
-        raise ValueError(f"{name}: scores are (batch, beams), got {tuple(scores.shape)}")
-    b, k = scores.shape
+    shape = scores.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"{name}: scores are (batch, beams), got {tuple(shape)}")
+    b, k = shape
     if logits.dim() == 2 and logits.shape[0] == b * k:
         logits = logits.unflatten(0, (b, k))
-    if logits.dim() != 3 or logits.shape[:2] != scores.shape or logits.shape[2] == 0:
-        raise ValueError(f"{name}: logits are {(b, k, 'V')} or {(b * k, 'V')}, got {tuple(logits.shape)}")
-    v = logits.shape[2]
+    ls = logits.shape
+    if len(ls) != 3 or ls[0] != b or ls[1] != k or ls[2] == 0:
+        raise ValueError(f"{name}: logits are {(b, k, 'V')} or {(b * k, 'V')}, got {tuple(ls)}")
+    v = ls[2]
     num = k if num is None else int(num)
     if k > _MAX_BEAMS or v > _MAX_VOCAB or not 1 <= num <= min(_MAX_NUM, k * v):
         raise ValueError(f"{name}: at most {_MAX_BEAMS} beams, {_MAX_VOCAB} tokens, and 1 to {_MAX_NUM} continuations of "
                          f"those there are; got {k}, {v}, {num}")
-    if not 0 <= int(end_token) < v:
+    end_token = int(end_token)
+    if not 0 <= end_token < v:
         raise ValueError(f"{name}: end_token {end_token} is outside the vocabulary of {v}")
-    at = logits.get_device()
-    if scores.get_device() != at or (finished is not None and finished.get_device() != at):
+    if scores.get_device() != dev.index or (finished is not None and finished.get_device() != dev.index):
         raise RuntimeError(f"{name}: logits, scores and finished must be on one device")
     if scores.dtype is not torch.float32:
         raise TypeError(f"{name}: scores must be float32, got {scores.dtype}")
     if finished is not None:
-        if finished.shape != scores.shape:
+        if finished.shape != shape:
             raise ValueError(f"{name}: finished of shape {tuple(finished.shape)}, expected {(b, k)}")
-        finished = finished.view(torch.uint8) if finished.dtype is torch.bool else (finished != 0).view(torch.uint8)
-    logits = _inner(logits.detach())
-    dev = logits.device
-    out = torch.empty(b, num, dtype=torch.float32, device=dev)
-    parents = torch.empty(b, num, dtype=torch.int64, device=dev)
-    tokens = torch.empty(b, num, dtype=torch.int64, device=dev)
+        if finished.dtype is not torch.bool:
+            finished = finished != 0
+    if logits.stride(2) != 1 and v > 1:
+        logits = logits.contiguous()
+    out = torch.empty((b, num), dtype=torch.float32, device=dev)
+    parents = torch.empty((b, num), dtype=torch.int64, device=dev)
+    tokens = torch.empty_like(parents)
     lib = L.load()
     with L.on_device(dev):
         code = L._DTYPE_CODE[logits.dtype]
         nbytes = lib.m3_beam_select_workspace_size(b, k, v, num, code)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        a = L.Records([*L.rec3(logits, code, b, k, v), *L.rec2(scores, L.M3_FLOAT32, b, k),
-                       *(L.NO_RECORD if finished is None else L.rec2(finished, L.M3_UINT8, b, k)),
-                       *L.rec2(out, L.M3_FLOAT32, b, num), *L.rec2(parents, L.M3_INT64, b, num),
-                       *L.rec2(tokens, L.M3_INT64, b, num)])
-        rc = lib.m3_beam_select(a.at(0), a.at(1), None if finished is None else a.at(2), int(end_token), a.at(3), a.at(4),
-                                a.at(5), ws.data_ptr() or None, nbytes, L.stream_ptr(dev))
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        vals = [*L.rec3(logits, code, b, k, v), *L.rec2(scores, L.M3_FLOAT32, b, k)]
+        vals += L.NO_RECORD if finished is None else L.rec2(finished, L.M3_UINT8, b, k)
+        tail = (2, b, num, 0, 0, 0, 0, num, 1, 0, 0, 0, 0)
+        vals += (out.data_ptr() or 1, L.M3_FLOAT32, *tail, parents.data_ptr() or 1, L.M3_INT64, *tail,
+                 tokens.data_ptr() or 1, L.M3_INT64, *tail)
+        a = L.Records(vals)
+        at = a.base
+        rc = lib.m3_beam_select(at, at + 112, None if finished is None else at + 224, end_token, at + 336, at + 448,
+                                at + 560, ws.data_ptr() or None, nbytes, L.stream_ptr(dev))
     L.check(rc, "m3_beam_select")
     return BeamSelection(out, parents, tokens)
 
@@ -107,14 +115,17 @@ def _pitches(what, ts, rows, index):
         raise RuntimeError(f"reorder_states_: {what} must be CUDA tensors of the parents' device (no CPU path)")
     pitches, sizes = [], []
     for t in ts:
-        shape = t.shape
-        if not shape or shape[0] != rows:
-            raise ValueError(f"reorder_states_: {what} of {rows} rows expected, got {tuple(shape)}")
-        n = t.numel()
-        if not t.is_contiguous() and n and not t[0].is_contiguous():
+        if not t.dim() or t.size(0) != rows:
+            raise ValueError(f"reorder_states_: {what} of {rows} rows expected, got {tuple(t.shape)}")
+        if rows and t.is_contiguous():
+            pitch = t.nbytes // rows
+            pitches.append(pitch)
+            sizes.append(pitch)
+            continue
+        n, es = t.numel(), t.element_size()
+        if n and not t[0].is_contiguous():
             raise ValueError(f"reorder_states_: rows of {what} must be dense in memory, got strides {t.stride()} for "
-                             f"{tuple(shape)}")
-        es = t.element_size()
+                             f"{tuple(t.shape)}")
         pitches.append(t.stride(0) * es)
         sizes.append(n // rows * es if rows else 0)
     return [t.data_ptr() for t in ts], pitches, sizes

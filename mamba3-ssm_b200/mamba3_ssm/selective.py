@@ -141,15 +141,17 @@ def _conv_forward(x, weight, bias, initial, lengths, silu, want):
     b, n, e = x.shape
     k = weight.shape[1]
     dev = x.device
-    y = torch.empty((b, n, e), dtype=x.dtype, device=dev)
+    y = torch.empty_like(x)
     last = torch.empty((b, k - 1, e), dtype=x.dtype, device=dev) if want else None
     vals = _conv_vals(x, weight, bias, initial, lengths, b, n, e, k)
     vals += _r3(y, b, n, e)
     vals += _r3(last, b, k - 1, e)
     a = L.Records(vals)
-    p = [_at(a.base, vals, i) for i in range(7)]
+    at = a.base
     with L.on_device(dev):
-        rc = L.load().m3_causal_conv(p[0], p[1], p[2], p[3], p[4], silu, p[5], p[6], L.stream_ptr(dev))
+        rc = L.load().m3_causal_conv(at, at + 112, at + 224 if bias is not None else None,
+                                     at + 336 if initial is not None else None, at + 448 if lengths is not None else None,
+                                     silu, at + 560, at + 672 if want else None, L.stream_ptr(dev))
     if rc:
         L.check(rc, "m3_causal_conv")
     return y, last
@@ -250,8 +252,10 @@ def causal_conv_step_(state, x, weight, bias=None, *, activation=None):
         raise TypeError(f"{name}: state must be of x's dtype {x.dtype}, got {state.dtype}")
     x = _inner(x)
     dev = x.device
-    y = torch.empty((b, e), dtype=x.dtype, device=dev)
-    vals = [*_r3(state, b, k - 1, e), *_r2(x, b, e), *_r2(weight, e, k), *_r1(bias, e), *_r2(y, b, e)]
+    y = torch.empty_like(x)
+    code = _CODE[x.dtype]
+    vals = [*L.rec3(state, code, b, k - 1, e), *L.rec2(x, code, b, e), *L.rec2(weight, _CODE[weight.dtype], e, k),
+            *_r1(bias, e), y.data_ptr() or 1, code, 2, b, e, 0, 0, 0, 0, e, 1, 0, 0, 0, 0]
     a = L.Records(vals)
     at = a.base
     with L.on_device(dev):
@@ -287,7 +291,7 @@ def _scan_forward(u, delta, A, B, C, D, z, bias, initial, lengths, softplus, wan
     m = A.shape[1]
     dev = u.device
     lib = L.load()
-    y = torch.empty((b, n, e), dtype=u.dtype, device=dev)
+    y = torch.empty_like(u)
     last = torch.empty((b, e, m), dtype=_F32, device=dev) if want else None
     vals = _scan_vals(u, delta, A, B, C, D, z, bias, initial, lengths, b, n, e, m)
     vals += _r3(y, b, n, e)
@@ -437,7 +441,7 @@ def ssm_step_selective_(state, u, delta, A, B_proj, C_proj, D=None, *, z=None, d
     if state.dtype is not _F32:
         raise TypeError(f"{name}: state must be float32, got {state.dtype}")
     dev = u.device
-    y = torch.empty((b, e), dtype=u.dtype, device=dev)
+    y = torch.empty_like(u)
     code = _CODE[B.dtype]
     vals = [*_r3(state, b, e, m), *_r2(u, b, e), *_r2(delta, b, e), *_r2(A, e, m)]
     if B.dim() == 2:  # one group
