@@ -81,15 +81,47 @@ __device__ __forceinline__ Two log_two(const Two& s) {
   return plus(plus(Two{n * 0.693145751953125f, 0.f}, Two{n * 1.42860682030941723212e-6f, 0.f}), logm);
 }
 
-constexpr int kGroups = NT / 4;  // threads whose largest elements give the first threshold
-static_assert(kGroups >= kMaxCandidates, "the first threshold is the num-th largest of the groups' maxima");
+// put(i, r) for each of n <= NT elements, r of which are above element i. As many threads an element as there are for it
+// (one thread an element, or a warp, took 14000 cycles for 128 elements where this takes 1000).
+template <typename X, typename Above, typename Put>
+__device__ __forceinline__ void ranks(const X* x, int n, Above&& above, Put&& put) {
+  int per = 1;
+  while (per < 32 && 2 * per * n <= NT) per *= 2;
+  const int part = threadIdx.x & (per - 1), i = threadIdx.x / per;
+  int r = 0;
+  if (i < n) {
+    const X mine = x[i];
+#pragma unroll 4
+    for (int k = part; k < n; k += per) r += above(x[k], mine);
+  }
+  for (int o = per / 2; o > 0; o /= 2) r += __shfl_xor_sync(0xffffffffu, r, o);
+  if (i < n && part == 0) put(i, r);
+}
+
+// A t with count(t) >= num, bit by bit from the highest of `bits` down to `lowest`: the largest one, or the first whose
+// count, which falls as t rises, is `enough` at most. had: the count, left alone where no bit could be set.
+template <typename Count>
+__device__ __forceinline__ uint64_t bisect(int bits, int lowest, int num, int enough, int* had, Count&& count) {
+  uint64_t t = 0;
+  for (int bit = bits - 1; bit >= lowest; --bit) {
+    const uint64_t with = t | 1ull << bit;
+    const int c = count(with);
+    if (c >= num) {
+      t = with;
+      *had = c;
+      if (c <= enough) break;
+    }
+  }
+  return t;
+}
+constexpr int kRanked = NT / 2;  // more elements than these are cut before they are ranked
+static_assert(kRanked >= kMaxCandidates, "the candidates themselves have to be ranked");
 
 template <typename T, int U>
 struct Rows {
   static constexpr int VN = 16 / sizeof(T), TILE = NT * U * VN;
   static constexpr int CAP = 1024;  // listed elements; more of a tile wait until the threshold has risen
-  uint64_t list[CAP], best[kMaxCandidates];
-  uint32_t group[kGroups];
+  uint64_t list[CAP], best[kRanked];
   Two sum[NT / 32];
   float max[NT / 32];
   int n;
@@ -100,38 +132,50 @@ struct Rows {
 template <typename R>
 __device__ __forceinline__ int compact(R& sh, int num) {
   __syncthreads();
-  const int n = min(sh.n, R::CAP);
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const uint64_t k = sh.list[i];
-    int r = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) r += sh.list[j] > k;
-    if (r < num) sh.best[r] = k;
+  const int n = min(sh.n, R::CAP), m = min(n, num);
+  auto larger = [](uint64_t a, uint64_t b) { return a > b; };
+  if (n > kRanked) {  // (pairs of a full list's elements are too many to compare)
+    int had = n;
+    const uint64_t low = bisect(64, 0, num, kRanked, &had, [&](uint64_t t) {
+      int c = 0;
+      for (int i0 = 0; i0 < n; i0 += NT) c += __syncthreads_count(i0 + (int)threadIdx.x < n && sh.list[i0 + threadIdx.x] >= t);
+      return c;
+    });
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += NT)
+      if (sh.list[i] >= low) sh.best[atomicAdd(&sh.n, 1)] = sh.list[i];
+    __syncthreads();
+    ranks(sh.best, had, larger, [&](int i, int r) {
+      if (r < num) sh.list[r] = sh.best[i];
+    });
+  } else {
+    ranks(sh.list, n, larger, [&](int i, int r) {
+      if (r < num) sh.best[r] = sh.list[i];
+    });
+    __syncthreads();
+    if (threadIdx.x < m) sh.list[threadIdx.x] = sh.best[threadIdx.x];
   }
   __syncthreads();
-  const int m = min(n, num);
-  if (threadIdx.x < m) sh.list[threadIdx.x] = sh.best[threadIdx.x];
   if (threadIdx.x == 0) {
     sh.n = m;
-    if (m == num) sh.tau = max(sh.tau, sh.best[num - 1]);
+    if (m == num) sh.tau = max(sh.tau, sh.list[num - 1]);
   }
   __syncthreads();
   return m;
 }
 
+// Whether a beam's logits are needed at all.
+__device__ __forceinline__ bool beam_counts(const BeamParams& p, int64_t b, int j) {
+  return !(p.finished != nullptr && p.finished[b * p.fb + j * p.fk] != 0) && p.scores[b * p.sb + j * p.sk] != -INFINITY;
+}
+
+// Elements s0 .. s1 - 1 of a row, by one CTA.
 template <typename T, int U>
-__global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part* parts, uint64_t* keys, int seg) {
+__device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, const T* x, int s0, int s1, Part* part, uint64_t* keys) {
   using R = Rows<T, U>;
   constexpr int VN = R::VN, TILE = R::TILE;
-  __shared__ R sh;
   const int tid = threadIdx.x;
-  const int64_t row = blockIdx.y;
-  const int64_t b = row / p.beams;
-  const int j = (int)(row % p.beams);
-  if (p.finished != nullptr && p.finished[b * p.fb + j * p.fk] != 0) return;
-  if (p.scores[b * p.sb + j * p.sk] == -INFINITY) return;
-  const T* x = static_cast<const T*>(p.logits) + b * p.lb + j * p.lk;
-  const int s0 = blockIdx.x * seg, s1 = min(p.V, s0 + seg);
   // vectors lie on 16-byte boundaries: the first begins up to VN - 1 elements in front of the part
   const int off = (int)((reinterpret_cast<uintptr_t>(x + s0) & 15) / sizeof(T));
   if (tid == 0) { sh.n = 0; sh.tau = 0; }
@@ -240,19 +284,11 @@ __global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part*
         sum += a0 + a1;
       }
       if (t0 == begin) {
-        // the first threshold: just below the num-th largest of the maxima of groups of four threads
-        uint32_t o = ordered(tm);
-        o = max(o, __shfl_xor_sync(0xffffffffu, o, 1));
-        o = max(o, __shfl_xor_sync(0xffffffffu, o, 2));
-        if ((tid & 3) == 0) sh.group[tid >> 2] = o;
-        __syncthreads();
-        if (tid < kGroups) {
-          const uint32_t mine = sh.group[tid];
-          int r = 0;
-#pragma unroll 8
-          for (int i = 0; i < kGroups; ++i) r += sh.group[i] > mine || (sh.group[i] == mine && i < tid);
-          if (r == p.num - 1) sh.tau = ((uint64_t)mine << 32) - 1;
-        }
+        // the first threshold: just below what the maxima of `num` threads reach, to the upper 16 bits
+        const uint32_t o = ordered(tm);
+        int had = 0;
+        const uint32_t low = (uint32_t)bisect(32, 16, p.num, p.num, &had, [&](uint64_t t) { return __syncthreads_count(o >= (uint32_t)t); });
+        if (tid == 0) sh.tau = ((uint64_t)max(low, ordered(-INFINITY)) << 32) - 1;  // (what lies below -inf are NaNs)
         __syncthreads();
       }
       uint32_t left = ~0u;
@@ -286,8 +322,7 @@ __global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part*
     held = compact(sh, p.num);
   }
   const int n = held;
-  const int64_t part = row * gridDim.x + blockIdx.x;
-  if (tid < n) keys[part * p.num + tid] = sh.list[tid];
+  if (tid < n) keys[tid] = sh.list[tid];
   // the sum over the CTA, to one base
   float m = run;
 #pragma unroll
@@ -305,8 +340,18 @@ __global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part*
   if (tid == 0) {
 #pragma unroll
     for (int w = 1; w < NT / 32; ++w) d.add(sh.sum[w]);
-    parts[part] = Part{d, m, n};
+    *part = Part{d, m, n};
   }
+}
+
+template <typename T, int U>
+__global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part* parts, uint64_t* keys, int seg) {
+  __shared__ Rows<T, U> sh;
+  const int64_t row = blockIdx.y, b = row / p.beams;
+  const int j = (int)(row % p.beams), s0 = blockIdx.x * seg;
+  if (!beam_counts(p, b, j)) return;
+  const int64_t part = row * gridDim.x + blockIdx.x;
+  row_part<T, U>(p, sh, static_cast<const T*>(p.logits) + b * p.lb + j * p.lk, s0, min(p.V, s0 + seg), parts + part, keys + part * p.num);
 }
 
 struct Cand { uint64_t value, tie; };  // score in order of integers; then beam, logit, token
@@ -319,24 +364,30 @@ __device__ __forceinline__ uint64_t tie_of(int beam, uint32_t logit, int token) 
   return ((uint64_t)(63 - beam) << (32 + kTokenBits)) | ((uint64_t)logit << kTokenBits) | (uint32_t)((1 << kTokenBits) - 1 - token);
 }
 
-// Lists that reach into the num best are num at most, with num elements each.
-__host__ __device__ inline int most_candidates(int lists, int num) { return (lists < num ? lists : num) * num; }
+// Lists that reach into the num best are num at most, with num elements each; twice as many are let through where they are
+// not told apart at once.
+constexpr int kHeads = 2;
+__host__ __device__ inline int most_candidates(int lists, int num) { return (lists < kHeads * num ? lists : kHeads * num) * num; }
 
-__global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const Part* parts, const uint64_t* keys, int splits) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  Cand* head = reinterpret_cast<Cand*>(smem_raw);  // beams * splits
-  Cand* cand = head + p.beams * splits;            // most_candidates
+__host__ __device__ inline size_t join_bytes(int lists, int num) { return (size_t)(lists + most_candidates(lists, num)) * sizeof(Cand); }
+
+// A prompt's continuations from the parts of its beams' rows, by one CTA. room: join_bytes.
+__device__ __forceinline__ void join_parts(const BeamParams& p, int64_t b, const Part* parts, const uint64_t* keys, int splits,
+                                           unsigned char* room) {
+  Cand* head = reinterpret_cast<Cand*>(room);  // beams * splits
+  Cand* cand = head + p.beams * splits;        // most_candidates
   // a logarithm of probability is (l - max) - log(sum): l - (max + log(sum)) would lose the digits of large logits
   __shared__ float s_max[kMaxBeams], s_score[kMaxBeams];
   __shared__ Two s_log[kMaxBeams];
-  __shared__ int s_kind[kMaxBeams], s_n;                 // 0 listed, 1 ended, 2 nothing, 3 NaN
-  __shared__ Cand s_tau;
+  __shared__ int s_kind[kMaxBeams];  // 0 listed, 1 ended, 2 nothing, 3 NaN
+  __shared__ int s_n, s_lists, s_list[kHeads * kMaxCandidates];  // candidates; lists that may hold some of the best
+  __shared__ uint64_t s_tau;
+  __shared__ Cand s_best[kRanked];
   const int tid = threadIdx.x, lane = tid & 31, K = p.beams, lists = K * splits;
-  const int64_t b = blockIdx.x;
-  if (tid == 0) { s_n = 0; s_tau = Cand{0, 0}; }
+  if (tid == 0) { s_n = 0; s_lists = 0; s_tau = 0; }
   // what the first element of this thread's list will need, on its way while the sums are joined (not used where it was not written)
-  const int first_n = tid < lists ? parts[b * lists + tid].n : 0;
-  const uint64_t first_key = tid < lists ? keys[(b * lists + tid) * p.num] : 0;
+  const int first_n = tid < lists ? parts[tid].n : 0;
+  const uint64_t first_key = tid < lists ? keys[tid * p.num] : 0;
   // a warp a beam joins its parts' sums
   for (int j = tid >> 5; j < K; j += NT / 32) {
     const float score = p.scores[b * p.sb + j * p.sk];
@@ -347,7 +398,7 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
     else if (!(score < INFINITY)) kind = 3;
     else if (p.finished != nullptr && p.finished[b * p.fb + j * p.fk] != 0) kind = 1;
     else {
-      const Part* q = parts + (b * K + j) * splits;
+      const Part* q = parts + j * splits;
       const Part mine = lane < splits ? q[lane] : Part{Two{0.f, 0.f}, -INFINITY, 0};
       float m = mine.max;
       for (int i = lane + 32; i < splits; i += 32) m = fmaxf(m, q[i].max);
@@ -394,66 +445,149 @@ __global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const
     *c = Cand{kind == 3 ? ~0ull : ordered64(Two{-INFINITY, 0.f}), tie_of(j, 0, token)};
     return true;
   };
-  auto get = [&](int l, int i, Cand* c) { return make(l, i, parts[b * lists + l].n, keys[(b * lists + l) * p.num + i], c); };
+  auto get = [&](int l, int i, Cand* c) { return make(l, i, parts[l].n, keys[l * p.num + i], c); };
   if (tid < lists && !make(tid, 0, first_n, first_key, &head[tid])) head[tid] = Cand{0, 0};
   for (int l = tid + NT; l < lists; l += NT)
     if (!get(l, 0, &head[l])) head[l] = Cand{0, 0};
   __syncthreads();
   // nothing below the num-th best head can be among the num best
-  if (lists > p.num) {
+  uint64_t tau = 0;
+  if (lists <= kRanked) {
+    ranks(head, lists, [](const Cand& a, const Cand& b) { return above(a, b); }, [&](int l, int r) {
+      if (r == p.num - 1) s_tau = head[l].value;
+      if (r < p.num && head[l].tie != 0) s_list[atomicAdd(&s_lists, 1)] = l;
+    });
+    __syncthreads();
+    tau = s_tau;
+  } else {
+    int had = 0;
+    tau = bisect(64, 0, p.num, kHeads * p.num, &had, [&](uint64_t t) {
+      int c = 0;
+      for (int l0 = 0; l0 < lists; l0 += NT) c += __syncthreads_count(l0 + tid < lists && head[l0 + tid].value >= t);
+      return c;
+    });
+    const bool equal = had > kHeads * p.num;  // heads, of which the first lists (and beams) come first
     for (int l = tid; l < lists; l += NT) {
-      // (equal values in the order of the lists, which is that of their beams)
-      const Cand mine = head[l];
+      const uint64_t mine = head[l].value;
+      if (head[l].tie == 0 || mine < tau) continue;
       int r = 0;
-#pragma unroll 4
-      for (int i = 0; i < l; ++i) r += head[i].value >= mine.value;
-#pragma unroll 4
-      for (int i = l + 1; i < lists; ++i) r += head[i].value > mine.value;
-      if (r == p.num - 1 && mine.tie != 0) s_tau = mine;
-      if (r >= p.num) head[l].tie = 0;  // the list is left out
+      if (equal) {
+        for (int i = 0; i < lists; ++i) r += head[i].value > mine || (head[i].value == mine && i < l);
+      }
+      if (r < p.num) s_list[atomicAdd(&s_lists, 1)] = l;
     }
     __syncthreads();
   }
-  const Cand tau = s_tau;
-  for (int i = tid; i < lists * p.num; i += NT) {
-    const int l = i / p.num;
-    const Cand h = head[l];
+  const int left = s_lists * p.num;
+  for (int i = tid; i < left; i += NT) {
     Cand c;
-    if (h.tie != 0 && get(l, i % p.num, &c) && !above(tau, c)) cand[atomicAdd(&s_n, 1)] = c;
+    if (get(s_list[i / p.num], i % p.num, &c) && c.value >= tau) cand[atomicAdd(&s_n, 1)] = c;
   }
   __syncthreads();
-  const int n = s_n;
-  for (int i = tid >> 5; i < n; i += NT / 32) {  // a warp a candidate: how many are above it
-    const Cand mine = cand[i];
-    int r = 0;
-    for (int k = lane; k - lane < n; k += 32) r += __popc(__ballot_sync(0xffffffffu, k < n && above(cand[k], mine)));
-    if (lane == 0 && r < p.num) {
-      const int64_t at = b * p.num + r;
-      p.out_scores[at] = score_of(mine.value);
-      p.parents[at] = 63 - (int)(mine.tie >> (32 + kTokenBits));
-      p.tokens[at] = (1 << kTokenBits) - 1 - (int)(mine.tie & ((1 << kTokenBits) - 1));
-    }
+  int n = s_n;
+  const Cand* from = cand;
+  if (n > kRanked) {  // the best of them, the last of which is found bit by bit: its value, and among many equal ones its tie
+    int had = n;
+    auto at_least = [&](uint64_t value, uint64_t tie) {
+      int c = 0;
+      for (int i0 = 0; i0 < n; i0 += NT) {
+        const int i = i0 + tid;
+        c += __syncthreads_count(i < n && (cand[i].value > value || (cand[i].value == value && cand[i].tie >= tie)));
+      }
+      return c;
+    };
+    Cand low{0, 0};
+    low.value = bisect(64, 0, p.num, kRanked, &had, [&](uint64_t t) { return at_least(t, 0); });
+    if (had > kRanked) low.tie = bisect(64, 0, p.num, kRanked, &had, [&](uint64_t t) { return at_least(low.value, t); });
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += NT)
+      if (!above(low, cand[i])) s_best[atomicAdd(&s_n, 1)] = cand[i];
+    __syncthreads();
+    from = s_best;
+    n = had;
   }
+  ranks(from, n, [](const Cand& a, const Cand& b) { return above(a, b); }, [&](int i, int r) {
+    if (r >= p.num) return;
+    const Cand c = from[i];
+    const int64_t at = b * p.num + r;
+    p.out_scores[at] = score_of(c.value);
+    p.parents[at] = 63 - (int)(c.tie >> (32 + kTokenBits));
+    p.tokens[at] = (1 << kTokenBits) - 1 - (int)(c.tie & ((1 << kTokenBits) - 1));
+  });
 }
 
-#ifndef M3_W
-#define M3_W 4
-#endif
-#ifndef M3_U
-#define M3_U 4
-#endif
-struct BeamPlan { int u, seg, splits; };
+__global__ void __launch_bounds__(NT) beam_join_kernel(const BeamParams p, const Part* parts, const uint64_t* keys, int splits) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const int64_t b = blockIdx.x, lists = (int64_t)p.beams * splits;
+  join_parts(p, b, parts + b * lists, keys + b * lists * p.num, splits, smem_raw);
+}
 
-// Parts of a row: tiles of four vectors a thread where the rows alone fill the GPU, of one where they do not;
-// then as many parts as bring the rows to about four CTAs an SM.
-BeamPlan plan(int64_t rows, int V, int es, int sms) {
+// Both in one launch for few and small prompts, where the second launch and the workspace would cost more than they
+// spread: a cluster of eight CTAs a prompt, with a part each, which go into the first one's shared memory, which joins them.
+constexpr int kCluster = 8;
+constexpr int kClusterPart = 32768;  // elements a CTA
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+template <typename X>
+__device__ __forceinline__ X* of_first(X* p) {  // the same place in the shared memory of the cluster's first CTA
+  uint64_t r;
+  asm("mapa.u64 %0, %1, 0;" : "=l"(r) : "l"((uint64_t)p));
+  return reinterpret_cast<X*>(r);
+}
+
+template <typename T, int U>
+__global__ void __launch_bounds__(NT) beam_cluster_kernel(const BeamParams p, int splits, int seg) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ Rows<T, U> sh;
+  const int lists = p.beams * splits, rank = blockIdx.x % kCluster;
+  const int64_t b = blockIdx.x / kCluster;
+  Part* parts = reinterpret_cast<Part*>(smem_raw);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(parts + lists);
+  cluster_arrive();  // every CTA runs before any writes into the first one's memory
+  cluster_wait();
+  if (rank < lists) {
+    const int j = rank / splits, s0 = rank % splits * seg;
+    if (beam_counts(p, b, j) && s0 < p.V)
+      row_part<T, U>(p, sh, static_cast<const T*>(p.logits) + b * p.lb + j * p.lk, s0, min(p.V, s0 + seg), of_first(parts + rank),
+                     of_first(keys + rank * p.num));
+    else if (threadIdx.x == 0)
+      *of_first(parts + rank) = Part{Two{0.f, 0.f}, -INFINITY, 0};
+  }
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0) join_parts(p, b, parts, keys, splits, reinterpret_cast<unsigned char*>(keys + lists * p.num));
+}
+
+struct BeamPlan {
+  bool cluster;
+  int u, seg, splits;
+};
+
+// In one launch, as many parts a row as there are CTAs of the cluster for it. In two, tiles of four vectors a
+// thread where the rows alone fill the GPU, of one where they do not, and as many parts as bring the rows to about four CTAs
+// an SM (finer parts cost more in thresholds than their balance gives: 48 us at eight an SM, 42 at four, 64 x 8 rows of 131072).
+BeamPlan plan(int64_t batch, int beams, int V, int num, int es, int sms) {
   const int vn = 16 / es;
   BeamPlan w;
-  const int64_t big = (V + M3_U * NT * vn - 1) / (M3_U * NT * vn);
-  w.u = rows * big >= 2 * sms ? M3_U : 1;
+  const int64_t rows = batch * beams;
+  w.splits = beams <= kCluster ? kCluster / beams : 0;
+  const int one = w.splits > 0 ? (V + w.splits - 1) / w.splits : 0;
+  // One launch, two launches, us a call by itself (and in a CUDA graph, without the host): 1 x 4 x 16384 of 8: 19.0, 24.8
+  // (9.3, 8.8); 32 x 4 x 16384 of 8: 19.0, 24.6 (10.5, 12.6); 1 x 4 x 50000 of 4: 19.0, 25.0 (12.1, 11.3), of 16: 20.7, 24.8
+  // (18.6, 11.7). Of more prompts than the GPU holds at once the clusters would take turns.
+  w.cluster = w.splits > 0 && one <= kClusterPart && batch * kCluster <= 2 * sms;
+  if (w.cluster) {
+    w.seg = (one + vn - 1) / vn * vn;
+    w.u = w.seg > 2 * NT * vn ? 4 : 1;
+    return w;
+  }
+  const int64_t big = (V + 4 * NT * vn - 1) / (4 * NT * vn);
+  w.u = rows * big >= 2 * sms ? 4 : 1;
   const int tile = NT * w.u * vn;
   const int64_t tiles = (V + tile - 1) / tile;
-  const int64_t want = std::max<int64_t>(1, (int64_t)M3_W * sms / std::max<int64_t>(1, rows));
+  const int64_t want = std::max<int64_t>(1, (int64_t)4 * sms / std::max<int64_t>(1, rows));
   const int64_t per = (tiles + std::min(want, tiles) - 1) / std::min(want, tiles);
   w.seg = (int)(per * tile);
   w.splits = (int)((V + w.seg - 1) / w.seg);
@@ -465,35 +599,56 @@ constexpr int kMaxLists = 4096;
 }  // namespace
 
 size_t beam_workspace_bytes(int64_t batch, int beams, int V, int num, int dtype, int sms) {
-  const int64_t rows = batch * beams;
-  const BeamPlan w = plan(rows, V, (int)dtype_size(dtype), sms);
-  return (size_t)rows * w.splits * (sizeof(Part) + (size_t)num * sizeof(uint64_t));
+  const BeamPlan w = plan(batch, beams, V, num, (int)dtype_size(dtype), sms);
+  return w.cluster ? 0 : (size_t)batch * beams * w.splits * (sizeof(Part) + (size_t)num * sizeof(uint64_t));
+}
+
+template <typename T, int U>
+static int launch_cluster(const BeamParams& p, const BeamPlan& w, cudaStream_t s) {
+  const int lists = p.beams * w.splits;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kCluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.batch * kCluster));
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = (size_t)lists * (sizeof(Part) + p.num * sizeof(uint64_t)) + join_bytes(lists, p.num);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, beam_cluster_kernel<T, U>, p, w.splits, w.seg);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(M3_ERR_CUDA, std::string("beam_cluster_kernel: ") + cudaGetErrorString(e));
+  }
+  return M3_OK;
 }
 
 int launch_beam_select(const BeamParams& p, int dtype, void* ws, cudaStream_t s) {
   int sms = 0;
   M3_TRY(device_sm_count(&sms));
   const int64_t rows = p.batch * p.beams;
-  const BeamPlan w = plan(rows, p.V, (int)dtype_size(dtype), sms);
+  const BeamPlan w = plan(p.batch, p.beams, p.V, p.num, (int)dtype_size(dtype), sms);
   if (p.beams * w.splits > kMaxLists) return fail(M3_ERR_UNSUPPORTED, "beam_select: too many parts");
   Part* parts = static_cast<Part*>(ws);
   uint64_t* keys = reinterpret_cast<uint64_t*>(parts + rows * w.splits);
   const dim3 grid((unsigned)w.splits, (unsigned)rows);
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (w.u == M3_U) beam_rows_kernel<T, M3_U><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
+    if (w.cluster) return w.u == 4 ? launch_cluster<T, 4>(p, w, s) : launch_cluster<T, 1>(p, w, s);
+    if (w.u == 4) beam_rows_kernel<T, 4><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
     else beam_rows_kernel<T, 1><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
     return check_launch("beam_rows_kernel");
   };
   if (dtype == M3_FLOAT32) M3_TRY(go(float{}));
   else if (dtype == M3_BFLOAT16) M3_TRY(go(__nv_bfloat16{}));
   else M3_TRY(go(__half{}));
+  if (w.cluster) return M3_OK;
   static std::atomic<bool> done[kMaxDevices];
-  const size_t most = (size_t)(kMaxCandidates * kMaxCandidates + kMaxLists) * sizeof(Cand);
+  const size_t most = join_bytes(kMaxLists, kMaxCandidates);
   M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(&beam_join_kernel), most, done));
-  const int lists = p.beams * w.splits;
-  const size_t smem = (size_t)(lists + most_candidates(lists, p.num)) * sizeof(Cand);
-  beam_join_kernel<<<(unsigned)p.batch, NT, smem, s>>>(p, parts, keys, w.splits);
+  beam_join_kernel<<<(unsigned)p.batch, NT, join_bytes(p.beams * w.splits, p.num), s>>>(p, parts, keys, w.splits);
   return check_launch("beam_join_kernel");
 }
 

@@ -1765,8 +1765,8 @@ int m3_beam_select(const m3_tensor* logits, const m3_tensor* scores, const m3_te
     }
   }
   if (batch == 0) return M3_OK;
-  M3_TRY(workspace_ok(workspace, workspace_bytes,
-                      beam_workspace_bytes(batch, (int)K, (int)V, (int)num, logits->dtype, sms_here()), "beam_select"));
+  const size_t need = beam_workspace_bytes(batch, (int)K, (int)V, (int)num, logits->dtype, sms_here());
+  if (need > 0) M3_TRY(workspace_ok(workspace, workspace_bytes, need, "beam_select"));
   BeamParams p{};
   p.logits = logits->data; p.lb = logits->stride[0]; p.lk = logits->stride[1];
   p.scores = sc.p; p.sb = sc.sb; p.sk = sc.st;

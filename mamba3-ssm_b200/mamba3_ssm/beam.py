@@ -86,7 +86,7 @@ def beam_select(logits, scores, num=None, *, finished=None, end_token=0):
     with L.on_device(dev):
         code = L._DTYPE_CODE[logits.dtype]
         nbytes = lib.m3_beam_select_workspace_size(b, k, v, num, code)
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None  # none where one launch does
         vals = [*L.rec3(logits, code, b, k, v), *L.rec2(scores, L.M3_FLOAT32, b, k)]
         vals += L.NO_RECORD if finished is None else L.rec2(finished, L.M3_UINT8, b, k)
         tail = (2, b, num, 0, 0, 0, 0, num, 1, 0, 0, 0, 0)
@@ -95,7 +95,7 @@ def beam_select(logits, scores, num=None, *, finished=None, end_token=0):
         a = L.Records(vals)
         at = a.base
         rc = lib.m3_beam_select(at, at + 112, None if finished is None else at + 224, end_token, at + 336, at + 448,
-                                at + 560, ws.data_ptr() or None, nbytes, L.stream_ptr(dev))
+                                at + 560, ws.data_ptr() if nbytes else None, nbytes, L.stream_ptr(dev))
     L.check(rc, "m3_beam_select")
     return BeamSelection(out, parents, tokens)
 

@@ -1,7 +1,7 @@
 """beam_select and reorder_states_ against plain implementations (the selection in float64).
 
 Scores: exp and sums in 32 bits a thread (each off by at most 2^-21 relative: the hardware's 2^x, its
-argument for elements that matter, and additions), joined in 64 bits, so a log-sum is off by at most
+argument for elements that matter, and additions), joined in two floats, so a log-sum is off by at most
 2^-20 absolute; the returned score is rounded to fp32 once. Which candidates are chosen is compared exactly
 where the float64 scores of neighbours are further apart than that, or equal."""
 
@@ -84,6 +84,19 @@ def test_ties_go_to_the_lowest_beam_and_token(dtype):
     logits[1, :, ::3] = -0.0  # equal to 0
     logits[1, 2, 5:9] = 2.0
     check(logits, torch.tensor([[0.0, 0.0, 0.0], [-1.0, -2.0, -1.0]], device=DEV), 40)
+
+
+@pytest.mark.parametrize("b,k,v,num,equal", [
+    (1, 32, 40, 64, True), (2, 32, 3000, 64, False), (1, 8, 20000, 64, True), (1, 7, 5001, 14, False), (1, 3, 70000, 64, False),
+    (38, 2, 2050, 4, False), (37, 5, 999, 8, True), (1, 6, 3, 18, False)])
+def test_many_candidates_and_one_or_two_launches(b, k, v, num, equal):
+    # equal: few values, so that most of what is ranked at the end differs in its beam and token alone
+    logits, scores = inputs(b, k, v, torch.float32, seed=k + v)
+    if equal:
+        logits = (logits * 0.5).round()
+        scores = torch.zeros_like(scores)
+    check(logits, scores, num)
+    check(logits.bfloat16(), scores, num)
 
 
 @pytest.mark.parametrize("order", ["ascending", "descending", "blocks"])

@@ -207,7 +207,8 @@ def test_beam_refusals(lib):
     _says(lib, select(num=0), 1, b"candidates")
     _says(lib, select(l=(0, 2, 100), num=65), 2, b"more than 64")
     _says(lib, select(pt=F32), 1, b"parents")
-    assert lib.m3_beam_select_workspace_size(1, 4, 50000, 4, BF16) > 0
+    assert lib.m3_beam_select_workspace_size(64, 8, 50000, 4, BF16) > 0
+    assert lib.m3_beam_select_workspace_size(1, 4, 50000, 4, BF16) == 0  # one launch, which needs none
     assert lib.m3_beam_select_workspace_size(1, 33, 50000, 4, BF16) == 0
 
 
