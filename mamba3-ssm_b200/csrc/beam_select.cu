@@ -344,8 +344,9 @@ __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, co
   }
 }
 
+// (three CTAs an SM, at 80 registers a thread: 43 us at 64 x 8 x 131072; two 50, four, which spill, 72)
 template <typename T, int U>
-__global__ void __launch_bounds__(NT) beam_rows_kernel(const BeamParams p, Part* parts, uint64_t* keys, int seg) {
+__global__ void __launch_bounds__(NT, 3) beam_rows_kernel(const BeamParams p, Part* parts, uint64_t* keys, int seg) {
   __shared__ Rows<T, U> sh;
   const int64_t row = blockIdx.y, b = row / p.beams;
   const int j = (int)(row % p.beams), s0 = blockIdx.x * seg;
