@@ -5,6 +5,11 @@
 // memory as (row, step), so that a lane reads four steps of one operand at once; the sums over a
 // channel's lanes are formed for several steps together by halving exchanges, and y leaves
 // through shared memory in whole rows. The next tile's operands are loaded while this one is scanned.
+//
+// Bound by the issue of instructions: about 11 a step, channel and state, of which the exponential alone holds its unit (16 a
+// clock and SM) for as long as eight issues. 8 x 2048 x 2048 x 16 of bf16 with a gate take 309 us (270 MB and the states that the
+// backward needs, 537 MB, at 1.7 TB/s; the exponentials alone would take 120). In other shapes, us: 128 threads 327; 32 threads and
+// two channels a lane 344, 64 and two 331 to 348; a quarter of the decays by a polynomial on the FMA pipe 323; K = 2, P = 8 727.
 #include <algorithm>
 #include <type_traits>
 
@@ -16,40 +21,28 @@ namespace {
 constexpr int TT = kSelTile;
 constexpr int TS = kSelPitch;
 
-// states of a lane whose decays the FMA pipe forms
-#ifndef M3_POLY
-#define M3_POLY 0
-#endif
-template <int K> constexpr int kPolyStates() { return K >= 4 ? M3_POLY : 0; }
-
 // steps whose sums over the lanes are formed together
 template <int P> constexpr int group_steps() { return P < 4 ? 4 : P; }
 
-template <int K, int P, int M, int NT>
+template <int K, int P, int NT>
 struct FwdSmem {
-  static constexpr int NP = K * P, EC = NT / P * M;
+  static constexpr int NP = K * P, EC = NT / P;
   float dt[EC][TS], dx[EC][TS];
   float B[NP][TS], C[NP][TS];
   float y[TT][EC + 8];
 };
 
-template <int NT>
-__device__ __forceinline__ void tile_sync() {
-  if constexpr (NT == 32) __syncwarp();
-  else __syncthreads();
-}
-
 // OUT: the scan proper. Else only the state that a piece of the sequence leaves, from zero, and
 // the sum of its step sizes. FAST: every operand is of u's type and read two elements at a time.
-template <typename T, int K, int P, int M, int NT, bool OUT, bool FAST>
+template <typename T, int K, int P, int NT, bool OUT, bool FAST>
 __global__ void __launch_bounds__(NT) sel_scan_kernel(const SelScanParams p) {
-  using S = FwdSmem<K, P, M, NT>;
+  using S = FwdSmem<K, P, NT>;
   constexpr int NP = S::NP, EC = S::EC, GS = group_steps<P>();
-  constexpr int R = TT * M / (2 * P) > 0 ? TT * M / (2 * P) : 1;  // steps of a pair of channels that a thread brings
-  constexpr bool kAhead = BcTile<T, K, P, NT, FAST>::J <= 2;      // B and C of the next tile are loaded ahead too
+  constexpr int R = TT / (2 * P) > 0 ? TT / (2 * P) : 1;  // steps of a pair of channels that a thread brings
+  constexpr bool kAhead = BcTile<T, K, P, NT, FAST>::J <= 2;  // B and C of the next tile are loaded ahead too
   extern __shared__ __align__(16) unsigned char smem_raw[];
   S& sh = *reinterpret_cast<S*>(smem_raw);
-  const int tid = threadIdx.x, q = tid % P, el = tid / P;  // channels el, el + NT / P, ..
+  const int tid = threadIdx.x, q = tid % P, el = tid / P;
   const int Eg = p.E / p.G, tiles = (Eg + EC - 1) / EC;
   const int g = blockIdx.x / tiles, e_first = g * Eg + (blockIdx.x % tiles) * EC, e_end = (g + 1) * Eg;
   const int b = blockIdx.z, c = blockIdx.y;
@@ -63,20 +56,16 @@ __global__ void __launch_bounds__(NT) sel_scan_kernel(const SelScanParams p) {
   const bool lelive = brings && e_first + le < e_end;
   const bool vu = FAST || p.vec_u, vd = FAST || p.vec_d, vz = FAST || p.vec_z, vy = FAST || p.vec_y;
 
-  float A2[M][K], h[M][K], dts[M];
+  float A2[K], h[K], dts = 0.f;
+  const int ec = min(e_first + el, e_end - 1);
 #pragma unroll
-  for (int m = 0; m < M; ++m) {
-    const int ec = min(e_first + el + m * (NT / P), e_end - 1);
-    dts[m] = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int n = q * K + k;
-      A2[m][k] = n < p.N ? p.A[(int64_t)ec * p.N + n] * kLog2e : 0.f;
-      h[m][k] = 0.f;
-      if (OUT) {
-        if (p.nchunk > 1) h[m][k] = p.states[(((int64_t)b * p.nchunk + c) * p.E + ec) * NP + n];
-        else if (p.h0 != nullptr && n < p.N) h[m][k] = p.h0[((int64_t)b * p.E + ec) * p.N + n];
-      }
+  for (int k = 0; k < K; ++k) {
+    const int n = q * K + k;
+    A2[k] = n < p.N ? p.A[(int64_t)ec * p.N + n] * kLog2e : 0.f;
+    h[k] = 0.f;
+    if (OUT) {
+      if (p.nchunk > 1) h[k] = p.states[(((int64_t)b * p.nchunk + c) * p.E + ec) * NP + n];
+      else if (p.h0 != nullptr && n < p.N) h[k] = p.h0[((int64_t)b * p.E + ec) * p.N + n];
     }
   }
   const float bias0 = p.bias != nullptr ? p.bias[l0] : 0.f, bias1 = p.bias != nullptr ? p.bias[l0 + second] : 0.f;
@@ -133,7 +122,7 @@ __global__ void __launch_bounds__(NT) sel_scan_kernel(const SelScanParams p) {
     }
     tb.put(sh.B, p.bc_f32, p.N, t0, len, tid);
     if (OUT) tc.put(sh.C, p.bc_f32, p.N, t0, len, tid);
-    tile_sync<NT>();
+    __syncthreads();
     if (OUT && zp != nullptr && brings) {
 #pragma unroll
       for (int j = 0; j < R; ++j) zz[j] = load2<T>(zp + (int64_t)min(t0 + lt + j, len - 1) * p.z.sl, vz, second);
@@ -144,83 +133,60 @@ __global__ void __launch_bounds__(NT) sel_scan_kernel(const SelScanParams p) {
     }
     constexpr int BS = GS < kSelSub ? kSelSub : GS;  // steps between two looks at whether states are kept
 #pragma unroll 1
-    for (int tb8 = 0; tb8 < TT; tb8 += BS) {
+    for (int tb8 = 0; tb8 < TT; tb8 += BS)
 #pragma unroll
-    for (int tg = tb8; tg < tb8 + BS; tg += GS) {
-      float yv[M][GS];
+      for (int tg = tb8; tg < tb8 + BS; tg += GS) {
+        float yv[GS];
 #pragma unroll
-      for (int i4 = 0; i4 < GS; i4 += 4) {
-        if (OUT && (GS < kSelSub ? tg == tb8 : i4 % kSelSub == 0) && p.save != nullptr && t0 + tg + i4 < len) {
-          float* sv = p.save + (((int64_t)b * ((p.L + kSelSub - 1) / kSelSub) + (t0 + tg + i4) / kSelSub) * p.E + e_first + el) * NP + q * K;
-#pragma unroll
-          for (int m = 0; m < M; ++m)
-            if (e_first + el + m * (NT / P) < e_end) {
-              float* at = sv + (int64_t)m * (NT / P) * NP;
-              if constexpr (K == 4) *reinterpret_cast<float4*>(at) = make_float4(h[m][0], h[m][1], h[m][2], h[m][3]);
+        for (int i4 = 0; i4 < GS; i4 += 4) {
+          if (OUT && (GS < kSelSub ? tg == tb8 : i4 % kSelSub == 0) && p.save != nullptr && t0 + tg + i4 < len) {
+            float* sv = p.save + (((int64_t)b * ((p.L + kSelSub - 1) / kSelSub) + (t0 + tg + i4) / kSelSub) * p.E + e_first + el) * NP + q * K;
+            if (e_first + el < e_end) {
+              if constexpr (K == 4) *reinterpret_cast<float4*>(sv) = make_float4(h[0], h[1], h[2], h[3]);
               else {
 #pragma unroll
-                for (int k = 0; k < K; ++k) at[k] = h[m][k];
+                for (int k = 0; k < K; ++k) sv[k] = h[k];
               }
             }
-        }
-        ulonglong2 d4[M], x4[M];
-        f2 ya[M], yb[M];
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-          d4[m] = *reinterpret_cast<const ulonglong2*>(&sh.dt[el + m * (NT / P)][tg + i4]);
-          x4[m] = *reinterpret_cast<const ulonglong2*>(&sh.dx[el + m * (NT / P)][tg + i4]);
-          ya[m] = yb[m] = 0;
+          }
+          const ulonglong2 d4 = *reinterpret_cast<const ulonglong2*>(&sh.dt[el][tg + i4]);
+          const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(&sh.dx[el][tg + i4]);
+          f2 ya = 0, yb = 0;
           if (!OUT) {
             float s0, s1;
-            unpack2(add2(d4[m].x, d4[m].y), s0, s1);
-            dts[m] += s0 + s1;
+            unpack2(add2(d4.x, d4.y), s0, s1);
+            dts += s0 + s1;
           }
-        }
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const ulonglong2 b4 = *reinterpret_cast<const ulonglong2*>(&sh.B[k * P + q][tg + i4]);
-          ulonglong2 c4{0, 0};
-          if (OUT) c4 = *reinterpret_cast<const ulonglong2*>(&sh.C[k * P + q][tg + i4]);
-#pragma unroll
-          for (int m = 0; m < M; ++m) {
-            const f2 A2k = pack2(A2[m][k], A2[m][k]), mean = pack2(kEx2Mean, kEx2Mean);
+          for (int k = 0; k < K; ++k) {
+            const ulonglong2 b4 = *reinterpret_cast<const ulonglong2*>(&sh.B[k * P + q][tg + i4]);
+            ulonglong2 c4{0, 0};
+            if (OUT) c4 = *reinterpret_cast<const ulonglong2*>(&sh.C[k * P + q][tg + i4]);
+            const f2 A2k = pack2(A2[k], A2[k]), mean = pack2(kEx2Mean, kEx2Mean);
             float a[4], x[4], hv[4];
-            if (k < kPolyStates<K>()) {
-              unpack2(ex2_poly2(mul2(d4[m].x, A2k)), a[0], a[1]);
-              unpack2(ex2_poly2(mul2(d4[m].y, A2k)), a[2], a[3]);
-            } else {
-              unpack2(fma2(d4[m].x, A2k, mean), a[0], a[1]);
-              unpack2(fma2(d4[m].y, A2k, mean), a[2], a[3]);
+            unpack2(fma2(d4.x, A2k, mean), a[0], a[1]);
+            unpack2(fma2(d4.y, A2k, mean), a[2], a[3]);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) a[i] = ex2(a[i]);
-            }
-            unpack2(mul2(x4[m].x, b4.x), x[0], x[1]);
-            unpack2(mul2(x4[m].y, b4.y), x[2], x[3]);
+            for (int i = 0; i < 4; ++i) a[i] = ex2(a[i]);
+            unpack2(mul2(x4.x, b4.x), x[0], x[1]);
+            unpack2(mul2(x4.y, b4.y), x[2], x[3]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) hv[i] = h[m][k] = fmaf(a[i], h[m][k], x[i]);
+            for (int i = 0; i < 4; ++i) hv[i] = h[k] = fmaf(a[i], h[k], x[i]);
             if (OUT) {
-              ya[m] = fma2(pack2(hv[0], hv[1]), c4.x, ya[m]);
-              yb[m] = fma2(pack2(hv[2], hv[3]), c4.y, yb[m]);
+              ya = fma2(pack2(hv[0], hv[1]), c4.x, ya);
+              yb = fma2(pack2(hv[2], hv[3]), c4.y, yb);
             }
           }
+          unpack2(ya, yv[i4], yv[i4 + 1]);
+          unpack2(yb, yv[i4 + 2], yv[i4 + 3]);
         }
+        if (OUT) {
+          const int at = spread_sum<GS, P>(yv, q);
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-          unpack2(ya[m], yv[m][i4], yv[m][i4 + 1]);
-          unpack2(yb[m], yv[m][i4 + 2], yv[m][i4 + 3]);
-        }
-      }
-      if (OUT) {
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-          const int at = spread_sum<GS, P>(yv[m], q);
-#pragma unroll
-          for (int j = 0; j < GS / P; ++j) sh.y[tg + at + j][el + m * (NT / P)] = yv[m][j];
+          for (int j = 0; j < GS / P; ++j) sh.y[tg + at + j][el] = yv[j];
         }
       }
-    }
-    }
-    tile_sync<NT>();
+    __syncthreads();
     if (OUT && lelive) {
 #pragma unroll
       for (int j = 0; j < R; ++j) {
@@ -248,22 +214,19 @@ __global__ void __launch_bounds__(NT) sel_scan_kernel(const SelScanParams p) {
         if (lelive && t0 + lt + j < end) store2<T>(yp + (int64_t)(t0 + lt + j) * p.y.sl, vy, second, 0.f, 0.f);
     }
   }
+  const int e = e_first + el;
+  if (e < e_end) {
+    if (OUT) {
+      if (p.h_last != nullptr && c == p.nchunk - 1) {
 #pragma unroll
-  for (int m = 0; m < M; ++m) {
-    const int e = e_first + el + m * (NT / P);
-    if (e < e_end) {
-      if (OUT) {
-        if (p.h_last != nullptr && c == p.nchunk - 1) {
-#pragma unroll
-          for (int k = 0; k < K; ++k)
-            if (q * K + k < p.N) p.h_last[((int64_t)b * p.E + e) * p.N + q * K + k] = h[m][k];
-        }
-      } else {
-        const int64_t at = ((int64_t)b * p.nchunk + c) * p.E + e;
-#pragma unroll
-        for (int k = 0; k < K; ++k) p.states[at * NP + q * K + k] = h[m][k];
-        if (q == 0) p.dtsum[at] = dts[m];
+        for (int k = 0; k < K; ++k)
+          if (q * K + k < p.N) p.h_last[((int64_t)b * p.E + e) * p.N + q * K + k] = h[k];
       }
+    } else {
+      const int64_t at = ((int64_t)b * p.nchunk + c) * p.E + e;
+#pragma unroll
+      for (int k = 0; k < K; ++k) p.states[at * NP + q * K + k] = h[k];
+      if (q == 0) p.dtsum[at] = dts;
     }
   }
 }
@@ -386,24 +349,18 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
-#ifndef M3_M
-#define M3_M 1
-#endif
-#ifndef M3_NT
-#define M3_NT 64
-#endif
 template <typename T, int K, int P, bool OUT>
 int launch_pass(const SelScanParams& p, cudaStream_t s) {
-  constexpr int M = P >= 4 ? M3_M : 1, NT = P >= 16 ? 128 : M3_NT;
-  using S = FwdSmem<K, P, M, NT>;
+  constexpr int NT = P >= 16 ? 128 : 64;  // (a CTA has eight channels at least: the pair of a thread needs them)
+  using S = FwdSmem<K, P, NT>;
   const int Eg = p.E / p.G;
   // what the last piece leaves enters no other
   const dim3 grid((unsigned)(p.G * ((Eg + S::EC - 1) / S::EC)), (unsigned)(OUT ? p.nchunk : p.nchunk - 1), (unsigned)p.batch);
   auto go = [&](auto fast) {
     static std::atomic<bool> done[kMaxDevices];
     constexpr bool FAST = decltype(fast)::value;
-    M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(&sel_scan_kernel<T, K, P, M, NT, OUT, FAST>), sizeof(S), done));
-    sel_scan_kernel<T, K, P, M, NT, OUT, FAST><<<grid, NT, sizeof(S), s>>>(p);
+    M3_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(&sel_scan_kernel<T, K, P, NT, OUT, FAST>), sizeof(S), done));
+    sel_scan_kernel<T, K, P, NT, OUT, FAST><<<grid, NT, sizeof(S), s>>>(p);
     return check_launch("sel_scan_kernel");
   };
   const bool f32 = sizeof(T) == 4;

@@ -89,31 +89,6 @@ int sel_pieces(const SelScanParams& p, int lanes, int sms, int* chunk);
 // exponent in the product's own rounding, this halves it where it is largest and keeps 2^0 = 1.
 constexpr float kEx2Mean = 1.5e-8f;
 
-// 2^x of two numbers on the FMA and integer pipes, for a share of the decays: the exponential's own unit does 16 a
-// clock and SM, which would bound the scan. x = n + f with n the nearest whole number (by adding 1.5 2^23), 2^f by
-// a polynomial of degree 5 on [-1/2, 1/2] that is 1 at 0, fitted here for the smallest relative error (1.7e-7 at
-// most with its roundings, 7e-8 rms), n added to the exponent's bits. From -126 down the result is 2^-126, from 128 up infinite.
-__device__ __forceinline__ f2 ex2_poly2(f2 x) {
-  float x0, x1, t0, t1, p0, p1;
-  unpack2(x, x0, x1);
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x0));
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x1));
-  asm("min.NaN.f32 %0, %0, 0f43000000;" : "+f"(x0));
-  asm("min.NaN.f32 %0, %0, 0f43000000;" : "+f"(x1));
-  x = pack2(x0, x1);
-  const f2 magic = pack2(12582912.f, 12582912.f), less = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f);
-  const f2 t = add2(x, magic), f = fma2(add2(t, less), minus, x);
-  f2 p = fma2(pack2(1.3264728050203965e-3f, 1.3264728050203965e-3f), f, pack2(9.671513139367519e-3f, 9.671513139367519e-3f));
-  p = fma2(p, f, pack2(5.550733745779106e-2f, 5.550733745779106e-2f));
-  p = fma2(p, f, pack2(2.4022242077762193e-1f, 2.4022242077762193e-1f));
-  p = fma2(p, f, pack2(6.931469775948809e-1f, 6.931469775948809e-1f));
-  p = fma2(p, f, pack2(1.f, 1.f));
-  unpack2(t, t0, t1);
-  unpack2(p, p0, p1);
-  return pack2(__int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23)),
-               __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)));
-}
-
 // a row that is either T or fp32
 template <typename T>
 struct RawAny { uint32_t a, b; };

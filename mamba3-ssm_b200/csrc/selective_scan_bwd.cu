@@ -5,9 +5,16 @@
 // The forward keeps the state in front of every eighth step, so eight steps at a time are done
 // again and then walked backwards, all in registers: P lanes share a channel and hold K states each,
 // M channels follow one another in a lane. Sums over the states of a channel (three a step and channel)
-// and over the channels (dB, dC) are formed for eight steps together by halving exchanges; M and K set
-// how many there are of each. Sums over channels of other warps go through shared memory, those of
-// other CTAs through the workspace and a second kernel, in a fixed order.
+// and over the channels (dB, dC) are formed for eight steps together by halving exchanges; K sets how many
+// exchanges the first take, M K how many the second. Sums over channels of other warps go through shared
+// memory, those of other CTAs through the workspace and a second kernel, in a fixed order.
+//
+// Bound by the issue of instructions and by shared memory's port together: about 24 instructions a step, channel and
+// state, four of them reads of shared memory (dt, dx, dy, B, C, whose broadcasts cost as much as other reads), at 0.43 a clock
+// with the two warps a scheduler that 255 registers leave. 8 x 2048 x 2048 x 16 of bf16 with a gate take 855 us and 18 to join
+// (742 MB, the forward's too, would take 113); the same in other shapes, us: K = 2, P = 8, M = 2 with all sums by shuffles 2690;
+// K = 4, P = 4, M = 1 1043; 64 threads 838 and 31 to join; 85 or 128 registers, which spill, 1320 to 1360; four steps at a time,
+// with the upper four's first state formed again, 1008 at two CTAs an SM and 1077 at three.
 #include <algorithm>
 
 #include "selective_scan.cuh"
@@ -48,10 +55,7 @@ __device__ __forceinline__ void lds4(const float* p, f2& a, f2& b) {
 }
 
 template <typename T, int K, int P, int M, int NT, bool FAST>
-#ifndef M3_BMIN
-#define M3_BMIN 1
-#endif
-__global__ void __launch_bounds__(NT, M3_BMIN) sel_bwd_kernel(const SelScanParams p, const SelScanGrads g) {
+__global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, const SelScanGrads g) {
   using S = BwdSmem<K, P, M, NT>;
   constexpr int NP = S::NP, EC = S::EC, W = S::W, Q = 32 / P;
   constexpr int R = TT * EC / 2 / NT > 0 ? TT * EC / 2 / NT : 1;  // steps of a pair of channels that a thread brings and stores
@@ -535,46 +539,43 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
-#ifndef M3_BK
-#define M3_BK 4
-#endif
-#ifndef M3_BM
-#define M3_BM 2
-#endif
-#ifndef M3_BNT
-#define M3_BNT 128
-#endif
-// states a lane, lanes, channels a lane by the padded number of states
+constexpr int kBwdThreads = 128;
+
+// f(K, P, M) as types: states a lane, lanes, channels a lane by the padded number of states. single: one channel a lane,
+// for launches that leave SMs idle otherwise (3 x 341 x 507 x 16: 55 us, with two channels 96).
 template <int K, int P, int M> struct KPM { static constexpr int k = K, p = P, m = M; };
 template <typename F>
-int by_states(int n, F&& f) {
+int by_states(int n, bool single, F&& f) {
   switch (sel_padded_states(n)) {
     case 4: return f(KPM<2, 2, 1>{});
     case 8: return f(KPM<4, 2, 1>{});
-    case 16: return f(KPM<M3_BK, 16 / M3_BK, M3_BM>{});
-    case 32: return f(KPM<4, 8, 2>{});
-    case 64: return f(KPM<4, 16, 2>{});
-    default: return f(KPM<4, 32, 2>{});
+    case 16: return single ? f(KPM<4, 4, 1>{}) : f(KPM<4, 4, 2>{});
+    case 32: return single ? f(KPM<4, 8, 1>{}) : f(KPM<4, 8, 2>{});
+    case 64: return single ? f(KPM<4, 16, 1>{}) : f(KPM<4, 16, 2>{});
+    default: return single ? f(KPM<4, 32, 1>{}) : f(KPM<4, 32, 2>{});
   }
 }
 
-constexpr int kBwdThreads = M3_BNT;
-
 struct BwdPlan {
   int np, tiles, nchunk, chunk;
+  bool single;
   size_t bc, a, states, dtsum;  // floats
 };
 
 BwdPlan plan(const SelScanParams& p, int sms) {
   BwdPlan w;
   w.np = sel_padded_states(p.N);
-  by_states(p.N, [&](auto l) {
-    using L_ = decltype(l);
-    const int ec = kBwdThreads / L_::p * L_::m, Eg = p.E / p.G;
-    w.tiles = (Eg + ec - 1) / ec;
-    w.nchunk = sel_pieces(p, std::max(1, L_::p / L_::m), sms, &w.chunk);
-    return 0;
-  });
+  for (const bool single : {false, true}) {
+    by_states(p.N, single, [&](auto l) {
+      using L_ = decltype(l);
+      const int ec = kBwdThreads / L_::p * L_::m, Eg = p.E / p.G;
+      w.tiles = (Eg + ec - 1) / ec;
+      if (!single) w.nchunk = sel_pieces(p, std::max(1, L_::p / L_::m), sms, &w.chunk);
+      return 0;
+    });
+    w.single = single;
+    if ((int64_t)p.batch * p.G * w.tiles * w.nchunk > sms) break;
+  }
   w.bc = (size_t)p.batch * p.L * p.G * w.tiles * 2 * w.np;
   w.a = (size_t)p.batch * w.nchunk * p.E * (w.np + 2);
   w.states = w.nchunk > 1 ? (size_t)p.batch * w.nchunk * p.E * w.np : 0;
@@ -608,7 +609,7 @@ int launch_sel_scan_bwd(SelScanParams p, SelScanGrads g, int dtype, void* ws, cu
   const int Eg = p.E / p.G;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    M3_TRY(by_states(p.N, [&](auto l) {
+    M3_TRY(by_states(p.N, w.single, [&](auto l) {
       using L_ = decltype(l);
       constexpr int K = L_::k, P = L_::p, M = L_::m, NT = kBwdThreads;
       if (p.batch == 0) return (int)M3_OK;  // parameters' gradients of zero
