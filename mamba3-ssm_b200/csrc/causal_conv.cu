@@ -1,9 +1,13 @@
 // Short depthwise causal convolution over (batch, length, channels), forward, backward, one step:
 //   pre[t] = bias + sum_k w[k] x[t - K + 1 + k],   y = pre or silu(pre)
 //   d = dy act'(pre),  dx[t] = sum_k w[k] d[t + K - 1 - k],  dw[k] = sum d[t] x[t - K + 1 + k],  dbias = sum d
-// Bound by the memory. A lane holds V neighbouring channels (a vector load where the rows allow it),
-// a warp 32 V of them, and walks a run of rows with the last K rows in registers, so each element is
-// read once but for the K - 1 rows between runs. The backward forms pre again from x.
+// Bound by the memory's latency: the rows that 24 (forward) or 16 (backward) warps an SM have on their way. A lane holds
+// one or two pairs of neighbouring channels (vector loads where the rows allow it) and walks a run of rows with the last K
+// rows in registers, so each element is read once but for the K - 1 rows between runs; the next four rows are
+// loaded while four are worked on, a multiple of the window so that it turns without moves. The backward forms
+// pre again from x. 8 x 2048 x 2048 of bf16 with four taps, us: forward 36 (134 MB, 3.7 TB/s), backward 74 (201 MB) and 3.4 to
+// join; with one pair a lane 45 and 103; runs of 16 rows 42 and 89, of 64 39 and 72; weights read four at a time, which
+// takes registers, 40 and 96; two or three rows ahead in the backward 155, 157.
 #include <algorithm>
 
 #include "causal_conv.cuh"
@@ -430,7 +434,8 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
-// Rows that a warp walks: 32, fewer where that leaves less than about two CTAs an SM (rows between two runs are read twice).
+// Rows that a warp walks: 32, fewer where that leaves less than about two CTAs an SM (rows between two runs are read twice;
+// 4 x 777 x 2048 forward: 10.2 us, in runs of 32 12.2).
 int run_rows(int64_t batch, int64_t L, int64_t E) {
   int run = 32;
   while (run > 8 && batch * ((E + 127) / 128) * ((L + run * kWarps - 1) / (run * kWarps)) < 296) run /= 2;

@@ -388,8 +388,9 @@ int by_states(int n, F&& f) {
 static int sel_lanes(int np) { return std::max(2, np / 4); }
 
 // Pieces that the sequence is cut into: one, unless the channels alone leave most of the GPU idle. A
-// piece's state has to be formed ahead (about as much work again), so cutting begins where
-// there are less than a quarter of the warps that keep an SM busy.
+// piece's state has to be formed ahead (about as much work again), so cutting begins where there are less than a quarter of
+// the warps that keep an SM busy, and a piece has 256 steps at least. Steps x channels of 16 states, us cut and not:
+// 8192 x 2048 233, 569; 8192 x 4096 449, 586; 8192 x 8192 793, 755; 1024 x 1024 36, 74; 512 x 1024 33, 39.
 int sel_pieces(const SelScanParams& p, int lanes, int sms, int* chunk) {
   const int64_t warps = (int64_t)p.batch * p.E * lanes / 32 + 1, want = (int64_t)sms * 16;
   int n = 1;
@@ -460,8 +461,9 @@ int launch_sel_step(const SelStepParams& p, int dtype, cudaStream_t s) {
     const int es = sizeof(T) == 4 || p.bc_f32 ? 4 : 2;
     const bool vec_bc = p.N % 4 == 0 && p.sB % 4 == 0 && p.sC % 4 == 0 && p.sBg % 4 == 0 && p.sCg % 4 == 0 &&
                         ((reinterpret_cast<uintptr_t>(p.B) | reinterpret_cast<uintptr_t>(p.C)) & (4 * es - 1)) == 0;
-    // four sequences a thread where that leaves some warps for every SM
-    const bool four = p.batch >= 4 && p.batch * p.E * P >= 4 * 128 * 1024;
+    // four sequences a thread where that leaves some warps for every SM: sequences of 5120 x 16, us, four a thread and one:
+    // 8 5.5, 4.5; 16 5.7, 6.9; 32 8.0, 11.0; 256 46, 71 (179 MB: 3.9 TB/s)
+    const bool four = p.batch >= 4 && p.batch * p.E * P >= 2 * 128 * 1024;
     const int64_t threads = (four ? (p.batch + 3) / 4 : p.batch) * p.E * P;
     const unsigned grid = (unsigned)((threads + 255) / 256);
     if (four) sel_step_kernel<T, P, 4><<<grid, 256, 0, s>>>(p, vec, vec_bc);
