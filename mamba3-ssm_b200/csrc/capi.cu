@@ -1605,6 +1605,12 @@ int m3_causal_conv_step(m3_tensor* state, const m3_tensor* x, const m3_tensor* w
   M3_TRY(operand(state, "state", 3, ss, 1u << x->dtype, false, false, some));
   M3_TRY(operand(y, "y", 2, x->shape, 1u << x->dtype, true, false, some));
   if (!some) return M3_OK;
+  // rows of E elements, one after the other in either order of sequences and rows
+  const int64_t sb = state->stride[0], sl = state->stride[1], rows = taps - 1;
+  const bool apart = batch == 1 ? rows == 1 || sl >= E
+                     : rows == 1 ? sb >= E
+                                 : (sl >= E && sb >= (rows - 1) * sl + E) || (sb >= E && sl >= (batch - 1) * sb + E);
+  if (!apart) return fail(M3_ERR_INVALID_ARGUMENT, "state: rows overlap");
   ConvStepParams p{state->data, state->stride[0], state->stride[1], x->data, x->stride[0], weight->data, weight->stride[0],
                    fptr<const void>(bias), weight->dtype == M3_FLOAT32, silu != 0, y->data, batch, (int)E, false};
   return launch_conv_step(p, (int)taps, x->dtype, reinterpret_cast<cudaStream_t>(stream));
@@ -1708,6 +1714,7 @@ int m3_selective_step(m3_tensor* state, const m3_tensor* u, const m3_tensor* del
   M3_TRY(operand(state, "state", 3, hs, kF32, false, false, some));
   if (some && E > 1 && state->stride[1] != N)
     return fail(M3_ERR_INVALID_ARGUMENT, "state: each sequence's part must be contiguous");
+  if (some && batch > 1 && state->stride[0] < E * N) return fail(M3_ERR_INVALID_ARGUMENT, "state: sequences overlap");
   M3_TRY(operand(y, "y", 2, u->shape, 1u << u->dtype, false, false, some));
   M3_TRY(flag(softplus, "softplus"));
   if (E > INT32_MAX / (2 * kSelMaxStates) || batch > (INT64_C(1) << 36) / std::max<int64_t>(1, E))

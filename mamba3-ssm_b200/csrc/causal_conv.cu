@@ -439,6 +439,7 @@ int by_type(int dtype, F&& f) {
 int run_rows(int64_t batch, int64_t L, int64_t E) {
   int run = 32;
   while (run > 8 && batch * ((E + 127) / 128) * ((L + run * kWarps - 1) / (run * kWarps)) < 296) run /= 2;
+  while (L > (int64_t)run * kWarps * 65535) run *= 2;  // of a grid's rows there are no more
   return run;
 }
 unsigned runs(int64_t L, int run) { return (unsigned)std::max<int64_t>(1, (L + run * kWarps - 1) / (run * kWarps)); }

@@ -13,6 +13,13 @@ def silu_slope(v):
     return p * (1 + v * (1 - p))
 
 
+def silu_slope_terms(v):
+    """The magnitudes of the slope's two terms s + s v (1 - s). They cancel at v = -1.2785, where the slope is 0 but a sigmoid
+    that is off by a relative d (a few 2^-23) moves it by s |v| s d or so: the bound there is one on the terms."""
+    p = torch.sigmoid(v)
+    return p + p * v.abs() * (1 - p)
+
+
 def valid(lengths, batch, length, device):
     n = torch.full((batch,), length, device=device) if lengths is None else lengths.clamp(0, length)
     return torch.arange(length, device=device) < n[:, None]
@@ -73,7 +80,7 @@ def scan(u, delta, A, B, C, D=None, z=None, bias=None, softplus=True, h0=None, l
     out.update(u=torch.where(k1, du, zero), delta=draw, A=dA, B=torch.where(k2, dB, zero), C=torch.where(k2, dC, zero),
                D=(dp * uv).sum((0, 1)), bias=draw.sum((0, 1)), h0=G)
     if z is not None:
-        out["z"] = torch.where(k1, dout * pre * mag(silu_slope(z)), zero)
+        out["z"] = torch.where(k1, dout * pre * (silu_slope_terms(z) if magnitudes else silu_slope(z)), zero)
     return out
 
 

@@ -188,6 +188,23 @@ def test_select_in_a_graph_and_on_streams():
             assert torch.equal(o.parents, want[1]) and torch.equal(o.tokens, want[2])
 
 
+@pytest.mark.parametrize("batch,vocab", [(3, 9000), (60, 9000)])
+def test_select_on_two_streams_at_once(batch, vocab):
+    """In one launch and in two."""
+    from mamba3_ssm import beam_select
+    xs = [inputs(batch, 4, vocab, torch.bfloat16, seed=s) for s in (21, 22)]
+    want = [beam_select(*x, 8) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(beam_select(*x, 8))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for g, w in zip(got, want) for p, q in zip(g, w))
+
+
 # ---------------------------------------------------------------------------------- states
 def moved(t, parents, batch):
     """Rows by the definition."""

@@ -86,6 +86,43 @@ def test_scan(b, n, e, m, g, dtype):
     check_scan(x, h0=h0, dstate=torch.randn(b, e, m, device=DEV, generator=_gen(6)))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("b,n,e,m,g", [(20, 19, 513, 16, 1), (20, 9, 250, 32, 1), (21, 12, 130, 64, 2), (20, 5, 66, 100, 1)])
+def test_scan_of_many_sequences(b, n, e, m, g, dtype):
+    """As many as give the backward two channels a lane; the smaller ones have one."""
+    x = scan_inputs(b, n, e, m, g, DTYPES[dtype], seed=m)
+    lengths = torch.tensor([n - i % 3 for i in range(b)], device=DEV)
+    check_scan(x, h0=torch.randn(b, e, m, device=DEV, generator=_gen(5)), lengths=lengths)
+
+
+def test_steps_before_sequences_in_memory():
+    """(length, batch, channels) seen as (batch, length, channels), forward, backward and in steps."""
+    b, n, e, m = 3, 41, 36, 16
+    x = scan_inputs(b, n, e, m, dtype=torch.bfloat16)
+    turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    y, state = check_scan({k: turned(t) if t is not None and t.dim() > 2 else t for k, t in x.items()})
+    z, again = check_scan(x)
+    assert torch.equal(y, z) and torch.equal(state, again)
+    cx, w, bias, init, dy, dlast = conv_inputs(b, n, e, 4, torch.bfloat16)
+    check_conv(turned(cx), w, bias, turned(init), turned(dy), turned(dlast), True)
+
+
+def test_steps_refuse_states_that_overlap():
+    from mamba3_ssm import causal_conv_step_, ssm_step_selective_
+    e, m = 24, 16
+    u = torch.randn(4, e, device=DEV)
+    A, w, B = torch.randn(e, m, device=DEV), torch.randn(e, 4, device=DEV), torch.randn(4, m, device=DEV)
+    for state in (torch.zeros(1, e, m, device=DEV).expand(4, e, m), torch.zeros(2000, device=DEV).as_strided((4, e, m), (e * m - 4, m, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ssm_step_selective_(state, u, u, A, B, B)
+    flat = torch.zeros(2000, device=DEV)
+    for strides in ((0, e, 1), (3 * e, 0, 1), (2 * e, e, 1), (3 * e, e - 1, 1), (e, 3 * e, 1)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            causal_conv_step_(flat.as_strided((4, 3, e), strides), u, w)
+    for strides in ((3 * e, e, 1), (e, 4 * e, 1), (4 * e + 1, e + 3, 1)):
+        causal_conv_step_(flat.as_strided((4, 3, e), strides), u, w)
+
+
 @pytest.mark.parametrize("drop", ["z", "D", "bias", "all", "softplus"])
 def test_scan_without_optional_operands(drop):
     x = scan_inputs(2, 45, 48, 16, dtype=torch.bfloat16, softplus=drop != "softplus")
