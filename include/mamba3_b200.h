@@ -464,7 +464,7 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
  *   x's dtype: the last K - 1 rows, what the next call takes as initial or m3_causal_conv_step as state.
  * m3_causal_conv_bwd: dx, dweight, dbias, dinitial (the last two optional) from dy and dlast
  *   (optional); dweight, dbias of weight's dtype, contiguous.
- * m3_causal_conv_step: one row; state (batch, K - 1, E) moves on in place. x, y (batch, E).
+ * m3_causal_conv_step: one row; state (batch, K - 1, E) moves on in place, its rows apart. x, y (batch, E).
  * m3_selective_scan:  dt = delta + delta_bias, with softplus = 1 log(1 + exp(.)) of it;
  *   h[t] = exp(dt A) h[t - 1] + dt u B[t];  y = (sum_n C[t] h[t] + D u) (z sigmoid(z))
  *   u (batch, seqlen, E); delta the same, u's dtype or f32; z as u, optional (no gate); B, C
@@ -510,13 +510,13 @@ int m3_selective_step(m3_tensor* state, const m3_tensor* u, const m3_tensor* del
 /* ---------------------------------------------------------------------------------
  * Beam search (no counterpart in the reference's package).
  * m3_beam_select: of each prompt, the num largest of scores[j] + logits[j, v] - log sum exp
- *   logits[j, :] over its beams j and tokens v, largest first, formed and compared in 64 bits; ties to the
- *   lowest (j, v). A finished beam offers end_token alone, at no cost (its logits are not read);
+ *   logits[j, :] over its beams j and tokens v, largest first, joined and compared in two f32 (about 48
+ *   bits), the sums of exp within a thread in one; ties to the lowest (j, v). A finished beam offers end_token alone, at no cost (its logits are not read);
  *   a beam with score -inf, or all of whose logits are -inf, offers -inf; one with a NaN or +inf
  *   among its logits, or as its score, offers NaN, which ranks first.
  *   logits (batch, beams, V), beams <= 32, V <= 2^24; scores (batch, beams) f32; finished (batch,
  *   beams) u8, optional; out_scores f32, parents (j) and tokens (v) i64: (batch, num) contiguous,
- *   num <= 64. workspace: m3_beam_select_workspace_size bytes, 16-byte aligned.
+ *   num <= 64. workspace: m3_beam_select_workspace_size bytes (0 where one launch does it all), 16-byte aligned.
  * m3_reorder_states: row b T + j of every tensor becomes its row b S + parents[b, j], zeros where
  *   the parent is outside [0, S). parents (batch, T) i64. Tensors are given as host arrays: device
  *   addresses of (batch S) rows of row_bytes bytes, their pitches, and those of the (batch T) rows that receive

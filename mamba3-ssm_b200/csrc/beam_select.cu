@@ -4,12 +4,15 @@
 // are, offers -inf; one with a NaN or an infinite logit or score offers NaN, which ranks first.
 // beam_rows_kernel reads the logits once: a CTA a part of a row keeps its largest element and the sum of
 // exponentials (one float a thread, two where they join) and the part's `num` largest elements. Those pass a
-// threshold, at first the num-th largest of the maxima of groups of threads, which rises whenever the list of those that
+// threshold, at first the num-th largest of the threads' maxima, which rises whenever the list of those that
 // passed has grown, so that later tiles are mostly dismissed by one comparison a vector. Where more pass than the list
 // holds (rising or equal logits), the rest of the tile waits for the risen threshold; keys are unique (value, then the
 // lower index), so that each look lists a full list's worth of them. beam_join_kernel, a CTA a prompt,
 // joins the sums and ranks the parts' elements by their score, both in two floats (about 48 bits).
-// Bound by the memory where there are many rows, by latency where there are few.
+// beam_cluster_kernel does both for few and short rows.
+// Bound by latency where there are few rows: 1 x 4 x 50000 of bf16 take 12 us in one launch (0.4 MB), of which the rows are 5,
+// the join 3. Where there are many, by the rows' threads between two barriers: 64 x 8 x 131072 of bf16, a quarter ended, take
+// 43 us (101 MB, 15 us of memory; with groups' maxima and a list cut at every tile 158) and 8 to join.
 #include <algorithm>
 
 #include "beam.cuh"

@@ -9,6 +9,7 @@
 // join; with one pair a lane 45 and 103; runs of 16 rows 42 and 89, of 64 39 and 72; weights read four at a time, which
 // takes registers, 40 and 96; two or three rows ahead in the backward 155, 157.
 #include <algorithm>
+#include <type_traits>
 
 #include "causal_conv.cuh"
 #include "m3_common.cuh"
@@ -135,11 +136,17 @@ __global__ void __launch_bounds__(32 * kWarps) conv_fwd_kernel(const ConvParams 
   const int t1 = min(t0 + p.run, p.L), end = min(t1, n);
   constexpr int U = 4;
   RawRow<T, NV> in[U];  // the next rows, on their way while those before them are worked on
+  const T* next = static_cast<const T*>(p.x) + (int64_t)b * p.xb + (int64_t)t0 * p.xl + e;
   auto fetch = [&](int t) {
     const Chan<T, NV> ch{p.vec, e + 1 < p.E ? 1 : 0};
-    const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.xb + e;
+    if (t + U <= end) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) in[u] = ch.load(x + (int64_t)min(t + u, end - 1) * p.xl);
+      for (int u = 0; u < U; ++u) in[u] = ch.load(next + u * p.xl);
+    } else {  // rows behind the end read the last one; nothing is made of them
+#pragma unroll
+      for (int u = 0; u < U; ++u) in[u] = ch.load(next + min(u, end - 1 - t) * p.xl);
+    }
+    next += U * p.xl;
   };
   if (t0 < end) fetch(t0);
   const Lane<T, NV, K> ln(p, b, e);
@@ -161,6 +168,7 @@ __global__ void __launch_bounds__(32 * kWarps) conv_fwd_kernel(const ConvParams 
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) ln.row(t0 - (K - 1) + k, win[k + 1]);
   }
+  T* to = y + (int64_t)t0 * p.yl;
 #pragma unroll 1
   for (int t = t0; t < end; t += U) {
     RawRow<T, NV> now[U];
@@ -169,18 +177,18 @@ __global__ void __launch_bounds__(32 * kWarps) conv_fwd_kernel(const ConvParams 
     if (t + U < end) fetch(t + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (t + u < end) {
-        f2 v[NV];
-        shift(win);
-        values<T, NV>(now[u], win[K - 1]);
-        ln.pre(win, v);
-        if (p.silu) {
+      // (the window turns whatever is stored: within a branch its registers would have to be moved back)
+      f2 v[NV];
+      shift(win);
+      values<T, NV>(now[u], win[K - 1]);
+      ln.pre(win, v);
+      if (p.silu) {
 #pragma unroll
-          for (int i = 0; i < NV; ++i) v[i] = mul2(v[i], sigmoid2(v[i]));
-        }
-        ln.ch.store(y + (int64_t)(t + u) * p.yl, v);
+        for (int i = 0; i < NV; ++i) v[i] = mul2(v[i], sigmoid2(v[i]));
       }
+      if (t + u < end) ln.ch.store(to + u * p.yl, v);
     }
+    to += U * p.yl;
   }
   f2 none[NV];
   zero(none);
@@ -213,7 +221,7 @@ __device__ __forceinline__ void add_last(const Lane<T, NV, K>& ln, const ConvGra
 }
 
 template <typename T, int NV, int K>
-__global__ void __launch_bounds__(32 * kWarps) conv_bwd_kernel(const ConvParams p, const ConvGrads g) {
+__global__ void __launch_bounds__(32 * kWarps, 2) conv_bwd_kernel(const ConvParams p, const ConvGrads g) {
   __shared__ f2 sums[kWarps][K + 1][32 * NV];
   const int e = (blockIdx.x * 32 + threadIdx.x) * 2 * NV, b = blockIdx.z;
   const int t0 = (blockIdx.y * kWarps + threadIdx.y) * p.run, t1 = min(t0 + p.run, p.L);
@@ -265,15 +273,61 @@ __global__ void __launch_bounds__(32 * kWarps) conv_bwd_kernel(const ConvParams 
       constexpr int U = 4;
       const int ahead = min(end + K - 1, n);  // rows whose d this run needs
       RawRow<T, NV> xn[U], dn[U];             // the next rows, on their way while those before them are worked on
+      const T *xr = ln.x + (int64_t)t0 * p.xl, *dr = dy + (int64_t)t0 * g.dyl;
       auto fetch = [&](int t) {
+        if (t + U <= ahead) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int64_t r = min(t + u, ahead - 1);
-          xn[u] = ln.ch.load(ln.x + r * p.xl);
-          dn[u] = ln.ch.load(dy + r * g.dyl);
+          for (int u = 0; u < U; ++u) {
+            xn[u] = ln.ch.load(xr + u * p.xl);
+            dn[u] = ln.ch.load(dr + u * g.dyl);
+          }
+        } else {  // rows behind the end read the last one; nothing is made of them
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int64_t r = min(u, ahead - 1 - t);
+            xn[u] = ln.ch.load(xr + r * p.xl);
+            dn[u] = ln.ch.load(dr + r * g.dyl);
+          }
         }
+        xr += U * p.xl;
+        dr += U * g.dyl;
       };
       fetch(t0);
+      T* to = dx + (int64_t)(t0 - (K - 1)) * g.dxl;
+      // U rows, all of which count and complete the gradient of a row of this run (ALL; the last rows' gradient falls on none
+      // of those: t - K + 1 < n - K + 1), or each looked at
+      auto rows = [&](auto all, int t, const RawRow<T, NV> (&in)[U], const RawRow<T, NV> (&din)[U]) {
+        constexpr bool ALL = decltype(all)::value;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          shift(win);
+          shift(dwin);
+          values<T, NV>(in[u], win[K - 1]);
+          values<T, NV>(din[u], dwin[K - 1]);
+          slope(ln, win, dwin[K - 1]);
+          if (!ALL && t + u >= ahead) zero(dwin[K - 1]);
+          if (ALL || t + u < end) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+              for (int k = 0; k < K; ++k) dw[k][i] = fma2(dwin[K - 1][i], win[k][i], dw[k][i]);
+              dw[K][i] = add2(dw[K][i], dwin[K - 1][i]);
+            }
+          }
+          const int at = t + u - (K - 1);  // all of d[at ..  at + K - 1] is at hand
+          if (ALL || (at >= t0 && at < end)) {
+            f2 v[NV];
+            zero(v);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+              for (int k = 0; k < K; ++k) v[i] = fma2(ln.w[k][i], dwin[K - 1 - k][i], v[i]);
+            if (!ALL) add_last<T, NV, K>(ln, g, b, e, n, at, v);
+            ln.ch.store(to + u * g.dxl, v);
+          }
+        }
+        to += U * g.dxl;
+      };
 #pragma unroll 1
       for (int t = t0; t < end + K - 1; t += U) {
         RawRow<T, NV> in[U], din[U];
@@ -283,37 +337,8 @@ __global__ void __launch_bounds__(32 * kWarps) conv_bwd_kernel(const ConvParams 
           din[u] = dn[u];
         }
         if (t + U < ahead) fetch(t + U);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          shift(win);
-          shift(dwin);
-          if (t + u < ahead) {
-            values<T, NV>(in[u], win[K - 1]);
-            values<T, NV>(din[u], dwin[K - 1]);
-            slope(ln, win, dwin[K - 1]);
-          } else {
-            zero(dwin[K - 1]);
-          }
-          if (t + u < end) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-#pragma unroll
-              for (int k = 0; k < K; ++k) dw[k][i] = fma2(dwin[K - 1][i], win[k][i], dw[k][i]);
-              dw[K][i] = add2(dw[K][i], dwin[K - 1][i]);
-            }
-          }
-          const int at = t + u - (K - 1);  // all of d[at ..  at + K - 1] is at hand
-          if (at >= t0 && at < end) {
-            f2 v[NV];
-            zero(v);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-              for (int k = 0; k < K; ++k) v[i] = fma2(ln.w[k][i], dwin[K - 1 - k][i], v[i]);
-            add_last<T, NV, K>(ln, g, b, e, n, at, v);
-            ln.ch.store(dx + (int64_t)at * g.dxl, v);
-          }
-        }
+        if (t >= t0 + K - 1 && t + U <= end) rows(std::true_type{}, t, in, din);
+        else rows(std::false_type{}, t, in, din);
       }
     }
     f2 none[NV];

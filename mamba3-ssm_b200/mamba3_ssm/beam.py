@@ -34,7 +34,7 @@ class BeamSelection(NamedTuple):
 def beam_select(logits, scores, num=None, *, finished=None, end_token=0):
     """The ``num`` (as many as beams by default, at most 64) best continuations of each prompt by
     scores[b, j] + log_softmax(logits[b, j])[v], over its beams j and tokens v, the largest first;
-    formed and compared in 64 bits, ties to the lowest (j, v). logits (batch, beams, V), or (batch * beams, V)
+    compared in about 48 bits (two floats), ties to the lowest (j, v). logits (batch, beams, V), or (batch * beams, V)
     as a model returns them, fp32, bf16 or fp16; at most 32 beams; scores (batch, beams) fp32: the
     beams' sums of log-probabilities so far.
 
