@@ -5,9 +5,9 @@
 // one or two pairs of neighbouring channels (vector loads where the rows allow it) and walks a run of rows with the last K
 // rows in registers, so each element is read once but for the K - 1 rows between runs; the next four rows are
 // loaded while four are worked on, a multiple of the window so that it turns without moves. The backward forms
-// pre again from x. 8 x 2048 x 2048 of bf16 with four taps, us: forward 36 (134 MB, 3.7 TB/s), backward 74 (201 MB) and 3.4 to
-// join; with one pair a lane 45 and 103; runs of 16 rows 42 and 89, of 64 39 and 72; weights read four at a time, which
-// takes registers, 40 and 96; two or three rows ahead in the backward 155, 157.
+// pre again from x. 8 x 2048 x 2048 of bf16 with four taps, us: forward 36 (134 MB, 3.7 TB/s), backward 57 (201 MB, 3.5 TB/s)
+// and 3 to join. Before, with a look at each row of the backward 74; with one pair a lane 45 and 103; weights read four at a time,
+// which takes registers, 40 and 96; two or three rows ahead in the backward 155, 157.
 #include <algorithm>
 #include <type_traits>
 
@@ -459,10 +459,11 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
-// Rows that a warp walks: 32, fewer where that leaves less than about two CTAs an SM (rows between two runs are read twice;
+// Rows that a warp walks, `most` or fewer where that leaves less than about two CTAs an SM (rows between two runs are read twice;
 // 4 x 777 x 2048 forward: 10.2 us, in runs of 32 12.2).
-int run_rows(int64_t batch, int64_t L, int64_t E) {
-  int run = 32;
+constexpr int kFwdRun = 32, kBwdRun = 64;  // (8 x 2048 x 2048, us: forward 36, with 64 37; backward 57, with 32 62)
+int run_rows(int64_t batch, int64_t L, int64_t E, int most) {
+  int run = most;
   while (run > 8 && batch * ((E + 127) / 128) * ((L + run * kWarps - 1) / (run * kWarps)) < 296) run /= 2;
   while (L > (int64_t)run * kWarps * 65535) run *= 2;  // of a grid's rows there are no more
   return run;
@@ -472,7 +473,7 @@ unsigned runs(int64_t L, int run) { return (unsigned)std::max<int64_t>(1, (L + r
 }  // namespace
 
 int launch_conv_fwd(ConvParams p, int taps, int dtype, cudaStream_t s) {
-  p.run = run_rows(p.batch, p.L, p.E);
+  p.run = run_rows(p.batch, p.L, p.E, kFwdRun);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto ok = [&](int v) {
@@ -491,12 +492,12 @@ int launch_conv_fwd(ConvParams p, int taps, int dtype, cudaStream_t s) {
 }
 
 size_t conv_bwd_workspace(int64_t batch, int64_t L, int64_t E, int taps) {
-  return (size_t)batch * runs(L, run_rows(batch, L, E)) * E * (taps + 1) * sizeof(float);
+  return (size_t)batch * runs(L, run_rows(batch, L, E, kBwdRun)) * E * (taps + 1) * sizeof(float);
 }
 
 int launch_conv_bwd(ConvParams p, ConvGrads g, int taps, int dtype, void* ws, cudaStream_t s) {
   g.part = static_cast<float*>(ws);
-  p.run = run_rows(p.batch, p.L, p.E);
+  p.run = run_rows(p.batch, p.L, p.E, kBwdRun);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int es = sizeof(T);
