@@ -6,10 +6,11 @@
 // channel's lanes are formed for several steps together by halving exchanges, and y leaves
 // through shared memory in whole rows. The next tile's operands are loaded while this one is scanned.
 //
-// Bound by the issue of instructions: about 11 a step, channel and state, of which the exponential alone holds its unit (16 a
-// clock and SM) for as long as eight issues. 8 x 2048 x 2048 x 16 of bf16 with a gate take 309 us (270 MB and the states that the
-// backward needs, 537 MB, at 1.7 TB/s; the exponentials alone would take 120). In other shapes, us: 128 threads 327; 32 threads and
-// two channels a lane 344, 64 and two 331 to 348; a quarter of the decays by a polynomial on the FMA pipe 323; K = 2, P = 8 727.
+// Bound by the issue of instructions: about 10 a step, channel and state, of which the exponential alone holds its unit (16 a
+// clock and SM) for as long as eight issues. 8 x 2048 x 2048 x 16 of bf16 with a gate take 309 us (268 MB and as much of states that
+// the backward needs, 1.7 TB/s; the exponentials alone would take 120). In other shapes, us: 128 threads 327; 32 threads and
+// two channels a lane 344, 64 and two 331 to 348; a quarter of the decays by a polynomial on the FMA pipe 323; without
+// pairs, in its first form, 727.
 #include <algorithm>
 #include <type_traits>
 
