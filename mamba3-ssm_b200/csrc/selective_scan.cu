@@ -144,10 +144,7 @@ __global__ void __launch_bounds__(NT) sel_scan_kernel(const SelScanParams p) {
             float* sv = p.save + (((int64_t)b * ((p.L + kSelSub - 1) / kSelSub) + (t0 + tg + i4) / kSelSub) * p.E + e_first + el) * NP + q * K;
             if (e_first + el < e_end) {
               if constexpr (K == 4) *reinterpret_cast<float4*>(sv) = make_float4(h[0], h[1], h[2], h[3]);
-              else {
-#pragma unroll
-                for (int k = 0; k < K; ++k) sv[k] = h[k];
-              }
+              else *reinterpret_cast<float2*>(sv) = make_float2(h[0], h[1]);
             }
           }
           const ulonglong2 d4 = *reinterpret_cast<const ulonglong2*>(&sh.dt[el][tg + i4]);
@@ -350,13 +347,38 @@ int by_type(int dtype, F&& f) {
   return f(__half{});
 }
 
+// f(K, P) as types: lanes and states a lane by the padded number of states. wide: twice the lanes with half the
+// states each, for the pass that forms the pieces' states, whose sums over lanes it has not to form (2048 channels x 16 states of 8192
+// steps: 81 us, not wide 90), and for launches of no more CTAs than SMs, where a warp's own time counts (3 x 341 x 507 x 16: 34 us,
+// not wide 46; 200 x 1024 of 16 and 32: 13, 12; 18, 17). In larger ones it costs more (8 x 2048 x 2048 x 16: 335, not wide 310).
+template <int K, int P> struct KP { static constexpr int k = K, p = P; };
+template <typename F>
+int by_states(int n, bool wide, F&& f) {
+  switch (sel_padded_states(n)) {
+    case 4: return f(KP<2, 2>{});
+    case 8: return f(KP<4, 2>{});
+    case 16: return wide ? f(KP<2, 8>{}) : f(KP<4, 4>{});
+    case 32: return wide ? f(KP<2, 16>{}) : f(KP<4, 8>{});
+    case 64: return f(KP<4, 16>{});
+    default: return f(KP<4, 32>{});
+  }
+}
+
+// threads of a CTA (which has eight channels, or four with 128 states) and CTAs of one piece of one sequence
+template <int K, int P> constexpr int pass_threads() { return P >= 16 || (K == 2 && P == 8) ? 128 : 64; }
+template <int K, int P>
+int64_t pass_tiles(const SelScanParams& p) {
+  using S = FwdSmem<K, P, pass_threads<K, P>()>;
+  const int Eg = p.E / p.G;
+  return (int64_t)p.G * ((Eg + S::EC - 1) / S::EC);
+}
+
 template <typename T, int K, int P, bool OUT>
 int launch_pass(const SelScanParams& p, cudaStream_t s) {
-  constexpr int NT = P >= 16 ? 128 : 64;  // (a CTA has eight channels at least: the pair of a thread needs them)
+  constexpr int NT = pass_threads<K, P>();
   using S = FwdSmem<K, P, NT>;
-  const int Eg = p.E / p.G;
   // what the last piece leaves enters no other
-  const dim3 grid((unsigned)(p.G * ((Eg + S::EC - 1) / S::EC)), (unsigned)(OUT ? p.nchunk : p.nchunk - 1), (unsigned)p.batch);
+  const dim3 grid((unsigned)pass_tiles<K, P>(p), (unsigned)(OUT ? p.nchunk : p.nchunk - 1), (unsigned)p.batch);
   auto go = [&](auto fast) {
     static std::atomic<bool> done[kMaxDevices];
     constexpr bool FAST = decltype(fast)::value;
@@ -368,20 +390,6 @@ int launch_pass(const SelScanParams& p, cudaStream_t s) {
   const bool fast = p.vec_u && p.vec_d && (p.vec_z || p.z.p == nullptr) && p.vec_y && p.vec_B && p.vec_C &&
                     (f32 || (!p.delta_f32 && !p.bc_f32));
   return fast ? go(std::true_type{}) : go(std::false_type{});
-}
-
-// f(K, P) as types: lanes and states a lane by the padded number of states
-template <int K, int P> struct KP { static constexpr int k = K, p = P; };
-template <typename F>
-int by_states(int n, F&& f) {
-  switch (sel_padded_states(n)) {
-    case 4: return f(KP<2, 2>{});
-    case 8: return f(KP<4, 2>{});
-    case 16: return f(KP<4, 4>{});
-    case 32: return f(KP<4, 8>{});
-    case 64: return f(KP<4, 16>{});
-    default: return f(KP<4, 32>{});
-  }
 }
 
 }  // namespace
@@ -441,16 +449,18 @@ int launch_sel_scan_fwd(SelScanParams p, int dtype, void* ws, cudaStream_t s) {
   }
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    return by_states(p.N, [&](auto kp) {
-      using L_ = decltype(kp);
-      if (p.nchunk > 1) {
-        M3_TRY((launch_pass<T, L_::k, L_::p, false>(p, s)));
-        const dim3 grid((unsigned)(((int64_t)p.E * np + 255) / 256), (unsigned)p.batch);
-        sel_carry_kernel<<<grid, 256, 0, s>>>(p, np);
-        M3_TRY(check_launch("sel_carry_kernel"));
-      }
-      return launch_pass<T, L_::k, L_::p, true>(p, s);
+    if (p.nchunk > 1) {
+      M3_TRY(by_states(p.N, true, [&](auto kp) { return launch_pass<T, decltype(kp)::k, decltype(kp)::p, false>(p, s); }));
+      const dim3 grid((unsigned)(((int64_t)p.E * np + 255) / 256), (unsigned)p.batch);
+      sel_carry_kernel<<<grid, 256, 0, s>>>(p, np);
+      M3_TRY(check_launch("sel_carry_kernel"));
+    }
+    bool few = false;
+    by_states(p.N, false, [&](auto kp) {
+      few = pass_tiles<decltype(kp)::k, decltype(kp)::p>(p) * p.nchunk * p.batch <= sms;
+      return 0;
     });
+    return by_states(p.N, few, [&](auto kp) { return launch_pass<T, decltype(kp)::k, decltype(kp)::p, true>(p, s); });
   });
 }
 
