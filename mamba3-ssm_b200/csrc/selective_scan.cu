@@ -399,7 +399,7 @@ static int sel_lanes(int np) { return std::max(2, np / 4); }
 // Pieces that the sequence is cut into: one, unless the channels alone leave most of the GPU idle. A
 // piece's state has to be formed ahead (about as much work again), so cutting begins where there are less than a quarter of
 // the warps that keep an SM busy, and a piece has 256 steps at least. Steps x channels of 16 states, us cut and not:
-// 8192 x 2048 233, 569; 8192 x 4096 449, 586; 8192 x 8192 793, 755; 1024 x 1024 36, 74; 512 x 1024 33, 39.
+// 8192 x 4096 447, 586; 8192 x 8192 793, 755.
 int sel_pieces(const SelScanParams& p, int lanes, int sms, int* chunk) {
   const int64_t warps = (int64_t)p.batch * p.E * lanes / 32 + 1, want = (int64_t)sms * 16;
   int n = 1;
