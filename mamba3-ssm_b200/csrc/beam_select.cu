@@ -251,7 +251,8 @@ __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, co
   float run = -INFINITY, sum = 0.f;
   int held = 0;  // listed elements at the last barrier
   __syncthreads();
-  // a few tiles between two barriers, at which the list is cut to its best and the threshold rises
+  // a few tiles between two barriers, at which the list is cut to its best and the threshold rises (64 x 8 x 131072: 43 us with
+  // four, 46 with two, 45 with eight; half as many vectors a thread at four CTAs an SM 61)
   constexpr int kTiles = 4;
 #pragma unroll 1
   for (int g0 = begin; g0 < s1; g0 += kTiles * TILE) {
