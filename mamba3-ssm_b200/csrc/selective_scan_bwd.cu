@@ -126,9 +126,9 @@ __global__ void __launch_bounds__(NT) sel_bwd_kernel(const SelScanParams p, cons
     else store2<T>(static_cast<T*>(d) + i, FAST || g.vec_dd, second, v0, v1);
   };
 
-  // padding behind the sequence: gradients of zero
-  if (lelive)
-    for (int t = max(beg, len) + (R == 1 ? lt : lt / R); t < end; t += NT / (EC / 2)) {
+  // padding behind the sequence: gradients of zero, by all threads of a pair of channels (also those that bring nothing)
+  if (e_first + le < e_end)
+    for (int t = max(beg, len) + tid / (EC / 2); t < end; t += NT / (EC / 2)) {
       store2<T>(dup + (int64_t)t * g.du.sl, FAST || g.vec_du, second, 0.f, 0.f);
       put_ddelta(t, 0.f, 0.f);
       if (has_z) store2<T>(dzp + (int64_t)t * g.dz.sl, FAST || g.vec_dz, second, 0.f, 0.f);
