@@ -155,17 +155,10 @@ class MambaLMHeadModel(nn.Module):
         return graph.search(input_ids, max_new_tokens, length_penalty)
 
 
-class DecodeGraph:
-    """Replays one whole decode step (embedding, every layer's norm / in_proj / fused step
-    kernel / out_proj / residual, norm_f, lm_head and, with ``greedy``, the argmax) as one
-    CUDA graph. The decode cache lives in static tensors updated in place; ``logits`` and
-    ``tokens`` are static buffers overwritten by every call.
-
-        g = model.decode_graph(batch)          # captures on the current device
-        g.prefill(prompt)                      # whole prompt through the chunked scans
-        for _ in range(n): tok = g.next()      # greedy: the argmax becomes the next input
-    (``g.reset()`` then ``g.feed(t)`` per prompt token also works, like step().)
-    """
+class _StepGraph:
+    """One whole decode step (embedding, every layer's norm / in_proj / fused step kernel / out_proj /
+    residual, norm_f, lm_head and, with ``greedy``, the argmax) as one CUDA graph over static
+    tensors: the decode cache, updated in place, ``tokens`` and ``logits``."""
 
     def __init__(self, model: "MambaLMHeadModel", batch_size: int, greedy: bool = True):
         dev = model.embedding.weight.device
@@ -209,6 +202,19 @@ class DecodeGraph:
             s.zero_()
             b.zero_()
 
+
+class DecodeGraph(_StepGraph):
+    """Replays one whole decode step (embedding, every layer's norm / in_proj / fused step
+    kernel / out_proj / residual, norm_f, lm_head and, with ``greedy``, the argmax) as one
+    CUDA graph. The decode cache lives in static tensors updated in place; ``logits`` and
+    ``tokens`` are static buffers overwritten by every call.
+
+        g = model.decode_graph(batch)          # captures on the current device
+        g.prefill(prompt)                      # whole prompt through the chunked scans
+        for _ in range(n): tok = g.next()      # greedy: the argmax becomes the next input
+    (``g.reset()`` then ``g.feed(t)`` per prompt token also works, like step().)
+    """
+
     def prefill(self, prompt: torch.Tensor) -> torch.Tensor:
         """Replace the cache by that of the prompt (B, L), computed by MambaLMHeadModel.prefill
         (chunked scans, not one replay per token), and return the last position's logits
@@ -235,11 +241,11 @@ class DecodeGraph:
         return self.tokens
 
 
-class BeamGraph(DecodeGraph):
+class BeamGraph(_StepGraph):
     """Beam search with one CUDA graph a token: the selection among the previous step's logits
     (beam.beam_select), the beams' states moved to the beams that continue them
     (beam.reorder_states_, in place), and the decode step of DecodeGraph for batch_size * num_beams
-    rows.
+    rows. The tokens come from the selection, so there is no feeding of single ones.
 
         g = model.beam_graph(batch, beams, end_token)
         tokens, scores = g.search(prompt, max_new_tokens)
@@ -275,6 +281,12 @@ class BeamGraph(DecodeGraph):
         logits = super()._body()
         self.ahead.copy_(logits.view_as(self.ahead))
         return logits
+
+    def reset(self):
+        """As before any search."""
+        super().reset()
+        for t in (self.ahead, self.scores, self.parents, self.finished, self.tokens):
+            t.zero_()
 
     @torch.no_grad()
     def search(self, prompt: torch.Tensor, max_new_tokens: int, length_penalty: float = 0.0):
