@@ -10,6 +10,7 @@ Next to ``ssm_scan_siso`` / ``ssm_scan_mimo``, whose decay is one number a head 
 taps: here every channel e and state n decays by exp(dt[e] A[e, n]). Tensors are (batch, length,
 channels) with contiguous channels, read in place at any strides of batch and length (columns
 of a projection's output), in fp32, bf16 or fp16; states and sums are fp32.
+Parameters, step sizes, B and C of other real dtypes than the call allows are converted to fp32; complex ones are refused.
 
 ``lengths`` (batch) holds the positions that count of each sequence of a padded batch, on the device.
 Positions from there on are not read; outputs and gradients are 0 there, and returned states are those in
@@ -85,11 +86,18 @@ def _dense(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _param(t):
+def _f32(name, what, t):
+    """Another real dtype as fp32; a complex one would lose its imaginary part."""
+    if t.dtype.is_complex:
+        raise TypeError(f"{name}: {what} must be real, got {t.dtype} (complex operands are not supported)")
+    return t.float()
+
+
+def _param(name, what, t):
     """A parameter of the channels as the kernels read it: fp32, contiguous."""
     if t is None:
         return None
-    return _dense(t if t.dtype is _F32 else t.float())
+    return _dense(t if t.dtype is _F32 else _f32(name, what, t))
 
 
 def _needs_grad(ts):
@@ -204,9 +212,9 @@ def _conv_weights(name, x, weight, bias, e):
         raise ValueError(f"{name}: 2, 3 or 4 taps, got {weight.shape[1]}")
     _shape(name, "bias", bias, (e,))
     if weight.dtype is not x.dtype and weight.dtype is not _F32:
-        weight = weight.float()
+        weight = _f32(name, "weight", weight)
     if bias is not None and bias.dtype is not weight.dtype:
-        bias = bias.to(weight.dtype)
+        bias = _f32(name, "bias", bias).to(weight.dtype)
     return _inner(weight), _dense(bias)
 
 
@@ -386,11 +394,11 @@ def _scan_operands(name, u, delta, A, B, C, D, z, bias, lead):
         raise TypeError(f"{name}: z must be of u's dtype {u.dtype}, got {z.dtype}")
     dtype, dd, bd = u.dtype, delta.dtype, B.dtype
     if dd is not dtype and dd is not _F32:
-        delta = delta.float()
+        delta = _f32(name, "delta", delta)
     if bd is not C.dtype or (bd is not dtype and bd is not _F32):
-        B, C = B.float(), C.float()
-    return (_inner(u), _inner(delta), _param(A), _inner(B), _inner(C), _param(D), None if z is None else _inner(z),
-            _param(bias))
+        B, C = _f32(name, "B_proj", B), _f32(name, "C_proj", C)
+    return (_inner(u), _inner(delta), _param(name, "A", A), _inner(B), _inner(C), _param(name, "D", D),
+            None if z is None else _inner(z), _param(name, "delta_bias", bias))
 
 
 def ssm_scan_selective(u, delta, A, B_proj, C_proj, D=None, *, z=None, delta_bias=None, delta_softplus=True,
@@ -418,7 +426,7 @@ def ssm_scan_selective(u, delta, A, B_proj, C_proj, D=None, *, z=None, delta_bia
     b, _, e = u.shape
     if initial_state is not None:
         _shape(name, "initial_state", initial_state, (b, e, A.shape[1]))
-        initial_state = _param(initial_state)
+        initial_state = _param(name, "initial_state", initial_state)
     args = (*ops, initial_state, _lengths(name, lengths, b), 1 if delta_softplus else 0, bool(return_state))
     y, last = (_SelectiveScanFn.apply if _needs_grad(args[:9]) else _scan_forward)(*args)
     return (y, last) if return_state else y

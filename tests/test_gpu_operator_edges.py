@@ -3,10 +3,36 @@
 import pytest
 import torch
 
-from test_gpu_selective import _gen
+from test_gpu_selective import _gen, scan_inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+def test_complex_operands_are_refused():
+    from mamba3_ssm import causal_conv, causal_conv_step_, ssm_scan_selective, ssm_step_selective_
+    x = scan_inputs(2, 5, 8, 4)
+    h0 = torch.zeros(2, 8, 4, device=DEV)
+    c = lambda t: t.to(torch.complex64) * (1 + 1j)  # noqa: E731
+    for k in ("delta", "A", "B", "C", "D", "bias", "h0"):
+        y = {**x, "h0": h0}
+        y[k] = c(y[k])
+        with pytest.raises(TypeError, match="complex"):
+            ssm_scan_selective(*(y[i] for i in ("u", "delta", "A", "B", "C", "D")), z=y["z"], delta_bias=y["bias"], initial_state=y["h0"])
+        if k == "h0":
+            continue
+        for i in ("u", "delta", "B", "C", "z"):
+            y[i] = y[i][:, 0]
+        state = torch.ones_like(h0)
+        with pytest.raises(TypeError, match="complex"):
+            ssm_step_selective_(state, *(y[i] for i in ("u", "delta", "A", "B", "C", "D")), z=y["z"], delta_bias=y["bias"])
+        assert (state == 1).all()
+    w, bias = torch.randn(8, 4, device=DEV), torch.randn(8, device=DEV)
+    for ww, bb in ((c(w), bias), (w, c(bias)), (c(w), None), (c(w), c(bias))):
+        with pytest.raises(TypeError, match="complex"):
+            causal_conv(x["u"], ww, bb)
+        with pytest.raises(TypeError, match="complex"):
+            causal_conv_step_(torch.zeros(2, 3, 8, device=DEV), x["u"][:, 0], ww, bb)
 
 
 @pytest.mark.parametrize("mimo", [False, True])
