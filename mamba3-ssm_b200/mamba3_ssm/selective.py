@@ -211,17 +211,18 @@ def _conv_weights(name, x, weight, bias, e):
     if not 2 <= weight.shape[1] <= 4:
         raise ValueError(f"{name}: 2, 3 or 4 taps, got {weight.shape[1]}")
     _shape(name, "bias", bias, (e,))
-    if weight.dtype is not x.dtype and weight.dtype is not _F32:
+    # the kernels read both in x's dtype or both in fp32, which holds all bits of either
+    if (weight.dtype is not x.dtype and weight.dtype is not _F32) or (bias is not None and bias.dtype is not weight.dtype):
         weight = _f32(name, "weight", weight)
-    if bias is not None and bias.dtype is not weight.dtype:
-        bias = _f32(name, "bias", bias).to(weight.dtype)
+        bias = None if bias is None else _f32(name, "bias", bias)
     return _inner(weight), _dense(bias)
 
 
 def causal_conv(x, weight, bias=None, *, activation=None, initial_state=None, lengths=None, return_state=False):
     """y[b, t, e] = act(bias[e] + sum_k weight[e, k] x[b, t - K + 1 + k, e]) for x (batch, length,
     channels), weight (channels, K) with K = 2, 3 or 4, bias (channels); ``activation`` None or
-    "silu". y has x's shape and dtype. Weight and bias may be fp32 or of x's dtype.
+    "silu". y has x's shape and dtype. Weight and bias may be fp32 or of x's dtype, each by itself (two
+    dtypes are brought to fp32 first).
 
     ``initial_state`` (batch, K - 1, channels) of x's dtype: the rows in front of the first
     (zeros without it). With ``return_state`` returns (y, state), the last K - 1 rows in that layout: the

@@ -3,10 +3,12 @@
 import pytest
 import torch
 
-from test_gpu_selective import _gen, scan_inputs
+import selective_ref as R
+from test_gpu_selective import _gen, _near, check_conv, conv_inputs, scan_inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 
 
 def test_complex_operands_are_refused():
@@ -33,6 +35,21 @@ def test_complex_operands_are_refused():
             causal_conv(x["u"], ww, bb)
         with pytest.raises(TypeError, match="complex"):
             causal_conv_step_(torch.zeros(2, 3, 8, device=DEV), x["u"][:, 0], ww, bb)
+
+
+@pytest.mark.parametrize("xt,wt,bt", [("bf16", "bf16", "fp32"), ("fp16", "fp16", "fp32"), ("bf16", "fp32", "bf16"), ("bf16", "bf16", "fp16"),
+                                      ("bf16", "fp16", "bf16"), ("fp32", "bf16", "fp32"), ("fp16", "bf16", "bf16")])
+def test_convolution_keeps_the_bits_of_weight_and_bias(xt, wt, bt):
+    """Each may be of any of the dtypes by itself; none is rounded to the other's."""
+    from mamba3_ssm import causal_conv_step_
+    x, w, bias, init, dy, dlast = conv_inputs(2, 50, 40, 4, DTYPES[xt], wdtype=torch.float32)
+    w, bias = w.to(DTYPES[wt]), (4 * bias).to(DTYPES[bt])
+    check_conv(x, w, bias, init, dy, dlast, False)
+    check_conv(x, w, bias, init, dy, dlast, True)
+    state = init.clone()
+    y = causal_conv_step_(state, x[:, 0], w, bias)
+    args = (x[:, :1], w, bias, False, init)
+    _near(y, R.conv(*args)["y"], R.conv(*args, magnitudes=True)["y"], 64 * 2.0 ** -24)
 
 
 @pytest.mark.parametrize("mimo", [False, True])
