@@ -14,6 +14,7 @@
 // the join 3. Where there are many, by the rows' threads between two barriers: 64 x 8 x 131072 of bf16, a quarter ended, take
 // 43 us (101 MB, 15 us of memory; with groups' maxima and a list cut at every tile 158) and 8 to join.
 #include <algorithm>
+#include <type_traits>
 
 #include "beam.cuh"
 #include "m3_common.cuh"
@@ -173,35 +174,79 @@ __device__ __forceinline__ bool beam_counts(const BeamParams& p, int64_t b, int 
   return !(p.finished != nullptr && p.finished[b * p.fb + j * p.fk] != 0) && p.scores[b * p.sb + j * p.sk] != -INFINITY;
 }
 
-// Elements s0 .. s1 - 1 of a row, by one CTA.
-template <typename T, int U>
+// 16 bytes of the 32 in a and b, from byte 4 W + bits / 8 on.
+template <int W>
+__device__ __forceinline__ uint4 funnel(const uint4& a, const uint4& b, int bits) {
+  const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __funnelshift_r(v[W + i], v[W + i + 1], bits);
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Elements s0 .. s1 - 1 of a row, by one CTA. Which thread takes which elements, and so the sum's last bits, goes by their indices
+// alone: beams with the same logits have the same scores wherever their rows lie. Where these are not all on 16-byte boundaries
+// (ALIGNED false), floats are loaded one by one (64 x 8 x 50257: 55 us, as many as with aligned rows; shifted 63), and of 16-bit
+// elements the 16 bytes from the boundary in front of the thread's own, which are then shifted up to the next ones (47 us, 43 with
+// aligned rows; with shuffles from the neighbour's registers 51).
+template <typename T, int U, bool ALIGNED>
 __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, const T* x, int s0, int s1, Part* part, uint64_t* keys) {
   using R = Rows<T, U>;
   constexpr int VN = R::VN, TILE = R::TILE;
   const int tid = threadIdx.x;
-  // vectors lie on 16-byte boundaries: the first begins up to VN - 1 elements in front of the part
-  const int off = (int)((reinterpret_cast<uintptr_t>(x + s0) & 15) / sizeof(T));
+  constexpr bool SHIFT = !ALIGNED && sizeof(T) == 2;
+  const int off = !SHIFT ? 0 : (int)((reinterpret_cast<uintptr_t>(x + s0) & 15) / sizeof(T));
   if (tid == 0) { sh.n = 0; sh.tau = 0; }
+  // 16 bytes, element i0 the first; -inf outside the part
+  auto load = [&](int i0) {
+    if ((!SHIFT || i0 >= s0) && i0 + VN <= s1) {
+      if constexpr (!ALIGNED && !SHIFT) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(x + i0);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      return *reinterpret_cast<const uint4*>(x + i0);
+    }
+    alignas(16) T e[VN];
+#pragma unroll
+    for (int k = 0; k < VN; ++k) e[k] = i0 + k >= s0 && i0 + k < s1 ? x[i0 + k] : from_f32<T>(-INFINITY);
+    return *reinterpret_cast<const uint4*>(e);
+  };
   uint4 next[U];
   auto fetch = [&](int t0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i0 = t0 + (u * NT + tid) * VN;
-      if (i0 >= s0 && i0 + VN <= s1) {
-        next[u] = *reinterpret_cast<const uint4*>(x + i0);
-      } else {
-        alignas(16) T e[VN];
+    for (int u = 0; u < U; ++u) next[u] = load(t0 + (u * NT + tid) * VN - off);
+  };
+  // this thread's elements of the tile at t0, which has been fetched; its neighbours' bytes are in L1
+  auto take = [&](int t0, uint4 (&raw)[U]) {
 #pragma unroll
-        for (int k = 0; k < VN; ++k) e[k] = i0 + k >= s0 && i0 + k < s1 ? x[i0 + k] : from_f32<T>(-INFINITY);
-        next[u] = *reinterpret_cast<const uint4*>(e);
-      }
+    for (int u = 0; u < U; ++u) raw[u] = next[u];
+    if (!SHIFT || off == 0) return;
+    uint4 b[U];
+    const int i0 = t0 + (tid + 1) * VN - off;
+    if (t0 + TILE + VN <= s1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) b[u] = *reinterpret_cast<const uint4*>(x + i0 + u * NT * VN);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) b[u] = load(i0 + u * NT * VN);
+    }
+    const int bits = off % 2 * 16;
+    auto shift = [&](auto words) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = funnel<decltype(words)::value>(raw[u], b[u], bits);
+    };
+    switch (off / 2) {
+      case 0: return shift(std::integral_constant<int, 0>{});
+      case 1: return shift(std::integral_constant<int, 1>{});
+      case 2: return shift(std::integral_constant<int, 2>{});
+      default: return shift(std::integral_constant<int, 3>{});
     }
   };
   // Lists the tile's elements above the threshold, of those left; false where some found no place.
   auto look = [&](const uint4 (&raw)[U], const float (&vm)[U], float tm, int t0, uint32_t& left) {
     const uint64_t tau = sh.tau;
     const float tau_v = unordered((uint32_t)((tau + 1) >> 32));  // the lowest value that may pass,
-    const bool ties = key_of(tau_v, max(t0, s0)) > tau;           // and whether it may from this tile on
+    const bool ties = key_of(tau_v, t0) > tau;                    // and whether it may from this tile on
     auto may = [&](float v) { return ties ? v >= tau_v : v > tau_v; };
     const uint32_t all = 0xffffffffu;
     bool placed = true;
@@ -219,7 +264,7 @@ __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, co
       while (pass) {
         const int bit = __ffs(pass) - 1, i = t0 + (bit / VN * NT + tid) * VN + bit % VN;
         pass &= pass - 1;
-        const uint64_t key = i >= s0 && i < s1 ? key_of(to_f32(x[i]), i) : 0;
+        const uint64_t key = i < s1 ? key_of(to_f32(x[i]), i) : 0;
         if (key > tau) {
           const int at = *const_cast<volatile int*>(&sh.n) < R::CAP ? atomicAdd(&sh.n, 1) : R::CAP;
           if (at >= R::CAP) {
@@ -246,8 +291,7 @@ __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, co
     }
     return tm;
   };
-  const int begin = s0 - off;
-  fetch(begin);
+  fetch(s0);
   float run = -INFINITY, sum = 0.f;
   int held = 0;  // listed elements at the last barrier
   __syncthreads();
@@ -255,14 +299,13 @@ __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, co
   // four, 46 with two, 45 with eight; half as many vectors a thread at four CTAs an SM 61)
   constexpr int kTiles = 4;
 #pragma unroll 1
-  for (int g0 = begin; g0 < s1; g0 += kTiles * TILE) {
+  for (int g0 = s0; g0 < s1; g0 += kTiles * TILE) {
     const int g1 = min(g0 + kTiles * TILE, s1);
     bool placed = true;
 #pragma unroll 1
     for (int t0 = g0; t0 < g1; t0 += TILE) {
       uint4 raw[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = next[u];
+      take(t0, raw);
       if (t0 + TILE < s1) fetch(t0 + TILE);
       float vm[U];
       const float tm = largest(raw, vm);
@@ -287,7 +330,7 @@ __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, co
         unpack2(s, a0, a1);
         sum += a0 + a1;
       }
-      if (t0 == begin) {
+      if (t0 == s0) {
         // the first threshold: just below what the maxima of `num` threads reach, to the upper 16 bits
         const uint32_t o = ordered(tm);
         int had = 0;
@@ -308,11 +351,9 @@ __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, co
 #pragma unroll
         for (int u = 0; u < U; ++u) keep[u] = next[u];
         fetch(t0);
+        take(t0, raw);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          raw[u] = next[u];
-          next[u] = keep[u];
-        }
+        for (int u = 0; u < U; ++u) next[u] = keep[u];
         float vm[U];
         const float tm = largest(raw, vm);
         uint32_t left = ~0u;  // of this thread's U VN elements
@@ -349,14 +390,14 @@ __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, co
 }
 
 // (three CTAs an SM, at 80 registers a thread: 43 us at 64 x 8 x 131072; two 50, four, which spill, 72)
-template <typename T, int U>
+template <typename T, int U, bool ALIGNED>
 __global__ void __launch_bounds__(NT, 3) beam_rows_kernel(const BeamParams p, Part* parts, uint64_t* keys, int seg) {
   __shared__ Rows<T, U> sh;
   const int64_t row = blockIdx.y, b = row / p.beams;
   const int j = (int)(row % p.beams), s0 = blockIdx.x * seg;
   if (!beam_counts(p, b, j)) return;
   const int64_t part = row * gridDim.x + blockIdx.x;
-  row_part<T, U>(p, sh, static_cast<const T*>(p.logits) + b * p.lb + j * p.lk, s0, min(p.V, s0 + seg), parts + part, keys + part * p.num);
+  row_part<T, U, ALIGNED>(p, sh, static_cast<const T*>(p.logits) + b * p.lb + j * p.lk, s0, min(p.V, s0 + seg), parts + part, keys + part * p.num);
 }
 
 struct Cand { uint64_t value, tie; };  // score in order of integers; then beam, logit, token
@@ -542,7 +583,7 @@ __device__ __forceinline__ X* of_first(X* p) {  // the same place in the shared 
   return reinterpret_cast<X*>(r);
 }
 
-template <typename T, int U>
+template <typename T, int U, bool ALIGNED>
 __global__ void __launch_bounds__(NT) beam_cluster_kernel(const BeamParams p, int splits, int seg) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ Rows<T, U> sh;
@@ -555,8 +596,8 @@ __global__ void __launch_bounds__(NT) beam_cluster_kernel(const BeamParams p, in
   if (rank < lists) {
     const int j = rank / splits, s0 = rank % splits * seg;
     if (beam_counts(p, b, j) && s0 < p.V)
-      row_part<T, U>(p, sh, static_cast<const T*>(p.logits) + b * p.lb + j * p.lk, s0, min(p.V, s0 + seg), of_first(parts + rank),
-                     of_first(keys + rank * p.num));
+      row_part<T, U, ALIGNED>(p, sh, static_cast<const T*>(p.logits) + b * p.lb + j * p.lk, s0, min(p.V, s0 + seg), of_first(parts + rank),
+                              of_first(keys + rank * p.num));
     else if (threadIdx.x == 0)
       *of_first(parts + rank) = Part{Two{0.f, 0.f}, -INFINITY, 0};
   }
@@ -608,7 +649,7 @@ size_t beam_workspace_bytes(int64_t batch, int beams, int V, int num, int dtype,
   return w.cluster ? 0 : (size_t)batch * beams * w.splits * (sizeof(Part) + (size_t)num * sizeof(uint64_t));
 }
 
-template <typename T, int U>
+template <typename T, int U, bool ALIGNED>
 static int launch_cluster(const BeamParams& p, const BeamPlan& w, cudaStream_t s) {
   const int lists = p.beams * w.splits;
   cudaLaunchAttribute attr{};
@@ -622,7 +663,7 @@ static int launch_cluster(const BeamParams& p, const BeamPlan& w, cudaStream_t s
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, beam_cluster_kernel<T, U>, p, w.splits, w.seg);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, beam_cluster_kernel<T, U, ALIGNED>, p, w.splits, w.seg);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(M3_ERR_CUDA, std::string("beam_cluster_kernel: ") + cudaGetErrorString(e));
@@ -639,12 +680,22 @@ int launch_beam_select(const BeamParams& p, int dtype, void* ws, cudaStream_t s)
   Part* parts = static_cast<Part*>(ws);
   uint64_t* keys = reinterpret_cast<uint64_t*>(parts + rows * w.splits);
   const dim3 grid((unsigned)w.splits, (unsigned)rows);
-  auto go = [&](auto t) {
+  // parts of a row begin at multiples of a vector
+  const uint64_t any = reinterpret_cast<uintptr_t>(p.logits) | (uint64_t)(p.batch > 1 ? p.lb : 0) * dtype_size(dtype) |
+                       (uint64_t)(p.beams > 1 ? p.lk : 0) * dtype_size(dtype);
+  auto launch = [&](auto t, auto u, auto aligned) {
     using T = decltype(t);
-    if (w.cluster) return w.u == 4 ? launch_cluster<T, 4>(p, w, s) : launch_cluster<T, 1>(p, w, s);
-    if (w.u == 4) beam_rows_kernel<T, 4><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
-    else beam_rows_kernel<T, 1><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
+    constexpr int U = decltype(u)::value;
+    constexpr bool ALIGNED = decltype(aligned)::value;
+    if (w.cluster) return launch_cluster<T, U, ALIGNED>(p, w, s);
+    beam_rows_kernel<T, U, ALIGNED><<<grid, NT, 0, s>>>(p, parts, keys, w.seg);
     return check_launch("beam_rows_kernel");
+  };
+  auto by_place = [&](auto t, auto u) {
+    return any % 16 == 0 ? launch(t, u, std::true_type{}) : launch(t, u, std::false_type{});
+  };
+  auto go = [&](auto t) {
+    return w.u == 4 ? by_place(t, std::integral_constant<int, 4>{}) : by_place(t, std::integral_constant<int, 1>{});
   };
   if (dtype == M3_FLOAT32) M3_TRY(go(float{}));
   else if (dtype == M3_BFLOAT16) M3_TRY(go(__nv_bfloat16{}));
