@@ -511,7 +511,8 @@ int m3_selective_step(m3_tensor* state, const m3_tensor* u, const m3_tensor* del
  * Beam search (no counterpart in the reference's package).
  * m3_beam_select: of each prompt, the num largest of scores[j] + logits[j, v] - log sum exp
  *   logits[j, :] over its beams j and tokens v, largest first, joined and compared in two f32 (about 48
- *   bits), the sums of exp within a thread in one; ties to the lowest (j, v). A finished beam offers end_token alone, at no cost (its logits are not read);
+ *   bits), the sums of exp within a thread in one. Of equal ones the lower beam's come first, within a beam the
+ *   larger logit's, then the lower token's. A finished beam offers end_token alone, at no cost (its logits are not read);
  *   a beam with score -inf, or all of whose logits are -inf, offers -inf; one with a NaN or +inf
  *   among its logits, or as its score, offers NaN, which ranks first.
  *   logits (batch, beams, V), beams <= 32, V <= 2^24; scores (batch, beams) f32; finished (batch,

@@ -1,5 +1,6 @@
 // Selection of a step of beam search: with lse_j = log sum_v exp(l[j, v]) of beam j's logits,
-//   the `num` largest of score_j + l[j, v] - lse_j over all beams j and tokens v, ties to the lowest (j, v).
+//   the `num` largest of score_j + l[j, v] - lse_j over all beams j and tokens v. Of equal ones the lower beam's come first, and
+//   within a beam the larger logit's, then the lower token's (the order of the sums before they are rounded).
 // A beam that has ended offers its end token at no cost; one whose score is -inf, or all of whose logits
 // are, offers -inf; one with a NaN or an infinite logit or score offers NaN, which ranks first.
 // beam_rows_kernel reads the logits once: a CTA a part of a row keeps its largest element and the sum of
@@ -512,13 +513,13 @@ __device__ __forceinline__ void join_parts(const BeamParams& p, int64_t b, const
       for (int l0 = 0; l0 < lists; l0 += NT) c += __syncthreads_count(l0 + tid < lists && head[l0 + tid].value >= t);
       return c;
     });
-    const bool equal = had > kHeads * p.num;  // heads, of which the first lists (and beams) come first
+    const bool equal = had > kHeads * p.num;  // heads, which their ties' keys tell apart
     for (int l = tid; l < lists; l += NT) {
-      const uint64_t mine = head[l].value;
-      if (head[l].tie == 0 || mine < tau) continue;
+      const Cand mine = head[l];
+      if (mine.tie == 0 || mine.value < tau) continue;
       int r = 0;
       if (equal) {
-        for (int i = 0; i < lists; ++i) r += head[i].value > mine || (head[i].value == mine && i < l);
+        for (int i = 0; i < lists; ++i) r += above(head[i], mine);
       }
       if (r < p.num) s_list[atomicAdd(&s_lists, 1)] = l;
     }
