@@ -114,6 +114,13 @@ def _no_grad_only(name, ts):
         raise RuntimeError(f"{name}: works in place, without gradients; call it under torch.no_grad()")
 
 
+def _like(t):
+    """An uninitialised tensor of t's shape, dtype and order of dimensions in memory, with contiguous channels: of rows one
+    element apart empty_like may turn the order round."""
+    y = torch.empty_like(t)
+    return y if y.stride(-1) == 1 or y.shape[-1] <= 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _written(t):
     if not t.is_inference():
         torch.autograd.graph.increment_version(t)
@@ -149,7 +156,7 @@ def _conv_forward(x, weight, bias, initial, lengths, silu, want):
     b, n, e = x.shape
     k = weight.shape[1]
     dev = x.device
-    y = torch.empty_like(x)
+    y = _like(x)
     last = torch.empty((b, k - 1, e), dtype=x.dtype, device=dev) if want else None
     vals = _conv_vals(x, weight, bias, initial, lengths, b, n, e, k)
     vals += _r3(y, b, n, e)
@@ -184,7 +191,7 @@ class _CausalConvFn(torch.autograd.Function):
         dev = x.device
         dy = torch.zeros((b, n, e), dtype=x.dtype, device=dev) if dy is None else _inner(dy)
         dlast = None if dlast is None else _inner(dlast)
-        dx = torch.empty_like(x)
+        dx = _like(x)
         dw = torch.empty((e, k), dtype=weight.dtype, device=dev)
         db = None if bias is None else torch.empty_like(bias)
         di = None
@@ -262,6 +269,8 @@ def causal_conv_step_(state, x, weight, bias=None, *, activation=None):
     x = _inner(x)
     dev = x.device
     y = torch.empty_like(x)
+    if not y.is_contiguous():  # rows of x one element apart
+        y = torch.empty((b, e), dtype=x.dtype, device=dev)
     code = _CODE[x.dtype]
     vals = [*L.rec3(state, code, b, k - 1, e), *L.rec2(x, code, b, e), *L.rec2(weight, _CODE[weight.dtype], e, k),
             *_r1(bias, e), y.data_ptr() or 1, code, 2, b, e, 0, 0, 0, 0, e, 1, 0, 0, 0, 0]
@@ -300,7 +309,7 @@ def _scan_forward(u, delta, A, B, C, D, z, bias, initial, lengths, softplus, wan
     m = A.shape[1]
     dev = u.device
     lib = L.load()
-    y = torch.empty_like(u)
+    y = _like(u)
     last = torch.empty((b, e, m), dtype=_F32, device=dev) if want else None
     vals = _scan_vals(u, delta, A, B, C, D, z, bias, initial, lengths, b, n, e, m)
     vals += _r3(y, b, n, e)
@@ -343,11 +352,11 @@ class _SelectiveScanFn(torch.autograd.Function):
         dlast = _dense(dlast)
         # (empty_like costs half of empty; it keeps the order of the dimensions in memory, which B's and C's gradients may not)
         like = torch.empty_like
-        du, ddelta, dA = like(u), like(delta), like(A)
+        du, ddelta, dA = _like(u), _like(delta), like(A)
         dB = like(B) if B.is_contiguous() else empty(B.shape, dtype=B.dtype, device=dev)
         dC = like(C) if C.is_contiguous() else empty(B.shape, dtype=B.dtype, device=dev)
         dD = None if D is None else like(D)
-        dz = None if z is None else like(z)
+        dz = None if z is None else _like(z)
         dbias = None if bias is None else like(bias)
         di = empty((b, e, m), dtype=_F32, device=dev) if initial is not None and ctx.needs_input_grad[8] else None
         vals = _scan_vals(u, delta, A, B, C, D, z, bias, initial, lengths, b, n, e, m)
@@ -450,7 +459,7 @@ def ssm_step_selective_(state, u, delta, A, B_proj, C_proj, D=None, *, z=None, d
     if state.dtype is not _F32:
         raise TypeError(f"{name}: state must be float32, got {state.dtype}")
     dev = u.device
-    y = torch.empty_like(u)
+    y = _like(u)
     code = _CODE[B.dtype]
     vals = [*_r3(state, b, e, m), *_r2(u, b, e), *_r2(delta, b, e), *_r2(A, e, m)]
     if B.dim() == 2:  # one group

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import selective_ref as R
-from test_gpu_selective import _gen, _near, check_conv, conv_inputs, scan_inputs
+from test_gpu_selective import _gen, _near, check_conv, check_scan, conv_inputs, scan_inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -50,6 +50,36 @@ def test_convolution_keeps_the_bits_of_weight_and_bias(xt, wt, bt):
     y = causal_conv_step_(state, x[:, 0], w, bias)
     args = (x[:, :1], w, bias, False, init)
     _near(y, R.conv(*args)["y"], R.conv(*args, magnitudes=True)["y"], 64 * 2.0 ** -24)
+
+
+# ------------------------------------------------------------------------------ strides
+@pytest.mark.parametrize("shape,strides", [((2, 4, 8), (16, 1, 1)), ((1, 4, 8), (1, 8, 1)), ((3, 8, 12), (1, 12, 1)), ((1, 2, 4), (1, 1, 1)),
+                                           ((2, 4, 6), (1, 0, 1)), ((3, 2, 4), (0, 0, 1))])
+def test_rows_one_element_apart(shape, strides):
+    """Windows over one buffer, and a batch of one with any stride: outputs have strides of their own."""
+    b, n, e = shape
+    window = lambda dtype, seed, f=lambda t: t: f(torch.randn(200, device=DEV, generator=_gen(seed))).to(dtype).as_strided(shape, strides)  # noqa: E731
+    for dtype in (torch.float32, torch.bfloat16):
+        x = scan_inputs(b, n, e, 16, dtype=dtype)
+        x["u"], x["z"], x["delta"] = window(dtype, 1), window(dtype, 2), window(dtype, 3, lambda t: -t.abs())
+        check_scan(x)
+        _, w, bias, init, dy, dlast = conv_inputs(b, n, e, 4, dtype)
+        check_conv(x["u"], w, bias, init, dy, dlast, True)
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 8), (1, 1)), ((2, 4), (1, 1)), ((3, 8), (0, 1)), ((8, 4), (1, 1))])
+def test_single_steps_of_rows_one_element_apart(shape, strides):
+    from mamba3_ssm import causal_conv_step_, ssm_step_selective_
+    b, e = shape
+    x = torch.randn(40, device=DEV, generator=_gen(1)).as_strided(shape, strides)
+    w, state = torch.randn(e, 4, device=DEV, generator=_gen(2)), torch.randn(b, 3, e, device=DEV, generator=_gen(3))
+    want = causal_conv_step_(state.clone(), x.contiguous(), w)
+    assert torch.equal(causal_conv_step_(state, x, w), want)
+    o = scan_inputs(b, 1, e, 16)
+    h = torch.randn(b, e, 16, device=DEV, generator=_gen(4))
+    args = (o["delta"][:, 0], o["A"], o["B"][:, 0], o["C"][:, 0])
+    want = ssm_step_selective_(h.clone(), x.contiguous(), *args)
+    assert torch.equal(ssm_step_selective_(h, x, *args), want)
 
 
 @pytest.mark.parametrize("mimo", [False, True])
