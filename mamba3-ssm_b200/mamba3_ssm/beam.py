@@ -159,7 +159,7 @@ def reorder_states_(states, parents, *, out=None):
     first = src[0].shape
     if not first or (batch and first[0] % batch):
         raise ValueError(f"{name}: states of {tuple(first)} for a batch of {batch}")
-    source = first[0] // batch if batch else 0
+    source = first[0] // batch if batch else rows  # (of an empty batch nothing is moved)
     dev = parents.device
     ptrs, pitch, size = _pitches("states", src, source * batch, dev.index)
     dst = src

@@ -82,6 +82,16 @@ def test_single_steps_of_rows_one_element_apart(shape, strides):
     assert torch.equal(ssm_step_selective_(h, x, *args), want)
 
 
+def test_moves_of_an_empty_batch():
+    from mamba3_ssm import reorder_states_
+    par = torch.zeros(0, 4, dtype=torch.long, device=DEV)
+    t, o = torch.zeros(0, 7, device=DEV), torch.zeros(0, 7, device=DEV)
+    assert reorder_states_(t, par) is t
+    assert reorder_states_([t], par, out=[o])[0] is o
+    with pytest.raises(ValueError):
+        reorder_states_(torch.zeros(4, 7, device=DEV), par)
+
+
 @pytest.mark.parametrize("mimo", [False, True])
 def test_beam_graph_starts_over(mimo):
     """reset() leaves nothing of an earlier search; what DecodeGraph does token by token is not offered."""
