@@ -177,6 +177,8 @@ def reorder_states_(states, parents, *, out=None):
         for t, o in zip(src, dst):
             if t.shape[1:] != o.shape[1:] or t.dtype is not o.dtype:
                 raise ValueError(f"{name}: output of rows {tuple(o.shape[1:])} {o.dtype} for rows {tuple(t.shape[1:])} {t.dtype}")
+            if t.dtype.is_complex and t.is_conj() != o.is_conj():  # their memory holds different numbers
+                raise ValueError(f"{name}: states and out are lazily conjugated both or neither; see torch.Tensor.resolve_conj")
         if not source:
             size = osize
     if torch.is_grad_enabled() and (any([t.requires_grad for t in src]) or (out is not None and any([t.requires_grad for t in dst]))):

@@ -92,6 +92,25 @@ def test_moves_of_an_empty_batch():
         reorder_states_(torch.zeros(4, 7, device=DEV), par)
 
 
+def test_moves_of_conjugated_states():
+    """A lazily conjugated tensor holds the other numbers in memory."""
+    from mamba3_ssm import reorder_states_
+    t = torch.randn(4, 6, dtype=torch.complex64, device=DEV)
+    par = torch.tensor([[1, 1, 3, 0]], device=DEV)
+    for src in (t, t.conj()):
+        for dst in (torch.empty_like(t), torch.empty_like(t).conj()):
+            if src.is_conj() == dst.is_conj():
+                reorder_states_(src, par, out=dst)
+                assert torch.equal(dst.resolve_conj(), src.resolve_conj()[par[0]])
+            else:
+                with pytest.raises(ValueError, match="conjugat"):
+                    reorder_states_(src, par, out=dst)
+    c = t.clone().conj()
+    want = c.resolve_conj()[par[0]]
+    reorder_states_(c, par)
+    assert torch.equal(c.resolve_conj(), want)
+
+
 @pytest.mark.parametrize("mimo", [False, True])
 def test_beam_graph_starts_over(mimo):
     """reset() leaves nothing of an earlier search; what DecodeGraph does token by token is not offered."""
