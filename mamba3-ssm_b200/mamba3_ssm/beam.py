@@ -13,6 +13,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from .ops import _require_cuda
@@ -51,6 +52,12 @@ def beam_select(logits, scores, num=None, *, finished=None, end_token=0):
     dev = logits.device
     if not (logits.is_cuda and scores.is_cuda):
         _require_cuda(name, logits, scores, finished)
+    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+        raise RuntimeError(f"{name}: works without gradients; call it under torch.no_grad()")
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for k, t in (("logits", logits), ("scores", scores)):
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name}: no forward-mode derivative, but {k} carry a tangent")
     if logits.dtype not in _FLOATS:
         raise TypeError(f"{name}: logits must be float32, bfloat16 or float16, got {logits.dtype}")
     shape = scores.shape

@@ -111,6 +111,23 @@ def test_moves_of_conjugated_states():
     assert torch.equal(c.resolve_conj(), want)
 
 
+def test_selection_refuses_what_carries_derivatives():
+    from mamba3_ssm import beam_select
+    from torch.autograd import forward_ad
+    logits, scores = torch.randn(2, 3, 50, device=DEV), torch.zeros(2, 3, device=DEV)
+    want = beam_select(logits, scores)
+    for a, b in ((logits.clone().requires_grad_(True), scores), (logits, scores.clone().requires_grad_(True))):
+        with pytest.raises(RuntimeError, match="without gradients"):
+            beam_select(a, b)
+        with torch.no_grad():
+            assert all(torch.equal(p, q) for p, q in zip(beam_select(a, b), want))
+    with forward_ad.dual_level():
+        for a, b in ((forward_ad.make_dual(logits, logits), scores), (logits, forward_ad.make_dual(scores, scores))):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                beam_select(a, b)
+        assert all(torch.equal(p, q) for p, q in zip(beam_select(logits, scores), want))
+
+
 @pytest.mark.parametrize("mimo", [False, True])
 def test_beam_graph_starts_over(mimo):
     """reset() leaves nothing of an earlier search; what DecodeGraph does token by token is not offered."""
