@@ -459,7 +459,7 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
  * m3_causal_conv:  pre[t] = bias + sum_k weight[:, k] x[t - K + 1 + k], y = pre, or
  *   pre * sigmoid(pre) with silu = 1; K = 2, 3 or 4. Rows in front of the first are those of
  *   initial, absent = zeros.
- *   x (batch, seqlen, E), weight (E, K) and bias (E, optional) of f32 or x's dtype, initial
+ *   x (batch, seqlen, E), weight (E, K) and bias (E, optional) of one dtype, f32 or x's, initial
  *   (batch, K - 1, E, optional) of x's dtype; y as x; last (batch, K - 1, E, optional), contiguous,
  *   x's dtype: the last K - 1 rows, what the next call takes as initial or m3_causal_conv_step as state.
  * m3_causal_conv_bwd: dx, dweight, dbias, dinitial (the last two optional) from dy and dlast
@@ -470,7 +470,7 @@ int m3_clip_grads(int64_t count, const void* const* grads, const int64_t* numel,
  *   u (batch, seqlen, E); delta the same, u's dtype or f32; z as u, optional (no gate); B, C
  *   (batch, seqlen, G, N), u's dtype or f32 both, E a multiple of G; N <= 128; A (E, N), D (E,
  *   optional), delta_bias (E, optional) f32 contiguous; initial, last (batch, E, N, optional) f32
- *   contiguous; y as u. states, optional: m3_selective_scan_states_size bytes that keep what
+ *   contiguous; y as u. batch <= 65535, as in m3_causal_conv (not in the single steps). states, optional: m3_selective_scan_states_size bytes that keep what
  *   m3_selective_scan_bwd needs. workspace: m3_selective_scan_workspace_size bytes.
  * m3_selective_scan_bwd: all gradients from dy and dlast (optional); dA, dD, ddelta_bias f32, dB
  *   and dC contiguous of B's dtype, dinitial optional.
@@ -515,7 +515,7 @@ int m3_selective_step(m3_tensor* state, const m3_tensor* u, const m3_tensor* del
  *   larger logit's, then the lower token's. A finished beam offers end_token alone, at no cost (its logits are not read);
  *   a beam with score -inf, or all of whose logits are -inf, offers -inf; one with a NaN or +inf
  *   among its logits, or as its score, offers NaN, which ranks first.
- *   logits (batch, beams, V), beams <= 32, V <= 2^24; scores (batch, beams) f32; finished (batch,
+ *   logits (batch, beams, V), beams <= 32, batch * beams <= 65535, V <= 2^24; scores (batch, beams) f32; finished (batch,
  *   beams) u8, optional; out_scores f32, parents (j) and tokens (v) i64: (batch, num) contiguous,
  *   num <= 64. workspace: m3_beam_select_workspace_size bytes (0 where one launch does it all), 16-byte aligned.
  * m3_reorder_states: row b T + j of every tensor becomes its row b S + parents[b, j], zeros where

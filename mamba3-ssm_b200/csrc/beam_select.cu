@@ -13,7 +13,7 @@
 // beam_cluster_kernel does both for few and short rows.
 // Bound by latency where there are few rows: 1 x 4 x 50000 of bf16 take 12 us in one launch (0.4 MB), of which the rows are 5,
 // the join 3. Where there are many, by the rows' threads between two barriers: 64 x 8 x 131072 of bf16, a quarter ended, take
-// 43 us (101 MB, 15 us of memory; with groups' maxima and a list cut at every tile 158) and 8 to join.
+// 42 us (101 MB, 15 us of memory; with groups' maxima and a list cut at every tile 158) and 8 to join.
 #include <algorithm>
 #include <type_traits>
 
@@ -187,9 +187,9 @@ __device__ __forceinline__ uint4 funnel(const uint4& a, const uint4& b, int bits
 
 // Elements s0 .. s1 - 1 of a row, by one CTA. Which thread takes which elements, and so the sum's last bits, goes by their indices
 // alone: beams with the same logits have the same scores wherever their rows lie. Where these are not all on 16-byte boundaries
-// (ALIGNED false), floats are loaded one by one (64 x 8 x 50257: 55 us, as many as with aligned rows; shifted 63), and of 16-bit
-// elements the 16 bytes from the boundary in front of the thread's own, which are then shifted up to the next ones (47 us, 43 with
-// aligned rows; with shuffles from the neighbour's registers 51).
+// (ALIGNED false), floats are loaded one by one (64 x 8 x 50257: 44 us, as many as with aligned rows), and of 16-bit elements the
+// 16 bytes from the boundary in front of the thread's own and those behind it, which are shifted (36 us, 32 with aligned rows). Both
+// kernels in a graph: floats 55 us, shifted 63; 16-bit elements 47, by shuffles from the neighbour's registers 51.
 template <typename T, int U, bool ALIGNED>
 __device__ __forceinline__ void row_part(const BeamParams& p, Rows<T, U>& sh, const T* x, int s0, int s1, Part* part, uint64_t* keys) {
   using R = Rows<T, U>;

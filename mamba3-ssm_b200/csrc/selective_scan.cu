@@ -364,7 +364,8 @@ int by_states(int n, bool wide, F&& f) {
   }
 }
 
-// threads of a CTA (which has eight channels, or four with 128 states) and CTAs of one piece of one sequence
+// threads of a CTA, which has 32, 32, 16, 8, 8 and 4 channels with 4, 8, 16, 32, 64 and 128 states, and CTAs of one piece of one
+// sequence
 template <int K, int P> constexpr int pass_threads() { return P >= 16 || (K == 2 && P == 8) ? 128 : 64; }
 template <int K, int P>
 int64_t pass_tiles(const SelScanParams& p) {

@@ -39,7 +39,7 @@ def beam_select(logits, scores, num=None, *, finished=None, end_token=0):
     thread, so that the difference between two beams is good to about 2^-20. Of equal sums the lower beam's come
     first, and within a beam the larger logit's, then the lower token's; beams with the same logits and scores tie.
     logits (batch, beams, V), or (batch * beams, V) as a model returns them, fp32, bf16 or fp16; at most 32
-    beams; scores (batch, beams) fp32: the beams' sums of log-probabilities so far.
+    beams and 65535 rows; scores (batch, beams) fp32: the beams' sums of log-probabilities so far.
 
     ``finished`` (batch, beams), optional: such a beam offers ``end_token`` alone, with its score
     unchanged. A beam with score -inf (an empty place, as all but one in a search's first step), or

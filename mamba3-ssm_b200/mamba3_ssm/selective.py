@@ -11,6 +11,7 @@ taps: here every channel e and state n decays by exp(dt[e] A[e, n]). Tensors are
 channels) with contiguous channels, read in place at any strides of batch and length (columns
 of a projection's output), in fp32, bf16 or fp16; states and sums are fp32.
 Parameters, step sizes, B and C of other real dtypes than the call allows are converted to fp32; complex ones are refused.
+A sequence call takes at most 65535 sequences. A is finite (0 times an infinite one would be NaN at a step size of 0, as in padding).
 
 ``lengths`` (batch) holds the positions that count of each sequence of a padded batch, on the device.
 Positions from there on are not read; outputs and gradients are 0 there, and returned states are those in
